@@ -19,6 +19,7 @@ ALU_SHIFT32, ALU_SILU32, ALU_EMUL32, ALU_SHIFT32W = 1, 6, 8, 9
 MOVY_PAIRS32, MOVY_INT16 = 0, 1
 PLAN_GRAPH, PLAN_PERSISTENT, PLAN_PERSISTENT_COOP = 0, 1, 2
 FENCE_ALL, FENCE_AUTO = 0, 1
+DT_F32, DT_BF16, DT_F16, DT_I16 = 0, 1, 2, 3
 WAIT_NONE, WAIT_GRID, WAIT_INPUT = 0, 1, 2   # w4a8_plan_fences
 
 _P = ctypes.c_void_p
@@ -70,6 +71,21 @@ SIGNATURES = {
     "w4a8_head_topk32_async": [_P, _P, _I32, _P, _P, _I32, _I32, _I32, _P],
     "w4a8_head_topk32_noalloc_async": [_P, _P, _I32, _P, _P, _I32, _I32, _I32, _P],
     "w4a8_mlp_async": [_P, _P, _P, _P, _I32, _I32, _I32, _P, _P, _I32, _I32, _P, _P],
+    "w4a8_kv_create": [_P] + [_I32] * 8 + [_P] * 4 + [ctypes.POINTER(_P)],
+    "w4a8_kv_destroy": [_P],
+    "w4a8_kv_extend_async": [_P, _P, _P, _I32],
+    "w4a8_kv_append_async": [_P, _I32, _I32, _I32, _P, _I64, _I64, _P, _I64, _I64, _P, _P,
+                             _I32],
+    "w4a8_kv_fork_async": [_P, _P, _P, _I32],
+    "w4a8_kv_free_async": [_P, _P, _I32],
+    "w4a8_kv_compact_async": [_P],
+    "w4a8_kv_copy_async": [_P, _P, _P, _I32],
+    "w4a8_kv_attend_workspace": [_P, _I32, _I32, _P],
+    "w4a8_kv_attend_async": [_P, _I32, _I32, _I32, _I32, _P, _I64, _I64, _P, _I64, _I64, _P,
+                             _P, _I32, _I32, ctypes.c_double, _P, _I64],
+    "w4a8_delta_step_async": [_P, _P],
+    "w4a8_delta_chunk_workspace": [_P, _I64, _I64, _I64, _P],
+    "w4a8_delta_chunk_async": [_P, _P],
     "w4a8_plan_create": [_P, ctypes.POINTER(_P)],
     "w4a8_plan_add_site": [_P, _I32, _PP, _P, _P, _PP, _I32, _P, _P, _I32, _I32,
                            _I32, _P, _P, _P],

@@ -11,11 +11,13 @@
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
 #include "../../include/fable5_w4a8.h"
 #include "w4a8_internal.h"
+#include "w4a8_mixers.h"
 
 using namespace w4a8;
 
@@ -203,6 +205,18 @@ int take_err(w4a8_ctx *c) {
       return fail(W4A8_E_HIP, "TOPK-32's wait for the lists of earlier chunks timed out");
     if (h & 1) return fail(W4A8_E_Y32_OVF, "y32 overflow — sh miscomputed");
     if (h & 16) return fail(W4A8_E_RANGE, "MOVX source is not int8-packed");
+    if (h & kErrKvFull)
+      return fail(W4A8_E_RANGE, "KV cache: too few free pages; the call changed nothing");
+    if (h & kErrKvList)
+      return fail(W4A8_E_RANGE, "KV cache: a sequence listed twice, or a fork's child that is "
+                                "not empty or a parent too; the call changed nothing");
+    if (h & kErrKvRange)
+      return fail(W4A8_E_RANGE, "KV cache: a sequence, position, length or page outside the "
+                                "cache; it was not followed");
+    if (h & kErrDelta)
+      return fail(W4A8_E_RANGE, "delta rule: a state slot named twice or outside the states, or "
+                                "bounds that do not lie in order within the tokens; those rows "
+                                "were not run");
   }
   return W4A8_OK;
 }
@@ -1981,5 +1995,273 @@ int w4a8_plan_destroy(w4a8_plan *p) {
   delete p;
   return W4A8_OK;
 }
+
+// ------------------------------------------------------------------ mixers
+struct w4a8_kv {
+  w4a8_ctx *ctx = nullptr;
+  KvCache c{};
+};
+
+namespace {
+
+// Activations of the mixers: 16-byte aligned, every stride whole 16 bytes.
+bool rows_ok(const void *p, int dtype, int64_t a, int64_t b) {
+  const int64_t per = 16 / dtype_size(dtype);
+  return p && aligned16(p) && a >= 0 && b >= 0 && a % per == 0 && b % per == 0;
+}
+
+int check_act(int32_t cache_dtype, int32_t dtype, int32_t frac) {
+  if (dtype != cache_dtype && dtype != DT_I16)
+    return fail(W4A8_E_ARG, "activations must have the cache's dtype or int16");
+  if (frac < 0 || frac > 31) return fail(W4A8_E_ARG, "fraction bits must be 0..31");
+  return W4A8_OK;
+}
+
+float unit_of(int32_t dtype, int64_t frac) {
+  return dtype == DT_I16 ? ldexpf(1.f, -(int)frac) : 1.f;
+}
+
+int check_list(const w4a8_kv *kv, const void *list, const void *list2, int32_t n) {
+  if (!kv) return fail(W4A8_E_ARG, "null cache");
+  if (n < 0 || (n > 0 && (!list || !list2))) return fail(W4A8_E_ARG, "bad list");
+  return W4A8_OK;
+}
+
+const char *delta_fault(const w4a8_delta *d, bool chunk) {
+  if (d->dtype < DT_F32 || d->dtype > DT_I16) return "unknown dtype";
+  if (d->dk != 64 && d->dk != 128) return "dk must be 64 or 128";
+  if (d->dv < 16 || d->dv > 256 || d->dv % 16) return "dv must be a multiple of 16, 16..256";
+  if (d->hk < 1 || d->hv < 1 || d->hv % d->hk || d->hv > 65535)
+    return "hv must be a multiple of hk";
+  if (d->rows < 0 || d->tokens < 0 || d->rows > INT32_MAX || d->tokens > INT32_MAX ||
+      d->nslots < 0 || d->nslots > INT32_MAX)
+    return "rows, tokens and slots must be 0..2^31 - 1";
+  if (!chunk && d->tokens != d->rows) return "a step has one token per row";
+  if (d->frac < 0 || d->frac > 31 || d->out_frac < 0 || d->out_frac > 31)
+    return "fraction bits must be 0..31";
+  if (d->rows == 0) return nullptr;
+  if (!d->slots && d->nslots < d->rows) return "fewer states than rows";
+  if (chunk && !d->cu) return "cu is needed";
+  const int t = (int)d->dtype;
+  if (!d->state || !aligned16(d->state)) return "state must be 16-byte aligned";
+  if (d->tokens > 0) {
+    if (!rows_ok(d->q, t, d->q_token, d->q_head) || !rows_ok(d->k, t, d->k_token, d->k_head) ||
+        !rows_ok(d->v, t, d->v_token, d->v_head) ||
+        !rows_ok(d->out, t, d->out_token, d->out_head))
+      return "q, k, v and out must be 16-byte aligned, their strides whole 16 bytes";
+    if (!d->g || !d->beta || ((uintptr_t)d->g & 3) || ((uintptr_t)d->beta & 3) ||
+        d->g_token < 0 || d->beta_token < 0)
+      return "g and beta must be 4-byte aligned";
+  }
+  return nullptr;
+}
+
+int delta_launch(w4a8_ctx *c, const w4a8_delta *d, bool chunk) {
+  if (!c || !d) return fail(W4A8_E_ARG, "null argument");
+  if (const char *why = delta_fault(d, chunk)) return fail(W4A8_E_ARG, why);
+  if (d->rows == 0) return W4A8_OK;
+  const int64_t need = chunk ? delta_workspace(d->tokens, d->rows, d->hv) : 0;
+  if (need > 0 && (!d->ws || !aligned16(d->ws) || d->ws_bytes < need))
+    return fail(W4A8_E_ARG, "delta rule: the workspace holds " + std::to_string(d->ws_bytes) +
+                                " bytes, the call needs " + std::to_string(need));
+  Delta p{};
+  p.q = d->q, p.k = d->k, p.v = d->v, p.g = d->g, p.beta = d->beta;
+  p.state = d->state, p.out = d->out, p.slots = d->slots;
+  p.cu = chunk ? d->cu : nullptr;
+  p.ws = d->ws;
+  p.q_token = d->q_token, p.q_head = d->q_head, p.k_token = d->k_token, p.k_head = d->k_head;
+  p.v_token = d->v_token, p.v_head = d->v_head, p.out_token = d->out_token,
+  p.out_head = d->out_head;
+  p.g_token = d->g_token, p.beta_token = d->beta_token;
+  p.tokens = (int32_t)d->tokens, p.rows = (int32_t)d->rows;
+  p.hk = (int32_t)d->hk, p.hv = (int32_t)d->hv, p.dk = (int32_t)d->dk, p.dv = (int32_t)d->dv;
+  p.nslots = (int32_t)d->nslots, p.dtype = (int32_t)d->dtype;
+  p.norm = d->norm != 0, p.fresh = d->fresh != 0;
+  p.scale = (float)d->scale, p.eps = (float)d->eps;
+  p.unit = unit_of(p.dtype, d->frac);
+  p.out_unit = 1.f / unit_of(p.dtype, d->out_frac);
+  p.err = c->d_err;
+  DeviceGuard g(c->device);
+  HIP_TRY(launch_delta(p, c->stream));
+  return W4A8_OK;
+}
+
+}  // namespace
+
+int w4a8_kv_create(w4a8_ctx *c, int32_t dtype, int32_t pages, int32_t layers, int32_t kv_heads,
+                   int32_t page_tokens, int32_t head_dim, int32_t seqs, int32_t max_pages,
+                   void *d_pool, int32_t *d_refs, int32_t *d_tables, int32_t *d_lens,
+                   w4a8_kv **out) {
+  if (!c || !out || !d_pool || !d_refs || !d_tables || !d_lens)
+    return fail(W4A8_E_ARG, "null argument");
+  if (dtype < DT_F32 || dtype > DT_F16)
+    return fail(W4A8_E_ARG, "a cache is float32, bfloat16 or float16");
+  if (page_tokens < 16 || page_tokens > 1024 || (page_tokens & (page_tokens - 1)))
+    return fail(W4A8_E_ARG, "page_tokens must be a power of two, 16..1024");
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return fail(W4A8_E_ARG, "head_dim must be 64, 128 or 256");
+  // list positions and page counts are 32-bit; 2^30 leaves the scans room
+  if (pages < 1 || pages > (1 << 30) || layers < 1 || layers > 65535 || kv_heads < 1 ||
+      kv_heads > 4096 || seqs < 1 || seqs > (1 << 30) || max_pages < 1 || max_pages > (1 << 21))
+    return fail(W4A8_E_ARG, "pages, layers, kv_heads, seqs or max_pages out of range");
+  if (!aligned16(d_pool) || !aligned16(d_refs) || ((uintptr_t)d_tables & 3) ||
+      ((uintptr_t)d_lens & 3))
+    return fail(W4A8_E_ARG, "pool and refs must be 16-byte, tables and lens 4-byte aligned");
+  w4a8_kv *kv = new (std::nothrow) w4a8_kv();
+  if (!kv) return fail(W4A8_E_HIP, "out of host memory");
+  kv->ctx = c;
+  KvCache &k = kv->c;
+  k.pool = (uint8_t *)d_pool;
+  k.refs = d_refs, k.tables = d_tables, k.lens = d_lens;
+  k.err = c->d_err;
+  k.pages = pages, k.seqs = seqs, k.max_pages = max_pages;
+  k.lg_page = __builtin_ctz(page_tokens);
+  k.layers = layers, k.heads = kv_heads, k.dim = head_dim;
+  k.esize = dtype_size(dtype), k.dtype = dtype;
+  k.page_bytes = (int64_t)layers * 2 * kv_heads * page_tokens * head_dim * k.esize;
+  DeviceGuard g(c->device);
+  const int64_t words = (int64_t)kv_scratch_words(seqs, pages);
+  void *p = nullptr;
+  hipError_t e = hipMalloc(&p, sizeof(int32_t) * (size_t)words);
+  if (e == hipSuccess && (e = launch_fill_i32((int32_t *)p, 0, words, c->stream)) == hipSuccess)
+    e = hipStreamSynchronize(c->stream);
+  if (e != hipSuccess) {
+    if (p) (void)hipFree(p);
+    delete kv;
+    return fail(W4A8_E_HIP, std::string("KV cache scratch: ") + hipGetErrorString(e));
+  }
+  k.scratch = (int32_t *)p;
+  *out = kv;
+  return W4A8_OK;
+}
+
+int w4a8_kv_destroy(w4a8_kv *kv) {
+  if (!kv) return W4A8_OK;
+  DeviceGuard g(kv->ctx->device);
+  (void)hipStreamSynchronize(kv->ctx->stream);
+  (void)hipFree(kv->c.scratch);
+  delete kv;
+  return W4A8_OK;
+}
+
+int w4a8_kv_extend_async(w4a8_kv *kv, const int32_t *d_seqs, const int32_t *d_counts,
+                         int32_t n) {
+  if (int rc = check_list(kv, d_seqs, d_counts, n)) return rc;
+  if (n == 0) return W4A8_OK;
+  DeviceGuard g(kv->ctx->device);
+  HIP_TRY(launch_kv_extend(kv->c, d_seqs, d_counts, n, kv->ctx->stream));
+  return W4A8_OK;
+}
+
+int w4a8_kv_fork_async(w4a8_kv *kv, const int32_t *d_parents, const int32_t *d_children,
+                       int32_t n) {
+  if (int rc = check_list(kv, d_parents, d_children, n)) return rc;
+  if (n == 0) return W4A8_OK;
+  DeviceGuard g(kv->ctx->device);
+  HIP_TRY(launch_kv_fork(kv->c, d_parents, d_children, n, kv->ctx->stream));
+  return W4A8_OK;
+}
+
+int w4a8_kv_free_async(w4a8_kv *kv, const int32_t *d_seqs, int32_t n) {
+  if (int rc = check_list(kv, d_seqs, d_seqs, n)) return rc;
+  if (n == 0) return W4A8_OK;
+  DeviceGuard g(kv->ctx->device);
+  HIP_TRY(launch_kv_free(kv->c, d_seqs, n, kv->ctx->stream));
+  return W4A8_OK;
+}
+
+int w4a8_kv_compact_async(w4a8_kv *kv) {
+  if (!kv) return fail(W4A8_E_ARG, "null cache");
+  DeviceGuard g(kv->ctx->device);
+  HIP_TRY(launch_kv_compact(kv->c, kv->ctx->num_cu, kv->ctx->stream));
+  return W4A8_OK;
+}
+
+int w4a8_kv_copy_async(w4a8_kv *kv, const int32_t *d_src, const int32_t *d_dst, int32_t n) {
+  if (int rc = check_list(kv, d_src, d_dst, n)) return rc;
+  if (n == 0) return W4A8_OK;
+  DeviceGuard g(kv->ctx->device);
+  HIP_TRY(launch_kv_copy(kv->c, d_src, d_dst, n, kv->ctx->num_cu, kv->ctx->stream));
+  return W4A8_OK;
+}
+
+int w4a8_kv_append_async(w4a8_kv *kv, int32_t layer, int32_t dtype, int32_t frac,
+                         const void *d_k, int64_t k_token, int64_t k_head, const void *d_v,
+                         int64_t v_token, int64_t v_head, const int32_t *d_seqs,
+                         const int32_t *d_pos, int32_t n) {
+  if (int rc = check_list(kv, d_seqs, d_seqs, n)) return rc;
+  if (layer < 0 || layer >= kv->c.layers) return fail(W4A8_E_ARG, "no such layer");
+  if (int rc = check_act(kv->c.dtype, dtype, frac)) return rc;
+  if (n == 0) return W4A8_OK;
+  if (!rows_ok(d_k, dtype, k_token, k_head) || !rows_ok(d_v, dtype, v_token, v_head))
+    return fail(W4A8_E_ARG, "k and v must be 16-byte aligned, their strides whole 16 bytes");
+  DeviceGuard g(kv->ctx->device);
+  const KvAppend a{d_k,  d_v, k_token, k_head, v_token, v_head, d_seqs, d_pos,
+                   n,    layer, dtype, unit_of(dtype, frac)};
+  HIP_TRY(launch_kv_append(kv->c, a, kv->ctx->stream));
+  return W4A8_OK;
+}
+
+namespace {
+int check_heads(const w4a8_kv *kv, int32_t rows, int32_t q_heads) {
+  if (!kv) return fail(W4A8_E_ARG, "null cache");
+  if (rows < 0 || q_heads < 1 || q_heads > 65535 || q_heads % kv->c.heads)
+    return fail(W4A8_E_ARG, "q_heads must be a multiple of the cache's kv_heads");
+  // the workgroups of a launch: rows x splits, at most 2^30 rows each
+  if (rows > (1 << 24)) return fail(W4A8_E_ARG, "at most 2^24 rows");
+  return W4A8_OK;
+}
+}  // namespace
+
+int w4a8_kv_attend_workspace(const w4a8_kv *kv, int32_t rows, int32_t q_heads, int64_t *bytes) {
+  if (!bytes) return fail(W4A8_E_ARG, "null argument");
+  if (int rc = check_heads(kv, rows, q_heads)) return rc;
+  *bytes = rows ? attend_workspace(kv->c, rows, q_heads, kv->ctx->num_cu) : 0;
+  return W4A8_OK;
+}
+
+int w4a8_kv_attend_async(w4a8_kv *kv, int32_t layer, int32_t dtype, int32_t frac,
+                         int32_t out_frac, const void *d_q, int64_t q_row, int64_t q_head,
+                         void *d_out, int64_t out_row, int64_t out_head, const int32_t *d_seqs,
+                         const int32_t *d_upto, int32_t rows, int32_t q_heads, double scale,
+                         void *d_ws, int64_t ws_bytes) {
+  if (int rc = check_heads(kv, rows, q_heads)) return rc;
+  if (layer < 0 || layer >= kv->c.layers) return fail(W4A8_E_ARG, "no such layer");
+  if (int rc = check_act(kv->c.dtype, dtype, frac)) return rc;
+  if (int rc = check_act(kv->c.dtype, dtype, out_frac)) return rc;
+  if (rows == 0) return W4A8_OK;
+  if (!d_seqs) return fail(W4A8_E_ARG, "null argument");
+  if (!rows_ok(d_q, dtype, q_row, q_head) || !rows_ok(d_out, dtype, out_row, out_head))
+    return fail(W4A8_E_ARG, "q and out must be 16-byte aligned, their strides whole 16 bytes");
+  const int64_t need = attend_workspace(kv->c, rows, q_heads, kv->ctx->num_cu);
+  if (need > 0 && (!d_ws || !aligned16(d_ws) || ws_bytes < need))
+    return fail(W4A8_E_ARG, "attention: the workspace holds " + std::to_string(ws_bytes) +
+                                " bytes, the call needs " + std::to_string(need));
+  Attend a{};
+  a.q = d_q, a.out = d_out;
+  a.q_row = q_row, a.q_head = q_head, a.out_row = out_row, a.out_head = out_head;
+  a.seqs = d_seqs, a.upto = d_upto;
+  a.part = (float *)d_ws;
+  a.rows = rows, a.hq = q_heads, a.layer = layer, a.dtype = dtype;
+  a.splits = attend_splits(kv->c, rows, q_heads, kv->ctx->num_cu);
+  a.scale = (float)(scale * unit_of(dtype, frac) * 1.4426950408889634);
+  a.out_unit = 1.f / unit_of(dtype, out_frac);
+  DeviceGuard g(kv->ctx->device);
+  HIP_TRY(launch_attend(kv->c, a, kv->ctx->stream));
+  return W4A8_OK;
+}
+
+int w4a8_delta_step_async(w4a8_ctx *c, const w4a8_delta *d) { return delta_launch(c, d, false); }
+
+int w4a8_delta_chunk_workspace(w4a8_ctx *c, int64_t tokens, int64_t rows, int64_t hv,
+                               int64_t *bytes) {
+  if (!c || !bytes || tokens < 0 || rows < 0 || hv < 1 || tokens > INT32_MAX ||
+      rows > INT32_MAX || hv > 65535)
+    return fail(W4A8_E_ARG, "bad argument");
+  *bytes = rows ? delta_workspace(tokens, rows, hv) : 0;
+  return W4A8_OK;
+}
+
+int w4a8_delta_chunk_async(w4a8_ctx *c, const w4a8_delta *d) { return delta_launch(c, d, true); }
 
 }  // extern "C"

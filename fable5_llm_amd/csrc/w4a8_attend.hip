@@ -1,0 +1,473 @@
+// Attention of one new token per row over a paged key-value cache.
+//
+//   o_h = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale q_h . k_t - m),
+//
+// in one pass over the cache with a running maximum m and sum; a row's tokens
+// are split over workgroups when there are few rows, each split leaving its
+// maximum, sum and unnormalised output for a second kernel to join.
+//
+// The query heads that share a key-value head (up to 16 at a time) are the
+// columns of the matrix instructions, so that keys and values are read once.
+// A wavefront takes 32 tokens at a time (16 of a float32 cache) and keeps them
+// in registers from the load to the product, without LDS:
+//   scores^T = K Q^T: lane (r, g) = (lane & 15, lane >> 4) holds 16 bytes of
+//     token r at every 64-byte step of the head, the instruction's A operand;
+//     the result's lane holds tokens 4 g + i of head r.
+//   out^T = V^T P^T: those are the 8 (or 4) k-slots of lane group g in the
+//     B operand, so P goes from one product to the next as it lies.  The A
+//     operand wants one element of d of those tokens: a lane loads 16 bytes of
+//     each of its group's tokens (16 lanes: a row's whole 256 bytes) and picks
+//     the pairs apart with byte permutes.  The order of d over lanes and
+//     instructions is free, and is undone where out is written.
+#include "w4a8_mixers.h"
+
+namespace w4a8 {
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kWaves = 4;
+
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+// what exponents are taken against: the maximum, or 0 where no score is above
+// -infinity, so that every weight there is 0 and not a NaN
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
+
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Per cache type: a lane's 16 bytes as matrix operand.
+template <typename T>
+struct Half {
+  typedef T x8 __attribute__((ext_vector_type(8)));
+};
+
+struct Range {
+  int seq, n, t0, t1, used;   // the row's tokens, this split's, splits in use
+};
+
+// the row's length and this split's tokens of it: whole chunks, the same
+// count for every split but the last
+__device__ __forceinline__ Range range_of(const KvCache &kv, const Attend &a, int row, int split) {
+  Range r{a.seqs[row], 0, 0, 0, 0};
+  if (r.seq >= 0 && r.seq < kv.seqs) {
+    int n = kv.lens[r.seq];
+    const int64_t most = (int64_t)kv.max_pages << kv.lg_page;
+    if (n > most) n = (int)most;
+    if (a.upto) n = min(n, a.upto[row]);
+    r.n = max(n, 0);
+  }
+  const int each = max((r.n + a.splits - 1) / a.splits, 1);
+  const int per = (each + kAttendChunk - 1) / kAttendChunk * kAttendChunk;
+  r.used = (int)(((int64_t)r.n + per - 1) / per);
+  const int64_t t0 = (int64_t)split * per;
+  r.t0 = (int)(t0 < r.n ? t0 : r.n);
+  r.t1 = (int)(t0 + per < r.n ? t0 + per : r.n);
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_row(T *p, const float *x, int n) {
+#pragma unroll
+  for (int i = 0; i < n; ++i) p[i] = (T)x[i];
+}
+
+// out[d .. d + n) of a head: rounded once
+__device__ __forceinline__ void store_out(const Attend &a, int cache_dtype, int64_t at,
+                                          const float *x, int n) {
+  if (a.dtype == DT_I16) {
+    int16_t *p = (int16_t *)a.out + at;
+    for (int i = 0; i < n; ++i)
+      p[i] = (int16_t)fminf(fmaxf(rintf(x[i] * a.out_unit), -32768.f), 32767.f);
+  } else if (cache_dtype == DT_F32) {
+    store_row((float *)a.out + at, x, n);
+  } else if (cache_dtype == DT_BF16) {
+    store_row((__bf16 *)a.out + at, x, n);
+  } else {
+    store_row((_Float16 *)a.out + at, x, n);
+  }
+}
+
+// I16: q is int16 (its value of a step is part of a.scale), exact as the sum
+// of two 8-bit halves in the cache's type; P then goes as the sum of two
+// values too, so that a 16-bit result keeps its bits.  Otherwise P is rounded
+// to the cache's type for the second product, its sum is not: an error of
+// half a step of that type per token, which averages out over the tokens.
+template <int D, typename T, bool I16>
+__global__ __launch_bounds__(64 * kWaves) void attend_kernel(KvCache kv, Attend a) {
+  constexpr bool F32 = sizeof(T) == 4;
+  constexpr int kTok = F32 ? 16 : 32;              // tokens of a turn
+  constexpr int NT = kTok / 16;                    // 16-token tiles of them
+  constexpr int KS = F32 ? D / 16 : D / 32;        // 64-byte steps of a key
+  constexpr int VEC = F32 ? 4 : (D == 64 ? 4 : 8); // elements of a value load
+  constexpr int NC = D / (16 * VEC);               // loads of a value row
+  constexpr int ROWS = F32 ? 4 : 8;                // value rows of a lane group
+  constexpr int SPLIT = I16 && !F32 ? 2 : 1;       // operands q and P are the sum of
+  constexpr int LD = D + 4;                        // floats of a head's row in LDS
+  __shared__ float obuf[2][16 * LD];
+  __shared__ float mbuf[kWaves][16], lbuf[kWaves][16];
+
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = blockIdx.x / a.splits, split = blockIdx.x - row * a.splits;
+  const int group = a.hq / kv.heads, tiles = (group + 15) / 16;
+  const int kvh = blockIdx.y / tiles, h0 = (blockIdx.y - kvh * tiles) * 16;
+  const int heads = min(16, group - h0);           // of this tile
+  const Range R = range_of(kv, a, row, split);
+  if (R.seq >= kv.seqs && split == 0 && threadIdx.x == 0) atomicOr(kv.err, kErrKvRange);
+  const int hq = kvh * group + h0 + r;             // this lane's query head
+  if (R.used == 0 && split == 0) {                 // nothing to attend to: zeros
+    const float zero[4] = {0, 0, 0, 0};
+    for (int e = threadIdx.x * 4; e < heads * D; e += 64 * kWaves * 4)
+      store_out(a, kv.dtype,
+                row * a.out_row + (kvh * group + h0 + e / D) * a.out_head + e % D, zero, 4);
+  }
+  if (split >= R.used) return;
+
+  // q as B operand: head r, elements 8 g .. (4 g ..) of each step
+  typedef typename Half<T>::x8 x8;
+  x8 qh[SPLIT][F32 ? 1 : KS];
+  f32x4 qf[F32 ? KS : 1];
+  {
+    const int64_t at = row * a.q_row + hq * a.q_head;
+    const bool on = r < heads;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      if constexpr (F32) {
+        const int64_t e = at + s * 16 + g * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          qf[s][i] = !on ? 0.f : I16 ? (float)((const int16_t *)a.q)[e + i]
+                                     : ((const float *)a.q)[e + i];
+      } else {
+        const int64_t e = at + s * 32 + g * 8;
+        const u32x4 w = on ? *(const u32x4 *)((const T *)a.q + e) : u32x4{0, 0, 0, 0};
+        if constexpr (I16) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int x = (int16_t)(w[i >> 1] >> (16 * (i & 1)));
+            const int lo = (int)(int8_t)x;
+            qh[0][s][i] = (T)(float)(x - lo);
+            qh[1][s][i] = (T)(float)lo;
+          }
+        } else {
+          qh[0][s] = __builtin_bit_cast(x8, w);
+        }
+      }
+    }
+  }
+
+  const int page = kv.page(), lg = kv.lg_page;
+  const int32_t *table = kv.tables + (int64_t)R.seq * kv.max_pages;
+  const int64_t plane = (int64_t)page * D;          // elements of a head's page
+  const T *pool = (const T *)kv.pool;
+  const int64_t page_elems = kv.page_bytes / (int)sizeof(T);
+  const int64_t kbase = (((int64_t)a.layer * 2) * kv.heads + kvh) * plane;
+  const int64_t vbase = kbase + kv.heads * plane;
+
+  f32x4 acc[NC * VEC];
+#pragma unroll
+  for (int i = 0; i < NC * VEC; ++i) acc[i] = f32x4{0, 0, 0, 0};
+  float m = -INFINITY, l = 0.f;
+  int bad = 0;
+
+  for (int t = R.t0 + wave * kTok; t < R.t1; t += kWaves * kTok) {
+    // the pages of the turn's 16-token tiles; a tile past the end, or whose
+    // page is none of the pool's, reads page 0 and is masked
+    const T *kp[NT], *vp[NT];
+    int lim[NT];                                    // tokens below it count
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int tt = t + 16 * j;
+      int p = tt < R.t1 ? table[tt >> lg] : 0;
+      lim[j] = R.t1;
+      if ((uint32_t)p >= (uint32_t)kv.pages) {
+        bad = 1;
+        p = 0;
+        lim[j] = 0;
+      }
+      const T *base = pool + p * page_elems + (int64_t)(tt & (page - 1)) * D;
+      kp[j] = base + kbase;
+      vp[j] = base + vbase;
+    }
+    u32x4 kr[NT][KS];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        constexpr int step = F32 ? 16 : 32, per = F32 ? 4 : 8;
+        kr[j][s] = load16_nt(kp[j] + r * D + s * step + g * per);
+      }
+    u32x4 vr[ROWS][NC];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const T *src = vp[i >> 2] + (4 * g + (i & 3)) * D + c * 16 * VEC + r * VEC;
+        if constexpr (VEC * sizeof(T) == 16) {
+          vr[i][c] = load16_nt(src);
+        } else {
+          const u32x2 x = __builtin_nontemporal_load((const u32x2 *)src);
+          vr[i][c] = u32x4{x.x, x.y, 0, 0};
+        }
+      }
+    // scores of tokens t + 16 j + 4 g + i for head r
+    f32x4 sc[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      sc[j] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        if constexpr (F32) {
+          const f32x4 k4 = __builtin_bit_cast(f32x4, kr[j][s]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            sc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(k4[i], qf[s][i], sc[j], 0, 0, 0);
+        } else {
+          const x8 k8 = __builtin_bit_cast(x8, kr[j][s]);
+#pragma unroll
+          for (int q = 0; q < SPLIT; ++q) sc[j] = mfma(k8, qh[q][s], sc[j]);
+        }
+      }
+    }
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool live = t + 16 * j + 4 * g + i < lim[j];
+        sc[j][i] = live ? sc[j][i] * a.scale : -INFINITY;
+        top = fmaxf(top, sc[j][i]);
+      }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float base = base_of(top), fall = exp2_of(m - base);
+    m = top;
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sc[j][i] = exp2_of(sc[j][i] - base);
+        sum += sc[j][i];
+      }
+    l = l * fall + sum;
+    if (__any(fall != 1.f)) {
+#pragma unroll
+      for (int i = 0; i < NC * VEC; ++i) acc[i] *= fall;
+    }
+    // what lies in a masked value row may be anything: not a factor of 0
+    if (t + kTok > R.t1 || lim[0] == 0 || lim[NT - 1] == 0) {
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i)
+        if (t + 16 * (i >> 2) + 4 * g + (i & 3) >= lim[i >> 2])
+#pragma unroll
+          for (int c = 0; c < NC; ++c) vr[i][c] = u32x4{0, 0, 0, 0};
+    }
+    if constexpr (F32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const f32x4 v4 = __builtin_bit_cast(f32x4, vr[i][c]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            acc[c * VEC + e] =
+                __builtin_amdgcn_mfma_f32_16x16x4f32(v4[e], sc[0][i], acc[c * VEC + e], 0, 0, 0);
+        }
+    } else {
+      x8 p[SPLIT];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = sc[i >> 2][i & 3];
+        p[0][i] = (T)x;
+        if constexpr (SPLIT == 2) p[1][i] = (T)(x - (float)p[0][i]);
+      }
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          u32x4 w;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            w[i] = __builtin_amdgcn_perm(vr[2 * i + 1][c][e >> 1], vr[2 * i][c][e >> 1],
+                                         e & 1 ? 0x07060302u : 0x05040100u);
+          const x8 v8 = __builtin_bit_cast(x8, w);
+#pragma unroll
+          for (int q = 0; q < SPLIT; ++q) acc[c * VEC + e] = mfma(v8, p[q], acc[c * VEC + e]);
+        }
+    }
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (bad && lane == 0) atomicOr(kv.err, kErrKvRange);
+
+  // the wavefronts' parts on one maximum, then added: 2, 3 to 0, 1, then 1 to 0
+  if (g == 0) {
+    mbuf[wave][r] = m;
+    lbuf[wave][r] = l;
+  }
+  __syncthreads();
+  float M = mbuf[0][r], L = 0.f;
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) M = fmaxf(M, mbuf[w][r]);
+  M = base_of(M);
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) L += lbuf[w][r] * exp2_of(mbuf[w][r] - M);
+  const float mine = exp2_of(m - M);
+#pragma unroll
+  for (int i = 0; i < NC * VEC; ++i) acc[i] *= mine;
+  // element e of load c and result i is d = (16 c + 4 g + i) VEC + e
+  auto put = [&](float *o) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; e += 4)
+          *(f32x4 *)(o + r * LD + (16 * c + 4 * g + i) * VEC + e) =
+              f32x4{acc[c * VEC + e][i], acc[c * VEC + e + 1][i], acc[c * VEC + e + 2][i],
+                    acc[c * VEC + e + 3][i]};
+  };
+  auto add = [&](const float *o) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; e += 4) {
+          const f32x4 x = *(const f32x4 *)(o + r * LD + (16 * c + 4 * g + i) * VEC + e);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) acc[c * VEC + e + k][i] += x[k];
+        }
+  };
+  if (wave >= 2) put(obuf[wave - 2]);
+  __syncthreads();
+  if (wave < 2) add(obuf[wave]);
+  __syncthreads();
+  if (wave == 1) put(obuf[0]);
+  __syncthreads();
+  if (wave != 0) return;
+  add(obuf[0]);
+  if (r >= heads) return;
+  if (R.used == 1) {
+    const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[e] = acc[c * VEC + e][i] * inv;
+        store_out(a, kv.dtype, row * a.out_row + hq * a.out_head + (16 * c + 4 * g + i) * VEC, x,
+                  VEC);
+      }
+    return;
+  }
+  const int64_t slot = ((int64_t)row * a.hq + hq) * a.splits + split;
+  float *part = a.part + slot * D;
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < VEC; e += 4)
+        *(f32x4 *)(part + (16 * c + 4 * g + i) * VEC + e) =
+            f32x4{acc[c * VEC + e][i], acc[c * VEC + e + 1][i], acc[c * VEC + e + 2][i],
+                  acc[c * VEC + e + 3][i]};
+  if (g == 0) {
+    float *ml = a.part + (int64_t)a.rows * a.hq * a.splits * D + slot * 2;
+    ml[0] = M;
+    ml[1] = L;
+  }
+}
+
+// The splits of a row and head joined: out = sum_s 2^(m_s - M) o_s / sum_s
+// 2^(m_s - M) l_s.  A workgroup per row and head, D / 4 threads per split.
+template <int D>
+__global__ __launch_bounds__(256) void attend_join_kernel(KvCache kv, Attend a) {
+  constexpr int LANES = D / 4, GROUPS = 256 / LANES;
+  __shared__ f32x4 obuf[GROUPS][LANES];
+  __shared__ float red[2][4];
+  const int row = blockIdx.x, h = blockIdx.y;
+  const Range R = range_of(kv, a, row, 0);
+  if (R.used <= 1) return;
+  const int64_t slot = ((int64_t)row * a.hq + h) * a.splits;
+  const float *ml = a.part + (int64_t)a.rows * a.hq * a.splits * D + slot * 2;
+  float M = -INFINITY;
+  for (int s = threadIdx.x; s < R.used; s += 256) M = fmaxf(M, ml[2 * s]);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) M = fmaxf(M, __shfl_xor(M, d));
+  if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6] = M;
+  __syncthreads();
+  M = base_of(fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3])));
+  float L = 0.f;
+  for (int s = threadIdx.x; s < R.used; s += 256) L += ml[2 * s + 1] * exp2_of(ml[2 * s] - M);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) L += __shfl_xor(L, d);
+  if ((threadIdx.x & 63) == 0) red[1][threadIdx.x >> 6] = L;
+  const int lane = threadIdx.x % LANES, grp = threadIdx.x / LANES;
+  const float *part = a.part + slot * D + lane * 4;
+  f32x4 o{0, 0, 0, 0};
+#pragma unroll 4
+  for (int s = grp; s < R.used; s += GROUPS)
+    o += *(const f32x4 *)(part + (int64_t)s * D) * exp2_of(ml[2 * s] - M);
+  obuf[grp][lane] = o;
+  __syncthreads();
+  if (grp != 0) return;
+  L = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+#pragma unroll
+  for (int k = 1; k < GROUPS; ++k) o += obuf[k][lane];
+  const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
+  const float x[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+  store_out(a, kv.dtype, row * a.out_row + h * a.out_head + lane * 4, x, 4);
+}
+
+template <int D, typename T>
+void launch_typed(const KvCache &kv, const Attend &a, dim3 grid, hipStream_t s) {
+  if (a.dtype == DT_I16) attend_kernel<D, T, true><<<grid, 64 * kWaves, 0, s>>>(kv, a);
+  else attend_kernel<D, T, false><<<grid, 64 * kWaves, 0, s>>>(kv, a);
+}
+
+template <int D>
+void launch_dim(const KvCache &kv, const Attend &a, dim3 grid, hipStream_t s) {
+  if (kv.dtype == DT_F32) launch_typed<D, float>(kv, a, grid, s);
+  else if (kv.dtype == DT_BF16) launch_typed<D, __bf16>(kv, a, grid, s);
+  else launch_typed<D, _Float16>(kv, a, grid, s);
+  if (a.splits > 1) attend_join_kernel<D><<<dim3(a.rows, a.hq), 256, 0, s>>>(kv, a);
+}
+
+}  // namespace
+
+// Splits of a row: enough workgroups to fill the chip four times over at the
+// cache's longest sequence, but none of less than a chunk.
+int attend_splits(const KvCache &kv, int64_t rows, int64_t hq, int num_cu) {
+  const int64_t group = hq / kv.heads, base = rows * kv.heads * ((group + 15) / 16);
+  const int64_t most = (((int64_t)kv.max_pages << kv.lg_page) + kAttendChunk - 1) / kAttendChunk;
+  const int64_t want = (4ll * num_cu + base - 1) / base;
+  return (int)(want < 1 ? 1 : want < most ? want : most);
+}
+
+int64_t attend_workspace(const KvCache &kv, int64_t rows, int64_t hq, int num_cu) {
+  const int64_t splits = attend_splits(kv, rows, hq, num_cu);
+  return splits > 1 ? rows * hq * splits * (kv.dim + 2) * 4 : 0;
+}
+
+hipError_t launch_attend(const KvCache &kv, const Attend &a, hipStream_t s) {
+  const int group = a.hq / kv.heads, tiles = (group + 15) / 16;
+  const dim3 grid((uint32_t)a.rows * a.splits, kv.heads * tiles);
+  if (kv.dim == 64) launch_dim<64>(kv, a, grid, s);
+  else if (kv.dim == 128) launch_dim<128>(kv, a, grid, s);
+  else launch_dim<256>(kv, a, grid, s);
+  return hipGetLastError();
+}
+
+}  // namespace w4a8

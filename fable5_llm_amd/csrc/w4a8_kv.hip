@@ -1,0 +1,505 @@
+// The pages of a key-value cache on the device: reserving, forking, freeing
+// and compacting them, and writing new tokens' keys and values into them.
+// Every decision (which page is free, what moves where) is taken from the
+// device's own counts and tables, so that a step with them can be captured
+// and replayed, and is the same from run to run: free pages are handed out
+// lowest first, in the order of the list.
+#include "w4a8_mixers.h"
+
+namespace w4a8 {
+
+namespace {
+
+constexpr int kOne = 1024;        // threads of the single-workgroup kernels
+constexpr int kRefsPerThread = 16;
+constexpr int kPiece = 16 << 10;  // bytes a workgroup copies at a time
+
+__device__ __forceinline__ int32_t *marks(const KvCache &kv) { return kv.scratch + kKvHead; }
+__device__ __forceinline__ int32_t *jobs(const KvCache &kv) { return marks(kv) + kv.seqs; }
+__device__ __forceinline__ int32_t *list_a(const KvCache &kv) { return jobs(kv) + kv.seqs; }
+__device__ __forceinline__ int32_t *list_b(const KvCache &kv) { return list_a(kv) + kv.pages; }
+
+__device__ __forceinline__ int32_t held_pages(const KvCache &kv, int32_t len) {
+  return (int32_t)(((int64_t)len + kv.page() - 1) >> kv.lg_page);
+}
+
+// exclusive scan of one value per thread of a kOne-thread workgroup, and the
+// total; every thread of it calls
+__device__ int scan_excl(int v, int *total) {
+  __shared__ int sums[kOne / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int x = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  __syncthreads();              // the last call's sums are read
+  if (lane == 63) sums[wave] = x;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kOne / 64; ++w) {
+    const int s = sums[w];
+    before += w < wave ? s : 0;
+    all += s;
+  }
+  *total = all;
+  return before + x - v;
+}
+
+// refs[p0 .. p0 + 16), pages past the end as 1 (in use) or 0
+__device__ __forceinline__ void load_refs(const KvCache &kv, int p0, int past, int *r) {
+  if (p0 + kRefsPerThread <= kv.pages) {
+#pragma unroll
+    for (int i = 0; i < kRefsPerThread / 4; ++i) {
+      const int4 v = *(const int4 *)(kv.refs + p0 + 4 * i);
+      r[4 * i] = v.x, r[4 * i + 1] = v.y, r[4 * i + 2] = v.z, r[4 * i + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kRefsPerThread; ++i) r[i] = p0 + i < kv.pages ? kv.refs[p0 + i] : past;
+  }
+}
+
+// the need lowest free pages, in order, to list; how many there were (fewer
+// than need: not enough).  One workgroup.
+__device__ int find_free(const KvCache &kv, int need, int32_t *list) {
+  int found = 0;
+  for (int base = 0; base < kv.pages && found < need; base += kOne * kRefsPerThread) {
+    int r[kRefsPerThread], mine = 0, all;
+    const int p0 = base + (int)threadIdx.x * kRefsPerThread;
+    load_refs(kv, p0, 1, r);
+#pragma unroll
+    for (int i = 0; i < kRefsPerThread; ++i) mine += r[i] == 0;
+    int at = found + scan_excl(mine, &all);
+#pragma unroll
+    for (int i = 0; i < kRefsPerThread; ++i)
+      if (r[i] == 0) {
+        if (at < need) list[at] = p0 + i;
+        ++at;
+      }
+    found += all;
+  }
+  __syncthreads();              // list is written (for this workgroup's reads)
+  return found;
+}
+
+// ------------------------------------------------------------------ reserve
+// One workgroup.  First pass: what is wrong with the list; second: the pages
+// each sequence needs, their ranks by a scan in list order; nothing is written
+// to the cache unless everything fits.
+__global__ __launch_bounds__(kOne) void kv_extend_kernel(KvCache kv, const int32_t *seqs,
+                                                         const int32_t *counts, int n) {
+  __shared__ int bad;
+  int32_t *mark = marks(kv), *list = list_a(kv);
+  if (threadIdx.x == 0) bad = 0;
+  __syncthreads();
+  int need = 0;
+  const int64_t most = (int64_t)kv.max_pages << kv.lg_page;
+  for (int i = threadIdx.x; i < n; i += kOne) {
+    const int s = seqs[i];
+    if (s < 0) continue;
+    if (s >= kv.seqs) {
+      atomicOr(&bad, kErrKvRange);
+      continue;
+    }
+    if (atomicAdd(mark + s, 1) != 0) atomicOr(&bad, kErrKvList);
+    const int64_t len = kv.lens[s], c = counts[i];
+    if (len < 0 || c < 0 || len + c > most || len + c > INT32_MAX)
+      atomicOr(&bad, kErrKvRange);
+    else
+      need += held_pages(kv, (int32_t)(len + c)) - held_pages(kv, (int32_t)len);
+  }
+  int all;
+  scan_excl(need, &all);        // synchronises: bad is whole
+  if (!bad && all > 0 && find_free(kv, all, list) < all) {
+    if (threadIdx.x == 0) bad = kErrKvFull;
+  }
+  __syncthreads();
+  if (!bad) {
+    int from = 0;
+    for (int base = 0; base < n; base += kOne) {
+      const int i = base + threadIdx.x;
+      const int s = i < n ? seqs[i] : -1;
+      int h0 = 0, h1 = 0, len = 0, sum;
+      if (s >= 0) {
+        len = kv.lens[s];
+        h0 = held_pages(kv, len);
+        h1 = held_pages(kv, len + counts[i]);
+      }
+      const int at = from + scan_excl(h1 - h0, &sum);
+      from += sum;
+      // a thread writes its own sequence's few pages; a long run of them (a
+      // prompt's) is written by its whole wavefront
+      const int add = h1 - h0;
+      if (s >= 0) {
+        if (add <= 8)
+          for (int j = 0; j < add; ++j) {
+            const int p = list[at + j];
+            kv.tables[(int64_t)s * kv.max_pages + h0 + j] = p;
+            kv.refs[p] = 1;
+          }
+        kv.lens[s] = len + counts[i];
+      }
+      uint64_t lots = __ballot(s >= 0 && add > 8);
+      while (lots) {
+        const int src = __builtin_ctzll(lots);
+        lots &= lots - 1;
+        const int ws = __shfl(s, src), wh = __shfl(h0, src), wa = __shfl(add, src),
+                  wat = __shfl(at, src);
+        for (int j = threadIdx.x & 63; j < wa; j += 64) {
+          const int p = list[wat + j];
+          kv.tables[(int64_t)ws * kv.max_pages + wh + j] = p;
+          kv.refs[p] = 1;
+        }
+      }
+    }
+  } else if (threadIdx.x == 0) {
+    atomicOr(kv.err, bad);
+  }
+  for (int i = threadIdx.x; i < n; i += kOne) {
+    const int s = seqs[i];
+    if (s >= 0 && s < kv.seqs) atomicExch(mark + s, 0);
+  }
+}
+
+// --------------------------------------------------------------------- fork
+// First kernel, one workgroup: the list's faults, a free page for each child
+// of a parent whose last page is not full (jobs[child], -1 where none), the
+// children's lengths.  scratch[0]: whether the second kernel runs.
+__global__ __launch_bounds__(kOne) void kv_fork_kernel(KvCache kv, const int32_t *parents,
+                                                       const int32_t *children, int n) {
+  __shared__ int bad;
+  int32_t *mark = marks(kv), *job = jobs(kv), *list = list_a(kv);
+  if (threadIdx.x == 0) bad = 0;
+  __syncthreads();
+  int need = 0;
+  for (int i = threadIdx.x; i < n; i += kOne) {
+    const int p = parents[i], c = children[i];
+    if (p < 0 || c < 0) continue;
+    if (p >= kv.seqs || c >= kv.seqs) {
+      atomicOr(&bad, kErrKvRange);
+      if (c < kv.seqs) atomicAdd(mark + c, 1);
+      continue;
+    }
+    if (atomicAdd(mark + c, 1) != 0 || kv.lens[c] != 0) atomicOr(&bad, kErrKvList);
+    const int64_t len = kv.lens[p];
+    if (len < 0 || len > ((int64_t)kv.max_pages << kv.lg_page))
+      atomicOr(&bad, kErrKvRange);
+    else
+      need += (len & (kv.page() - 1)) != 0;
+  }
+  int all;
+  scan_excl(need, &all);
+  for (int i = threadIdx.x; i < n; i += kOne) {   // a child that is a parent too
+    const int p = parents[i], c = children[i];
+    if (p >= 0 && c >= 0 && p < kv.seqs && atomicAdd(mark + p, 0) != 0)
+      atomicOr(&bad, kErrKvList);
+  }
+  __syncthreads();
+  const bool fine = bad == 0;
+  if (fine && all > 0 && find_free(kv, all, list) < all) {
+    if (threadIdx.x == 0) bad = kErrKvFull;
+  }
+  __syncthreads();
+  if (!bad) {
+    int from = 0;
+    for (int base = 0; base < n; base += kOne) {
+      const int i = base + threadIdx.x;
+      const int p = i < n ? parents[i] : -1, c = i < n ? children[i] : -1;
+      const bool on = p >= 0 && c >= 0;
+      const int len = on ? kv.lens[p] : 0;
+      const int rest = (len & (kv.page() - 1)) != 0;
+      int sum;
+      const int at = from + scan_excl(rest, &sum);
+      from += sum;
+      if (on) {
+        int page = -1;
+        if (rest) {
+          page = list[at];
+          kv.refs[page] = 1;
+        }
+        job[c] = page;
+        kv.lens[c] = len;
+      }
+    }
+  } else if (threadIdx.x == 0) {
+    atomicOr(kv.err, bad);
+  }
+  if (threadIdx.x == 0) kv.scratch[0] = bad == 0;
+  for (int i = threadIdx.x; i < n; i += kOne) {
+    const int p = parents[i], c = children[i];
+    if (p >= 0 && c >= 0 && c < kv.seqs) atomicExch(mark + c, 0);
+  }
+}
+
+// Second kernel, a row of workgroups per pair: the shared pages' entries and
+// counts, and the used tokens of the last page, one run of memory per layer,
+// keys or values, and head.
+__global__ __launch_bounds__(256) void kv_fork_rows_kernel(KvCache kv, const int32_t *parents,
+                                                           const int32_t *children) {
+  if (kv.scratch[0] == 0) return;
+  const int p = parents[blockIdx.x], c = children[blockIdx.x];
+  if (p < 0 || c < 0) return;
+  const int len = kv.lens[p], full = len >> kv.lg_page, rest = len & (kv.page() - 1);
+  const int32_t *from = kv.tables + (int64_t)p * kv.max_pages;
+  int32_t *to = kv.tables + (int64_t)c * kv.max_pages;
+  for (int j = blockIdx.y * 256 + threadIdx.x; j < full; j += gridDim.y * 256) {
+    const int page = from[j];
+    to[j] = page;
+    if ((uint32_t)page < (uint32_t)kv.pages)
+      atomicAdd(kv.refs + page, 1);
+    else
+      atomicOr(kv.err, kErrKvRange);
+  }
+  if (!rest) return;
+  const int dst = jobs(kv)[c], src = from[full];
+  if (blockIdx.y == 0 && threadIdx.x == 0) to[full] = dst;
+  if ((uint32_t)src >= (uint32_t)kv.pages) {
+    if (threadIdx.x == 0) atomicOr(kv.err, kErrKvRange);
+    return;
+  }
+  const int runs = kv.layers * 2 * kv.heads;
+  const int64_t run = (int64_t)kv.page() * kv.dim * kv.esize;
+  const int used = rest * kv.dim * kv.esize;   // a multiple of 128
+  const uint8_t *a = kv.pool + src * kv.page_bytes;
+  uint8_t *b = kv.pool + dst * kv.page_bytes;
+  for (int r = blockIdx.y; r < runs; r += gridDim.y)
+    for (int o = threadIdx.x * 16; o < used; o += 256 * 16)
+      store16_nt(b + r * run + o, load16_nt(a + r * run + o));
+}
+
+// --------------------------------------------------------------------- free
+// A workgroup per listed sequence; a sequence listed again, or already empty,
+// is left alone.
+__global__ __launch_bounds__(256) void kv_free_kernel(KvCache kv, const int32_t *seqs) {
+  const int i = blockIdx.x, s = seqs[i];
+  if (s < 0) return;
+  if (s >= kv.seqs) {
+    if (threadIdx.x == 0) atomicOr(kv.err, kErrKvRange);
+    return;
+  }
+  int again = 0;
+  for (int j = threadIdx.x; j < i; j += 256) again |= seqs[j] == s;
+  if (__syncthreads_or(again)) return;
+  const int len = kv.lens[s];
+  const int held = min(held_pages(kv, max(len, 0)), kv.max_pages);
+  const int32_t *row = kv.tables + (int64_t)s * kv.max_pages;
+  for (int j = threadIdx.x; j < held; j += 256) {
+    const int page = row[j];
+    if ((uint32_t)page >= (uint32_t)kv.pages) {
+      atomicOr(kv.err, kErrKvRange);
+    } else if (atomicAdd(kv.refs + page, -1) <= 0) {
+      atomicAdd(kv.refs + page, 1);
+      atomicOr(kv.err, kErrKvRange);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) kv.lens[s] = 0;
+}
+
+// ------------------------------------------------------------------ compact
+// First kernel, one workgroup: U pages are in use; the k-th page in use at U
+// or above moves to the k-th free page below U (there are as many of either).
+// list_a: where it is, list_b[page]: where it goes; the counts move with it.
+// scratch[0] = moves, scratch[1] = U.
+__global__ __launch_bounds__(kOne) void kv_compact_kernel(KvCache kv) {
+  int32_t *holes = list_a(kv), *to = list_b(kv);
+  int used = 0, U;
+  for (int p0 = (int)threadIdx.x * kRefsPerThread; p0 < kv.pages; p0 += kOne * kRefsPerThread) {
+    int r[kRefsPerThread];
+    load_refs(kv, p0, 0, r);
+#pragma unroll
+    for (int i = 0; i < kRefsPerThread; ++i) used += r[i] != 0;
+  }
+  scan_excl(used, &U);
+  const int moves = find_free(kv, U, holes);   // free pages, lowest first, up to U of them
+  // those below U are the holes: as many as pages in use at U or above
+  int from = 0;
+  const int first = U / kRefsPerThread * kRefsPerThread;
+  for (int base = first; base < kv.pages; base += kOne * kRefsPerThread) {
+    const int p0 = base + (int)threadIdx.x * kRefsPerThread;
+    int r[kRefsPerThread], mine = 0, all;
+    load_refs(kv, p0, 0, r);
+#pragma unroll
+    for (int i = 0; i < kRefsPerThread; ++i) mine += r[i] != 0 && p0 + i >= U;
+    int at = from + scan_excl(mine, &all);
+    from += all;
+#pragma unroll
+    for (int i = 0; i < kRefsPerThread; ++i)
+      if (r[i] != 0 && p0 + i >= U) {
+        const int hole = at < min(moves, U) ? holes[at] : -1;
+        if (hole >= 0) {
+          to[p0 + i] = hole;
+          to[hole] = p0 + i;      // below U: the page that comes here
+          kv.refs[hole] = r[i];
+          kv.refs[p0 + i] = 0;
+        }
+        ++at;
+      }
+  }
+  if (threadIdx.x == 0) {
+    kv.scratch[0] = from;
+    kv.scratch[1] = U;
+  }
+}
+
+__device__ __forceinline__ void copy_piece(uint8_t *b, const uint8_t *a, int64_t o, int64_t end) {
+  u32x4 v[kPiece / (256 * 16)];
+#pragma unroll
+  for (int u = 0; u < kPiece / (256 * 16); ++u) {
+    const int64_t at = o + (u * 256 + (int)threadIdx.x) * 16;
+    if (at < end) v[u] = load16_nt(a + at);
+  }
+#pragma unroll
+  for (int u = 0; u < kPiece / (256 * 16); ++u) {
+    const int64_t at = o + (u * 256 + (int)threadIdx.x) * 16;
+    if (at < end) store16_nt(b + at, v[u]);
+  }
+}
+
+// Second kernel: the tables follow, and the pages are copied, a piece per
+// workgroup at a time.  Sources lie at U or above and destinations below, so
+// no copy reads what another writes.
+__global__ __launch_bounds__(256) void kv_move_kernel(KvCache kv) {
+  const int moves = kv.scratch[0], U = kv.scratch[1];
+  const int32_t *holes = list_a(kv), *to = list_b(kv);
+  for (int s = blockIdx.x; s < kv.seqs; s += gridDim.x) {
+    const int held = min(held_pages(kv, max(kv.lens[s], 0)), kv.max_pages);
+    int32_t *row = kv.tables + (int64_t)s * kv.max_pages;
+    for (int j = threadIdx.x; j < held; j += 256) {
+      const int p = row[j];
+      if ((uint32_t)p >= (uint32_t)kv.pages)
+        atomicOr(kv.err, kErrKvRange);
+      else if (p >= U)
+        row[j] = to[p];
+    }
+  }
+  const int64_t pieces = (kv.page_bytes + kPiece - 1) / kPiece;
+  for (int64_t w = blockIdx.x; w < moves * pieces; w += gridDim.x) {
+    const int m = (int)(w / pieces);
+    const int dst = holes[m], src = to[dst];
+    copy_piece(kv.pool + dst * kv.page_bytes, kv.pool + src * kv.page_bytes,
+               (w - m * pieces) * kPiece, kv.page_bytes);
+  }
+}
+
+__global__ __launch_bounds__(256) void kv_copy_kernel(KvCache kv, const int32_t *src,
+                                                      const int32_t *dst, int n) {
+  const int64_t pieces = (kv.page_bytes + kPiece - 1) / kPiece;
+  for (int64_t w = blockIdx.x; w < n * pieces; w += gridDim.x) {
+    const int m = (int)(w / pieces);
+    const int a = src[m], b = dst[m];
+    if (a < 0 || b < 0 || a == b) continue;
+    if (a >= kv.pages || b >= kv.pages) {
+      if (threadIdx.x == 0) atomicOr(kv.err, kErrKvRange);
+      continue;
+    }
+    copy_piece(kv.pool + b * kv.page_bytes, kv.pool + a * kv.page_bytes,
+               (w - m * pieces) * kPiece, kv.page_bytes);
+  }
+}
+
+// ------------------------------------------------------------------- append
+template <typename T>
+__device__ __forceinline__ T from_float(float x) {
+  return (T)x;
+}
+
+// 16 bytes of the cache per thread and turn; rows are tokens
+template <typename T, bool I16>
+__global__ __launch_bounds__(256) void kv_append_kernel(KvCache kv, KvAppend a) {
+  constexpr int V = 16 / sizeof(T);
+  const int per = kv.heads * kv.dim / V;      // vectors of a token's keys
+  const int64_t all = (int64_t)a.n * per * 2;
+  for (int64_t w = blockIdx.x * 256ll + threadIdx.x; w < all; w += gridDim.x * 256ll) {
+    const int i = (int)(w / (2 * per));
+    const int x = (int)(w - (int64_t)i * 2 * per);
+    const int which = x >= per;
+    const int e = (x - which * per) * V, h = e / kv.dim, d = e - h * kv.dim;
+    const int s = a.seqs[i];
+    if (s < 0) continue;
+    bool ok = s < kv.seqs;
+    int page = -1, pos = 0;
+    if (ok) {
+      const int len = kv.lens[s];
+      pos = a.pos ? a.pos[i] : len - 1;
+      ok = pos >= 0 && pos < len && (pos >> kv.lg_page) < kv.max_pages;
+      if (ok) page = kv.tables[(int64_t)s * kv.max_pages + (pos >> kv.lg_page)];
+      ok = ok && (uint32_t)page < (uint32_t)kv.pages;
+    }
+    if (!ok) {
+      if (x == 0) atomicOr(kv.err, kErrKvRange);
+      continue;
+    }
+    const int64_t at = i * (which ? a.v_token : a.k_token) + h * (which ? a.v_head : a.k_head) + d;
+    const void *src = which ? a.v : a.k;
+    uint8_t *dst = kv.pool + page * kv.page_bytes +
+                   ((((int64_t)a.layer * 2 + which) * kv.heads + h) * kv.page() +
+                    (pos & (kv.page() - 1))) * kv.dim * (int)sizeof(T) + d * (int)sizeof(T);
+    if constexpr (I16) {
+      T v[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = from_float<T>(((const int16_t *)src)[at + j] * a.unit);
+      *(u32x4 *)dst = *(const u32x4 *)v;
+    } else {
+      *(u32x4 *)dst = load16_nt((const T *)src + at);
+    }
+  }
+}
+
+}  // namespace
+
+hipError_t launch_kv_extend(const KvCache &kv, const int32_t *seqs, const int32_t *counts,
+                            int32_t n, hipStream_t s) {
+  kv_extend_kernel<<<1, kOne, 0, s>>>(kv, seqs, counts, n);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv_fork(const KvCache &kv, const int32_t *parents, const int32_t *children,
+                          int32_t n, hipStream_t s) {
+  kv_fork_kernel<<<1, kOne, 0, s>>>(kv, parents, children, n);
+  const int runs = kv.layers * 2 * kv.heads;
+  kv_fork_rows_kernel<<<dim3(n, runs < 64 ? runs : 64), 256, 0, s>>>(kv, parents, children);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv_free(const KvCache &kv, const int32_t *seqs, int32_t n, hipStream_t s) {
+  kv_free_kernel<<<n, 256, 0, s>>>(kv, seqs);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv_compact(const KvCache &kv, int num_cu, hipStream_t s) {
+  kv_compact_kernel<<<1, kOne, 0, s>>>(kv);
+  kv_move_kernel<<<num_cu * 8, 256, 0, s>>>(kv);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv_copy(const KvCache &kv, const int32_t *src, const int32_t *dst, int32_t n,
+                          int num_cu, hipStream_t s) {
+  const int64_t work = n * ((kv.page_bytes + kPiece - 1) / kPiece);
+  const int grid = (int)(work < num_cu * 8 ? work : num_cu * 8);
+  kv_copy_kernel<<<grid, 256, 0, s>>>(kv, src, dst, n);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv_append(const KvCache &kv, const KvAppend &a, hipStream_t s) {
+  const int64_t vecs = (int64_t)a.n * 2 * kv.heads * kv.dim * kv.esize / 16;
+  const int64_t want = (vecs + 255) / 256;
+  const int grid = (int)(want < 16384 ? want : 16384);
+  const bool i16 = a.dtype == DT_I16;
+  if (kv.dtype == DT_F32) {
+    if (i16) kv_append_kernel<float, true><<<grid, 256, 0, s>>>(kv, a);
+    else kv_append_kernel<float, false><<<grid, 256, 0, s>>>(kv, a);
+  } else if (kv.dtype == DT_BF16) {
+    if (i16) kv_append_kernel<__bf16, true><<<grid, 256, 0, s>>>(kv, a);
+    else kv_append_kernel<__bf16, false><<<grid, 256, 0, s>>>(kv, a);
+  } else {
+    if (i16) kv_append_kernel<_Float16, true><<<grid, 256, 0, s>>>(kv, a);
+    else kv_append_kernel<_Float16, false><<<grid, 256, 0, s>>>(kv, a);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace w4a8

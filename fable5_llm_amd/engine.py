@@ -11,6 +11,8 @@ from array import array
 import numpy as np
 
 from . import _native as N
+from . import mixers
+from .mixers import PagedKV  # noqa: F401
 
 _c = ctypes.c_void_p
 
@@ -410,6 +412,35 @@ class Context:
         N.check(N.lib().w4a8_mlp_async(
             self.h, gate.h, up.h, down.h, pg, pu, pd, _dptr(x16), _dptr(norm_w),
             int(in_f), 1 if one_plus else 0, _dptr(mlp_out), _dptr(res_out)), "mlp")
+
+    # ------------------------------------------- gated delta rule (async)
+    def delta_step_async(self, q, k, v, g, beta, state, out, slots=None, scale=None, norm=True,
+                         eps=1e-6, frac=0, out_frac=0):
+        """One token of each row through the gated delta rule, on device
+        tensors (w4a8_delta_step_async): q, k [rows, hk, dk], v and out [rows,
+        hv, dv] of one type, g (log decay) and beta float32 [rows, hv], state
+        float32 [slots, hv, dk, dv], updated in place.  slots[row]: the row's
+        state, negative for a padded row (its out is zeros); row i's is i
+        without.  norm: q and k are normalised.  scale: 1 / sqrt(dk) unless
+        given.  frac, out_frac: fraction bits of int16 q, k, v and out."""
+        N.check(N.lib().w4a8_delta_step_async(self.h, mixers.delta_args(
+            self, q, k, v, g, beta, state, out, None, None, slots, scale, norm, eps, False, frac,
+            out_frac)), "delta_step")
+
+    def delta_chunk_workspace(self, tokens, rows, hv):
+        """Device memory for delta_chunk_async with this many tokens, rows and
+        value heads; calls that can overlap need one each."""
+        return mixers.delta_workspace(self, tokens, rows, hv)
+
+    def delta_chunk_async(self, q, k, v, g, beta, state, out, cu, ws, slots=None, fresh=False,
+                          scale=None, norm=True, eps=1e-6, frac=0, out_frac=0):
+        """Whole prompts through the gated delta rule: the arguments of
+        delta_step_async with tokens of several rows side by side, row i's
+        from cu[i] to cu[i + 1] (int32 [rows + 1], on the device).  fresh: the
+        states start from zeros and are not read."""
+        N.check(N.lib().w4a8_delta_chunk_async(self.h, mixers.delta_args(
+            self, q, k, v, g, beta, state, out, cu, ws, slots, scale, norm, eps, fresh, frac,
+            out_frac)), "delta_chunk")
 
 
 _DEFAULT = None

@@ -398,6 +398,132 @@ int w4a8_plan_profile(w4a8_plan *plan, int32_t n, float *ms);
 int w4a8_plan_time_launches(w4a8_plan *plan, int32_t n, float *ms);
 int w4a8_plan_destroy(w4a8_plan *plan);
 
+/* ---- the mixers between a step's sites ---------------------------------
+ * What a decoder layer does between its projections, on device buffers:
+ * attention over a paged key-value cache, the cache's pages, and the gated
+ * delta rule.  No counterpart in the reference's C interface; they are
+ * floating-point operators, not the fixed-point ones of its layers.
+ *
+ * Activations are float32, bfloat16, float16, or the engine's own int16 with
+ * `frac` fraction bits (value = x * 2^-frac), which a site writes and a DYNQ8
+ * site reads.  Their last dimension is contiguous; the strides of tokens (or
+ * rows) and heads are arguments, in elements.  Sums, softmax statistics and
+ * states are held in 32 bits.  Lists of sequences, pages and slots are int32
+ * device arrays; a negative entry is padding and is skipped.  What a list or
+ * a table holds is checked on the device: an entry outside the cache is not
+ * followed, and the next w4a8_ctx_sync() returns W4A8_E_RANGE. */
+#define W4A8_DT_F32   0
+#define W4A8_DT_BF16  1
+#define W4A8_DT_F16   2
+#define W4A8_DT_I16   3   /* activations only */
+
+/* A paged cache over device memory of the caller:
+ *   pool    [pages][layers][keys, values][kv_heads][page_tokens][head_dim] of
+ *           dtype (F32, BF16 or F16), 16-byte aligned
+ *   refs    int32[pages]: how many sequences hold the page, 0 = free (16-byte
+ *           aligned)
+ *   tables  int32[seqs][max_pages]: the pages of each sequence
+ *   lens    int32[seqs]: its tokens; the first ceil(len / page_tokens) entries
+ *           of its table are in use
+ * An empty cache is refs and lens of zeros.  page_tokens: a power of two,
+ * 16..1024; head_dim: 64, 128 or 256.  The calls below change refs, tables
+ * and lens on the context's stream, so calls on one cache from several
+ * streams need ordering by the caller; one handle serves one cache (its
+ * scratch memory is part of the cache's state). */
+typedef struct w4a8_kv w4a8_kv;
+int w4a8_kv_create(w4a8_ctx *ctx, int32_t dtype, int32_t pages, int32_t layers,
+                   int32_t kv_heads, int32_t page_tokens, int32_t head_dim,
+                   int32_t seqs, int32_t max_pages, void *d_pool,
+                   int32_t *d_refs, int32_t *d_tables, int32_t *d_lens,
+                   w4a8_kv **out);
+int w4a8_kv_destroy(w4a8_kv *kv);
+/* sequence d_seqs[i] grows by d_counts[i] tokens: pages are added as needed,
+   the lowest free ones first, in the order of the list.  All or nothing: with
+   too few free pages, a sequence listed twice or outside the cache, or one
+   that would pass max_pages, nothing changes and the next sync reports it. */
+int w4a8_kv_extend_async(w4a8_kv *kv, const int32_t *d_seqs,
+                         const int32_t *d_counts, int32_t n);
+/* token i's keys and values of one layer, k and v [n][kv_heads][head_dim] of
+   the cache's dtype or int16, to sequence d_seqs[i] at position d_pos[i] <
+   its length (null: its last token).  Two tokens for the same place leave
+   either one's values there. */
+int w4a8_kv_append_async(w4a8_kv *kv, int32_t layer, int32_t dtype, int32_t frac,
+                         const void *d_k, int64_t k_token, int64_t k_head,
+                         const void *d_v, int64_t v_token, int64_t v_head,
+                         const int32_t *d_seqs, const int32_t *d_pos, int32_t n);
+/* sequence d_children[i], empty, becomes a copy of d_parents[i]: full pages
+   are shared, the used tokens of a last page that is not full are copied to a
+   free page (lowest first, in the order of the list).  A parent may be listed
+   many times.  All or nothing as above; a child listed twice, not empty, or a
+   parent too, is refused. */
+int w4a8_kv_fork_async(w4a8_kv *kv, const int32_t *d_parents,
+                       const int32_t *d_children, int32_t n);
+/* the listed sequences become empty; their pages, where no other sequence
+   holds them, free.  Listing a sequence again changes nothing. */
+int w4a8_kv_free_async(w4a8_kv *kv, const int32_t *d_seqs, int32_t n);
+/* the U pages in use become pages 0..U-1: the k-th page in use at U or above
+   moves to the k-th free page below U, and refs and tables follow */
+int w4a8_kv_compact_async(w4a8_kv *kv);
+/* page d_src[i] copied to page d_dst[i], whole; no page of d_dst may be listed
+   twice or in d_src */
+int w4a8_kv_copy_async(w4a8_kv *kv, const int32_t *d_src, const int32_t *d_dst,
+                       int32_t n);
+/* bytes of workspace w4a8_kv_attend_async needs for this many rows and query
+   heads (may be 0).  Calls that can overlap need one each. */
+int w4a8_kv_attend_workspace(const w4a8_kv *kv, int32_t rows, int32_t q_heads,
+                             int64_t *bytes);
+/* Attention of one token per row: q [rows][q_heads][head_dim] against the
+   tokens of sequence d_seqs[i] (the first d_upto[i] of them, where d_upto is
+   given: several new tokens of a sequence are rows of their own), query heads
+   of a key-value head side by side (q_heads a multiple of kv_heads).
+     out = softmax(scale q K^T) V; a row without tokens gets zeros
+   dtype: the cache's, or I16 (q with frac, out with out_frac fraction bits);
+   q and out share it.  d_ws: 16-byte aligned. */
+int w4a8_kv_attend_async(w4a8_kv *kv, int32_t layer, int32_t dtype, int32_t frac,
+                         int32_t out_frac, const void *d_q, int64_t q_row,
+                         int64_t q_head, void *d_out, int64_t out_row,
+                         int64_t out_head, const int32_t *d_seqs,
+                         const int32_t *d_upto, int32_t rows, int32_t q_heads,
+                         double scale, void *d_ws, int64_t ws_bytes);
+
+/* The gated delta rule.  Per token t and value head h (key head h / (hv /
+ * hk)), with the head's state S float32 [dk][dv]:
+ *   S <- exp(g) S;  u = beta (v - S^T k);  S <- S + k u^T;  out = scale S^T q
+ * norm: q and k are divided by sqrt(sum of squares + eps) first.  A row is a
+ * sequence; its tokens lie side by side in q, k [tokens][hk][dk], v, out
+ * [tokens][hv][dv], g, beta float32 [tokens][hv].  dk: 64 or 128; dv: a
+ * multiple of 16, 16..256; hv a multiple of hk.  All members are 8 bytes
+ * wide. */
+typedef struct {
+  const void *q, *k, *v;
+  const float *g, *beta;
+  float *state;          /* [slots][hv][dk][dv], contiguous, updated in place */
+  void *out;
+  const int32_t *slots;  /* [rows]: the row's state, negative: none (a padded
+                            row, its out is zeros); null: row i's is i.  A slot
+                            named by two rows is the first one's; the other is
+                            treated as padding and the next sync reports it */
+  const int32_t *cu;     /* chunk: [rows + 1]: row i's tokens are cu[i] ..
+                            cu[i + 1] - 1; tokens past the last row's are left
+                            alone.  step: ignored */
+  void *ws;              /* chunk: w4a8_delta_chunk_workspace bytes; 16-byte
+                            aligned.  step: ignored */
+  int64_t ws_bytes;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
+  int64_t g_token, beta_token;              /* strides, in elements */
+  int64_t tokens, rows, hk, hv, dk, dv, nslots;
+  int64_t dtype, frac, out_frac;            /* of q, k, v and of out; fracs: I16 */
+  int64_t norm;
+  int64_t fresh;                            /* states start from zeros, unread */
+  double scale, eps;
+} w4a8_delta;
+/* one token of each row */
+int w4a8_delta_step_async(w4a8_ctx *ctx, const w4a8_delta *d);
+/* whole prompts */
+int w4a8_delta_chunk_workspace(w4a8_ctx *ctx, int64_t tokens, int64_t rows,
+                               int64_t hv, int64_t *bytes);
+int w4a8_delta_chunk_async(w4a8_ctx *ctx, const w4a8_delta *d);
+
 #ifdef __cplusplus
 }
 #endif
