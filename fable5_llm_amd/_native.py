@@ -84,7 +84,7 @@ SIGNATURES = {
     "w4a8_kv_attend_async": [_P, _I32, _I32, _I32, _I32, _P, _I64, _I64, _P, _I64, _I64, _P,
                              _P, _I32, _I32, ctypes.c_double, _P, _I64],
     "w4a8_delta_step_async": [_P, _P],
-    "w4a8_delta_chunk_workspace": [_P, _I64, _I64, _I64, _P],
+    "w4a8_delta_chunk_workspace": [_P, _I64, _I64, _I64, _I64, _I64, _I32, _P],
     "w4a8_delta_chunk_async": [_P, _P],
     "w4a8_plan_create": [_P, ctypes.POINTER(_P)],
     "w4a8_plan_add_site": [_P, _I32, _PP, _P, _P, _PP, _I32, _P, _P, _I32, _I32,

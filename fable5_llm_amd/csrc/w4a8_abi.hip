@@ -214,9 +214,9 @@ int take_err(w4a8_ctx *c) {
       return fail(W4A8_E_RANGE, "KV cache: a sequence, position, length or page outside the "
                                 "cache; it was not followed");
     if (h & kErrDelta)
-      return fail(W4A8_E_RANGE, "delta rule: a state slot named twice or outside the states, or "
-                                "bounds that do not lie in order within the tokens; those rows "
-                                "were not run");
+      return fail(W4A8_E_RANGE, "delta rule: a state slot named twice or outside the states "
+                                "(that row was not run), or bounds that do not lie in order "
+                                "within the tokens (nothing was run)");
   }
   return W4A8_OK;
 }
@@ -2042,6 +2042,7 @@ const char *delta_fault(const w4a8_delta *d, bool chunk) {
   if (d->rows == 0) return nullptr;
   if (!d->slots && d->nslots < d->rows) return "fewer states than rows";
   if (chunk && !d->cu) return "cu is needed";
+  if (d->rows * d->hv > (1 << 26)) return "more than 2^26 heads of states";
   const int t = (int)d->dtype;
   if (!d->state || !aligned16(d->state)) return "state must be 16-byte aligned";
   if (d->tokens > 0) {
@@ -2060,7 +2061,9 @@ int delta_launch(w4a8_ctx *c, const w4a8_delta *d, bool chunk) {
   if (!c || !d) return fail(W4A8_E_ARG, "null argument");
   if (const char *why = delta_fault(d, chunk)) return fail(W4A8_E_ARG, why);
   if (d->rows == 0) return W4A8_OK;
-  const int64_t need = chunk ? delta_workspace(d->tokens, d->rows, d->hv) : 0;
+  const int64_t need = chunk ? delta_workspace(d->tokens, d->rows, d->hk, d->hv, d->dk,
+                                               (int)d->dtype)
+                             : 0;
   if (need > 0 && (!d->ws || !aligned16(d->ws) || d->ws_bytes < need))
     return fail(W4A8_E_ARG, "delta rule: the workspace holds " + std::to_string(d->ws_bytes) +
                                 " bytes, the call needs " + std::to_string(need));
@@ -2207,7 +2210,6 @@ int check_heads(const w4a8_kv *kv, int32_t rows, int32_t q_heads) {
   if (!kv) return fail(W4A8_E_ARG, "null cache");
   if (rows < 0 || q_heads < 1 || q_heads > 65535 || q_heads % kv->c.heads)
     return fail(W4A8_E_ARG, "q_heads must be a multiple of the cache's kv_heads");
-  // the workgroups of a launch: rows x splits, at most 2^30 rows each
   if (rows > (1 << 24)) return fail(W4A8_E_ARG, "at most 2^24 rows");
   return W4A8_OK;
 }
@@ -2253,12 +2255,13 @@ int w4a8_kv_attend_async(w4a8_kv *kv, int32_t layer, int32_t dtype, int32_t frac
 
 int w4a8_delta_step_async(w4a8_ctx *c, const w4a8_delta *d) { return delta_launch(c, d, false); }
 
-int w4a8_delta_chunk_workspace(w4a8_ctx *c, int64_t tokens, int64_t rows, int64_t hv,
-                               int64_t *bytes) {
-  if (!c || !bytes || tokens < 0 || rows < 0 || hv < 1 || tokens > INT32_MAX ||
-      rows > INT32_MAX || hv > 65535)
+int w4a8_delta_chunk_workspace(w4a8_ctx *c, int64_t tokens, int64_t rows, int64_t hk, int64_t hv,
+                               int64_t dk, int32_t dtype, int64_t *bytes) {
+  if (!c || !bytes || tokens < 0 || rows < 0 || hk < 1 || hv < hk || tokens > INT32_MAX ||
+      rows > INT32_MAX || hv > 65535 || (dk != 64 && dk != 128) || dtype < DT_F32 ||
+      dtype > DT_I16)
     return fail(W4A8_E_ARG, "bad argument");
-  *bytes = rows ? delta_workspace(tokens, rows, hv) : 0;
+  *bytes = rows ? delta_workspace(tokens, rows, hk, hv, dk, dtype) : 0;
   return W4A8_OK;
 }
 

@@ -26,122 +26,642 @@ __device__ __forceinline__ T from_float(float x, float out_unit) {
     return (T)x;
 }
 
-// The tokens of a row and the slot of its state (-1: none, its tokens' out is
-// zeros).  A slot that an earlier row names too, or outside the states, and
-// bounds that do not lie in order within the tokens, are reported.
-struct Row {
-  int t0, t1, slot;
-};
-__device__ __forceinline__ Row row_of(const Delta &p, int row, int *flag) {
-  Row r;
-  int bad = 0, taken = 0;
-  r.t0 = p.cu ? p.cu[row] : row;
-  r.t1 = p.cu ? p.cu[row + 1] : row + 1;
-  if (r.t0 < 0 || r.t1 < r.t0 || r.t1 > p.tokens) {
-    bad = 1;
-    r.t0 = r.t1 = 0;
-  }
-  r.slot = p.slots ? p.slots[row] : row;
-  if (p.slots && r.slot >= 0)
-    for (int j = threadIdx.x; j < row; j += blockDim.x) taken |= p.slots[j] == r.slot;
-  taken = __syncthreads_or(taken) || r.slot >= p.nslots;
-  if (taken) r.slot = -1;
-  *flag = bad | taken;
-  return r;
+// The slot of a row's state, -1 for none: a padded row, or a slot that an
+// earlier row names too or that lies outside the states, which is reported.
+// The whole workgroup asks.
+__device__ __forceinline__ int slot_of(const Delta &p, int row, bool tell) {
+  const int slot = p.slots ? p.slots[row] : row;
+  int taken = 0;
+  if (p.slots && slot >= 0)
+    for (int j = threadIdx.x; j < row; j += blockDim.x) taken |= p.slots[j] == slot;
+  taken = __syncthreads_or(taken) || slot >= p.nslots;
+  if (taken && tell && threadIdx.x == 0) atomicOr(p.err, kErrDelta);
+  return taken ? -1 : slot;
 }
 
-// A wavefront holds 16 columns of a head's state in registers: lane (rg, cq) =
-// (lane >> 2, lane & 3) rows NR rg .. and columns 4 cq .., and takes the
-// row's tokens one after another.
+// One token of each row: a wavefront holds 16 columns of a head's state in
+// registers, lane (rg, cq) = (lane >> 2, lane & 3) its rows NR rg .. and
+// columns 4 cq ...
 template <int DK, typename T>
-__global__ __launch_bounds__(256) void delta_serial_kernel(Delta p) {
+__global__ __launch_bounds__(256) void delta_step_kernel(Delta p) {
   constexpr int NR = DK / 16;
   const int row = blockIdx.x, h = blockIdx.y;
-  int flag;
-  const Row R = row_of(p, row, &flag);
-  if (flag && threadIdx.x == 0 && h == 0 && blockIdx.z == 0) atomicOr(p.err, kErrDelta);
+  const int slot = slot_of(p, row, h == 0 && blockIdx.z == 0);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int rg = lane >> 2, col = (blockIdx.z * 4 + wave) * 16 + (lane & 3) * 4;
   if (col >= p.dv) return;
-  T *out = (T *)p.out + h * p.out_head + col;
-  if (R.slot < 0) {
+  T *out = (T *)p.out + row * p.out_token + h * p.out_head + col;
+  if (slot < 0) {
     if (rg == 0)
-      for (int t = R.t0; t < R.t1; ++t)
-        for (int c = 0; c < 4; ++c) out[t * p.out_token + c] = (T)0;
+      for (int c = 0; c < 4; ++c) out[c] = (T)0;
     return;
   }
-  if (R.t0 == R.t1) {
-    if (!p.fresh) return;
-  }
-  float *S = p.state + (((int64_t)R.slot * p.hv + h) * p.dk + rg * NR) * p.dv + col;
+  float *S = p.state + (((int64_t)slot * p.hv + h) * p.dk + rg * NR) * p.dv + col;
   f32x4 s[NR];
 #pragma unroll
-  for (int i = 0; i < NR; ++i)
-    s[i] = p.fresh ? f32x4{0, 0, 0, 0} : *(const f32x4 *)(S + (int64_t)i * p.dv);
+  for (int i = 0; i < NR; ++i) s[i] = *(const f32x4 *)(S + (int64_t)i * p.dv);
   const int hk = h / (p.hv / p.hk);
-  const T *q = (const T *)p.q + hk * p.q_head + rg * NR;
-  const T *k = (const T *)p.k + hk * p.k_head + rg * NR;
-  const T *v = (const T *)p.v + h * p.v_head + col;
-  for (int t = R.t0; t < R.t1; ++t) {
-    float qv[NR], kv[NR];
-    float qq = 0.f, kk = 0.f, kq = 0.f;
-    f32x4 pk{0, 0, 0, 0}, pq{0, 0, 0, 0};
+  const T *q = (const T *)p.q + row * p.q_token + hk * p.q_head + rg * NR;
+  const T *k = (const T *)p.k + row * p.k_token + hk * p.k_head + rg * NR;
+  const T *v = (const T *)p.v + row * p.v_token + h * p.v_head + col;
+  float qv[NR], kv[NR];
+  float qq = 0.f, kk = 0.f, kq = 0.f;
+  f32x4 pk{0, 0, 0, 0}, pq{0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < NR; ++i) {
-      qv[i] = to_float(q[t * p.q_token + i], p.unit);
-      kv[i] = to_float(k[t * p.k_token + i], p.unit);
-      qq += qv[i] * qv[i];
-      kk += kv[i] * kv[i];
-      kq += kv[i] * qv[i];
-      pk += s[i] * kv[i];
-      pq += s[i] * qv[i];
-    }
-#pragma unroll
-    for (int d = 4; d < 64; d <<= 1) {
-      qq += __shfl_xor(qq, d);
-      kk += __shfl_xor(kk, d);
-      kq += __shfl_xor(kq, d);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        pk[c] += __shfl_xor(pk[c], d);
-        pq[c] += __shfl_xor(pq[c], d);
-      }
-    }
-    const float rq = (p.norm ? 1.f / sqrtf(qq + p.eps) : 1.f) * p.scale;
-    const float rk = p.norm ? 1.f / sqrtf(kk + p.eps) : 1.f;
-    const float e = expf(p.g[t * p.g_token + h]), beta = p.beta[t * p.beta_token + h];
-    f32x4 u, o;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      u[c] = beta * (to_float(v[t * p.v_token + c], p.unit) - e * rk * pk[c]);
-      o[c] = rq * (e * pq[c] + rk * kq * u[c]);
-    }
-#pragma unroll
-    for (int i = 0; i < NR; ++i) s[i] = s[i] * e + u * (kv[i] * rk);
-    if (rg == 0)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) out[t * p.out_token + c] = from_float<T>(o[c], p.out_unit);
+  for (int i = 0; i < NR; ++i) {
+    qv[i] = to_float(q[i], p.unit);
+    kv[i] = to_float(k[i], p.unit);
+    qq += qv[i] * qv[i];
+    kk += kv[i] * kv[i];
+    kq += kv[i] * qv[i];
+    pk += s[i] * kv[i];
+    pq += s[i] * qv[i];
   }
 #pragma unroll
-  for (int i = 0; i < NR; ++i) *(f32x4 *)(S + (int64_t)i * p.dv) = s[i];
+  for (int d = 4; d < 64; d <<= 1) {
+    qq += __shfl_xor(qq, d);
+    kk += __shfl_xor(kk, d);
+    kq += __shfl_xor(kq, d);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      pk[c] += __shfl_xor(pk[c], d);
+      pq[c] += __shfl_xor(pq[c], d);
+    }
+  }
+  const float rq = (p.norm ? 1.f / sqrtf(qq + p.eps) : 1.f) * p.scale;
+  const float rk = p.norm ? 1.f / sqrtf(kk + p.eps) : 1.f;
+  const float e = expf(p.g[row * p.g_token + h]), beta = p.beta[row * p.beta_token + h];
+  f32x4 u;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    u[c] = beta * (to_float(v[c], p.unit) - e * rk * pk[c]);
+    const float o = rq * (e * pq[c] + rk * kq * u[c]);
+    if (rg == 0) out[c] = from_float<T>(o, p.out_unit);
+  }
+#pragma unroll
+  for (int i = 0; i < NR; ++i) *(f32x4 *)(S + (int64_t)i * p.dv) = s[i] * e + u * (kv[i] * rk);
+}
+
+// ------------------------------------------------------------ whole prompts
+// A prompt goes in chunks of C = 64 tokens.  With G the running sum of g in a
+// chunk, S0 the state before it, and rows of q, k, v as matrices, the tokens'
+// u are the solution of a triangular system (strictly lower A):
+//
+//   A_tj = beta_t e^(G_t - G_j) k_t . k_j  (j < t),   M = (I + A)^-1 diag(beta)
+//   U = M (V - diag(e^G) K S0)
+//   O = scale (diag(e^G) Q S0 + P U),  P_tj = e^(G_t - G_j) q_t . k_j  (j <= t)
+//   S = e^(G_C) S0 + K^T diag(e^(G_C - G)) U
+//
+// M and P of every chunk do not depend on the state: delta_prep_kernel makes
+// them, all chunks at once; delta_scan_kernel then walks a row's chunks, a
+// workgroup per head and 16 columns of the state, which stays in registers.
+// Decays are differences of sums of g in 64 bits (an e^g of 0 among them
+// would otherwise cost the others their bits), and each is at most 1 where g
+// is at most 0.
+//
+// The products run on the bfloat16 matrix instructions with float32 sums: a
+// float32 operand is the sum of three bfloat16 values, exactly (float16 and
+// int16 of two, bfloat16 of one), and of the products of two operands' terms
+// those below 2^-24 are left out.  So a state keeps its 24 bits through a
+// prompt; a norm of q or k is a factor of its row, applied to the sums.
+// A token that holds an infinity or a NaN spoils its whole chunk.
+constexpr int C = 64;
+constexpr int kPlane = 64 * 8;                   // bfloat16 of one operand: 8 per lane
+constexpr int kTriBytes = 6 * 3 * kPlane * 2;    // M or P: operands of tri_of, three terms
+constexpr int kVecFloats = 256;                  // a, b, c of 64 tokens, e^(G_C)
+constexpr int kChunkBytes = 2 * kTriBytes + kVecFloats * 4;
+constexpr float kNoDecay = -200.f;               // e^g is 0 in float32 from here on down
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+struct Terms {
+  static constexpr int n = sizeof(T) == 4 ? 3 : __is_same(T, __bf16) ? 1 : 2;
+};
+
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma4(f32x4 a, f32x4 b, f32x4 c) {   // 16 x 16 x 16, float32
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+  return c;
+}
+// sum of the products of terms a[i] b[j] with i + j <= 2
+template <int NA, int NB>
+__device__ __forceinline__ f32x4 mfma_terms(const bf16x8 *a, const bf16x8 *b, f32x4 c) {
+#pragma unroll
+  for (int i = NA - 1; i >= 0; --i)
+#pragma unroll
+    for (int j = NB - 1; j >= 0; --j)
+      if (i + j <= 2) c = mfma(a[i], b[j], c);
+  return c;
+}
+
+// x as a sum of N bfloat16 values
+template <int N>
+__device__ __forceinline__ void split(float x, __bf16 *t) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    t[i] = (__bf16)x;
+    x -= (float)t[i];
+  }
+}
+
+// Barrier of the workgroup for LDS alone: loads from memory stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// The order of a chunk's tokens in an operand of k-steps s = 0, 1: slot j of
+// lane group g is token 32 s + 16 (j >> 2) + 4 g + (j & 3), so that a lane's
+// four results of row tiles 2 s and 2 s + 1 are its own eight slots.
+__device__ __forceinline__ int token_of(int s, int g, int j) {
+  return 32 * s + 16 * (j >> 2) + 4 * g + (j & 3);
+}
+// M and P as operands: row tile w (of 16 tokens) and k-step s <= w / 2
+__device__ __forceinline__ constexpr int tri_of(int w, int s) {
+  return w < 2 ? w : w == 2 ? 2 + s : 4 + s;
+}
+
+// first chunk of a row in the workspace: rows do not share chunks
+__device__ __forceinline__ int first_chunk(const Delta &p, int row) {
+  return p.cu[row] / C + row;
+}
+
+// Whether every row's bounds lie in order within the tokens (the whole
+// workgroup asks), and which row chunk `slot` belongs to (-1: none).
+__device__ __forceinline__ bool bounds_ok(const Delta &p, int slot, int *row) {
+  __shared__ int found;
+  if (threadIdx.x == 0) found = -1;
+  __syncthreads();
+  int bad = 0;
+  for (int j = threadIdx.x; j < p.rows; j += blockDim.x) {
+    const int t0 = p.cu[j], t1 = p.cu[j + 1];
+    const bool off = t0 < 0 || t1 < t0 || t1 > p.tokens;
+    bad |= off;
+    const int at = slot - (t0 / C + j);
+    if (!off && at >= 0 && at < (t1 - t0 + C - 1) / C) found = j;
+  }
+  bad = __syncthreads_or(bad);
+  *row = found;
+  return !bad;
+}
+
+// Planes of q and k as bfloat16 terms [term][token][key head][dk]; bfloat16
+// itself is read where it lies.
+struct Planes {
+  const __bf16 *k, *q;
+  int64_t k_token, q_token, k_head, q_head, term;   // elements
+};
+template <typename T>
+__host__ __device__ inline Planes planes_of(const Delta &p) {
+  if (Terms<T>::n == 1)
+    return Planes{(const __bf16 *)p.k, (const __bf16 *)p.q, p.k_token, p.q_token, p.k_head,
+                  p.q_head, 0};
+  const int64_t term = (int64_t)p.tokens * p.hk * p.dk;
+  const int64_t chunks = p.tokens / C + p.rows;
+  __bf16 *k = (__bf16 *)((uint8_t *)p.ws + chunks * p.hv * kChunkBytes);
+  return Planes{k, k + Terms<T>::n * term, (int64_t)p.hk * p.dk, (int64_t)p.hk * p.dk, p.dk, p.dk,
+                term};
+}
+
+// A workgroup per chunk and key head.
+template <int DK, typename T>
+__global__ __launch_bounds__(256) void delta_prep_kernel(Delta p) {
+  constexpr int NK = Terms<T>::n, NS = DK / 32, LD = 68;
+  __shared__ double Gs[C];
+  __shared__ float rks[C], rqs[C], betas[C];
+  __shared__ __align__(16) float As[C * LD];
+  __shared__ __align__(16) float Ts[4][16 * 20];
+  __shared__ __align__(16) __bf16 planes[2][6 * 3 * kPlane];
+  const int slot = blockIdx.x, hk = blockIdx.y;
+  int row;
+  if (!bounds_ok(p, slot, &row)) {
+    if (slot == 0 && hk == 0 && threadIdx.x == 0) atomicOr(p.err, kErrDelta);
+    return;
+  }
+  if (row < 0) return;
+  const int chunk = slot - first_chunk(p, row);
+  const int t0 = p.cu[row] + chunk * C, len = min(C, p.cu[row + 1] - t0);
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+  // tiles above the diagonal that share a k-step with one below stay zeros
+  for (int i = threadIdx.x; i < 2 * kTriBytes / 16; i += 256)
+    ((u32x4 *)planes)[i] = u32x4{0, 0, 0, 0};
+
+  // rows 16 tile + r of x, elements 32 s + 8 g .., as terms; their squares' sum
+  auto load = [&](const void *x, int64_t token, int64_t head, int tile, bf16x8 (*f)[NK],
+                  float *squares) {
+    const int t = 16 * tile + r;
+    const bool on = t < len;
+    const T *src = (const T *)x + (t0 + min(t, len - 1)) * token + hk * head + 8 * g;
+    float sum = 0.f;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      T v[8];
+      *(u32x4 *)v = *(const u32x4 *)(src + 32 * s);
+      if constexpr (sizeof(T) == 4) *(u32x4 *)(v + 4) = *(const u32x4 *)(src + 32 * s + 4);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float y = on ? to_float(v[j], p.unit) : 0.f;
+        sum += y * y;
+        __bf16 h[NK];
+        split<NK>(y, h);
+#pragma unroll
+        for (int i = 0; i < NK; ++i) f[s][i][j] = h[i];
+      }
+    }
+    if (squares) *squares = sum;
+  };
+  bf16x8 kw[NS][NK], qw[NS][NK];
+  float kk2, qq2;
+  load(p.k, p.k_token, p.k_head, w, kw, &kk2);
+  load(p.q, p.q_token, p.q_head, w, qw, &qq2);
+  kk2 += __shfl_xor(kk2, 16);
+  kk2 += __shfl_xor(kk2, 32);
+  qq2 += __shfl_xor(qq2, 16);
+  qq2 += __shfl_xor(qq2, 32);
+  if (g == 0) {
+    const bool on = 16 * w + r < len;
+    rks[16 * w + r] = !on ? 0.f : p.norm ? 1.f / sqrtf(kk2 + p.eps) : 1.f;
+    rqs[16 * w + r] = !on ? 0.f : (p.norm ? 1.f / sqrtf(qq2 + p.eps) : 1.f) * p.scale;
+  }
+  if constexpr (NK > 1) {
+    const Planes pl = planes_of<T>(p);
+    if (16 * w + r < len) {
+      const int64_t at = (t0 + 16 * w + r) * pl.k_token + hk * pl.k_head + 8 * g;
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+          *(bf16x8 *)(const_cast<__bf16 *>(pl.k) + i * pl.term + at + 32 * s) = kw[s][i];
+          *(bf16x8 *)(const_cast<__bf16 *>(pl.q) + i * pl.term + at + 32 * s) = qw[s][i];
+        }
+    }
+  }
+  // k_t . k_j and q_t . k_j, t = 16 w + 4 g + i, j = 16 c + r, up to the diagonal
+  f32x4 kk[4], qk[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    kk[c] = qk[c] = f32x4{0, 0, 0, 0};
+    if (c <= w) {
+      bf16x8 kc[NS][NK];
+      load(p.k, p.k_token, p.k_head, c, kc, nullptr);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        kk[c] = mfma_terms<NK, NK>(kw[s], kc[s], kk[c]);
+        qk[c] = mfma_terms<NK, NK>(qw[s], kc[s], qk[c]);
+      }
+    }
+  }
+  // an element of M or P, row 16 tile + m, column 16 c + col
+  auto put = [&](int which, int tile, int c, int m, int col, float x) {
+    __bf16 h[3];
+    split<3>(x, h);
+    __bf16 *o = planes[which] + tri_of(tile, c >> 1) * 3 * kPlane + (m + 16 * (col >> 2)) * 8 +
+                4 * (c & 1) + (col & 3);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) o[i * kPlane] = h[i];
+  };
+
+  const int per = p.hv / p.hk;
+  for (int h = hk * per; h < (hk + 1) * per; ++h) {
+    uint8_t *ws = (uint8_t *)p.ws + ((int64_t)slot * p.hv + h) * kChunkBytes;
+    __syncthreads();                 // rks, rqs; the last head's planes are out
+    if (w == 0) {
+      const bool on = lane < len;
+      const int64_t t = t0 + min(lane, len - 1);
+      const float gt = on ? fmaxf(p.g[t * p.g_token + h], kNoDecay) : 0.f;
+      const float bt = on ? p.beta[t * p.beta_token + h] : 0.f;
+      double G = gt;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const double y = __shfl_up(G, d);
+        if (lane >= d) G += y;
+      }
+      Gs[lane] = G;
+      betas[lane] = bt;
+      const double GC = __shfl(G, 63);
+      float *vec = (float *)(ws + 2 * kTriBytes);
+      vec[lane] = on ? expf((float)G) * rks[lane] : 0.f;
+      vec[64 + lane] = on ? expf((float)G) * rqs[lane] : 0.f;
+      vec[128 + lane] = on ? expf((float)(GC - G)) * rks[lane] : 0.f;
+      if (lane == 0) vec[192] = expf((float)GC);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (c <= w) {
+        const int j = 16 * c + r;
+        const double Gj = Gs[j];
+        const float rkj = rks[j];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int t = 16 * w + 4 * g + i;
+          const float dec = j <= t ? expf((float)(Gs[t] - Gj)) * rkj : 0.f;
+          As[t * LD + j] = j < t ? betas[t] * rks[t] * dec * kk[c][i] : 0.f;
+          put(1, w, c, 4 * g + i, r, j <= t ? rqs[t] * dec * qk[c][i] : 0.f);
+        }
+      }
+    __syncthreads();
+    {   // the inverse of diagonal block w, column r by substitution
+      float x[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float y = i == r ? 1.f : 0.f;
+#pragma unroll
+        for (int j = 0; j < i; ++j) y -= As[(16 * w + i) * LD + 16 * w + j] * x[j];
+        x[i] = y;
+        if (g == 0) Ts[w][i * 20 + r] = y;
+      }
+    }
+    __syncthreads();
+    {   // block column w of the inverse: X_i = -T_ii sum_k A_ik X_k
+      f32x4 X[4];
+      const float bj = betas[16 * w + r];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        X[i] = f32x4{0, 0, 0, 0};
+        if (i == w) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) X[i][k] = Ts[w][(4 * g + k) * 20 + r];
+        } else if (i > w) {
+          f32x4 acc{0, 0, 0, 0};
+#pragma unroll
+          for (int k = 0; k < i; ++k)
+            if (k >= w)
+              acc = mfma4(*(const f32x4 *)(As + (16 * i + r) * LD + 16 * k + 4 * g), X[k], acc);
+          X[i] = mfma4(-*(const f32x4 *)(Ts[i] + r * 20 + 4 * g), acc, X[i]);
+        }
+        if (i >= w)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) put(0, i, w, 4 * g + k, r, X[i][k] * bj);
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * kTriBytes / 16; i += 256)
+      ((u32x4 *)ws)[i] = ((const u32x4 *)planes)[i];
+  }
+}
+
+// What a wavefront needs of one chunk, loaded a chunk ahead: its 16 tokens'
+// rows of K and Q, 32 columns of K of every token, its tokens' 16 values, its
+// row tile of M and P, and the factors of its tokens.
+template <int DK, typename T>
+struct ChunkData {
+  static constexpr int NK = Terms<T>::n, NS = DK / 32;
+  bf16x8 k[NS][NK], q[NS][NK];
+  uint32_t kt[2][8][NK];
+  T v[4];
+  bf16x8 m[2][3], pp[2][3];
+  f32x4 a, b, c;
+  float fall;
+  int t0, len;
+};
+
+template <int DK, typename T>
+__device__ __forceinline__ void load_chunk(const Delta &p, const Planes &pl, int t0, int len,
+                                           int64_t slot, int h, int hk, int col, int w, int lane,
+                                           ChunkData<DK, T> &d) {
+  constexpr int NK = Terms<T>::n, NS = DK / 32;
+  const int r = lane & 15, g = lane >> 4;
+  d.t0 = t0;
+  d.len = len;
+  const uint8_t *ws = (const uint8_t *)p.ws + (slot * p.hv + h) * kChunkBytes;
+  const bf16x8 *tri = (const bf16x8 *)ws + lane;
+  const int64_t row = t0 + min(16 * w + r, len - 1);
+  const __bf16 *k = pl.k + row * pl.k_token + hk * pl.k_head + 8 * g;
+  const __bf16 *q = pl.q + row * pl.q_token + hk * pl.q_head + 8 * g;
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      d.k[s][i] = *(const bf16x8 *)(k + i * pl.term + 32 * s);
+      d.q[s][i] = *(const bf16x8 *)(q + i * pl.term + 32 * s);
+    }
+  const T *v = (const T *)p.v + h * p.v_head + col;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) d.v[i] = v[(t0 + min(16 * w + 4 * g + i, len - 1)) * p.v_token];
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+    if (s <= w >> 1)
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        d.m[s][i] = tri[(tri_of(w, s) * 3 + i) * 64];
+        d.pp[s][i] = tri[(6 * 3 + tri_of(w, s) * 3 + i) * 64];
+      }
+  if (w < NS) {
+    const __bf16 *kt = pl.k + hk * pl.k_head + 32 * w + 2 * r;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int64_t t = t0 + min(token_of(s, g, j), len - 1);
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+          d.kt[s][j][i] = *(const uint32_t *)(kt + t * pl.k_token + i * pl.term);
+      }
+  }
+  const float *vec = (const float *)(ws + 2 * kTriBytes);
+  d.a = *(const f32x4 *)(vec + 16 * w + 4 * g);
+  d.b = *(const f32x4 *)(vec + 64 + 16 * w + 4 * g);
+  d.c = *(const f32x4 *)(vec + 128 + 16 * w + 4 * g);
+  d.fall = vec[192];
+}
+
+// A workgroup per row, value head and 16 columns; wavefront w has tokens
+// 16 w .. of a chunk, and rows 32 w .. of the state: lane (r, g) of it rows
+// 32 w + 8 g + e of column r, in register [e & 1][e >> 1].
+template <int DK, typename T>
+__global__ __launch_bounds__(256, 1) void delta_scan_kernel(Delta p) {
+  constexpr int NK = Terms<T>::n, NS = DK / 32;
+  __shared__ bf16x8 Sb[3][NS][64];                // the state, k-step s by wavefront s
+  __shared__ __align__(16) bf16x4 Rb[3][2][64][2], Ub[3][2][64][2], Wb[3][2][64][2];
+  const int tiles = p.dv / 16, units = p.rows * p.hv, each = (units + 7) / 8;
+  // a head's columns, and heads that share keys, on one XCD (workgroups go
+  // round the eight of them)
+  const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3;
+  const int unit = xcd * each + at / tiles;
+  if (at / tiles >= each || unit >= units) return;
+  const int row = unit / p.hv, h = unit - row * p.hv, hk = h / (p.hv / p.hk);
+  int dummy;
+  if (!bounds_ok(p, -1, &dummy)) return;          // reported by delta_prep_kernel
+  const int slot = slot_of(p, row, h == 0 && at % tiles == 0);
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = (at % tiles) * 16 + r;
+  const int begin = p.cu[row], end = p.cu[row + 1];
+  T *out = (T *)p.out + h * p.out_head + col;
+  if (slot < 0) {
+    for (int t = begin + (int)(threadIdx.x >> 4); t < end; t += 16) out[t * p.out_token] = (T)0;
+    return;
+  }
+  float *state = p.state + (((int64_t)slot * p.hv + h) * DK + 32 * w + 8 * g) * p.dv + col;
+  f32x4 S[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      S[e][i] = p.fresh || w >= NS ? 0.f : state[(int64_t)(2 * i + e) * p.dv];
+  auto put_state = [&]() {
+    if (w >= NS) return;
+    bf16x8 t[3];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      __bf16 x[3];
+      split<3>(S[j & 1][j >> 1], x);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) t[i][j] = x[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i) Sb[i][w][lane] = t[i];
+  };
+  auto put_rows = [&](bf16x4 (*b)[2][64][2], f32x4 x) {
+    bf16x4 t[3];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      __bf16 y[3];
+      split<3>(x[j], y);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) t[i][j] = y[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i) b[i][w >> 1][lane][w & 1] = t[i];
+  };
+  const Planes pl = planes_of<T>(p);
+  const int64_t slot0 = first_chunk(p, row);
+  const int n = (end - begin + C - 1) / C;
+  typedef ChunkData<DK, T> Data;
+  auto load = [&](int c, Data &d) {
+    if (c < n)
+      load_chunk<DK, T>(p, pl, begin + c * C, min(C, end - begin - c * C), slot0 + c, h, hk, col,
+                        w, lane, d);
+  };
+  auto step = [&](const Data &d) {
+    f32x4 ks{0, 0, 0, 0}, qs{0, 0, 0, 0};
+    {
+      bf16x8 sb[NS][3];
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int i = 0; i < 3; ++i) sb[s][i] = Sb[i][s][lane];
+#pragma unroll
+      for (int s = 0; s < NS; ++s) ks = mfma_terms<NK, 3>(d.k[s], sb[s], ks);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) qs = mfma_terms<NK, 3>(d.q[s], sb[s], qs);
+    }
+    f32x4 x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      x[i] = (16 * w + 4 * g + i < d.len ? to_float(d.v[i], p.unit) : 0.f) - d.a[i] * ks[i];
+    put_rows(Rb, x);
+    lds_barrier();
+    f32x4 u{0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      if (s <= w >> 1) {
+        bf16x8 b[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) b[i] = *(const bf16x8 *)Rb[i][s][lane];
+        u = mfma_terms<3, 3>(d.m[s], b, u);
+      }
+    put_rows(Ub, u);
+    put_rows(Wb, u * d.c);
+    lds_barrier();
+    if (w < NS) {
+      S[0] *= d.fall;
+      S[1] *= d.fall;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        bf16x8 b[3], a[2][NK];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) b[i] = *(const bf16x8 *)Wb[i][s][lane];
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            u32x4 y;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              y[j] = __builtin_amdgcn_perm(d.kt[s][2 * j + 1][i], d.kt[s][2 * j][i],
+                                           e ? 0x07060302u : 0x05040100u);
+            a[e][i] = __builtin_bit_cast(bf16x8, y);
+          }
+        S[0] = mfma_terms<NK, 3>(a[0], b, S[0]);
+        S[1] = mfma_terms<NK, 3>(a[1], b, S[1]);
+      }
+      put_state();
+    }
+    f32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = d.b[i] * qs[i];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      if (s <= w >> 1) {
+        bf16x8 b[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) b[i] = *(const bf16x8 *)Ub[i][s][lane];
+        o = mfma_terms<3, 3>(d.pp[s], b, o);
+      }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (16 * w + 4 * g + i < d.len)
+        out[(d.t0 + 16 * w + 4 * g + i) * p.out_token] = from_float<T>(o[i], p.out_unit);
+    lds_barrier();
+  };
+  Data d0, d1;
+  load(0, d0);
+  put_state();
+  lds_barrier();
+  for (int c = 0; c < n; c += 2) {
+    load(c + 1, d1);
+    step(d0);
+    if (c + 1 >= n) break;
+    load(c + 2, d0);
+    step(d1);
+  }
+  if (w < NS)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) state[(int64_t)(2 * i + e) * p.dv] = S[e][i];
+}
+
+template <int DK, typename T>
+void launch_typed(const Delta &d, hipStream_t s) {
+  if (!d.cu) {
+    delta_step_kernel<DK, T><<<dim3(d.rows, d.hv, (d.dv + 63) / 64), 256, 0, s>>>(d);
+    return;
+  }
+  delta_prep_kernel<DK, T><<<dim3(d.tokens / C + d.rows, d.hk), 256, 0, s>>>(d);
+  const int64_t each = ((int64_t)d.rows * d.hv + 7) / 8;
+  delta_scan_kernel<DK, T><<<(uint32_t)(8 * each * (d.dv / 16)), 256, 0, s>>>(d);
 }
 
 template <int DK>
-void launch_serial(const Delta &d, hipStream_t s) {
-  const dim3 grid(d.rows, d.hv, (d.dv + 63) / 64);
-  if (d.dtype == DT_F32) delta_serial_kernel<DK, float><<<grid, 256, 0, s>>>(d);
-  else if (d.dtype == DT_BF16) delta_serial_kernel<DK, __bf16><<<grid, 256, 0, s>>>(d);
-  else if (d.dtype == DT_F16) delta_serial_kernel<DK, _Float16><<<grid, 256, 0, s>>>(d);
-  else delta_serial_kernel<DK, int16_t><<<grid, 256, 0, s>>>(d);
+void launch_dim(const Delta &d, hipStream_t s) {
+  if (d.dtype == DT_F32) launch_typed<DK, float>(d, s);
+  else if (d.dtype == DT_BF16) launch_typed<DK, __bf16>(d, s);
+  else if (d.dtype == DT_F16) launch_typed<DK, _Float16>(d, s);
+  else launch_typed<DK, int16_t>(d, s);
 }
 
 }  // namespace
 
-int64_t delta_workspace(int64_t, int64_t, int64_t) { return 0; }
+int64_t delta_workspace(int64_t tokens, int64_t rows, int64_t hk, int64_t hv, int64_t dk,
+                        int dtype) {
+  const int64_t terms = dtype == DT_F32 ? 3 : dtype == DT_BF16 ? 0 : 2;
+  return (tokens / C + rows) * hv * kChunkBytes + 2 * terms * tokens * hk * dk * 2;
+}
 
 hipError_t launch_delta(const Delta &d, hipStream_t s) {
-  if (d.dk == 64) launch_serial<64>(d, s);
-  else launch_serial<128>(d, s);
+  if (d.dk == 64) launch_dim<64>(d, s);
+  else launch_dim<128>(d, s);
   return hipGetLastError();
 }
 

@@ -427,10 +427,12 @@ class Context:
             self, q, k, v, g, beta, state, out, None, None, slots, scale, norm, eps, False, frac,
             out_frac)), "delta_step")
 
-    def delta_chunk_workspace(self, tokens, rows, hv):
+    def delta_chunk_workspace(self, tokens, rows, hv, hk=None, dk=128, dtype=None):
         """Device memory for delta_chunk_async with this many tokens, rows and
-        value heads; calls that can overlap need one each."""
-        return mixers.delta_workspace(self, tokens, rows, hv)
+        value heads, of the largest such call's size; with the key heads, dk
+        and the type of q, k and v given, of that call's.  Calls that can
+        overlap need one each."""
+        return mixers.delta_workspace(self, tokens, rows, hv, hk, dk, dtype)
 
     def delta_chunk_async(self, q, k, v, g, beta, state, out, cu, ws, slots=None, fresh=False,
                           scale=None, norm=True, eps=1e-6, frac=0, out_frac=0):

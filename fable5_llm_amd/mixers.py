@@ -264,8 +264,12 @@ def delta_args(ctx, q, k, v, g, beta, state, out, cu, ws, slots, scale, norm, ep
         1.0 / math.sqrt(dk) if scale is None else scale, eps)
 
 
-def delta_workspace(ctx, tokens, rows, hv):
+def delta_workspace(ctx, tokens, rows, hv, hk, dk, dtype):
     b = ctypes.c_int64()
-    N.check(N.lib().w4a8_delta_chunk_workspace(ctx.h, tokens, rows, hv, ctypes.byref(b)),
-            "delta_chunk_workspace")
+    dt = N.DT_F32 if dtype is None else _dtypes().get(dtype)
+    if dt is None:
+        raise ValueError(f"dtype: float32, bfloat16, float16 or int16, not {dtype}")
+    N.check(N.lib().w4a8_delta_chunk_workspace(
+        ctx.h, tokens, rows, hv if hk is None else hk, hv, dk, dt, ctypes.byref(b)),
+        "delta_chunk_workspace")
     return _workspace(ctx, b.value)

@@ -130,10 +130,18 @@ def delta(**kw):
 def check_delta():
     step, chunk = lib.w4a8_delta_step_async, lib.w4a8_delta_chunk_async
     b = I64()
-    assert lib.w4a8_delta_chunk_workspace(ctx, I64(1000), I64(3), I64(4), ctypes.byref(b)) == OK
-    refused(lib.w4a8_delta_chunk_workspace, ctx, I64(-1), I64(3), I64(4), ctypes.byref(b))
-    refused(lib.w4a8_delta_chunk_workspace, ctx, I64(1), I64(3), I64(0), ctypes.byref(b))
-    refused(lib.w4a8_delta_chunk_workspace, ctx, I64(1), I64(3), I64(4), None)
+
+    def space(tokens=3, rows=3, hk=2, hv=4, dk=128, dtype=BF16, to=b):
+        return lib.w4a8_delta_chunk_workspace(ctx, I64(tokens), I64(rows), I64(hk), I64(hv),
+                                              I64(dk), dtype, None if to is None else ctypes.byref(to))
+    sizes = []
+    for dtype in (BF16, F16, F32):
+        assert space(dtype=dtype) == OK
+        sizes.append(b.value)
+    assert 0 < sizes[0] < sizes[1] < sizes[2]
+    for kw in (dict(tokens=-1), dict(rows=-1), dict(hk=0), dict(hv=1), dict(hv=1 << 16),
+               dict(dk=32), dict(dtype=4), dict(to=None), dict(tokens=1 << 31)):
+        refused(lambda kw=kw: space(**kw))
     for f in (step, chunk):
         assert f(ctx, ctypes.byref(delta())) == OK
         refused(f, ctx, None)
@@ -149,11 +157,11 @@ def check_delta():
             refused(f, ctx, ctypes.byref(delta(**kw)))
     refused(step, ctx, ctypes.byref(delta(tokens=4)))
     refused(chunk, ctx, ctypes.byref(delta(cu=None)))
-    need = I64()
-    assert lib.w4a8_delta_chunk_workspace(ctx, I64(3), I64(3), I64(4), ctypes.byref(need)) == OK
-    if need.value:
-        refused(chunk, ctx, ctypes.byref(delta(ws=None)))
-        refused(chunk, ctx, ctypes.byref(delta(ws_bytes=need.value - 1)))
+    refused(chunk, ctx, ctypes.byref(delta(ws=None)))
+    refused(chunk, ctx, ctypes.byref(delta(ws=ODD.value)))
+    for dtype, need in zip((BF16, F16, F32), sizes):
+        assert chunk(ctx, ctypes.byref(delta(dtype=dtype, ws_bytes=need))) == OK
+        refused(chunk, ctx, ctypes.byref(delta(dtype=dtype, ws_bytes=need - 1)))
 
 
 def check_launches():

@@ -273,18 +273,13 @@ def test_bad_slots_are_reported(engine, kind, slots):
 def test_bad_bounds_are_reported(engine, cu):
     gen = torch.Generator().manual_seed(27)
     d = inputs(gen, 100, 1, 1, 64, 16, torch.float32, 3)
-    spans = [(a, b) if 0 <= a <= b <= 100 else (0, 0) for a, b in zip(cu[:-1], cu[1:])]
-    want = recurrence(d, spans, [0, 1, 2])
+    state = d["state"].clone()
     out, ws, c = torch.ones_like(d["v"]), engine.delta_chunk_workspace(100, 3, 1), ints(cu)
     torch.cuda.synchronize()
     engine.delta_chunk_async(**d, out=out, cu=c, ws=ws)
     with pytest.raises(AssertionError, match="bounds"):
         engine.sync()
-    assert not torch.isnan(out).any()
-    # a row whose own bounds are in order is run, unless others overlap it
-    if cu == [0, 30, 60, 120]:
-        want[0][60:] = 1
-        check(out, d["state"], want)
+    assert (out == 1).all() and torch.equal(d["state"], state)   # nothing was run
 
 
 def test_captured_step_replays(engine):
