@@ -126,9 +126,8 @@ __global__ __launch_bounds__(256) void delta_step_kernel(Delta p) {
 // prompt; a norm of q or k is a factor of its row, applied to the sums.
 // A token that holds an infinity or a NaN spoils its whole chunk.
 constexpr int C = 64;
-constexpr int kPlane = 64 * 8;                   // bfloat16 of one operand: 8 per lane
-constexpr int kTriBytes = 6 * 3 * kPlane * 2;    // M or P: operands of tri_of, three terms
-constexpr int kVecFloats = 256;                  // a, b, c of 64 tokens, e^(G_C)
+constexpr int kTriBytes = 6 * 3 * 64 * 16;       // M or P: operands of tri_of, three terms
+constexpr int kVecFloats = 256;                  // a, b, c of 64 tokens, e^(G_C) 64 times
 constexpr int kChunkBytes = 2 * kTriBytes + kVecFloats * 4;
 constexpr float kNoDecay = -200.f;               // e^g is 0 in float32 from here on down
 
@@ -148,16 +147,22 @@ __device__ __forceinline__ f32x4 mfma4(f32x4 a, f32x4 b, f32x4 c) {   // 16 x 16
   for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
   return c;
 }
-// sum of the products of terms a[i] b[j] with i + j <= 2
-template <int NA, int NB>
+template <int N>
+struct Int {
+  static constexpr int value = N;
+};
+// sum of the products of terms a[i] b[j] with i + j <= L
+template <int NA, int NB, int L>
 __device__ __forceinline__ f32x4 mfma_terms(const bf16x8 *a, const bf16x8 *b, f32x4 c) {
 #pragma unroll
   for (int i = NA - 1; i >= 0; --i)
 #pragma unroll
     for (int j = NB - 1; j >= 0; --j)
-      if (i + j <= 2) c = mfma(a[i], b[j], c);
+      if (i + j <= L) c = mfma(a[i], b[j], c);
   return c;
 }
+
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // x as a sum of N bfloat16 values
 template <int N>
@@ -229,15 +234,16 @@ __host__ __device__ inline Planes planes_of(const Delta &p) {
                 term};
 }
 
-// A workgroup per chunk and key head.
+// A workgroup per chunk and key head.  Tiles of M and P are made transposed
+// (rows j, columns t), which leaves a lane with four neighbouring slots of the
+// operand that delta_scan_kernel reads: nothing is rearranged.
 template <int DK, typename T>
 __global__ __launch_bounds__(256) void delta_prep_kernel(Delta p) {
   constexpr int NK = Terms<T>::n, NS = DK / 32, LD = 68;
-  __shared__ double Gs[C];
-  __shared__ float rks[C], rqs[C], betas[C];
-  __shared__ __align__(16) float As[C * LD];
-  __shared__ __align__(16) float Ts[4][16 * 20];
-  __shared__ __align__(16) __bf16 planes[2][6 * 3 * kPlane];
+  __shared__ double Gs[C];                         // log2(e) times the running sum of g
+  __shared__ __align__(16) float rks[C], rqs[C], betas[C];
+  __shared__ __align__(16) float At[C * LD];       // A transposed
+  __shared__ __align__(16) float Tt[4][16 * 20];   // its diagonal blocks' inverses, transposed
   const int slot = blockIdx.x, hk = blockIdx.y;
   int row;
   if (!bounds_ok(p, slot, &row)) {
@@ -249,10 +255,6 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Delta p) {
   const int t0 = p.cu[row] + chunk * C, len = min(C, p.cu[row + 1] - t0);
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-
-  // tiles above the diagonal that share a k-step with one below stay zeros
-  for (int i = threadIdx.x; i < 2 * kTriBytes / 16; i += 256)
-    ((u32x4 *)planes)[i] = u32x4{0, 0, 0, 0};
 
   // rows 16 tile + r of x, elements 32 s + 8 g .., as terms; their squares' sum
   auto load = [&](const void *x, int64_t token, int64_t head, int tile, bf16x8 (*f)[NK],
@@ -304,41 +306,50 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Delta p) {
         }
     }
   }
-  // k_t . k_j and q_t . k_j, t = 16 w + 4 g + i, j = 16 c + r, up to the diagonal
-  f32x4 kk[4], qk[4];
+  // k_j . k_t and k_j . q_t, j = 16 c + 4 g + i, t = 16 w + r, up to the diagonal
+  f32x4 kk[4], kq[4];
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    kk[c] = qk[c] = f32x4{0, 0, 0, 0};
+    kk[c] = kq[c] = f32x4{0, 0, 0, 0};
     if (c <= w) {
       bf16x8 kc[NS][NK];
       load(p.k, p.k_token, p.k_head, c, kc, nullptr);
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        kk[c] = mfma_terms<NK, NK>(kw[s], kc[s], kk[c]);
-        qk[c] = mfma_terms<NK, NK>(qw[s], kc[s], qk[c]);
+        kk[c] = mfma_terms<NK, NK, 2>(kc[s], kw[s], kk[c]);
+        kq[c] = mfma_terms<NK, NK, 2>(kc[s], qw[s], kq[c]);
       }
     }
   }
-  // an element of M or P, row 16 tile + m, column 16 c + col
-  auto put = [&](int which, int tile, int c, int m, int col, float x) {
-    __bf16 h[3];
-    split<3>(x, h);
-    __bf16 *o = planes[which] + tri_of(tile, c >> 1) * 3 * kPlane + (m + 16 * (col >> 2)) * 8 +
-                4 * (c & 1) + (col & 3);
+  // row tile w of M (which 0) or P out of its transposed tiles X[c], c <= w
+  auto store = [&](uint8_t *ws, int which, const f32x4 *X) {
+    bf16x8 *out = (bf16x8 *)(ws + which * kTriBytes) + lane;
 #pragma unroll
-    for (int i = 0; i < 3; ++i) o[i * kPlane] = h[i];
+    for (int s = 0; s < 2; ++s)
+      if (s <= w >> 1) {
+        bf16x8 t[3];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          __bf16 h[3];
+          split<3>(X[2 * s + (j >> 2)][j & 3], h);
+#pragma unroll
+          for (int i = 0; i < 3; ++i) t[i][j] = h[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 3; ++i) out[(tri_of(w, s) * 3 + i) * 64] = t[i];
+      }
   };
 
   const int per = p.hv / p.hk;
   for (int h = hk * per; h < (hk + 1) * per; ++h) {
     uint8_t *ws = (uint8_t *)p.ws + ((int64_t)slot * p.hv + h) * kChunkBytes;
-    __syncthreads();                 // rks, rqs; the last head's planes are out
+    __syncthreads();                 // rks, rqs; the last head's Gs, betas, At, Tt are read
     if (w == 0) {
       const bool on = lane < len;
       const int64_t t = t0 + min(lane, len - 1);
       const float gt = on ? fmaxf(p.g[t * p.g_token + h], kNoDecay) : 0.f;
       const float bt = on ? p.beta[t * p.beta_token + h] : 0.f;
-      double G = gt;
+      double G = gt * 1.4426950408889634;
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) {
         const double y = __shfl_up(G, d);
@@ -348,140 +359,97 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Delta p) {
       betas[lane] = bt;
       const double GC = __shfl(G, 63);
       float *vec = (float *)(ws + 2 * kTriBytes);
-      vec[lane] = on ? expf((float)G) * rks[lane] : 0.f;
-      vec[64 + lane] = on ? expf((float)G) * rqs[lane] : 0.f;
-      vec[128 + lane] = on ? expf((float)(GC - G)) * rks[lane] : 0.f;
-      if (lane == 0) vec[192] = expf((float)GC);
+      vec[lane] = on ? exp2_of((float)G) * rks[lane] : 0.f;
+      vec[64 + lane] = on ? exp2_of((float)G) * rqs[lane] : 0.f;
+      vec[128 + lane] = on ? exp2_of((float)(GC - G)) * rks[lane] : 0.f;
+      vec[192 + lane] = exp2_of((float)GC);
     }
     __syncthreads();
+    {
+      const int t = 16 * w + r;
+      const double Gt = Gs[t];
+      const float rqt = rqs[t], bt = betas[t] * rks[t];
+      f32x4 P[4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (c <= w) {
-        const int j = 16 * c + r;
-        const double Gj = Gs[j];
-        const float rkj = rks[j];
+      for (int c = 0; c < 4; ++c) {
+        P[c] = f32x4{0, 0, 0, 0};
+        if (c <= w) {
+          const f32x4 rkj = *(const f32x4 *)(rks + 16 * c + 4 * g);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int t = 16 * w + 4 * g + i;
-          const float dec = j <= t ? expf((float)(Gs[t] - Gj)) * rkj : 0.f;
-          As[t * LD + j] = j < t ? betas[t] * rks[t] * dec * kk[c][i] : 0.f;
-          put(1, w, c, 4 * g + i, r, j <= t ? rqs[t] * dec * qk[c][i] : 0.f);
+          for (int i = 0; i < 4; ++i) {
+            const int j = 16 * c + 4 * g + i;
+            const float dec = exp2_of((float)(Gt - Gs[j])) * rkj[i];
+            At[j * LD + t] = j < t ? bt * dec * kk[c][i] : 0.f;
+            P[c][i] = j <= t ? rqt * dec * kq[c][i] : 0.f;
+          }
         }
       }
+      store(ws, 1, P);
+    }
     __syncthreads();
-    {   // the inverse of diagonal block w, column r by substitution
+    {   // the inverse of diagonal block w: lane r column r, by substitution
       float x[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float y = i == r ? 1.f : 0.f;
+      for (int i = 0; i < 16; ++i) x[i] = i == r ? 1.f : 0.f;
 #pragma unroll
-        for (int j = 0; j < i; ++j) y -= As[(16 * w + i) * LD + 16 * w + j] * x[j];
-        x[i] = y;
-        if (g == 0) Ts[w][i * 20 + r] = y;
+      for (int j = 0; j < 15; ++j) {
+        const float *a = At + (16 * w + j) * LD + 16 * w;
+#pragma unroll
+        for (int i = j + 1; i < 16; ++i) x[i] -= a[i] * x[j];
       }
+      if (g == 0)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          *(f32x4 *)(Tt[w] + r * 20 + i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
     }
     __syncthreads();
-    {   // block column w of the inverse: X_i = -T_ii sum_k A_ik X_k
+    {   // block row w of the inverse T, transposed: with T (I + A) = I,
+        // T_wc^T = -T_cc^T sum_(c < k <= w) A_kc^T T_wk^T
       f32x4 X[4];
-      const float bj = betas[16 * w + r];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        X[i] = f32x4{0, 0, 0, 0};
-        if (i == w) {
+      for (int c = 3; c >= 0; --c) {
+        X[c] = f32x4{0, 0, 0, 0};
+        if (c == w) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) X[i][k] = Ts[w][(4 * g + k) * 20 + r];
-        } else if (i > w) {
+          for (int i = 0; i < 4; ++i) X[c][i] = Tt[c][(4 * g + i) * 20 + r];
+        } else if (c < w) {
           f32x4 acc{0, 0, 0, 0};
 #pragma unroll
-          for (int k = 0; k < i; ++k)
-            if (k >= w)
-              acc = mfma4(*(const f32x4 *)(As + (16 * i + r) * LD + 16 * k + 4 * g), X[k], acc);
-          X[i] = mfma4(-*(const f32x4 *)(Ts[i] + r * 20 + 4 * g), acc, X[i]);
+          for (int k = c + 1; k < 4; ++k)
+            if (k <= w)
+              acc = mfma4(*(const f32x4 *)(At + (16 * c + r) * LD + 16 * k + 4 * g), X[k], acc);
+          X[c] = mfma4(-*(const f32x4 *)(Tt[c] + r * 20 + 4 * g), acc, X[c]);
         }
-        if (i >= w)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) put(0, i, w, 4 * g + k, r, X[i][k] * bj);
       }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) X[c] *= *(const f32x4 *)(betas + 16 * c + 4 * g);
+      store(ws, 0, X);
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 2 * kTriBytes / 16; i += 256)
-      ((u32x4 *)ws)[i] = ((const u32x4 *)planes)[i];
   }
 }
 
-// What a wavefront needs of one chunk, loaded a chunk ahead: its 16 tokens'
-// rows of K and Q, 32 columns of K of every token, its tokens' 16 values, its
-// row tile of M and P, and the factors of its tokens.
+// A workgroup per row, value head and 16 columns of the state, eight
+// wavefronts on 16 tokens each: the chain of a chunk, S0 -> V - a K S0 -> U ->
+// S, on four of them and the outputs, b Q S0 + P U, on the other four, so that
+// the chain's trips through LDS are filled with the outputs' products.  Where
+// there is one row, a chunk's chain and the instructions issued along it are
+// what bounds the kernel.  So every operand of the next chunk is loaded right
+// after this chunk's use of it, spread over the step, by offsets from the
+// chunk's first token that are the same in every whole chunk.
+//
+// Wavefront w of the chain has rows 32 w .. of the state too: lane (r, g) rows
+// 32 w + 8 g + e of column r, in register [e & 1][e >> 1], which is its slots
+// of the state as an operand; its results of U are slots of that operand
+// likewise (token_of).
+//
+// Outputs are rounded to 16 bits (bfloat16, float16): two terms of their
+// operands, an error of 2^-17, are enough for them.
 template <int DK, typename T>
-struct ChunkData {
-  static constexpr int NK = Terms<T>::n, NS = DK / 32;
-  bf16x8 k[NS][NK], q[NS][NK];
-  uint32_t kt[2][8][NK];
-  T v[4];
-  bf16x8 m[2][3], pp[2][3];
-  f32x4 a, b, c;
-  float fall;
-  int t0, len;
-};
-
-template <int DK, typename T>
-__device__ __forceinline__ void load_chunk(const Delta &p, const Planes &pl, int t0, int len,
-                                           int64_t slot, int h, int hk, int col, int w, int lane,
-                                           ChunkData<DK, T> &d) {
+__global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
   constexpr int NK = Terms<T>::n, NS = DK / 32;
-  const int r = lane & 15, g = lane >> 4;
-  d.t0 = t0;
-  d.len = len;
-  const uint8_t *ws = (const uint8_t *)p.ws + (slot * p.hv + h) * kChunkBytes;
-  const bf16x8 *tri = (const bf16x8 *)ws + lane;
-  const int64_t row = t0 + min(16 * w + r, len - 1);
-  const __bf16 *k = pl.k + row * pl.k_token + hk * pl.k_head + 8 * g;
-  const __bf16 *q = pl.q + row * pl.q_token + hk * pl.q_head + 8 * g;
-#pragma unroll
-  for (int s = 0; s < NS; ++s)
-#pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      d.k[s][i] = *(const bf16x8 *)(k + i * pl.term + 32 * s);
-      d.q[s][i] = *(const bf16x8 *)(q + i * pl.term + 32 * s);
-    }
-  const T *v = (const T *)p.v + h * p.v_head + col;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) d.v[i] = v[(t0 + min(16 * w + 4 * g + i, len - 1)) * p.v_token];
-#pragma unroll
-  for (int s = 0; s < 2; ++s)
-    if (s <= w >> 1)
-#pragma unroll
-      for (int i = 0; i < 3; ++i) {
-        d.m[s][i] = tri[(tri_of(w, s) * 3 + i) * 64];
-        d.pp[s][i] = tri[(6 * 3 + tri_of(w, s) * 3 + i) * 64];
-      }
-  if (w < NS) {
-    const __bf16 *kt = pl.k + hk * pl.k_head + 32 * w + 2 * r;
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int64_t t = t0 + min(token_of(s, g, j), len - 1);
-#pragma unroll
-        for (int i = 0; i < NK; ++i)
-          d.kt[s][j][i] = *(const uint32_t *)(kt + t * pl.k_token + i * pl.term);
-      }
-  }
-  const float *vec = (const float *)(ws + 2 * kTriBytes);
-  d.a = *(const f32x4 *)(vec + 16 * w + 4 * g);
-  d.b = *(const f32x4 *)(vec + 64 + 16 * w + 4 * g);
-  d.c = *(const f32x4 *)(vec + 128 + 16 * w + 4 * g);
-  d.fall = vec[192];
-}
-
-// A workgroup per row, value head and 16 columns; wavefront w has tokens
-// 16 w .. of a chunk, and rows 32 w .. of the state: lane (r, g) of it rows
-// 32 w + 8 g + e of column r, in register [e & 1][e >> 1].
-template <int DK, typename T>
-__global__ __launch_bounds__(256, 1) void delta_scan_kernel(Delta p) {
-  constexpr int NK = Terms<T>::n, NS = DK / 32;
+  constexpr int OT = __is_same(T, __bf16) || __is_same(T, _Float16) ? 2 : 3;
   __shared__ bf16x8 Sb[3][NS][64];                // the state, k-step s by wavefront s
-  __shared__ __align__(16) bf16x4 Rb[3][2][64][2], Ub[3][2][64][2], Wb[3][2][64][2];
+  __shared__ __align__(16) bf16x4 Rb[3][2][64][2], Ub[OT][2][64][2], Wb[3][2][64][2];
   const int tiles = p.dv / 16, units = p.rows * p.hv, each = (units + 7) / 8;
   // a head's columns, and heads that share keys, on one XCD (workgroups go
   // round the eight of them)
@@ -493,143 +461,289 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(Delta p) {
   if (!bounds_ok(p, -1, &dummy)) return;          // reported by delta_prep_kernel
   const int slot = slot_of(p, row, h == 0 && at % tiles == 0);
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
   const int col = (at % tiles) * 16 + r;
   const int begin = p.cu[row], end = p.cu[row + 1];
-  T *out = (T *)p.out + h * p.out_head + col;
   if (slot < 0) {
-    for (int t = begin + (int)(threadIdx.x >> 4); t < end; t += 16) out[t * p.out_token] = (T)0;
+    T *out = (T *)p.out + h * p.out_head + col;
+    for (int t = begin + (int)(threadIdx.x >> 4); t < end; t += 32) out[t * p.out_token] = (T)0;
     return;
   }
-  float *state = p.state + (((int64_t)slot * p.hv + h) * DK + 32 * w + 8 * g) * p.dv + col;
-  f32x4 S[2];
-#pragma unroll
-  for (int e = 0; e < 2; ++e)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      S[e][i] = p.fresh || w >= NS ? 0.f : state[(int64_t)(2 * i + e) * p.dv];
-  auto put_state = [&]() {
-    if (w >= NS) return;
-    bf16x8 t[3];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      __bf16 x[3];
-      split<3>(S[j & 1][j >> 1], x);
-#pragma unroll
-      for (int i = 0; i < 3; ++i) t[i][j] = x[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 3; ++i) Sb[i][w][lane] = t[i];
-  };
-  auto put_rows = [&](bf16x4 (*b)[2][64][2], f32x4 x) {
-    bf16x4 t[3];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      __bf16 y[3];
-      split<3>(x[j], y);
-#pragma unroll
-      for (int i = 0; i < 3; ++i) t[i][j] = y[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 3; ++i) b[i][w >> 1][lane][w & 1] = t[i];
-  };
-  const Planes pl = planes_of<T>(p);
-  const int64_t slot0 = first_chunk(p, row);
   const int n = (end - begin + C - 1) / C;
-  typedef ChunkData<DK, T> Data;
-  auto load = [&](int c, Data &d) {
-    if (c < n)
-      load_chunk<DK, T>(p, pl, begin + c * C, min(C, end - begin - c * C), slot0 + c, h, hk, col,
-                        w, lane, d);
+  const Planes pl = planes_of<T>(p);
+  // of the chunk whose operands are loaded next
+  const int64_t first = first_chunk(p, row);
+  const uint8_t *ws = (const uint8_t *)p.ws + (first * p.hv + h) * kChunkBytes;
+  const int64_t ws_step = (int64_t)p.hv * kChunkBytes;
+  // row tile w of M (which 0) or P, terms i of k-step s
+  auto tri = [&](int which, int s, int i) -> const bf16x8 & {
+    return ((const bf16x8 *)(ws + which * kTriBytes) + (tri_of(w, s) * 3 + i) * 64)[lane];
   };
-  auto step = [&](const Data &d) {
-    f32x4 ks{0, 0, 0, 0}, qs{0, 0, 0, 0};
-    {
-      bf16x8 sb[NS][3];
+  // a, b or c of tokens 16 w + 4 g ..
+  auto factor = [&](int which) {
+    return *(const f32x4 *)((const float *)(ws + 2 * kTriBytes) + 64 * which + 16 * w + 4 * g);
+  };
+  // where the operands of a chunk of len tokens lie, in bytes from its first
+  // token; past its end the last token's are read, whose factors and columns
+  // of M and P are zeros
+  auto row_at = [&](int t, int len, int64_t token, int e, int size) {
+    return (uint32_t)(min(t, len - 1) * (int)token + e) * (uint32_t)size;
+  };
+
+  auto chain = [&](auto upper) {
+    constexpr bool HI = upper.value;              // w >= 2: two k-steps of M
+    constexpr bool STATE = NS == 4 || !HI;        // rows of the state
+    float *state = p.state + (((int64_t)slot * p.hv + h) * DK + 32 * w + 8 * g) * p.dv + col;
+    f32x4 S[2];
+    if constexpr (STATE) {
 #pragma unroll
-      for (int s = 0; s < NS; ++s)
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int i = 0; i < 3; ++i) sb[s][i] = Sb[i][s][lane];
-#pragma unroll
-      for (int s = 0; s < NS; ++s) ks = mfma_terms<NK, 3>(d.k[s], sb[s], ks);
-#pragma unroll
-      for (int s = 0; s < NS; ++s) qs = mfma_terms<NK, 3>(d.q[s], sb[s], qs);
+        for (int i = 0; i < 4; ++i) S[e][i] = p.fresh ? 0.f : state[(int64_t)(2 * i + e) * p.dv];
     }
-    f32x4 x;
+    auto put_state = [&]() {
+      bf16x8 t[3];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        __bf16 x[3];
+        split<3>(S[j & 1][j >> 1], x);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) t[i][j] = x[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 3; ++i) Sb[i][w][lane] = t[i];
+    };
+    auto put_rows = [&](bf16x4 (*b)[2][64][2], f32x4 x, auto terms) {
+      bf16x4 t[3];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        __bf16 y[3];
+        split<terms.value>(x[j], y);
+#pragma unroll
+        for (int i = 0; i < terms.value; ++i) t[i][j] = y[i];
+      }
+#pragma unroll
+      for (int i = 0; i < terms.value; ++i) b[i][w >> 1][lane][w & 1] = t[i];
+    };
+    const uint8_t *kb = (const uint8_t *)(pl.k + begin * pl.k_token + hk * pl.k_head);
+    const uint8_t *vb = (const uint8_t *)((const T *)p.v + begin * p.v_token + h * p.v_head);
+    const int64_t k_step = pl.k_token * C * 2, v_step = p.v_token * C * (int)sizeof(T);
+    uint32_t k_at, v_at[4], kt_at[2][8];
+    auto offsets = [&](int len) {
+      k_at = row_at(16 * w + r, len, pl.k_token, 8 * g, 2);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v_at[i] = row_at(16 * w + 4 * g + i, len, p.v_token, col, sizeof(T));
+      if constexpr (STATE)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            kt_at[s][j] = row_at(token_of(s, g, j), len, pl.k_token, 32 * w + 2 * r, 2);
+    };
+    bf16x8 k[NS][NK], m[2][3];
+    uint32_t kt[2][8][NK];
+    T v[4];
+    f32x4 a, c;
+    float fall;
+    auto load_rows = [&]() {
+#pragma unroll
+      for (int i = 0; i < NK; ++i)
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+          k[s][i] = *(const bf16x8 *)(kb + 2 * i * pl.term + 64 * s + k_at);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = *(const T *)(vb + v_at[i]);
+      a = factor(0);
+    };
+    auto load_solve = [&]() {
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        m[0][i] = tri(0, 0, i);
+        if constexpr (HI) m[1][i] = tri(0, 1, i);
+      }
+      c = factor(2);
+    };
+    auto load_update = [&]() {
+      if constexpr (STATE) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int i = 0; i < NK; ++i)
+              kt[s][j][i] = *(const uint32_t *)(kb + 2 * i * pl.term + kt_at[s][j]);
+        fall = ((const float *)(ws + 2 * kTriBytes) + 192)[lane];
+      }
+    };
+    offsets(min(C, end - begin));
+    if (n > 0) {
+      load_rows();
+      load_solve();
+      load_update();
+      if constexpr (STATE) put_state();
+    }
+    lds_barrier();
+    for (int ch = 0; ch < n; ++ch) {
+      const int len = min(C, end - begin - ch * C);
+      if (ch + 1 < n) {
+        kb += k_step;
+        vb += v_step;
+        ws += ws_step;
+        if (len < 2 * C && end - begin - (ch + 1) * C < C) offsets(end - begin - (ch + 1) * C);
+      }
+      {
+        bf16x8 sb[NS][3];
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int i = 0; i < 3; ++i) sb[s][i] = Sb[i][s][lane];
+        f32x4 ks{0, 0, 0, 0}, x;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) ks = mfma_terms<NK, 3, 2>(k[s], sb[s], ks);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          x[i] = (16 * w + 4 * g + i < len ? to_float(v[i], p.unit) : 0.f) - a[i] * ks[i];
+        put_rows(Rb, x, Int<3>());
+      }
+      load_rows();
+      lds_barrier();
+      {
+        bf16x8 b[2][3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          b[0][i] = *(const bf16x8 *)Rb[i][0][lane];
+          if constexpr (HI) b[1][i] = *(const bf16x8 *)Rb[i][1][lane];
+        }
+        f32x4 u = mfma_terms<3, 3, 2>(m[0], b[0], f32x4{0, 0, 0, 0});
+        if constexpr (HI) u = mfma_terms<3, 3, 2>(m[1], b[1], u);
+        put_rows(Wb, u * c, Int<3>());
+        put_rows(Ub, u, Int<OT>());
+      }
+      load_solve();
+      lds_barrier();
+      if constexpr (STATE) {
+        bf16x8 b[2][3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          b[0][i] = *(const bf16x8 *)Wb[i][0][lane];
+          b[1][i] = *(const bf16x8 *)Wb[i][1][lane];
+        }
+        S[0] *= fall;
+        S[1] *= fall;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          bf16x8 x[2][NK];
+#pragma unroll
+          for (int i = 0; i < NK; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              u32x4 y;
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                y[j] = __builtin_amdgcn_perm(kt[s][2 * j + 1][i], kt[s][2 * j][i],
+                                             e ? 0x07060302u : 0x05040100u);
+              x[e][i] = __builtin_bit_cast(bf16x8, y);
+            }
+          S[0] = mfma_terms<NK, 3, 2>(x[0], b[s], S[0]);
+          S[1] = mfma_terms<NK, 3, 2>(x[1], b[s], S[1]);
+        }
+        put_state();
+        load_update();
+      }
+      lds_barrier();
+    }
+    if constexpr (STATE)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) state[(int64_t)(2 * i + e) * p.dv] = S[e][i];
+  };
+
+  auto output = [&](auto upper) {
+    constexpr bool HI = upper.value;
+    const uint8_t *qb = (const uint8_t *)(pl.q + begin * pl.q_token + hk * pl.q_head);
+    uint8_t *ob = (uint8_t *)((T *)p.out + begin * p.out_token + h * p.out_head);
+    const int64_t q_step = pl.q_token * C * 2, o_step = p.out_token * C * (int)sizeof(T);
+    uint32_t q_at, o_at[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      x[i] = (16 * w + 4 * g + i < d.len ? to_float(d.v[i], p.unit) : 0.f) - d.a[i] * ks[i];
-    put_rows(Rb, x);
-    lds_barrier();
-    f32x4 u{0, 0, 0, 0};
+      o_at[i] = row_at(16 * w + 4 * g + i, C, p.out_token, col, sizeof(T));
+    bf16x8 q[NS][NK], m[2][OT];
+    f32x4 b;
+    auto load_rows = [&]() {
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
-      if (s <= w >> 1) {
-        bf16x8 b[3];
+      for (int i = 0; i < NK; ++i)
 #pragma unroll
-        for (int i = 0; i < 3; ++i) b[i] = *(const bf16x8 *)Rb[i][s][lane];
-        u = mfma_terms<3, 3>(d.m[s], b, u);
+        for (int s = 0; s < NS; ++s)
+          q[s][i] = *(const bf16x8 *)(qb + 2 * i * pl.term + 64 * s + q_at);
+    };
+    auto load_weights = [&]() {
+#pragma unroll
+      for (int i = 0; i < OT; ++i) {
+        m[0][i] = tri(1, 0, i);
+        if constexpr (HI) m[1][i] = tri(1, 1, i);
       }
-    put_rows(Ub, u);
-    put_rows(Wb, u * d.c);
-    lds_barrier();
-    if (w < NS) {
-      S[0] *= d.fall;
-      S[1] *= d.fall;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        bf16x8 b[3], a[2][NK];
-#pragma unroll
-        for (int i = 0; i < 3; ++i) b[i] = *(const bf16x8 *)Wb[i][s][lane];
-#pragma unroll
-        for (int i = 0; i < NK; ++i)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            u32x4 y;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              y[j] = __builtin_amdgcn_perm(d.kt[s][2 * j + 1][i], d.kt[s][2 * j][i],
-                                           e ? 0x07060302u : 0x05040100u);
-            a[e][i] = __builtin_bit_cast(bf16x8, y);
-          }
-        S[0] = mfma_terms<NK, 3>(a[0], b, S[0]);
-        S[1] = mfma_terms<NK, 3>(a[1], b, S[1]);
-      }
-      put_state();
+      b = factor(1);
+    };
+    q_at = row_at(16 * w + r, min(C, end - begin), pl.q_token, 8 * g, 2);
+    if (n > 0) {
+      load_rows();
+      load_weights();
     }
-    f32x4 o;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = d.b[i] * qs[i];
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-      if (s <= w >> 1) {
-        bf16x8 b[3];
-#pragma unroll
-        for (int i = 0; i < 3; ++i) b[i] = *(const bf16x8 *)Ub[i][s][lane];
-        o = mfma_terms<3, 3>(d.pp[s], b, o);
-      }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (16 * w + 4 * g + i < d.len)
-        out[(d.t0 + 16 * w + 4 * g + i) * p.out_token] = from_float<T>(o[i], p.out_unit);
     lds_barrier();
+    for (int ch = 0; ch < n; ++ch) {
+      const int len = min(C, end - begin - ch * C);
+      if (ch + 1 < n) {
+        qb += q_step;
+        ws += ws_step;
+        q_at = row_at(16 * w + r, min(C, end - begin - (ch + 1) * C), pl.q_token, 8 * g, 2);
+      }
+      f32x4 o{0, 0, 0, 0};
+      {
+        bf16x8 sb[NS][OT];
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int i = 0; i < OT; ++i) sb[s][i] = Sb[i][s][lane];
+#pragma unroll
+        for (int s = 0; s < NS; ++s) o = mfma_terms<NK, OT, OT - 1>(q[s], sb[s], o);
+        o *= b;
+      }
+      load_rows();
+      lds_barrier();
+      lds_barrier();
+      {
+        bf16x8 ub[2][OT];
+#pragma unroll
+        for (int i = 0; i < OT; ++i) {
+          ub[0][i] = *(const bf16x8 *)Ub[i][0][lane];
+          if constexpr (HI) ub[1][i] = *(const bf16x8 *)Ub[i][1][lane];
+        }
+        o = mfma_terms<OT, OT, OT - 1>(m[0], ub[0], o);
+        if constexpr (HI) o = mfma_terms<OT, OT, OT - 1>(m[1], ub[1], o);
+      }
+      load_weights();
+      if (len == C) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *(T *)(ob + o_at[i]) = from_float<T>(o[i], p.out_unit);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (16 * w + 4 * g + i < len) *(T *)(ob + o_at[i]) = from_float<T>(o[i], p.out_unit);
+      }
+      ob += o_step;
+      lds_barrier();
+    }
   };
-  Data d0, d1;
-  load(0, d0);
-  put_state();
-  lds_barrier();
-  for (int c = 0; c < n; c += 2) {
-    load(c + 1, d1);
-    step(d0);
-    if (c + 1 >= n) break;
-    load(c + 2, d0);
-    step(d1);
+  // the same number of barriers on every way
+  if (wave < 4) {
+    if (w < 2) chain(Int<0>());
+    else chain(Int<1>());
+  } else {
+    if (w < 2) output(Int<0>());
+    else output(Int<1>());
   }
-  if (w < NS)
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) state[(int64_t)(2 * i + e) * p.dv] = S[e][i];
 }
 
 template <int DK, typename T>
@@ -640,7 +754,7 @@ void launch_typed(const Delta &d, hipStream_t s) {
   }
   delta_prep_kernel<DK, T><<<dim3(d.tokens / C + d.rows, d.hk), 256, 0, s>>>(d);
   const int64_t each = ((int64_t)d.rows * d.hv + 7) / 8;
-  delta_scan_kernel<DK, T><<<(uint32_t)(8 * each * (d.dv / 16)), 256, 0, s>>>(d);
+  delta_scan_kernel<DK, T><<<(uint32_t)(8 * each * (d.dv / 16)), 512, 0, s>>>(d);
 }
 
 template <int DK>
