@@ -164,21 +164,40 @@ __device__ __forceinline__ f32x4 mfma_terms(const bf16x8 *a, const bf16x8 *b, f3
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// x as a sum of N bfloat16 values
-template <int N>
-__device__ __forceinline__ void split(float x, __bf16 *t) {
+// x[0 .. M) as a sum of N vectors of bfloat16, a pair of values per conversion
+// (whose result is kept as one word: taken apart, the compiler converts each
+// value again, 17 instructions a pair instead of 11)
+__device__ __forceinline__ uint32_t pair_of(float a, float b) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  uint32_t w = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
+  asm("" : "+v"(w));
+  return w;
+}
+template <int N, int M, typename V>
+__device__ __forceinline__ void split(const float *x, V *t) {
+  uint32_t w[N][M / 2];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    t[i] = (__bf16)x;
-    x -= (float)t[i];
+  for (int j = 0; j < M / 2; ++j) {
+    float a = x[2 * j], b = x[2 * j + 1];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      w[i][j] = pair_of(a, b);
+      a -= __builtin_bit_cast(float, w[i][j] << 16);
+      b -= __builtin_bit_cast(float, w[i][j] & 0xFFFF0000u);
+    }
   }
+#pragma unroll
+  for (int i = 0; i < N; ++i) __builtin_memcpy(&t[i], w[i], sizeof(V));
 }
 
-// Barrier of the workgroup for LDS alone: loads from memory stay in flight.
+// Barrier of the workgroup for LDS alone: loads from memory stay in flight,
+// and what waits for them is not moved up across it.
 __device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 // The order of a chunk's tokens in an operand of k-steps s = 0, 1: slot j of
@@ -268,15 +287,13 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Delta p) {
       T v[8];
       *(u32x4 *)v = *(const u32x4 *)(src + 32 * s);
       if constexpr (sizeof(T) == 4) *(u32x4 *)(v + 4) = *(const u32x4 *)(src + 32 * s + 4);
+      float y[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float y = on ? to_float(v[j], p.unit) : 0.f;
-        sum += y * y;
-        __bf16 h[NK];
-        split<NK>(y, h);
-#pragma unroll
-        for (int i = 0; i < NK; ++i) f[s][i][j] = h[i];
+        y[j] = on ? to_float(v[j], p.unit) : 0.f;
+        sum += y[j] * y[j];
       }
+      split<NK, 8>(y, f[s]);
     }
     if (squares) *squares = sum;
   };
@@ -328,13 +345,10 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Delta p) {
     for (int s = 0; s < 2; ++s)
       if (s <= w >> 1) {
         bf16x8 t[3];
+        float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          __bf16 h[3];
-          split<3>(X[2 * s + (j >> 2)][j & 3], h);
-#pragma unroll
-          for (int i = 0; i < 3; ++i) t[i][j] = h[i];
-        }
+        for (int j = 0; j < 8; ++j) x[j] = X[2 * s + (j >> 2)][j & 3];
+        split<3, 8>(x, t);
 #pragma unroll
         for (int i = 0; i < 3; ++i) out[(tri_of(w, s) * 3 + i) * 64] = t[i];
       }
@@ -470,6 +484,12 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
     return;
   }
   const int n = (end - begin + C - 1) / C;
+  if (n == 0) {                                   // no tokens: the state stays, or is cleared
+    float *state = p.state + ((int64_t)slot * p.hv + h) * DK * p.dv + col;
+    if (p.fresh)
+      for (int d = threadIdx.x >> 4; d < DK; d += 32) state[(int64_t)d * p.dv] = 0.f;
+    return;
+  }
   const Planes pl = planes_of<T>(p);
   // of the chunk whose operands are loaded next
   const int64_t first = first_chunk(p, row);
@@ -494,34 +514,26 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
     constexpr bool HI = upper.value;              // w >= 2: two k-steps of M
     constexpr bool STATE = NS == 4 || !HI;        // rows of the state
     float *state = p.state + (((int64_t)slot * p.hv + h) * DK + 32 * w + 8 * g) * p.dv + col;
-    f32x4 S[2];
-    if constexpr (STATE) {
+    f32x4 S[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    if (STATE && !p.fresh) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) S[e][i] = p.fresh ? 0.f : state[(int64_t)(2 * i + e) * p.dv];
+        for (int i = 0; i < 4; ++i) S[e][i] = state[(int64_t)(2 * i + e) * p.dv];
     }
     auto put_state = [&]() {
       bf16x8 t[3];
+      float x[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        __bf16 x[3];
-        split<3>(S[j & 1][j >> 1], x);
-#pragma unroll
-        for (int i = 0; i < 3; ++i) t[i][j] = x[i];
-      }
+      for (int j = 0; j < 8; ++j) x[j] = S[j & 1][j >> 1];
+      split<3, 8>(x, t);
 #pragma unroll
       for (int i = 0; i < 3; ++i) Sb[i][w][lane] = t[i];
     };
     auto put_rows = [&](bf16x4 (*b)[2][64][2], f32x4 x, auto terms) {
       bf16x4 t[3];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        __bf16 y[3];
-        split<terms.value>(x[j], y);
-#pragma unroll
-        for (int i = 0; i < terms.value; ++i) t[i][j] = y[i];
-      }
+      const float y[4] = {x[0], x[1], x[2], x[3]};
+      split<terms.value, 4>(y, t);
 #pragma unroll
       for (int i = 0; i < terms.value; ++i) b[i][w >> 1][lane][w & 1] = t[i];
     };
@@ -577,12 +589,14 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
       }
     };
     offsets(min(C, end - begin));
-    if (n > 0) {
-      load_rows();
-      load_solve();
-      load_update();
-      if constexpr (STATE) put_state();
-    }
+    if constexpr (STATE) put_state();
+    // in the loop's order, so that its waits are for what it uses
+    __builtin_amdgcn_sched_barrier(0);
+    load_rows();
+    __builtin_amdgcn_sched_barrier(0);
+    load_solve();
+    __builtin_amdgcn_sched_barrier(0);
+    load_update();
     lds_barrier();
     for (int ch = 0; ch < n; ++ch) {
       const int len = min(C, end - begin - ch * C);
@@ -687,10 +701,9 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
       b = factor(1);
     };
     q_at = row_at(16 * w + r, min(C, end - begin), pl.q_token, 8 * g, 2);
-    if (n > 0) {
-      load_rows();
-      load_weights();
-    }
+    load_rows();
+    __builtin_amdgcn_sched_barrier(0);
+    load_weights();
     lds_barrier();
     for (int ch = 0; ch < n; ++ch) {
       const int len = min(C, end - begin - ch * C);
