@@ -2044,9 +2044,8 @@ const char *delta_fault(const w4a8_delta *d, bool chunk) {
   if (chunk && !d->cu) return "cu is needed";
   if (d->rows * d->hv > (1 << 26)) return "more than 2^26 heads of states";
   // 32-bit offsets within a chunk's 64 tokens
-  if (chunk && (d->q_token > kDeltaStride || d->k_token > kDeltaStride ||
-                d->v_token > kDeltaStride || d->out_token > kDeltaStride))
-    return "token strides of q, k, v and out must be at most 2^23";
+  if (chunk && (d->v_token > kDeltaStride || d->out_token > kDeltaStride))
+    return "token strides of v and out must be at most 2^23";
   const int t = (int)d->dtype;
   if (!d->state || !aligned16(d->state)) return "state must be 16-byte aligned";
   if (d->tokens > 0) {

@@ -128,7 +128,9 @@ __global__ __launch_bounds__(256) void delta_step_kernel(Delta p) {
 constexpr int C = 64;
 constexpr int kTriBytes = 6 * 3 * 64 * 16;       // M or P: operands of tri_of, three terms
 constexpr int kVecFloats = 256;                  // a, b, c of 64 tokens, e^(G_C) 64 times
-constexpr int kChunkBytes = 2 * kTriBytes + kVecFloats * 4;
+constexpr int kHeadBytes = 2 * kTriBytes + kVecFloats * 4;   // of a chunk and value head
+// K, Q and K transposed of a chunk and key head, as operands
+constexpr int64_t rows_bytes(int64_t dk, int terms) { return 3 * C * dk * 2 * terms; }
 constexpr float kNoDecay = -200.f;               // e^g is 0 in float32 from here on down
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -235,32 +237,35 @@ __device__ __forceinline__ bool bounds_ok(const Delta &p, int slot, int *row) {
   return !bad;
 }
 
-// Planes of q and k as bfloat16 terms [term][token][key head][dk]; bfloat16
-// itself is read where it lies.
-struct Planes {
-  const __bf16 *k, *q;
-  int64_t k_token, q_token, k_head, q_head, term;   // elements
+// A chunk in the workspace: M, P and factors per value head, rows per key head;
+// the chunks of a head lie side by side.
+template <int DK, typename T>
+struct Space {
+  static constexpr int64_t kRows = rows_bytes(DK, Terms<T>::n);
+  uint8_t *ws;
+  int64_t chunks, chunk, heads;
+  __device__ Space(const Delta &p, int64_t c)
+      : ws((uint8_t *)p.ws), chunks(p.tokens / C + p.rows), chunk(c), heads(p.hv) {}
+  __device__ uint8_t *head(int h) const { return ws + (h * chunks + chunk) * kHeadBytes; }
+  // 0: K, 1: Q, 2: K transposed
+  __device__ bf16x8 *rows(int hk, int which) const {
+    return (bf16x8 *)(ws + heads * chunks * kHeadBytes + (hk * chunks + chunk) * kRows +
+                      which * (kRows / 3));
+  }
 };
-template <typename T>
-__host__ __device__ inline Planes planes_of(const Delta &p) {
-  if (Terms<T>::n == 1)
-    return Planes{(const __bf16 *)p.k, (const __bf16 *)p.q, p.k_token, p.q_token, p.k_head,
-                  p.q_head, 0};
-  const int64_t term = (int64_t)p.tokens * p.hk * p.dk;
-  const int64_t chunks = p.tokens / C + p.rows;
-  __bf16 *k = (__bf16 *)((uint8_t *)p.ws + chunks * p.hv * kChunkBytes);
-  return Planes{k, k + Terms<T>::n * term, (int64_t)p.hk * p.dk, (int64_t)p.hk * p.dk, p.dk, p.dk,
-                term};
-}
 
-// A workgroup per chunk and key head.  Tiles of M and P are made transposed
-// (rows j, columns t), which leaves a lane with four neighbouring slots of the
-// operand that delta_scan_kernel reads: nothing is rearranged.
+// A workgroup per chunk and key head.  It lays K, Q and K transposed out as
+// the operands that delta_scan_kernel reads, in whole lines (read where they
+// lie, rows of a prompt 4 KB apart all fall to one channel of the L2: 70 us of
+// the scan's 257 at 8192 tokens, 16 key heads of 128).  Tiles of M and P are
+// made transposed (rows j, columns t), which leaves a lane with four
+// neighbouring slots of their operand: nothing is rearranged.
 template <int DK, typename T>
 __global__ __launch_bounds__(256) void delta_prep_kernel(Delta p) {
-  constexpr int NK = Terms<T>::n, NS = DK / 32, LD = 68;
-  __shared__ double Gs[C];                         // log2(e) times the running sum of g
-  __shared__ __align__(16) float rks[C], rqs[C], betas[C];
+  constexpr int NK = Terms<T>::n, NS = DK / 32, LD = 68, HEADS = 4;
+  __shared__ bf16x8 Ks[4][NS][NK][64];             // K by row tiles, as operand
+  __shared__ double Gs[HEADS][C];                  // log2(e) times the running sum of g
+  __shared__ __align__(16) float betas[HEADS][C], rks[C], rqs[C];
   __shared__ __align__(16) float At[C * LD];       // A transposed
   __shared__ __align__(16) float Tt[4][16 * 20];   // its diagonal blocks' inverses, transposed
   const int slot = blockIdx.x, hk = blockIdx.y;
@@ -274,14 +279,18 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Delta p) {
   const int t0 = p.cu[row] + chunk * C, len = min(C, p.cu[row + 1] - t0);
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Space<DK, T> space(p, slot);
+  const int per = p.hv / p.hk;
 
-  // rows 16 tile + r of x, elements 32 s + 8 g .., as terms; their squares' sum
-  auto load = [&](const void *x, int64_t token, int64_t head, int tile, bf16x8 (*f)[NK],
-                  float *squares) {
-    const int t = 16 * tile + r;
+  // rows 16 w + r of x, elements 32 s + 8 g .., as terms (zeros past the
+  // chunk's end), written as operand; the sum of their squares
+  bf16x8 kw[NS][NK], qw[NS][NK];
+  auto load = [&](const void *x, int64_t token, int64_t head, bf16x8 (*f)[NK], int which) {
+    const int t = 16 * w + r;
     const bool on = t < len;
     const T *src = (const T *)x + (t0 + min(t, len - 1)) * token + hk * head + 8 * g;
     float sum = 0.f;
+    bf16x8 *out = space.rows(hk, which) + lane;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       T v[8];
@@ -294,49 +303,60 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Delta p) {
         sum += y[j] * y[j];
       }
       split<NK, 8>(y, f[s]);
+#pragma unroll
+      for (int i = 0; i < NK; ++i) out[((w * NS + s) * NK + i) * 64] = f[s][i];
     }
-    if (squares) *squares = sum;
+    sum += __shfl_xor(sum, 16);
+    return sum + __shfl_xor(sum, 32);
   };
-  bf16x8 kw[NS][NK], qw[NS][NK];
-  float kk2, qq2;
-  load(p.k, p.k_token, p.k_head, w, kw, &kk2);
-  load(p.q, p.q_token, p.q_head, w, qw, &qq2);
-  kk2 += __shfl_xor(kk2, 16);
-  kk2 += __shfl_xor(kk2, 32);
-  qq2 += __shfl_xor(qq2, 16);
-  qq2 += __shfl_xor(qq2, 32);
+  const float kk2 = load(p.k, p.k_token, p.k_head, kw, 0);
+  const float qq2 = load(p.q, p.q_token, p.q_head, qw, 1);
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+#pragma unroll
+    for (int i = 0; i < NK; ++i) Ks[w][s][i][lane] = kw[s][i];
   if (g == 0) {
     const bool on = 16 * w + r < len;
     rks[16 * w + r] = !on ? 0.f : p.norm ? 1.f / sqrtf(kk2 + p.eps) : 1.f;
     rqs[16 * w + r] = !on ? 0.f : (p.norm ? 1.f / sqrtf(qq2 + p.eps) : 1.f) * p.scale;
   }
-  if constexpr (NK > 1) {
-    const Planes pl = planes_of<T>(p);
-    if (16 * w + r < len) {
-      const int64_t at = (t0 + 16 * w + r) * pl.k_token + hk * pl.k_head + 8 * g;
-#pragma unroll
-      for (int s = 0; s < NS; ++s)
-#pragma unroll
-        for (int i = 0; i < NK; ++i) {
-          *(bf16x8 *)(const_cast<__bf16 *>(pl.k) + i * pl.term + at + 32 * s) = kw[s][i];
-          *(bf16x8 *)(const_cast<__bf16 *>(pl.q) + i * pl.term + at + 32 * s) = qw[s][i];
-        }
-    }
-  }
+  __syncthreads();
   // k_j . k_t and k_j . q_t, j = 16 c + 4 g + i, t = 16 w + r, up to the diagonal
   f32x4 kk[4], kq[4];
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     kk[c] = kq[c] = f32x4{0, 0, 0, 0};
-    if (c <= w) {
-      bf16x8 kc[NS][NK];
-      load(p.k, p.k_token, p.k_head, c, kc, nullptr);
+    if (c <= w)
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        kk[c] = mfma_terms<NK, NK, 2>(kc[s], kw[s], kk[c]);
-        kq[c] = mfma_terms<NK, NK, 2>(kc[s], qw[s], kq[c]);
+        bf16x8 kc[NK];
+#pragma unroll
+        for (int i = 0; i < NK; ++i) kc[i] = Ks[c][s][i][lane];
+        kk[c] = mfma_terms<NK, NK, 2>(kc, kw[s], kk[c]);
+        kq[c] = mfma_terms<NK, NK, 2>(kc, qw[s], kq[c]);
       }
-    }
+  }
+  if (w < NS) {   // rows d = 32 w + 2 r + e of K transposed: pairs of its columns
+    bf16x8 *out = space.rows(hk, 2) + lane;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < NK; ++i) {
+        uint32_t x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int t = token_of(s, g, j);
+          x[j] = ((const uint32_t *)&Ks[t >> 4][w][i][(t & 15) + 16 * (r >> 2)])[r & 3];
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          u32x4 y;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            y[j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], e ? 0x07060302u : 0x05040100u);
+          out[(((w * 2 + s) * 2 + e) * NK + i) * 64] = __builtin_bit_cast(bf16x8, y);
+        }
+      }
   }
   // row tile w of M (which 0) or P out of its transposed tiles X[c], c <= w
   auto store = [&](uint8_t *ws, int which, const f32x4 *X) {
@@ -354,11 +374,10 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Delta p) {
       }
   };
 
-  const int per = p.hv / p.hk;
-  for (int h = hk * per; h < (hk + 1) * per; ++h) {
-    uint8_t *ws = (uint8_t *)p.ws + ((int64_t)slot * p.hv + h) * kChunkBytes;
-    __syncthreads();                 // rks, rqs; the last head's Gs, betas, At, Tt are read
-    if (w == 0) {
+  for (int first = 0; first < per; first += HEADS) {
+    const int count = min(HEADS, per - first);
+    if (w < count) {   // a wavefront per head: its tokens' factors
+      const int h = hk * per + first + w;
       const bool on = lane < len;
       const int64_t t = t0 + min(lane, len - 1);
       const float gt = on ? fmaxf(p.g[t * p.g_token + h], kNoDecay) : 0.f;
@@ -369,76 +388,80 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Delta p) {
         const double y = __shfl_up(G, d);
         if (lane >= d) G += y;
       }
-      Gs[lane] = G;
-      betas[lane] = bt;
+      Gs[w][lane] = G;
+      betas[w][lane] = bt;
       const double GC = __shfl(G, 63);
-      float *vec = (float *)(ws + 2 * kTriBytes);
+      float *vec = (float *)(space.head(h) + 2 * kTriBytes);
       vec[lane] = on ? exp2_of((float)G) * rks[lane] : 0.f;
       vec[64 + lane] = on ? exp2_of((float)G) * rqs[lane] : 0.f;
       vec[128 + lane] = on ? exp2_of((float)(GC - G)) * rks[lane] : 0.f;
       vec[192 + lane] = exp2_of((float)GC);
     }
-    __syncthreads();
-    {
-      const int t = 16 * w + r;
-      const double Gt = Gs[t];
-      const float rqt = rqs[t], bt = betas[t] * rks[t];
-      f32x4 P[4];
+    for (int b = 0; b < count; ++b) {
+      uint8_t *ws = space.head(hk * per + first + b);
+      __syncthreads();               // Gs, betas; the last head's At, Tt are read
+      {
+        const int t = 16 * w + r;
+        const double Gt = Gs[b][t];
+        const float rqt = rqs[t], bt = betas[b][t] * rks[t];
+        f32x4 P[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        P[c] = f32x4{0, 0, 0, 0};
-        if (c <= w) {
-          const f32x4 rkj = *(const f32x4 *)(rks + 16 * c + 4 * g);
+        for (int c = 0; c < 4; ++c) {
+          P[c] = f32x4{0, 0, 0, 0};
+          if (c <= w) {
+            const f32x4 rkj = *(const f32x4 *)(rks + 16 * c + 4 * g);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int j = 16 * c + 4 * g + i;
-            const float dec = exp2_of((float)(Gt - Gs[j])) * rkj[i];
-            At[j * LD + t] = j < t ? bt * dec * kk[c][i] : 0.f;
-            P[c][i] = j <= t ? rqt * dec * kq[c][i] : 0.f;
+            for (int i = 0; i < 4; ++i) {
+              const int j = 16 * c + 4 * g + i;
+              const float dec = exp2_of((float)(Gt - Gs[b][j])) * rkj[i];
+              At[j * LD + t] = j < t ? bt * dec * kk[c][i] : 0.f;
+              P[c][i] = j <= t ? rqt * dec * kq[c][i] : 0.f;
+            }
           }
         }
+        store(ws, 1, P);
       }
-      store(ws, 1, P);
-    }
-    __syncthreads();
-    {   // the inverse of diagonal block w: lane r column r, by substitution
-      float x[16];
+      __syncthreads();
+      {   // the inverse of diagonal block w: lane r column r, by substitution
+        float x[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = i == r ? 1.f : 0.f;
+        for (int i = 0; i < 16; ++i) x[i] = i == r ? 1.f : 0.f;
 #pragma unroll
-      for (int j = 0; j < 15; ++j) {
-        const float *a = At + (16 * w + j) * LD + 16 * w;
+        for (int j = 0; j < 15; ++j) {
+          const float *a = At + (16 * w + j) * LD + 16 * w;
 #pragma unroll
-        for (int i = j + 1; i < 16; ++i) x[i] -= a[i] * x[j];
-      }
-      if (g == 0)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4)
-          *(f32x4 *)(Tt[w] + r * 20 + i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
-    }
-    __syncthreads();
-    {   // block row w of the inverse T, transposed: with T (I + A) = I,
-        // T_wc^T = -T_cc^T sum_(c < k <= w) A_kc^T T_wk^T
-      f32x4 X[4];
-#pragma unroll
-      for (int c = 3; c >= 0; --c) {
-        X[c] = f32x4{0, 0, 0, 0};
-        if (c == w) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) X[c][i] = Tt[c][(4 * g + i) * 20 + r];
-        } else if (c < w) {
-          f32x4 acc{0, 0, 0, 0};
-#pragma unroll
-          for (int k = c + 1; k < 4; ++k)
-            if (k <= w)
-              acc = mfma4(*(const f32x4 *)(At + (16 * c + r) * LD + 16 * k + 4 * g), X[k], acc);
-          X[c] = mfma4(-*(const f32x4 *)(Tt[c] + r * 20 + 4 * g), acc, X[c]);
+          for (int i = j + 1; i < 16; ++i) x[i] -= a[i] * x[j];
         }
-      }
+        if (g == 0)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) X[c] *= *(const f32x4 *)(betas + 16 * c + 4 * g);
-      store(ws, 0, X);
+          for (int i = 0; i < 16; i += 4)
+            *(f32x4 *)(Tt[w] + r * 20 + i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+      }
+      __syncthreads();
+      {   // block row w of the inverse T, transposed: with T (I + A) = I,
+          // T_wc^T = -T_cc^T sum_(c < k <= w) A_kc^T T_wk^T
+        f32x4 X[4];
+#pragma unroll
+        for (int c = 3; c >= 0; --c) {
+          X[c] = f32x4{0, 0, 0, 0};
+          if (c == w) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) X[c][i] = Tt[c][(4 * g + i) * 20 + r];
+          } else if (c < w) {
+            f32x4 acc{0, 0, 0, 0};
+#pragma unroll
+            for (int k = c + 1; k < 4; ++k)
+              if (k <= w)
+                acc = mfma4(*(const f32x4 *)(At + (16 * c + r) * LD + 16 * k + 4 * g), X[k], acc);
+            X[c] = mfma4(-*(const f32x4 *)(Tt[c] + r * 20 + 4 * g), acc, X[c]);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) X[c] *= *(const f32x4 *)(betas[b] + 16 * c + 4 * g);
+        store(ws, 0, X);
+      }
     }
+    __syncthreads();                 // betas are read
   }
 }
 
@@ -490,11 +513,9 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
       for (int d = threadIdx.x >> 4; d < DK; d += 32) state[(int64_t)d * p.dv] = 0.f;
     return;
   }
-  const Planes pl = planes_of<T>(p);
   // of the chunk whose operands are loaded next
-  const int64_t first = first_chunk(p, row);
-  const uint8_t *ws = (const uint8_t *)p.ws + (first * p.hv + h) * kChunkBytes;
-  const int64_t ws_step = (int64_t)p.hv * kChunkBytes;
+  const Space<DK, T> space(p, first_chunk(p, row));
+  const uint8_t *ws = space.head(h);
   // row tile w of M (which 0) or P, terms i of k-step s
   auto tri = [&](int which, int s, int i) -> const bf16x8 & {
     return ((const bf16x8 *)(ws + which * kTriBytes) + (tri_of(w, s) * 3 + i) * 64)[lane];
@@ -503,11 +524,11 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
   auto factor = [&](int which) {
     return *(const f32x4 *)((const float *)(ws + 2 * kTriBytes) + 64 * which + 16 * w + 4 * g);
   };
-  // where the operands of a chunk of len tokens lie, in bytes from its first
-  // token; past its end the last token's are read, whose factors and columns
-  // of M and P are zeros
-  auto row_at = [&](int t, int len, int64_t token, int e, int size) {
-    return (uint32_t)(min(t, len - 1) * (int)token + e) * (uint32_t)size;
+  // where a chunk's values lie, in bytes from its first token; past its end of
+  // len tokens the last one's are read, whose factors and columns of M and P
+  // are zeros
+  auto row_at = [&](int t, int len, int64_t token) {
+    return (uint32_t)(min(t, len - 1) * (int)token + col) * (uint32_t)sizeof(T);
   };
 
   auto chain = [&](auto upper) {
@@ -537,24 +558,16 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
 #pragma unroll
       for (int i = 0; i < terms.value; ++i) b[i][w >> 1][lane][w & 1] = t[i];
     };
-    const uint8_t *kb = (const uint8_t *)(pl.k + begin * pl.k_token + hk * pl.k_head);
+    const uint8_t *kb = (const uint8_t *)space.rows(hk, 0);
+    const int64_t kt_off = Space<DK, T>::kRows / 3 * 2;
     const uint8_t *vb = (const uint8_t *)((const T *)p.v + begin * p.v_token + h * p.v_head);
-    const int64_t k_step = pl.k_token * C * 2, v_step = p.v_token * C * (int)sizeof(T);
-    uint32_t k_at, v_at[4], kt_at[2][8];
+    const int64_t v_step = p.v_token * C * (int)sizeof(T);
+    uint32_t v_at[4];
     auto offsets = [&](int len) {
-      k_at = row_at(16 * w + r, len, pl.k_token, 8 * g, 2);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v_at[i] = row_at(16 * w + 4 * g + i, len, p.v_token, col, sizeof(T));
-      if constexpr (STATE)
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            kt_at[s][j] = row_at(token_of(s, g, j), len, pl.k_token, 32 * w + 2 * r, 2);
+      for (int i = 0; i < 4; ++i) v_at[i] = row_at(16 * w + 4 * g + i, len, p.v_token);
     };
-    bf16x8 k[NS][NK], m[2][3];
-    uint32_t kt[2][8][NK];
+    bf16x8 k[NS][NK], m[2][3], kt[2][2][NK];
     T v[4];
     f32x4 a, c;
     float fall;
@@ -563,7 +576,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
       for (int i = 0; i < NK; ++i)
 #pragma unroll
         for (int s = 0; s < NS; ++s)
-          k[s][i] = *(const bf16x8 *)(kb + 2 * i * pl.term + 64 * s + k_at);
+          k[s][i] = ((const bf16x8 *)kb + ((w * NS + s) * NK + i) * 64)[lane];
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = *(const T *)(vb + v_at[i]);
       a = factor(0);
@@ -581,10 +594,11 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
+          for (int e = 0; e < 2; ++e)
 #pragma unroll
             for (int i = 0; i < NK; ++i)
-              kt[s][j][i] = *(const uint32_t *)(kb + 2 * i * pl.term + kt_at[s][j]);
+              kt[s][e][i] =
+                  ((const bf16x8 *)(kb + kt_off) + (((w * 2 + s) * 2 + e) * NK + i) * 64)[lane];
         fall = ((const float *)(ws + 2 * kTriBytes) + 192)[lane];
       }
     };
@@ -601,9 +615,9 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
     for (int ch = 0; ch < n; ++ch) {
       const int len = min(C, end - begin - ch * C);
       if (ch + 1 < n) {
-        kb += k_step;
+        kb += space.kRows;
         vb += v_step;
-        ws += ws_step;
+        ws += kHeadBytes;
         if (len < 2 * C && end - begin - (ch + 1) * C < C) offsets(end - begin - (ch + 1) * C);
       }
       {
@@ -647,20 +661,8 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
         S[1] *= fall;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          bf16x8 x[2][NK];
-#pragma unroll
-          for (int i = 0; i < NK; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              u32x4 y;
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                y[j] = __builtin_amdgcn_perm(kt[s][2 * j + 1][i], kt[s][2 * j][i],
-                                             e ? 0x07060302u : 0x05040100u);
-              x[e][i] = __builtin_bit_cast(bf16x8, y);
-            }
-          S[0] = mfma_terms<NK, 3, 2>(x[0], b[s], S[0]);
-          S[1] = mfma_terms<NK, 3, 2>(x[1], b[s], S[1]);
+          S[0] = mfma_terms<NK, 3, 2>(kt[s][0], b[s], S[0]);
+          S[1] = mfma_terms<NK, 3, 2>(kt[s][1], b[s], S[1]);
         }
         put_state();
         load_update();
@@ -676,13 +678,12 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
 
   auto output = [&](auto upper) {
     constexpr bool HI = upper.value;
-    const uint8_t *qb = (const uint8_t *)(pl.q + begin * pl.q_token + hk * pl.q_head);
+    const uint8_t *qb = (const uint8_t *)space.rows(hk, 1);
     uint8_t *ob = (uint8_t *)((T *)p.out + begin * p.out_token + h * p.out_head);
-    const int64_t q_step = pl.q_token * C * 2, o_step = p.out_token * C * (int)sizeof(T);
-    uint32_t q_at, o_at[4];
+    const int64_t o_step = p.out_token * C * (int)sizeof(T);
+    uint32_t o_at[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      o_at[i] = row_at(16 * w + 4 * g + i, C, p.out_token, col, sizeof(T));
+    for (int i = 0; i < 4; ++i) o_at[i] = row_at(16 * w + 4 * g + i, C, p.out_token);
     bf16x8 q[NS][NK], m[2][OT];
     f32x4 b;
     auto load_rows = [&]() {
@@ -690,7 +691,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
       for (int i = 0; i < NK; ++i)
 #pragma unroll
         for (int s = 0; s < NS; ++s)
-          q[s][i] = *(const bf16x8 *)(qb + 2 * i * pl.term + 64 * s + q_at);
+          q[s][i] = ((const bf16x8 *)qb + ((w * NS + s) * NK + i) * 64)[lane];
     };
     auto load_weights = [&]() {
 #pragma unroll
@@ -700,7 +701,6 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
       }
       b = factor(1);
     };
-    q_at = row_at(16 * w + r, min(C, end - begin), pl.q_token, 8 * g, 2);
     load_rows();
     __builtin_amdgcn_sched_barrier(0);
     load_weights();
@@ -708,9 +708,8 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
     for (int ch = 0; ch < n; ++ch) {
       const int len = min(C, end - begin - ch * C);
       if (ch + 1 < n) {
-        qb += q_step;
-        ws += ws_step;
-        q_at = row_at(16 * w + r, min(C, end - begin - (ch + 1) * C), pl.q_token, 8 * g, 2);
+        qb += space.kRows;
+        ws += kHeadBytes;
       }
       f32x4 o{0, 0, 0, 0};
       {
@@ -782,8 +781,9 @@ void launch_dim(const Delta &d, hipStream_t s) {
 
 int64_t delta_workspace(int64_t tokens, int64_t rows, int64_t hk, int64_t hv, int64_t dk,
                         int dtype) {
-  const int64_t terms = dtype == DT_F32 ? 3 : dtype == DT_BF16 ? 0 : 2;
-  return (tokens / C + rows) * hv * kChunkBytes + 2 * terms * tokens * hk * dk * 2;
+  const int terms = dtype == DT_F32 ? Terms<float>::n
+                    : dtype == DT_BF16 ? Terms<__bf16>::n : Terms<_Float16>::n;
+  return (tokens / C + rows) * (hv * kHeadBytes + hk * rows_bytes(dk, terms));
 }
 
 hipError_t launch_delta(const Delta &d, hipStream_t s) {

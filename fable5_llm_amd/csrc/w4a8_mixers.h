@@ -96,7 +96,7 @@ struct Delta {
   float unit, out_unit;         // DT_I16: the value of a step of q, k, v; 1 / that of out
   int32_t *err;
 };
-constexpr int64_t kDeltaStride = 1 << 23;   // of tokens, whole prompts
+constexpr int64_t kDeltaStride = 1 << 23;   // of v's and out's tokens, whole prompts
 int64_t delta_workspace(int64_t tokens, int64_t rows, int64_t hk, int64_t hv, int64_t dk,
                         int dtype);
 hipError_t launch_delta(const Delta &d, hipStream_t s);

@@ -520,7 +520,8 @@ typedef struct {
 /* one token of each row */
 int w4a8_delta_step_async(w4a8_ctx *ctx, const w4a8_delta *d);
 /* whole prompts, in chunks of 64 tokens (an infinity or a NaN among a token's
-   inputs can reach every output of its chunk).  Token strides: at most 2^23.  Bounds that do not lie in
+   inputs can reach every output of its chunk).  Token strides of v and
+   out: at most 2^23.  Bounds that do not lie in
    order within the tokens: nothing is run, and the next sync reports it. */
 int w4a8_delta_chunk_workspace(w4a8_ctx *ctx, int64_t tokens, int64_t rows,
                                int64_t hk, int64_t hv, int64_t dk, int32_t dtype,

@@ -157,7 +157,7 @@ def check_delta():
             refused(f, ctx, ctypes.byref(delta(**kw)))
     refused(step, ctx, ctypes.byref(delta(tokens=4)))
     refused(chunk, ctx, ctypes.byref(delta(cu=None)))
-    for n in ("q_token", "k_token", "v_token", "out_token"):
+    for n in ("v_token", "out_token"):
         refused(chunk, ctx, ctypes.byref(delta(**{n: (1 << 23) + 8})))
     refused(chunk, ctx, ctypes.byref(delta(ws=None)))
     refused(chunk, ctx, ctypes.byref(delta(ws=ODD.value)))
