@@ -2004,6 +2004,8 @@ struct w4a8_kv {
 
 namespace {
 
+constexpr int32_t kMostRows = 1 << 20;   // of a call: rows, list entries
+
 // Activations of the mixers: 16-byte aligned, every stride whole 16 bytes.
 bool rows_ok(const void *p, int dtype, int64_t a, int64_t b) {
   const int64_t per = 16 / dtype_size(dtype);
@@ -2023,7 +2025,8 @@ float unit_of(int32_t dtype, int64_t frac) {
 
 int check_list(const w4a8_kv *kv, const void *list, const void *list2, int32_t n) {
   if (!kv) return fail(W4A8_E_ARG, "null cache");
-  if (n < 0 || (n > 0 && (!list || !list2))) return fail(W4A8_E_ARG, "bad list");
+  if (n < 0 || n > kMostRows || (n > 0 && (!list || !list2)))
+    return fail(W4A8_E_ARG, "bad list (0 to 2^20 entries)");
   return W4A8_OK;
 }
 
@@ -2033,16 +2036,17 @@ const char *delta_fault(const w4a8_delta *d, bool chunk) {
   if (d->dv < 16 || d->dv > 256 || d->dv % 16) return "dv must be a multiple of 16, 16..256";
   if (d->hk < 1 || d->hv < 1 || d->hv % d->hk || d->hv > 65535)
     return "hv must be a multiple of hk";
-  if (d->rows < 0 || d->tokens < 0 || d->rows > INT32_MAX || d->tokens > INT32_MAX ||
+  if (d->rows < 0 || d->tokens < 0 || d->rows > kMostRows || d->tokens > (1 << 30) ||
       d->nslots < 0 || d->nslots > INT32_MAX)
-    return "rows, tokens and slots must be 0..2^31 - 1";
+    return "at most 2^20 rows, 2^30 tokens and 2^31 - 1 slots";
   if (!chunk && d->tokens != d->rows) return "a step has one token per row";
   if (d->frac < 0 || d->frac > 31 || d->out_frac < 0 || d->out_frac > 31)
     return "fraction bits must be 0..31";
   if (d->rows == 0) return nullptr;
   if (!d->slots && d->nslots < d->rows) return "fewer states than rows";
   if (chunk && !d->cu) return "cu is needed";
-  if (d->rows * d->hv > (1 << 26)) return "more than 2^26 heads of states";
+  if (d->rows * d->hv > (1 << 22) / (d->dv / 16))   // a launch has fewer than 2^32 threads
+    return "too many rows and heads for one call";
   // 32-bit offsets within a chunk's 64 tokens
   if (chunk && (d->v_token > kDeltaStride || d->out_token > kDeltaStride))
     return "token strides of v and out must be at most 2^23";
@@ -2213,7 +2217,11 @@ int check_heads(const w4a8_kv *kv, int32_t rows, int32_t q_heads) {
   if (!kv) return fail(W4A8_E_ARG, "null cache");
   if (rows < 0 || q_heads < 1 || q_heads > 65535 || q_heads % kv->c.heads)
     return fail(W4A8_E_ARG, "q_heads must be a multiple of the cache's kv_heads");
-  if (rows > (1 << 24)) return fail(W4A8_E_ARG, "at most 2^24 rows");
+  // a launch has fewer than 2^32 threads
+  if (rows > kMostRows ||
+      (int64_t)rows * q_heads * attend_splits(kv->c, rows ? rows : 1, q_heads, kv->ctx->num_cu) >
+          (1 << 23))
+    return fail(W4A8_E_ARG, "attention: too many rows and heads for one call");
   return W4A8_OK;
 }
 }  // namespace
@@ -2260,8 +2268,8 @@ int w4a8_delta_step_async(w4a8_ctx *c, const w4a8_delta *d) { return delta_launc
 
 int w4a8_delta_chunk_workspace(w4a8_ctx *c, int64_t tokens, int64_t rows, int64_t hk, int64_t hv,
                                int64_t dk, int32_t dtype, int64_t *bytes) {
-  if (!c || !bytes || tokens < 0 || rows < 0 || hk < 1 || hv < hk || tokens > INT32_MAX ||
-      rows > INT32_MAX || hv > 65535 || (dk != 64 && dk != 128) || dtype < DT_F32 ||
+  if (!c || !bytes || tokens < 0 || rows < 0 || hk < 1 || hv < hk || tokens > (1 << 30) ||
+      rows > kMostRows || hv > 65535 || (dk != 64 && dk != 128) || dtype < DT_F32 ||
       dtype > DT_I16)
     return fail(W4A8_E_ARG, "bad argument");
   *bytes = rows ? delta_workspace(tokens, rows, hk, hv, dk, dtype) : 0;

@@ -101,8 +101,11 @@ __device__ __forceinline__ void store_out(const Attend &a, int cache_dtype, int6
 // values too, so that a 16-bit result keeps its bits.  Otherwise P is rounded
 // to the cache's type for the second product, its sum is not: an error of
 // half a step of that type per token, which averages out over the tokens.
+// Workgroups: key-value heads fastest, then rows, then splits, so that those of
+// short rows that have nothing to do come last.  Two a CU at least (registers:
+// a head of 256 would take 267 and leave one, @@).
 template <int D, typename T, bool I16>
-__global__ __launch_bounds__(64 * kWaves) void attend_kernel(KvCache kv, Attend a) {
+__global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(KvCache kv, Attend a) {
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int kTok = F32 ? 16 : 32;              // tokens of a turn
   constexpr int NT = kTok / 16;                    // 16-token tiles of them
@@ -117,9 +120,11 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(KvCache kv, Attend 
 
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int row = blockIdx.x / a.splits, split = blockIdx.x - row * a.splits;
   const int group = a.hq / kv.heads, tiles = (group + 15) / 16;
-  const int kvh = blockIdx.y / tiles, h0 = (blockIdx.y - kvh * tiles) * 16;
+  const int heads_all = kv.heads * tiles, unit = blockIdx.x / heads_all;
+  const int tile = blockIdx.x - unit * heads_all, kvh = tile / tiles;
+  const int h0 = (tile - kvh * tiles) * 16;
+  const int split = unit / a.rows, row = unit - split * a.rows;
   const int heads = min(16, group - h0);           // of this tile
   const Range R = range_of(kv, a, row, split);
   if (R.seq >= kv.seqs && split == 0 && threadIdx.x == 0) atomicOr(kv.err, kErrKvRange);
@@ -179,15 +184,24 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(KvCache kv, Attend 
   float m = -INFINITY, l = 0.f;
   int bad = 0;
 
+  // the pages of a turn's 16-token tiles, looked up a turn ahead; a tile past
+  // the end, or whose page is none of the pool's, reads page 0 and is masked
+  int next[NT];
+  auto look_up = [&](int t) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int tt = t + 16 * j;
+      next[j] = table[(tt < R.t1 ? tt : R.t0) >> lg];
+    }
+  };
+  look_up(R.t0 + wave * kTok);
   for (int t = R.t0 + wave * kTok; t < R.t1; t += kWaves * kTok) {
-    // the pages of the turn's 16-token tiles; a tile past the end, or whose
-    // page is none of the pool's, reads page 0 and is masked
     const T *kp[NT], *vp[NT];
     int lim[NT];                                    // tokens below it count
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       const int tt = t + 16 * j;
-      int p = tt < R.t1 ? table[tt >> lg] : 0;
+      int p = tt < R.t1 ? next[j] : 0;
       lim[j] = R.t1;
       if ((uint32_t)p >= (uint32_t)kv.pages) {
         bad = 1;
@@ -198,6 +212,7 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(KvCache kv, Attend 
       kp[j] = base + kbase;
       vp[j] = base + vbase;
     }
+    look_up(t + kWaves * kTok);
     u32x4 kr[NT][KS];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
@@ -392,38 +407,43 @@ __global__ __launch_bounds__(64 * kWaves) void attend_kernel(KvCache kv, Attend 
 
 // The splits of a row and head joined: out = sum_s 2^(m_s - M) o_s / sum_s
 // 2^(m_s - M) l_s.  A workgroup per row and head, D / 4 threads per split.
+constexpr int kJoin = 512;
 template <int D>
-__global__ __launch_bounds__(256) void attend_join_kernel(KvCache kv, Attend a) {
-  constexpr int LANES = D / 4, GROUPS = 256 / LANES;
+__global__ __launch_bounds__(kJoin) void attend_join_kernel(KvCache kv, Attend a) {
+  constexpr int LANES = D / 4, GROUPS = kJoin / LANES, WAVES = kJoin / 64;
   __shared__ f32x4 obuf[GROUPS][LANES];
-  __shared__ float red[2][4];
+  __shared__ float red[2][WAVES];
   const int row = blockIdx.x, h = blockIdx.y;
   const Range R = range_of(kv, a, row, 0);
   if (R.used <= 1) return;
   const int64_t slot = ((int64_t)row * a.hq + h) * a.splits;
   const float *ml = a.part + (int64_t)a.rows * a.hq * a.splits * D + slot * 2;
   float M = -INFINITY;
-  for (int s = threadIdx.x; s < R.used; s += 256) M = fmaxf(M, ml[2 * s]);
+  for (int s = threadIdx.x; s < R.used; s += kJoin) M = fmaxf(M, ml[2 * s]);
 #pragma unroll
   for (int d = 32; d; d >>= 1) M = fmaxf(M, __shfl_xor(M, d));
   if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6] = M;
   __syncthreads();
-  M = base_of(fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3])));
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) M = fmaxf(M, red[0][w]);
+  M = base_of(M);
   float L = 0.f;
-  for (int s = threadIdx.x; s < R.used; s += 256) L += ml[2 * s + 1] * exp2_of(ml[2 * s] - M);
+  for (int s = threadIdx.x; s < R.used; s += kJoin) L += ml[2 * s + 1] * exp2_of(ml[2 * s] - M);
 #pragma unroll
   for (int d = 32; d; d >>= 1) L += __shfl_xor(L, d);
   if ((threadIdx.x & 63) == 0) red[1][threadIdx.x >> 6] = L;
   const int lane = threadIdx.x % LANES, grp = threadIdx.x / LANES;
   const float *part = a.part + slot * D + lane * 4;
   f32x4 o{0, 0, 0, 0};
-#pragma unroll 4
+#pragma unroll 8
   for (int s = grp; s < R.used; s += GROUPS)
     o += *(const f32x4 *)(part + (int64_t)s * D) * exp2_of(ml[2 * s] - M);
   obuf[grp][lane] = o;
   __syncthreads();
   if (grp != 0) return;
-  L = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  L = 0.f;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) L += red[1][w];
 #pragma unroll
   for (int k = 1; k < GROUPS; ++k) o += obuf[k][lane];
   const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
@@ -432,17 +452,17 @@ __global__ __launch_bounds__(256) void attend_join_kernel(KvCache kv, Attend a) 
 }
 
 template <int D, typename T>
-void launch_typed(const KvCache &kv, const Attend &a, dim3 grid, hipStream_t s) {
+void launch_typed(const KvCache &kv, const Attend &a, uint32_t grid, hipStream_t s) {
   if (a.dtype == DT_I16) attend_kernel<D, T, true><<<grid, 64 * kWaves, 0, s>>>(kv, a);
   else attend_kernel<D, T, false><<<grid, 64 * kWaves, 0, s>>>(kv, a);
 }
 
 template <int D>
-void launch_dim(const KvCache &kv, const Attend &a, dim3 grid, hipStream_t s) {
+void launch_dim(const KvCache &kv, const Attend &a, uint32_t grid, hipStream_t s) {
   if (kv.dtype == DT_F32) launch_typed<D, float>(kv, a, grid, s);
   else if (kv.dtype == DT_BF16) launch_typed<D, __bf16>(kv, a, grid, s);
   else launch_typed<D, _Float16>(kv, a, grid, s);
-  if (a.splits > 1) attend_join_kernel<D><<<dim3(a.rows, a.hq), 256, 0, s>>>(kv, a);
+  if (a.splits > 1) attend_join_kernel<D><<<dim3(a.rows, a.hq), kJoin, 0, s>>>(kv, a);
 }
 
 }  // namespace
@@ -452,7 +472,8 @@ void launch_dim(const KvCache &kv, const Attend &a, dim3 grid, hipStream_t s) {
 int attend_splits(const KvCache &kv, int64_t rows, int64_t hq, int num_cu) {
   const int64_t group = hq / kv.heads, base = rows * kv.heads * ((group + 15) / 16);
   const int64_t most = (((int64_t)kv.max_pages << kv.lg_page) + kAttendChunk - 1) / kAttendChunk;
-  const int64_t want = (4ll * num_cu + base - 1) / base;
+  const int64_t fill = (4ll * num_cu + base - 1) / base, even = (most + 3) / 4;
+  const int64_t want = fill > 16 ? fill : fill > even ? fill : even < 16 ? even : 16;
   return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
@@ -463,7 +484,7 @@ int64_t attend_workspace(const KvCache &kv, int64_t rows, int64_t hq, int num_cu
 
 hipError_t launch_attend(const KvCache &kv, const Attend &a, hipStream_t s) {
   const int group = a.hq / kv.heads, tiles = (group + 15) / 16;
-  const dim3 grid((uint32_t)a.rows * a.splits, kv.heads * tiles);
+  const uint32_t grid = (uint32_t)(kv.heads * tiles) * a.rows * a.splits;
   if (kv.dim == 64) launch_dim<64>(kv, a, grid, s);
   else if (kv.dim == 128) launch_dim<128>(kv, a, grid, s);
   else launch_dim<256>(kv, a, grid, s);

@@ -58,6 +58,7 @@ def check_lists():
         refused(f, h, None, PTR, 3)
         refused(f, h, PTR, None, 3)
         refused(f, h, PTR, PTR, -1)
+        refused(f, h, PTR, PTR, (1 << 20) + 1)
         refused(f, h, None, None, 0, what=OK)
     refused(lib.w4a8_kv_free_async, None, PTR, 1)
     refused(lib.w4a8_kv_free_async, h, None, 1)
@@ -100,7 +101,7 @@ def check_attend():
                dict(q=None), dict(out=None), dict(q=ODD), dict(out=ODD), dict(q0=1023),
                dict(q1=2), dict(o0=-1024), dict(o1=129), dict(seqs=None), dict(rows=-1),
                dict(heads=6), dict(heads=0), dict(ws=None), dict(ws=ODD),
-               dict(ws_bytes=b.value - 1), dict(rows=(1 << 24) + 1)):
+               dict(ws_bytes=b.value - 1), dict(rows=(1 << 20) + 1), dict(rows=1 << 20, heads=16)):
         refused(lambda kw=kw: attend(h, **kw))
     refused(lambda: attend(None))
     refused(lib.w4a8_kv_attend_workspace, h, 2, 9, ctypes.byref(b))
@@ -149,7 +150,8 @@ def check_delta():
         refused(f, ctx, ctypes.byref(delta(rows=0, tokens=0)), what=OK)
         for kw in (dict(dtype=4), dict(dtype=-1), dict(dk=96), dict(dv=24), dict(dv=8),
                    dict(dv=272), dict(hv=3), dict(hk=0), dict(hv=0), dict(rows=-1),
-                   dict(tokens=-1), dict(tokens=1 << 32), dict(nslots=-1), dict(frac=32),
+                   dict(tokens=-1), dict(tokens=(1 << 30) + 1), dict(rows=(1 << 20) + 1),
+                   dict(rows=1 << 20, tokens=1 << 20, nslots=1 << 20), dict(nslots=-1), dict(frac=32),
                    dict(out_frac=-1), dict(slots=None, nslots=2), dict(q=None), dict(k=ODD.value),
                    dict(v=None), dict(out=ODD.value), dict(state=None), dict(state=ODD.value),
                    dict(g=None), dict(beta=ODD.value), dict(q_token=1), dict(k_head=4),
