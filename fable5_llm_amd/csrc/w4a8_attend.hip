@@ -69,8 +69,8 @@ __device__ __forceinline__ Range range_of(const KvCache &kv, const Attend &a, in
   const int per = (each + kAttendChunk - 1) / kAttendChunk * kAttendChunk;
   r.used = (int)(((int64_t)r.n + per - 1) / per);
   const int64_t t0 = (int64_t)split * per;
-  r.t0 = (int)(t0 < r.n ? t0 : r.n);
-  r.t1 = (int)(t0 + per < r.n ? t0 + per : r.n);
+  r.t0 = __builtin_amdgcn_readfirstlane((int)(t0 < r.n ? t0 : r.n));
+  r.t1 = __builtin_amdgcn_readfirstlane((int)(t0 + per < r.n ? t0 + per : r.n));
   return r;
 }
 
@@ -105,7 +105,8 @@ __device__ __forceinline__ void store_out(const Attend &a, int cache_dtype, int6
 // short rows that have nothing to do come last.  Two a CU at least (registers:
 // a head of 256 would take 267 and leave one, @@).
 template <int D, typename T, bool I16>
-__global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(KvCache kv, Attend a) {
+__global__ __launch_bounds__(64 * kWaves, D == 256 && (I16 || sizeof(T) == 4) ? 1 : 2) void
+attend_kernel(KvCache kv, Attend a) {
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int kTok = F32 ? 16 : 32;              // tokens of a turn
   constexpr int NT = kTok / 16;                    // 16-token tiles of them
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(KvCache kv, Atte
   const int heads_all = kv.heads * tiles, unit = blockIdx.x / heads_all;
   const int tile = blockIdx.x - unit * heads_all, kvh = tile / tiles;
   const int h0 = (tile - kvh * tiles) * 16;
-  const int split = unit / a.rows, row = unit - split * a.rows;
+  const int row = unit / a.splits, split = unit - row * a.splits;
   const int heads = min(16, group - h0);           // of this tile
   const Range R = range_of(kv, a, row, split);
   if (R.seq >= kv.seqs && split == 0 && threadIdx.x == 0) atomicOr(kv.err, kErrKvRange);
@@ -173,10 +174,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(KvCache kv, Atte
   const int page = kv.page(), lg = kv.lg_page;
   const int32_t *table = kv.tables + (int64_t)R.seq * kv.max_pages;
   const int64_t plane = (int64_t)page * D;          // elements of a head's page
-  const T *pool = (const T *)kv.pool;
-  const int64_t page_elems = kv.page_bytes / (int)sizeof(T);
   const int64_t kbase = (((int64_t)a.layer * 2) * kv.heads + kvh) * plane;
-  const int64_t vbase = kbase + kv.heads * plane;
 
   f32x4 acc[NC * VEC];
 #pragma unroll
@@ -194,48 +192,50 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(KvCache kv, Atte
       next[j] = table[(tt < R.t1 ? tt : R.t0) >> lg];
     }
   };
-  look_up(R.t0 + wave * kTok);
-  for (int t = R.t0 + wave * kTok; t < R.t1; t += kWaves * kTok) {
-    const T *kp[NT], *vp[NT];
-    int lim[NT];                                    // tokens below it count
+  // a lane's bytes from a tile's first row: the tile's address is the same in
+  // every lane
+  const uint32_t k_at = (r * D + g * (F32 ? 4 : 8)) * (int)sizeof(T);
+  const uint32_t v_at = (4 * g * D + r * VEC) * (int)sizeof(T);
+  const uint8_t *vp[NT];
+  int lim[NT];                                      // tokens below it count
+  u32x4 kr[NT][KS], vr[ROWS][NC];
+  auto load_keys = [&](int t) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       const int tt = t + 16 * j;
-      int p = tt < R.t1 ? next[j] : 0;
+      int p = __builtin_amdgcn_readfirstlane(tt < R.t1 ? next[j] : 0);
       lim[j] = R.t1;
       if ((uint32_t)p >= (uint32_t)kv.pages) {
         bad = 1;
         p = 0;
         lim[j] = 0;
       }
-      const T *base = pool + p * page_elems + (int64_t)(tt & (page - 1)) * D;
-      kp[j] = base + kbase;
-      vp[j] = base + vbase;
+      const uint8_t *kp = kv.pool + p * kv.page_bytes +
+                          (kbase + (int64_t)(tt & (page - 1)) * D) * (int)sizeof(T);
+      vp[j] = kp + kv.heads * plane * (int)sizeof(T);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) kr[j][s] = load16_nt(kp + k_at + 64 * s);
     }
     look_up(t + kWaves * kTok);
-    u32x4 kr[NT][KS];
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        constexpr int step = F32 ? 16 : 32, per = F32 ? 4 : 8;
-        kr[j][s] = load16_nt(kp[j] + r * D + s * step + g * per);
-      }
-    u32x4 vr[ROWS][NC];
+  };
+  auto load_values = [&]() {
 #pragma unroll
     for (int i = 0; i < ROWS; ++i)
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const T *src = vp[i >> 2] + (4 * g + (i & 3)) * D + c * 16 * VEC + r * VEC;
+        const uint8_t *src =
+            vp[i >> 2] + v_at + ((i & 3) * D + c * 16 * VEC) * (int)sizeof(T);
         if constexpr (VEC * sizeof(T) == 16) {
           vr[i][c] = load16_nt(src);
         } else {
-          const u32x2 x = __builtin_nontemporal_load((const u32x2 *)src);
-          vr[i][c] = u32x4{x.x, x.y, 0, 0};
+          const u32x2 y = __builtin_nontemporal_load((const u32x2 *)src);
+          vr[i][c] = u32x4{y.x, y.y, 0, 0};
         }
       }
-    // scores of tokens t + 16 j + 4 g + i for head r
-    f32x4 sc[NT];
+  };
+  f32x4 sc[NT];
+  // scores of tokens t + 16 j + 4 g + i for head r
+  auto scores = [&]() {
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       sc[j] = f32x4{0, 0, 0, 0};
@@ -253,6 +253,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(KvCache kv, Atte
         }
       }
     }
+  };
+  // the weights of tokens t .., and their values added up.  The next turn's
+  // keys may be in flight already: lims are this turn's.
+  auto weigh = [&](int t, const int *lim) {
     float top = m;
 #pragma unroll
     for (int j = 0; j < NT; ++j)
@@ -302,9 +306,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(KvCache kv, Atte
       x8 p[SPLIT];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float x = sc[i >> 2][i & 3];
-        p[0][i] = (T)x;
-        if constexpr (SPLIT == 2) p[1][i] = (T)(x - (float)p[0][i]);
+        const float w = sc[i >> 2][i & 3];
+        p[0][i] = (T)w;
+        if constexpr (SPLIT == 2) p[1][i] = (T)(w - (float)p[0][i]);
       }
 #pragma unroll
       for (int c = 0; c < NC; ++c)
@@ -315,11 +319,35 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(KvCache kv, Atte
           for (int i = 0; i < 4; ++i)
             w[i] = __builtin_amdgcn_perm(vr[2 * i + 1][c][e >> 1], vr[2 * i][c][e >> 1],
                                          e & 1 ? 0x07060302u : 0x05040100u);
-          const x8 v8 = __builtin_bit_cast(x8, w);
+          const x8 v = __builtin_bit_cast(x8, w);
 #pragma unroll
-          for (int q = 0; q < SPLIT; ++q) acc[c * VEC + e] = mfma(v8, p[q], acc[c * VEC + e]);
+          for (int q = 0; q < SPLIT; ++q) acc[c * VEC + e] = mfma(v, p[q], acc[c * VEC + e]);
         }
     }
+  };
+  // A turn's registers are loaded with the next turn's keys once its scores are
+  // made, and with its values once those are added up, so that a tile of each
+  // wavefront is in flight throughout.
+  constexpr int kStep = kWaves * kTok;
+  int t = R.t0 + wave * kTok;
+  if (t < R.t1) {
+    look_up(t);
+    load_keys(t);
+    __builtin_amdgcn_sched_barrier(0);
+    load_values();
+    for (; t + kStep < R.t1; t += kStep) {
+      int now[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) now[j] = lim[j];
+      scores();
+      load_keys(t + kStep);
+      __builtin_amdgcn_sched_barrier(0);
+      weigh(t, now);
+      load_values();
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    scores();
+    weigh(t, lim);
   }
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
@@ -406,47 +434,57 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(KvCache kv, Atte
 }
 
 // The splits of a row and head joined: out = sum_s 2^(m_s - M) o_s / sum_s
-// 2^(m_s - M) l_s.  A workgroup per row and head, D / 4 threads per split.
-constexpr int kJoin = 512;
+// 2^(m_s - M) l_s.  A workgroup per row and head, D / 4 threads per split; what
+// it waits for is a chain of small loads, so the first two splits of a thread
+// are on their way before it knows how many there are.
+constexpr int kJoin = 256;
 template <int D>
 __global__ __launch_bounds__(kJoin) void attend_join_kernel(KvCache kv, Attend a) {
-  constexpr int LANES = D / 4, GROUPS = kJoin / LANES, WAVES = kJoin / 64;
+  constexpr int LANES = D / 4, GROUPS = kJoin / LANES, EARLY = 2;
   __shared__ f32x4 obuf[GROUPS][LANES];
-  __shared__ float red[2][WAVES];
+  __shared__ float mbuf[GROUPS], lbuf[GROUPS];
   const int row = blockIdx.x, h = blockIdx.y;
-  const Range R = range_of(kv, a, row, 0);
-  if (R.used <= 1) return;
-  const int64_t slot = ((int64_t)row * a.hq + h) * a.splits;
-  const float *ml = a.part + (int64_t)a.rows * a.hq * a.splits * D + slot * 2;
-  float M = -INFINITY;
-  for (int s = threadIdx.x; s < R.used; s += kJoin) M = fmaxf(M, ml[2 * s]);
-#pragma unroll
-  for (int d = 32; d; d >>= 1) M = fmaxf(M, __shfl_xor(M, d));
-  if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6] = M;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) M = fmaxf(M, red[0][w]);
-  M = base_of(M);
-  float L = 0.f;
-  for (int s = threadIdx.x; s < R.used; s += kJoin) L += ml[2 * s + 1] * exp2_of(ml[2 * s] - M);
-#pragma unroll
-  for (int d = 32; d; d >>= 1) L += __shfl_xor(L, d);
-  if ((threadIdx.x & 63) == 0) red[1][threadIdx.x >> 6] = L;
   const int lane = threadIdx.x % LANES, grp = threadIdx.x / LANES;
+  const int64_t slot = ((int64_t)row * a.hq + h) * a.splits;
   const float *part = a.part + slot * D + lane * 4;
+  const float *ml = a.part + (int64_t)a.rows * a.hq * a.splits * D + slot * 2;
+  f32x4 ahead[EARLY];
+  float am[EARLY], al[EARLY];
+#pragma unroll
+  for (int e = 0; e < EARLY; ++e) {
+    const int s = min(grp + e * GROUPS, a.splits - 1);
+    ahead[e] = *(const f32x4 *)(part + (int64_t)s * D);
+    am[e] = ml[2 * s];
+    al[e] = ml[2 * s + 1];
+  }
+  const int used = range_of(kv, a, row, 0).used;
+  if (used <= 1) return;
+  // this group's splits on one maximum
+  float m = -INFINITY, l = 0.f;
   f32x4 o{0, 0, 0, 0};
-#pragma unroll 8
-  for (int s = grp; s < R.used; s += GROUPS)
-    o += *(const f32x4 *)(part + (int64_t)s * D) * exp2_of(ml[2 * s] - M);
+  auto add = [&](float sm, float sl, f32x4 so) {
+    const float top = fmaxf(m, sm), base = base_of(top);
+    const float x = exp2_of(m - base), y = exp2_of(sm - base);
+    m = top;
+    l = l * x + sl * y;
+    o = o * x + so * y;
+  };
+#pragma unroll
+  for (int e = 0; e < EARLY; ++e)
+    if (grp + e * GROUPS < used) add(am[e], al[e], ahead[e]);
+#pragma unroll 4
+  for (int s = grp + EARLY * GROUPS; s < used; s += GROUPS)
+    add(ml[2 * s], ml[2 * s + 1], *(const f32x4 *)(part + (int64_t)s * D));
   obuf[grp][lane] = o;
+  if (lane == 0) {
+    mbuf[grp] = m;
+    lbuf[grp] = l;
+  }
   __syncthreads();
   if (grp != 0) return;
-  L = 0.f;
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) L += red[1][w];
-#pragma unroll
-  for (int k = 1; k < GROUPS; ++k) o += obuf[k][lane];
-  const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
+  for (int k = 1; k < GROUPS; ++k) add(mbuf[k], lbuf[k], obuf[k][lane]);
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
   const float x[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
   store_out(a, kv.dtype, row * a.out_row + h * a.out_head + lane * 4, x, 4);
 }
@@ -467,13 +505,18 @@ void launch_dim(const KvCache &kv, const Attend &a, uint32_t grid, hipStream_t s
 
 }  // namespace
 
-// Splits of a row: enough workgroups to fill the chip four times over at the
-// cache's longest sequence, but none of less than a chunk.
+// Splits of a row: workgroups for the chip twice over at least, and no more than
+// 512 tokens of the cache's longest sequence in one (a longer one is what a
+// ragged batch waits for), but no more than 16 for that (each is a part to
+// join), and none of less than a chunk.  Measured: 48 ragged rows to 4099, 8
+// key-value heads of 128, in 9 splits 37.5 us, in 3 51; 8 rows of 3450 in 8
+// 25.8, in 16 29.5; 24 rows of 9216 in 16 151, in 3 168.
 int attend_splits(const KvCache &kv, int64_t rows, int64_t hq, int num_cu) {
   const int64_t group = hq / kv.heads, base = rows * kv.heads * ((group + 15) / 16);
   const int64_t most = (((int64_t)kv.max_pages << kv.lg_page) + kAttendChunk - 1) / kAttendChunk;
-  const int64_t fill = (4ll * num_cu + base - 1) / base, even = (most + 3) / 4;
-  const int64_t want = fill > 16 ? fill : fill > even ? fill : even < 16 ? even : 16;
+  const int64_t fill = (2ll * num_cu + base - 1) / base;
+  const int64_t even = most > 64 ? 16 : (most + 3) / 4;
+  const int64_t want = fill > even ? fill : even;
   return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
