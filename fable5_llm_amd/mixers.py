@@ -23,15 +23,19 @@ def _dtypes():
         import torch
         _DTYPES.update({torch.float32: N.DT_F32, torch.bfloat16: N.DT_BF16,
                         torch.float16: N.DT_F16, torch.int16: N.DT_I16,
-                        torch.int32: None})
+                        torch.int32: None, None: torch.int32})
     return _DTYPES
 
 
 def _on(t, ctx, name):
+    try:
+        if t.get_device() == ctx.device:
+            return
+    except AttributeError:
+        pass
     if not getattr(t, "is_cuda", False):
         raise ValueError(f"{name}: must be a device tensor")
-    if t.device.index != ctx.device:
-        raise ValueError(f"{name}: is on device {t.device.index}, the context on {ctx.device}")
+    raise ValueError(f"{name}: is on device {t.device.index}, the context on {ctx.device}")
 
 
 def _act(t, ctx, name, shape, dtype=None):
@@ -51,6 +55,13 @@ def _act(t, ctx, name, shape, dtype=None):
 
 def _list(t, ctx, name, n=None):
     """Pointer of an int32 list of n entries (any number where n is None)."""
+    try:
+        shape = t.shape
+        if t.get_device() == ctx.device and len(shape) == 1 and (n is None or shape[0] == n) \
+                and t.dtype is _DTYPES.get(None) and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
     _on(t, ctx, name)
     if t.dim() != 1 or _dtypes().get(t.dtype, 0) is not None or not t.is_contiguous():
         raise ValueError(f"{name}: must be a contiguous int32 vector")
@@ -112,7 +123,7 @@ class PagedKV:
         self.pool, self.refs, self.tables, self.lens = pool, refs, tables, lens
         self.kv_heads, self.page_tokens, self.head_dim = heads, page, dim
         self.scale = 1.0 / math.sqrt(dim)
-        self._types = dt
+        self.dtype, self._type, self._types = pool.dtype, dt[pool.dtype], dt
 
     @classmethod
     def empty(cls, ctx, pages, layers, kv_heads, page_tokens, head_dim, seqs, max_pages, dtype):
@@ -128,9 +139,12 @@ class PagedKV:
         return kv
 
     def _act_type(self, t, name):
-        if t.dtype != self.pool.dtype and self._types.get(t.dtype) != N.DT_I16:
-            raise ValueError(f"{name}: must be {self.pool.dtype}, as the cache, or int16")
-        return self._types[t.dtype]
+        dtype = t.dtype
+        if dtype is self.dtype:
+            return self._type
+        if self._types.get(dtype) != N.DT_I16:
+            raise ValueError(f"{name}: must be {self.dtype}, as the cache, or int16")
+        return N.DT_I16
 
     def extend_async(self, seqs, counts):
         """Sequence seqs[i] grows by counts[i] tokens, pages added as needed:
@@ -143,11 +157,19 @@ class PagedKV:
     def append_async(self, layer, k, v, seqs, pos=None, frac=0):
         """Keys and values [n, kv_heads, head_dim] of n tokens of one layer, to
         sequence seqs[i] at position pos[i] (its last token without pos)."""
-        n = seqs.shape[0]
+        n, dev = seqs.shape[0], self.ctx.device
         shape = (n, self.kv_heads, self.head_dim)
         dt = self._act_type(k, "k")
-        kp, k0, k1 = _act(k, self.ctx, "k", shape)
-        vp, v0, v1 = _act(v, self.ctx, "v", shape, k.dtype)
+        if k.shape == shape and v.shape == shape and v.dtype is k.dtype \
+                and k.get_device() == dev and v.get_device() == dev:
+            (k0, k1, k2), (v0, v1, v2) = k.stride(), v.stride()
+        else:
+            k2 = None
+        if k2 != 1 or v2 != 1 or n <= 1 or self.kv_heads == 1:   # refused, or unused strides
+            kp, k0, k1 = _act(k, self.ctx, "k", shape)
+            vp, v0, v1 = _act(v, self.ctx, "v", shape, k.dtype)
+        else:
+            kp, vp = k.data_ptr(), v.data_ptr()
         N.check(N.lib().w4a8_kv_append_async(
             self.h, layer, dt, frac, kp, k0, k1, vp, v0, v1, _list(seqs, self.ctx, "seqs"),
             None if pos is None else _list(pos, self.ctx, "pos", n), n), "kv_append")
@@ -225,29 +247,64 @@ class PagedKV:
 _DELTA = struct.Struct("=10Q23q2d")
 
 
-def delta_args(ctx, q, k, v, g, beta, state, out, cu, ws, slots, scale, norm, eps, fresh, frac,
-               out_frac):
-    """The checked arguments of one delta-rule call, packed as w4a8_delta."""
+def _delta_fault(ctx, q, k, v, g, beta, state, out):
+    """What is wrong with the tensors of a delta-rule call, as a ValueError."""
     if q.dim() != 3 or v.dim() != 3 or state.dim() != 4:
         raise ValueError("q, k [tokens, hk, dk], v, out [tokens, hv, dv] and "
                          "state [slots, hv, dk, dv] are required")
     tokens, hk, dk = q.shape
     hv, dv = v.shape[1], v.shape[2]
-    dt = _dtypes().get(q.dtype)
-    if dt is None:
+    if _dtypes().get(q.dtype) is None:
         raise ValueError(f"q: float32, bfloat16, float16 or int16, not {q.dtype}")
-    qp, q0, q1 = _act(q, ctx, "q", (tokens, hk, dk))
-    kp, k0, k1 = _act(k, ctx, "k", (tokens, hk, dk), q.dtype)
-    vp, v0, v1 = _act(v, ctx, "v", (tokens, hv, dv), q.dtype)
-    op, o0, o1 = _act(out, ctx, "out", (tokens, hv, dv), q.dtype)
-    gp, g0 = _gate(g, ctx, "g", (tokens, hv))
-    bp, b0 = _gate(beta, ctx, "beta", (tokens, hv))
+    _act(q, ctx, "q", (tokens, hk, dk))
+    _act(k, ctx, "k", (tokens, hk, dk), q.dtype)
+    _act(v, ctx, "v", (tokens, hv, dv), q.dtype)
+    _act(out, ctx, "out", (tokens, hv, dv), q.dtype)
+    _gate(g, ctx, "g", (tokens, hv))
+    _gate(beta, ctx, "beta", (tokens, hv))
     _on(state, ctx, "state")
-    if state.shape[1:] != (hv, dk, dv) or not state.is_contiguous() or \
-            _dtypes().get(state.dtype) != N.DT_F32:
-        raise ValueError(f"state: must be contiguous float32 [slots, {hv}, {dk}, {dv}]")
+    raise ValueError(f"state: must be contiguous float32 [slots, {hv}, {dk}, {dv}]")
+
+
+def delta_args(ctx, q, k, v, g, beta, state, out, cu, ws, slots, scale, norm, eps, fresh, frac,
+               out_frac):
+    """The checked arguments of one delta-rule call, packed as w4a8_delta.
+    The checks of the tensors are one condition (a step is a few microseconds
+    on the device); what does not hold is told by _delta_fault."""
+    dts, dev, qt = _dtypes(), ctx.device, q.dtype
+    dt = dts.get(qt)
+    try:
+        tokens, hk, dk = qs = q.shape
+        _, hv, dv = vs = v.shape
+        q0, q1, q2 = q.stride()
+        k0, k1, k2 = k.stride()
+        v0, v1, v2 = v.stride()
+        o0, o1, o2 = out.stride()
+        g0, g1 = g.stride()
+        b0, b1 = beta.stride()
+        slots_n, *heads = state.shape
+        fine = (dt is not None and q.get_device() == dev and k.get_device() == dev
+                and v.get_device() == dev and out.get_device() == dev and g.get_device() == dev
+                and beta.get_device() == dev and state.get_device() == dev
+                and k.dtype is qt and v.dtype is qt and out.dtype is qt
+                and k.shape == qs and out.shape == vs and vs[0] == tokens
+                and g.shape == beta.shape == (tokens, hv) and heads == [hv, dk, dv]
+                and q2 == k2 == v2 == o2 == 1 and (g1 == b1 == 1 or hv == 1)
+                and dts.get(g.dtype) == dts.get(beta.dtype) == dts.get(state.dtype) == N.DT_F32
+                and state.is_contiguous())
+    except (AttributeError, TypeError, ValueError):
+        fine = False
+    if not fine:
+        _delta_fault(ctx, q, k, v, g, beta, state, out)
+    # the stride of a dimension of one entry is never used
+    if tokens == 1:
+        q0 = k0 = v0 = o0 = g0 = b0 = 0
+    if hk == 1:
+        q1 = k1 = 0
+    if hv == 1:
+        v1 = o1 = 0
     rows = tokens if cu is None else cu.shape[0] - 1
-    if cu is not None and rows < 0:
+    if rows < 0:
         raise ValueError("cu: needs an entry per row and one more")
     wp, wb = 0, 0
     if ws is not None:
@@ -256,10 +313,11 @@ def delta_args(ctx, q, k, v, g, beta, state, out, cu, ws, slots, scale, norm, ep
             raise ValueError("ws: must be contiguous")
         wp, wb = ws.data_ptr(), ws.nbytes
     return _DELTA.pack(
-        qp, kp, vp, gp, bp, state.data_ptr(), op,
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(),
+        state.data_ptr(), out.data_ptr(),
         0 if slots is None else _list(slots, ctx, "slots", rows),
         0 if cu is None else _list(cu, ctx, "cu"), wp, wb,
-        q0, q1, k0, k1, v0, v1, o0, o1, g0, b0, tokens, rows, hk, hv, dk, dv, state.shape[0], dt,
+        q0, q1, k0, k1, v0, v1, o0, o1, g0, b0, tokens, rows, hk, hv, dk, dv, slots_n, dt,
         frac, out_frac, 1 if norm else 0, 1 if fresh else 0,
         1.0 / math.sqrt(dk) if scale is None else scale, eps)
 
