@@ -136,6 +136,11 @@ constexpr float kNoDecay = -200.f;               // e^g is 0 in float32 from her
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 
+// terms of what goes into outputs alone
+template <typename T>
+constexpr int out_terms() {
+  return __is_same(T, __bf16) || __is_same(T, _Float16) ? 2 : 3;
+}
 template <typename T>
 struct Terms {
   static constexpr int n = sizeof(T) == 4 ? 3 : __is_same(T, __bf16) ? 1 : 2;
@@ -261,7 +266,7 @@ struct Space {
 // made transposed (rows j, columns t), which leaves a lane with four
 // neighbouring slots of their operand: nothing is rearranged.
 template <int DK, typename T>
-__global__ __launch_bounds__(256) void delta_prep_kernel(Delta p) {
+__global__ __launch_bounds__(256, 3) void delta_prep_kernel(Delta p) {
   constexpr int NK = Terms<T>::n, NS = DK / 32, LD = 68, HEADS = 4;
   __shared__ bf16x8 Ks[4][NS][NK][64];             // K by row tiles, as operand
   __shared__ double Gs[HEADS][C];                  // log2(e) times the running sum of g
@@ -359,8 +364,9 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Delta p) {
       }
   }
   // row tile w of M (which 0) or P out of its transposed tiles X[c], c <= w
-  auto store = [&](uint8_t *ws, int which, const f32x4 *X) {
-    bf16x8 *out = (bf16x8 *)(ws + which * kTriBytes) + lane;
+  auto store = [&](uint8_t *ws, auto which, const f32x4 *X) {
+    constexpr int N = which.value ? out_terms<T>() : 3;
+    bf16x8 *out = (bf16x8 *)(ws + which.value * kTriBytes) + lane;
 #pragma unroll
     for (int s = 0; s < 2; ++s)
       if (s <= w >> 1) {
@@ -368,9 +374,9 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Delta p) {
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = X[2 * s + (j >> 2)][j & 3];
-        split<3, 8>(x, t);
+        split<N, 8>(x, t);
 #pragma unroll
-        for (int i = 0; i < 3; ++i) out[(tri_of(w, s) * 3 + i) * 64] = t[i];
+        for (int i = 0; i < N; ++i) out[(tri_of(w, s) * 3 + i) * 64] = t[i];
       }
   };
 
@@ -419,7 +425,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Delta p) {
             }
           }
         }
-        store(ws, 1, P);
+        store(ws, Int<1>(), P);
       }
       __syncthreads();
       {   // the inverse of diagonal block w: lane r column r, by substitution
@@ -458,7 +464,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Delta p) {
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c) X[c] *= *(const f32x4 *)(betas[b] + 16 * c + 4 * g);
-        store(ws, 0, X);
+        store(ws, Int<0>(), X);
       }
     }
     __syncthreads();                 // betas are read
@@ -470,9 +476,8 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Delta p) {
 // S, on four of them and the outputs, b Q S0 + P U, on the other four, so that
 // the chain's trips through LDS are filled with the outputs' products.  Where
 // there is one row, a chunk's chain and the instructions issued along it are
-// what bounds the kernel.  So every operand of the next chunk is loaded right
-// after this chunk's use of it, spread over the step, by offsets from the
-// chunk's first token that are the same in every whole chunk.
+// what bounds the kernel.  So every operand is loaded right after an earlier
+// chunk's use of its registers, spread over the step.
 //
 // Wavefront w of the chain has rows 32 w .. of the state too: lane (r, g) rows
 // 32 w + 8 g + e of column r, in register [e & 1][e >> 1], which is its slots
@@ -484,9 +489,10 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Delta p) {
 template <int DK, typename T>
 __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
   constexpr int NK = Terms<T>::n, NS = DK / 32;
-  constexpr int OT = __is_same(T, __bf16) || __is_same(T, _Float16) ? 2 : 3;
+  constexpr int OT = out_terms<T>();
   __shared__ bf16x8 Sb[3][NS][64];                // the state, k-step s by wavefront s
   __shared__ __align__(16) bf16x4 Rb[3][2][64][2], Ub[OT][2][64][2], Wb[3][2][64][2];
+  __shared__ __align__(16) T Ts[8][16 * 16];      // a wavefront's tokens' values or outputs
   const int tiles = p.dv / 16, units = p.rows * p.hv, each = (units + 7) / 8;
   // a head's columns, and heads that share keys, on one XCD (workgroups go
   // round the eight of them)
@@ -524,11 +530,23 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
   auto factor = [&](int which) {
     return *(const f32x4 *)((const float *)(ws + 2 * kTriBytes) + 64 * which + 16 * w + 4 * g);
   };
-  // where a chunk's values lie, in bytes from its first token; past its end of
-  // len tokens the last one's are read, whose factors and columns of M and P
-  // are zeros
-  auto row_at = [&](int t, int len, int64_t token) {
-    return (uint32_t)(min(t, len - 1) * (int)token + col) * (uint32_t)sizeof(T);
+  // Values and outputs move in pieces of 16 bytes, PIECES a row of 16 columns
+  // (single values would be four loads and four stores for one), and change
+  // between pieces and results' places in LDS, within a wavefront.  piece_at:
+  // where this lane's lies, in bytes from a chunk's first token; past the
+  // chunk's end of len tokens the last one's is read, whose factors and
+  // columns of M and P are zeros.
+  constexpr int PIECES = sizeof(T);
+  const int prow = (lane / PIECES) & 15, piece = lane % PIECES;
+  T *tile = &Ts[wave][0];
+  auto piece_at = [&](int len, int64_t token) {
+    return (uint32_t)(min(16 * w + prow, len - 1) * (int)token + col - r) * (uint32_t)sizeof(T) +
+           (uint32_t)piece * 16;
+  };
+  auto exchange = [&]() {                         // a wavefront's writes before its reads
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
   };
 
   auto chain = [&](auto upper) {
@@ -562,34 +580,39 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
     const int64_t kt_off = Space<DK, T>::kRows / 3 * 2;
     const uint8_t *vb = (const uint8_t *)((const T *)p.v + begin * p.v_token + h * p.v_head);
     const int64_t v_step = p.v_token * C * (int)sizeof(T);
-    uint32_t v_at[4];
-    auto offsets = [&](int len) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v_at[i] = row_at(16 * w + 4 * g + i, len, p.v_token);
+    uint32_t v_at = piece_at(C, p.v_token);
+    struct In {
+      bf16x8 k[NS][NK], m[2][3], kt[2][2][NK];
+      u32x4 v;
+      f32x4 a, c;
+      float fall;
     };
-    bf16x8 k[NS][NK], m[2][3], kt[2][2][NK];
-    T v[4];
-    f32x4 a, c;
-    float fall;
-    auto load_rows = [&]() {
+    const uint8_t *const kb0 = kb, *const vb0 = vb, *const ws0 = ws;
+    auto next = [&](int ch) {                     // its operands are loaded from here on
+      ch = min(ch, n - 1);
+      kb = kb0 + ch * space.kRows;
+      vb = vb0 + ch * v_step;
+      ws = ws0 + (int64_t)ch * kHeadBytes;
+      if (end - begin - ch * C < C) v_at = piece_at(end - begin - ch * C, p.v_token);
+    };
+    auto load_rows = [&](In &x) {
 #pragma unroll
       for (int i = 0; i < NK; ++i)
 #pragma unroll
         for (int s = 0; s < NS; ++s)
-          k[s][i] = ((const bf16x8 *)kb + ((w * NS + s) * NK + i) * 64)[lane];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = *(const T *)(vb + v_at[i]);
-      a = factor(0);
+          x.k[s][i] = ((const bf16x8 *)kb + ((w * NS + s) * NK + i) * 64)[lane];
+      x.v = *(const u32x4 *)(vb + v_at);
+      x.a = factor(0);
     };
-    auto load_solve = [&]() {
+    auto load_solve = [&](In &x) {
 #pragma unroll
       for (int i = 0; i < 3; ++i) {
-        m[0][i] = tri(0, 0, i);
-        if constexpr (HI) m[1][i] = tri(0, 1, i);
+        x.m[0][i] = tri(0, 0, i);
+        if constexpr (HI) x.m[1][i] = tri(0, 1, i);
       }
-      c = factor(2);
+      x.c = factor(2);
     };
-    auto load_update = [&]() {
+    auto load_update = [&](In &x) {
       if constexpr (STATE) {
 #pragma unroll
         for (int s = 0; s < 2; ++s)
@@ -597,45 +620,38 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
           for (int e = 0; e < 2; ++e)
 #pragma unroll
             for (int i = 0; i < NK; ++i)
-              kt[s][e][i] =
+              x.kt[s][e][i] =
                   ((const bf16x8 *)(kb + kt_off) + (((w * 2 + s) * 2 + e) * NK + i) * 64)[lane];
-        fall = ((const float *)(ws + 2 * kTriBytes) + 192)[lane];
+        x.fall = ((const float *)(ws + 2 * kTriBytes) + 192)[lane];
       }
     };
-    offsets(min(C, end - begin));
-    if constexpr (STATE) put_state();
-    // in the loop's order, so that its waits are for what it uses
-    __builtin_amdgcn_sched_barrier(0);
-    load_rows();
-    __builtin_amdgcn_sched_barrier(0);
-    load_solve();
-    __builtin_amdgcn_sched_barrier(0);
-    load_update();
-    lds_barrier();
-    for (int ch = 0; ch < n; ++ch) {
+    // Loads go out behind a segment's reads of LDS, in the time those take.
+    auto step = [&](int ch, In &x) {
       const int len = min(C, end - begin - ch * C);
-      if (ch + 1 < n) {
-        kb += space.kRows;
-        vb += v_step;
-        ws += kHeadBytes;
-        if (len < 2 * C && end - begin - (ch + 1) * C < C) offsets(end - begin - (ch + 1) * C);
-      }
       {
         bf16x8 sb[NS][3];
+        T v[4];
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
           for (int i = 0; i < 3; ++i) sb[s][i] = Sb[i][s][lane];
-        f32x4 ks{0, 0, 0, 0}, x;
+        *(u32x4 *)(tile + prow * 16 + piece * (16 / (int)sizeof(T))) = x.v;
+        exchange();
 #pragma unroll
-        for (int s = 0; s < NS; ++s) ks = mfma_terms<NK, 3, 2>(k[s], sb[s], ks);
+        for (int i = 0; i < 4; ++i) v[i] = tile[(4 * g + i) * 16 + r];
+        __builtin_amdgcn_sched_barrier(0);
+        load_update(x);
+        __builtin_amdgcn_sched_barrier(0);
+        f32x4 ks{0, 0, 0, 0}, z;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) ks = mfma_terms<NK, 3, 2>(x.k[s], sb[s], ks);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          x[i] = (16 * w + 4 * g + i < len ? to_float(v[i], p.unit) : 0.f) - a[i] * ks[i];
-        put_rows(Rb, x, Int<3>());
+          z[i] = (16 * w + 4 * g + i < len ? to_float(v[i], p.unit) : 0.f) - x.a[i] * ks[i];
+        put_rows(Rb, z, Int<3>());
       }
-      load_rows();
       lds_barrier();
+      next(ch + 1);
       {
         bf16x8 b[2][3];
 #pragma unroll
@@ -643,12 +659,14 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
           b[0][i] = *(const bf16x8 *)Rb[i][0][lane];
           if constexpr (HI) b[1][i] = *(const bf16x8 *)Rb[i][1][lane];
         }
-        f32x4 u = mfma_terms<3, 3, 2>(m[0], b[0], f32x4{0, 0, 0, 0});
-        if constexpr (HI) u = mfma_terms<3, 3, 2>(m[1], b[1], u);
-        put_rows(Wb, u * c, Int<3>());
+        __builtin_amdgcn_sched_barrier(0);
+        load_rows(x);
+        __builtin_amdgcn_sched_barrier(0);
+        f32x4 u = mfma_terms<3, 3, 2>(x.m[0], b[0], f32x4{0, 0, 0, 0});
+        if constexpr (HI) u = mfma_terms<3, 3, 2>(x.m[1], b[1], u);
+        put_rows(Wb, u * x.c, Int<3>());
         put_rows(Ub, u, Int<OT>());
       }
-      load_solve();
       lds_barrier();
       if constexpr (STATE) {
         bf16x8 b[2][3];
@@ -657,18 +675,33 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
           b[0][i] = *(const bf16x8 *)Wb[i][0][lane];
           b[1][i] = *(const bf16x8 *)Wb[i][1][lane];
         }
-        S[0] *= fall;
-        S[1] *= fall;
+        __builtin_amdgcn_sched_barrier(0);
+        load_solve(x);
+        __builtin_amdgcn_sched_barrier(0);
+        S[0] *= x.fall;
+        S[1] *= x.fall;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          S[0] = mfma_terms<NK, 3, 2>(kt[s][0], b[s], S[0]);
-          S[1] = mfma_terms<NK, 3, 2>(kt[s][1], b[s], S[1]);
+          S[0] = mfma_terms<NK, 3, 2>(x.kt[s][0], b[s], S[0]);
+          S[1] = mfma_terms<NK, 3, 2>(x.kt[s][1], b[s], S[1]);
         }
         put_state();
-        load_update();
+      } else {
+        load_solve(x);
       }
       lds_barrier();
-    }
+    };
+    // the first chunks' operands, in the order of the loop, so that its waits
+    // are for what it uses
+    In in;
+    if constexpr (STATE) put_state();
+    next(0);
+    __builtin_amdgcn_sched_barrier(0);
+    load_rows(in);
+    __builtin_amdgcn_sched_barrier(0);
+    load_solve(in);
+    lds_barrier();
+    for (int ch = 0; ch < n; ++ch) step(ch, in);
     if constexpr (STATE)
 #pragma unroll
       for (int e = 0; e < 2; ++e)
@@ -681,72 +714,72 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
     const uint8_t *qb = (const uint8_t *)space.rows(hk, 1);
     uint8_t *ob = (uint8_t *)((T *)p.out + begin * p.out_token + h * p.out_head);
     const int64_t o_step = p.out_token * C * (int)sizeof(T);
-    uint32_t o_at[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o_at[i] = row_at(16 * w + 4 * g + i, C, p.out_token);
+    const uint32_t o_at = piece_at(C, p.out_token);
     bf16x8 q[NS][NK], m[2][OT];
-    f32x4 b;
-    auto load_rows = [&]() {
+    f32x4 b, o{0, 0, 0, 0};
+    const uint8_t *const qb0 = qb, *const ws0 = ws;
+    // a chunk's rows of Q and their factors; its rows of P
+    auto load_rows = [&](int ch) {
+      qb = qb0 + ch * space.kRows;
+      ws = ws0 + (int64_t)ch * kHeadBytes;
 #pragma unroll
       for (int i = 0; i < NK; ++i)
 #pragma unroll
         for (int s = 0; s < NS; ++s)
           q[s][i] = ((const bf16x8 *)qb + ((w * NS + s) * NK + i) * 64)[lane];
+      b = factor(1);
     };
-    auto load_weights = [&]() {
+    auto load_weights = [&](int ch) {
+      ws = ws0 + (int64_t)ch * kHeadBytes;
 #pragma unroll
       for (int i = 0; i < OT; ++i) {
         m[0][i] = tri(1, 0, i);
         if constexpr (HI) m[1][i] = tri(1, 1, i);
       }
-      b = factor(1);
     };
-    load_rows();
-    __builtin_amdgcn_sched_barrier(0);
-    load_weights();
+    auto write = [&](int ch) {
+      const int len = min(C, end - begin - ch * C);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tile[(4 * g + i) * 16 + r] = from_float<T>(o[i], p.out_unit);
+      exchange();
+      const u32x4 x = *(const u32x4 *)(tile + prow * 16 + piece * (16 / (int)sizeof(T)));
+      if (lane < 16 * PIECES && 16 * w + prow < len) *(u32x4 *)(ob + o_at) = x;
+      ob += o_step;
+    };
+    load_rows(0);
+    load_weights(0);
     lds_barrier();
     for (int ch = 0; ch < n; ++ch) {
-      const int len = min(C, end - begin - ch * C);
-      if (ch + 1 < n) {
-        qb += space.kRows;
-        ws += kHeadBytes;
-      }
-      f32x4 o{0, 0, 0, 0};
+      // beside the chain's first segment the last chunk's outputs are written,
+      // beside its second Q S0 is made, beside its third P U: no segment has
+      // more than its share of the loads and stores
+      if (ch) write(ch - 1);
+      lds_barrier();
       {
         bf16x8 sb[NS][OT];
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
           for (int i = 0; i < OT; ++i) sb[s][i] = Sb[i][s][lane];
+        o = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < NS; ++s) o = mfma_terms<NK, OT, OT - 1>(q[s], sb[s], o);
         o *= b;
       }
-      load_rows();
+      load_rows(min(ch + 1, n - 1));
       lds_barrier();
-      lds_barrier();
-      {
-        bf16x8 ub[2][OT];
+      bf16x8 ub[2][OT];
 #pragma unroll
-        for (int i = 0; i < OT; ++i) {
-          ub[0][i] = *(const bf16x8 *)Ub[i][0][lane];
-          if constexpr (HI) ub[1][i] = *(const bf16x8 *)Ub[i][1][lane];
-        }
-        o = mfma_terms<OT, OT, OT - 1>(m[0], ub[0], o);
-        if constexpr (HI) o = mfma_terms<OT, OT, OT - 1>(m[1], ub[1], o);
+      for (int i = 0; i < OT; ++i) {
+        ub[0][i] = *(const bf16x8 *)Ub[i][0][lane];
+        if constexpr (HI) ub[1][i] = *(const bf16x8 *)Ub[i][1][lane];
       }
-      load_weights();
-      if (len == C) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) *(T *)(ob + o_at[i]) = from_float<T>(o[i], p.out_unit);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (16 * w + 4 * g + i < len) *(T *)(ob + o_at[i]) = from_float<T>(o[i], p.out_unit);
-      }
-      ob += o_step;
+      o = mfma_terms<OT, OT, OT - 1>(m[0], ub[0], o);
+      if constexpr (HI) o = mfma_terms<OT, OT, OT - 1>(m[1], ub[1], o);
+      load_weights(min(ch + 1, n - 1));
       lds_barrier();
     }
+    write(n - 1);
   };
   // the same number of barriers on every way
   if (wave < 4) {
