@@ -62,14 +62,30 @@ __device__ __forceinline__ void load_refs(const KvCache &kv, int p0, int past, i
   }
 }
 
+// The counts of a thread's share of the first kOne * kRefsPerThread pages, so
+// that the scans' first turn does not wait for them.
+struct FirstRefs {
+  int r[kRefsPerThread];
+};
+__device__ __forceinline__ FirstRefs first_refs(const KvCache &kv, int past) {
+  FirstRefs f;
+  load_refs(kv, (int)threadIdx.x * kRefsPerThread, past, f.r);
+  return f;
+}
+
 // the need lowest free pages, in order, to list; how many there were (fewer
 // than need: not enough).  One workgroup.
-__device__ int find_free(const KvCache &kv, int need, int32_t *list) {
+__device__ int find_free(const KvCache &kv, int need, int32_t *list, const FirstRefs &f) {
   int found = 0;
   for (int base = 0; base < kv.pages && found < need; base += kOne * kRefsPerThread) {
     int r[kRefsPerThread], mine = 0, all;
     const int p0 = base + (int)threadIdx.x * kRefsPerThread;
-    load_refs(kv, p0, 1, r);
+    if (base == 0) {
+#pragma unroll
+      for (int i = 0; i < kRefsPerThread; ++i) r[i] = f.r[i];
+    } else {
+      load_refs(kv, p0, 1, r);
+    }
 #pragma unroll
     for (int i = 0; i < kRefsPerThread; ++i) mine += r[i] == 0;
     int at = found + scan_excl(mine, &all);
@@ -92,6 +108,7 @@ __device__ int find_free(const KvCache &kv, int need, int32_t *list) {
 __global__ __launch_bounds__(kOne) void kv_extend_kernel(KvCache kv, const int32_t *seqs,
                                                          const int32_t *counts, int n) {
   __shared__ int bad;
+  const FirstRefs refs = first_refs(kv, 1);
   int32_t *mark = marks(kv), *list = list_a(kv);
   if (threadIdx.x == 0) bad = 0;
   __syncthreads();
@@ -113,7 +130,7 @@ __global__ __launch_bounds__(kOne) void kv_extend_kernel(KvCache kv, const int32
   }
   int all;
   scan_excl(need, &all);        // synchronises: bad is whole
-  if (!bad && all > 0 && find_free(kv, all, list) < all) {
+  if (!bad && all > 0 && find_free(kv, all, list, refs) < all) {
     if (threadIdx.x == 0) bad = kErrKvFull;
   }
   __syncthreads();
@@ -171,6 +188,7 @@ __global__ __launch_bounds__(kOne) void kv_extend_kernel(KvCache kv, const int32
 __global__ __launch_bounds__(kOne) void kv_fork_kernel(KvCache kv, const int32_t *parents,
                                                        const int32_t *children, int n) {
   __shared__ int bad;
+  const FirstRefs refs = first_refs(kv, 1);
   int32_t *mark = marks(kv), *job = jobs(kv), *list = list_a(kv);
   if (threadIdx.x == 0) bad = 0;
   __syncthreads();
@@ -199,7 +217,7 @@ __global__ __launch_bounds__(kOne) void kv_fork_kernel(KvCache kv, const int32_t
   }
   __syncthreads();
   const bool fine = bad == 0;
-  if (fine && all > 0 && find_free(kv, all, list) < all) {
+  if (fine && all > 0 && find_free(kv, all, list, refs) < all) {
     if (threadIdx.x == 0) bad = kErrKvFull;
   }
   __syncthreads();
@@ -306,22 +324,34 @@ __global__ __launch_bounds__(256) void kv_free_kernel(KvCache kv, const int32_t 
 // scratch[0] = moves, scratch[1] = U.
 __global__ __launch_bounds__(kOne) void kv_compact_kernel(KvCache kv) {
   int32_t *holes = list_a(kv), *to = list_b(kv);
+  FirstRefs refs = first_refs(kv, 0);
   int used = 0, U;
-  for (int p0 = (int)threadIdx.x * kRefsPerThread; p0 < kv.pages; p0 += kOne * kRefsPerThread) {
+#pragma unroll
+  for (int i = 0; i < kRefsPerThread; ++i) used += refs.r[i] != 0;
+  const int turn = kOne * kRefsPerThread;
+  for (int p0 = turn + (int)threadIdx.x * kRefsPerThread; p0 < kv.pages; p0 += turn) {
     int r[kRefsPerThread];
     load_refs(kv, p0, 0, r);
 #pragma unroll
     for (int i = 0; i < kRefsPerThread; ++i) used += r[i] != 0;
   }
   scan_excl(used, &U);
-  const int moves = find_free(kv, U, holes);   // free pages, lowest first, up to U of them
+  FirstRefs free = refs;          // past the last page: not free
+#pragma unroll
+  for (int i = 0; i < kRefsPerThread; ++i)
+    if ((int)threadIdx.x * kRefsPerThread + i >= kv.pages) free.r[i] = 1;
+  const int moves = find_free(kv, U, holes, free);   // free pages, lowest first, up to U of them
   // those below U are the holes: as many as pages in use at U or above
   int from = 0;
-  const int first = U / kRefsPerThread * kRefsPerThread;
-  for (int base = first; base < kv.pages; base += kOne * kRefsPerThread) {
+  for (int base = U / turn * turn; base < kv.pages; base += kOne * kRefsPerThread) {
     const int p0 = base + (int)threadIdx.x * kRefsPerThread;
     int r[kRefsPerThread], mine = 0, all;
-    load_refs(kv, p0, 0, r);
+    if (base == 0) {
+#pragma unroll
+      for (int i = 0; i < kRefsPerThread; ++i) r[i] = refs.r[i];
+    } else {
+      load_refs(kv, p0, 0, r);
+    }
 #pragma unroll
     for (int i = 0; i < kRefsPerThread; ++i) mine += r[i] != 0 && p0 + i >= U;
     int at = from + scan_excl(mine, &all);
@@ -402,49 +432,62 @@ __global__ __launch_bounds__(256) void kv_copy_kernel(KvCache kv, const int32_t 
 }
 
 // ------------------------------------------------------------------- append
-template <typename T>
-__device__ __forceinline__ T from_float(float x) {
-  return (T)x;
-}
-
-// 16 bytes of the cache per thread and turn; rows are tokens
+// A wavefront per token: its keys and values, 16 bytes of the cache a lane, are
+// on their way while the token's place is looked up.
+constexpr int kAppendWaves = 4;
 template <typename T, bool I16>
-__global__ __launch_bounds__(256) void kv_append_kernel(KvCache kv, KvAppend a) {
-  constexpr int V = 16 / sizeof(T);
-  const int per = kv.heads * kv.dim / V;      // vectors of a token's keys
-  const int64_t all = (int64_t)a.n * per * 2;
-  for (int64_t w = blockIdx.x * 256ll + threadIdx.x; w < all; w += gridDim.x * 256ll) {
-    const int i = (int)(w / (2 * per));
-    const int x = (int)(w - (int64_t)i * 2 * per);
-    const int which = x >= per;
-    const int e = (x - which * per) * V, h = e / kv.dim, d = e - h * kv.dim;
-    const int s = a.seqs[i];
-    if (s < 0) continue;
-    bool ok = s < kv.seqs;
-    int page = -1, pos = 0;
-    if (ok) {
-      const int len = kv.lens[s];
-      pos = a.pos ? a.pos[i] : len - 1;
-      ok = pos >= 0 && pos < len && (pos >> kv.lg_page) < kv.max_pages;
-      if (ok) page = kv.tables[(int64_t)s * kv.max_pages + (pos >> kv.lg_page)];
-      ok = ok && (uint32_t)page < (uint32_t)kv.pages;
-    }
-    if (!ok) {
-      if (x == 0) atomicOr(kv.err, kErrKvRange);
-      continue;
-    }
+__global__ __launch_bounds__(64 * kAppendWaves) void kv_append_kernel(KvCache kv, KvAppend a) {
+  constexpr int V = 16 / sizeof(T), U = 4;
+  const int lane = threadIdx.x & 63;
+  const int i = blockIdx.x * kAppendWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (i >= a.n) return;
+  const int lg = __builtin_ctz(kv.dim / V);   // vectors of a head's row
+  const int per = kv.heads << lg, all = 2 * per;
+  auto load = [&](int x, T *v) {
+    const int which = x >= per, y = x - which * per;
+    const int h = y >> lg, d = (y - (h << lg)) * V;
     const int64_t at = i * (which ? a.v_token : a.k_token) + h * (which ? a.v_head : a.k_head) + d;
     const void *src = which ? a.v : a.k;
-    uint8_t *dst = kv.pool + page * kv.page_bytes +
-                   ((((int64_t)a.layer * 2 + which) * kv.heads + h) * kv.page() +
-                    (pos & (kv.page() - 1))) * kv.dim * (int)sizeof(T) + d * (int)sizeof(T);
     if constexpr (I16) {
-      T v[V];
+      int16_t w[V];
+      __builtin_memcpy(w, (const int16_t *)src + at, sizeof(w));
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = from_float<T>(((const int16_t *)src)[at + j] * a.unit);
-      *(u32x4 *)dst = *(const u32x4 *)v;
+      for (int j = 0; j < V; ++j) v[j] = (T)(w[j] * a.unit);
     } else {
-      *(u32x4 *)dst = load16_nt((const T *)src + at);
+      *(u32x4 *)v = load16_nt((const T *)src + at);
+    }
+  };
+  alignas(16) T v[U][V];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (lane + 64 * u < all) load(lane + 64 * u, v[u]);
+  const int s = a.seqs[i];
+  if (s < 0) return;
+  bool ok = s < kv.seqs;
+  int page = -1, pos = 0;
+  if (ok) {
+    const int len = kv.lens[s];
+    pos = a.pos ? a.pos[i] : len - 1;
+    ok = pos >= 0 && pos < len && (pos >> kv.lg_page) < kv.max_pages;
+    if (ok) page = kv.tables[(int64_t)s * kv.max_pages + (pos >> kv.lg_page)];
+    ok = ok && (uint32_t)page < (uint32_t)kv.pages;
+  }
+  if (!ok) {
+    if (lane == 0) atomicOr(kv.err, kErrKvRange);
+    return;
+  }
+  uint8_t *base = kv.pool + page * kv.page_bytes +
+                  ((int64_t)a.layer * 2 * kv.heads * kv.page() + (pos & (kv.page() - 1))) *
+                      kv.dim * (int)sizeof(T);
+  const int64_t row = (int64_t)kv.page() * kv.dim * (int)sizeof(T);   // from a head to the next
+  for (int x0 = lane; x0 < all; x0 += 64 * U) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int x = x0 + 64 * u;
+      if (x < all) {
+        if (x0 != lane) load(x, v[u]);
+        *(u32x4 *)(base + (x >> lg) * row + (x & ((1 << lg) - 1)) * 16) = *(const u32x4 *)v[u];
+      }
     }
   }
 }
@@ -485,19 +528,17 @@ hipError_t launch_kv_copy(const KvCache &kv, const int32_t *src, const int32_t *
 }
 
 hipError_t launch_kv_append(const KvCache &kv, const KvAppend &a, hipStream_t s) {
-  const int64_t vecs = (int64_t)a.n * 2 * kv.heads * kv.dim * kv.esize / 16;
-  const int64_t want = (vecs + 255) / 256;
-  const int grid = (int)(want < 16384 ? want : 16384);
+  const int grid = (a.n + kAppendWaves - 1) / kAppendWaves, threads = 64 * kAppendWaves;
   const bool i16 = a.dtype == DT_I16;
   if (kv.dtype == DT_F32) {
-    if (i16) kv_append_kernel<float, true><<<grid, 256, 0, s>>>(kv, a);
-    else kv_append_kernel<float, false><<<grid, 256, 0, s>>>(kv, a);
+    if (i16) kv_append_kernel<float, true><<<grid, threads, 0, s>>>(kv, a);
+    else kv_append_kernel<float, false><<<grid, threads, 0, s>>>(kv, a);
   } else if (kv.dtype == DT_BF16) {
-    if (i16) kv_append_kernel<__bf16, true><<<grid, 256, 0, s>>>(kv, a);
-    else kv_append_kernel<__bf16, false><<<grid, 256, 0, s>>>(kv, a);
+    if (i16) kv_append_kernel<__bf16, true><<<grid, threads, 0, s>>>(kv, a);
+    else kv_append_kernel<__bf16, false><<<grid, threads, 0, s>>>(kv, a);
   } else {
-    if (i16) kv_append_kernel<_Float16, true><<<grid, 256, 0, s>>>(kv, a);
-    else kv_append_kernel<_Float16, false><<<grid, 256, 0, s>>>(kv, a);
+    if (i16) kv_append_kernel<_Float16, true><<<grid, threads, 0, s>>>(kv, a);
+    else kv_append_kernel<_Float16, false><<<grid, threads, 0, s>>>(kv, a);
   }
   return hipGetLastError();
 }
