@@ -386,7 +386,8 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(Delta p) {
       const int h = hk * per + first + w;
       const bool on = lane < len;
       const int64_t t = t0 + min(lane, len - 1);
-      const float gt = on ? fmaxf(p.g[t * p.g_token + h], kNoDecay) : 0.f;
+      float gt = on ? p.g[t * p.g_token + h] : 0.f;
+      gt = gt < kNoDecay ? kNoDecay : gt;          // a NaN stays one
       const float bt = on ? p.beta[t * p.beta_token + h] : 0.f;
       double G = gt * 1.4426950408889634;
 #pragma unroll

@@ -111,7 +111,8 @@ def spans_of(lens):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("lens,hk,hv,dk,dv", [
     ([1], 1, 1, 64, 16), ([64], 1, 2, 64, 64), ([63, 65, 0, 1, 128], 2, 2, 128, 32),
-    ([0, 200], 1, 3, 128, 128), ([300], 2, 4, 128, 80), ([129, 7, 64, 2], 1, 2, 64, 256)])
+    ([0, 200], 1, 3, 128, 128), ([300], 2, 4, 128, 80), ([129, 7, 64, 2], 1, 2, 64, 256),
+    ([70, 40], 1, 6, 128, 16), ([5] * 40, 1, 1, 64, 16)])
 def test_chunk(engine, dtype, lens, hk, hv, dk, dv):
     gen = torch.Generator().manual_seed(sum(lens) + dv)
     cu = spans_of(lens)
@@ -212,6 +213,33 @@ def test_decays_from_none_to_all(engine, kind):
         engine.delta_chunk_async(**d, out=out, cu=c, ws=ws)
     engine.sync()
     check(out, d["state"], want)
+
+
+@pytest.mark.parametrize("kind", ["step", "chunk"])
+@pytest.mark.parametrize("name", ["q", "k", "v", "g", "beta"])
+def test_nan_stays_in_its_row(engine, kind, name):
+    # and reaches what depends on it: a token's outputs from there on
+    gen = torch.Generator().manual_seed(30)
+    lens = [1, 1] if kind == "step" else [100, 130]
+    cu = spans_of(lens)
+    d = inputs(gen, cu[-1], 1, 2, 64, 64, torch.float32, 2)
+    bad = 0 if kind == "step" else 70
+    want = recurrence(d, list(zip(cu[:-1], cu[1:])), [0, 1])
+    d[name][bad] = float("nan")
+    out, ws, c = torch.zeros_like(d["v"]), engine.delta_chunk_workspace(cu[-1], 2, 2), ints(cu)
+    torch.cuda.synchronize()
+    if kind == "step":
+        engine.delta_step_async(**d, out=out)
+    else:
+        engine.delta_chunk_async(**d, out=out, cu=c, ws=ws)
+    engine.sync()
+    assert torch.isnan(out[bad]).all()
+    assert name == "q" or torch.isnan(d["state"][0]).all()
+    # the chunks before it, and the other row
+    fine = [t for t in range(cu[-1]) if t >= cu[1] or t < bad // 64 * 64]
+    off = (out[fine].double().cpu() - want[0][fine]).abs()
+    assert (off <= want[2][fine][:, None, None] + 2.0 ** -24 * want[0][fine].abs()).all()
+    assert torch.isfinite(d["state"][1]).all()
 
 
 def test_values_far_from_one(engine):
