@@ -358,6 +358,9 @@ __global__ __launch_bounds__(kOne) void kv_compact_kernel(KvCache kv) {
     from += all;
 #pragma unroll
     for (int i = 0; i < kRefsPerThread; ++i)
+      if (r[i] == 0 && p0 + i >= U && p0 + i < kv.pages) to[p0 + i] = -1;
+#pragma unroll
+    for (int i = 0; i < kRefsPerThread; ++i)
       if (r[i] != 0 && p0 + i >= U) {
         const int hole = at < min(moves, U) ? holes[at] : -1;
         if (hole >= 0) {
@@ -400,10 +403,12 @@ __global__ __launch_bounds__(256) void kv_move_kernel(KvCache kv) {
     int32_t *row = kv.tables + (int64_t)s * kv.max_pages;
     for (int j = threadIdx.x; j < held; j += 256) {
       const int p = row[j];
-      if ((uint32_t)p >= (uint32_t)kv.pages)
+      if (p >= 0 && p < U) continue;
+      const int q = (uint32_t)p < (uint32_t)kv.pages ? to[p] : -1;
+      if (q < 0)              // no page, or one that no sequence holds
         atomicOr(kv.err, kErrKvRange);
-      else if (p >= U)
-        row[j] = to[p];
+      else
+        row[j] = q;
     }
   }
   const int64_t pieces = (kv.page_bytes + kPiece - 1) / kPiece;

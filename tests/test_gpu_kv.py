@@ -239,6 +239,25 @@ def test_append_strided_and_int16(engine, dtype):
         assert torch.equal(at[1], (i16[i, 2:, :128].double() / 512).to(dtype))
 
 
+def test_compact_reports_tables_that_disagree_with_the_counts(engine):
+    b = Both(engine, 9, 5, 6)
+    assert b.both("extend", [0, 1, 2], [40, 40, 20])
+    assert b.both("free", [0])
+    for wrong in (8, -3, 9):                       # a free page past the used ones; none at all
+        keep = int(b.kv.tables[1, 0])
+        b.kv.tables[1, 0] = wrong
+        torch.cuda.synchronize()
+        b.kv.compact_async()
+        with pytest.raises(AssertionError, match="outside the cache"):
+            engine.sync()
+        assert int(b.kv.tables[1, 0]) == wrong
+        b.kv.tables[1, 0] = keep
+        if wrong == 8:                             # the first call moved the rest
+            b.m.compact()
+            b.kv.tables[1, 0] = b.m.tables[1][0]
+    b.check()
+
+
 def test_copy_pages(engine):
     kv = PagedKV.empty(engine, 300, 3, 2, 16, 64, 1, 1, torch.bfloat16)
     kv.pool.normal_()
