@@ -2114,6 +2114,8 @@ int w4a8_kv_create(w4a8_ctx *c, int32_t dtype, int32_t pages, int32_t layers, in
   if (pages < 1 || pages > (1 << 30) || layers < 1 || layers > 65535 || kv_heads < 1 ||
       kv_heads > 4096 || seqs < 1 || seqs > (1 << 30) || max_pages < 1 || max_pages > (1 << 21))
     return fail(W4A8_E_ARG, "pages, layers, kv_heads, seqs or max_pages out of range");
+  if ((int64_t)max_pages * page_tokens > (1 << 30))
+    return fail(W4A8_E_ARG, "a sequence holds at most 2^30 tokens");
   if (!aligned16(d_pool) || !aligned16(d_refs) || ((uintptr_t)d_tables & 3) ||
       ((uintptr_t)d_lens & 3))
     return fail(W4A8_E_ARG, "pool and refs must be 16-byte, tables and lens 4-byte aligned");

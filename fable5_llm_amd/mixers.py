@@ -224,9 +224,9 @@ class PagedKV:
                                            _list(dst, self.ctx, "dst", n), n), "kv_copy")
 
     def close(self):
-        if self.h:
+        if self.h and self.ctx.h:
             N.lib().w4a8_kv_destroy(self.h)
-            self.h = None
+        self.h = None
 
     def __enter__(self):
         return self
@@ -236,8 +236,7 @@ class PagedKV:
 
     def __del__(self):
         try:
-            if self.h and self.ctx.h:
-                self.close()
+            self.close()
         except Exception:
             pass
 

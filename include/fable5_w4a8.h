@@ -427,7 +427,7 @@ int w4a8_plan_destroy(w4a8_plan *plan);
  *   lens    int32[seqs]: its tokens; the first ceil(len / page_tokens) entries
  *           of its table are in use
  * An empty cache is refs and lens of zeros.  page_tokens: a power of two,
- * 16..1024; head_dim: 64, 128 or 256.  The calls below change refs, tables
+ * 16..1024; head_dim: 64, 128 or 256; max_pages * page_tokens: at most 2^30.  The calls below change refs, tables
  * and lens on the context's stream, so calls on one cache from several
  * streams need ordering by the caller; one handle serves one cache (its
  * scratch memory is part of the cache's state). */

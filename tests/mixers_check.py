@@ -42,7 +42,8 @@ def check_cache():
                dict(page=8), dict(page=24), dict(page=2048), dict(dim=96), dict(dim=0),
                dict(seqs=0), dict(max_pages=0), dict(pool=None), dict(refs=None),
                dict(tables=None), dict(lens=None), dict(pool=ODD), dict(refs=ODD),
-               dict(tables=ODD), dict(lens=ODD), dict(pages=(1 << 30) + 1)):
+               dict(tables=ODD), dict(lens=ODD), dict(pages=(1 << 30) + 1),
+               dict(max_pages=(1 << 20) + 1, page=1024)):
         refused(lambda kw=kw: cache(**kw)[0])
     assert lib.w4a8_kv_destroy(None) == OK
     rt.fake_set(1, 0, 0, 0)              # the clearing of its scratch fails
