@@ -48,6 +48,20 @@ __device__ int scan_excl(int v, int *total) {
   return before + x - v;
 }
 
+// the sum of one value per thread, or most where it is above that (what a list
+// asks for can pass any integer); most and every value below 2^31
+__device__ uint32_t sum_up_to(uint32_t v, uint32_t most) {
+  __shared__ uint32_t sums[kOne / 64];
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v = min(v + __shfl_xor(v, d), most);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = v;
+  __syncthreads();
+  uint32_t all = 0;
+#pragma unroll
+  for (int w = 0; w < kOne / 64; ++w) all = min(all + sums[w], most);
+  return all;
+}
+
 // refs[p0 .. p0 + 16), pages past the end as 1 (in use) or 0
 __device__ __forceinline__ void load_refs(const KvCache &kv, int p0, int past, int *r) {
   if (p0 + kRefsPerThread <= kv.pages) {
@@ -112,7 +126,8 @@ __global__ __launch_bounds__(kOne) void kv_extend_kernel(KvCache kv, const int32
   int32_t *mark = marks(kv), *list = list_a(kv);
   if (threadIdx.x == 0) bad = 0;
   __syncthreads();
-  int need = 0;
+  const uint32_t over = (uint32_t)kv.pages + 1;   // more than there are
+  uint32_t need = 0;
   const int64_t most = (int64_t)kv.max_pages << kv.lg_page;
   for (int i = threadIdx.x; i < n; i += kOne) {
     const int s = seqs[i];
@@ -126,11 +141,12 @@ __global__ __launch_bounds__(kOne) void kv_extend_kernel(KvCache kv, const int32
     if (len < 0 || c < 0 || len + c > most || len + c > INT32_MAX)
       atomicOr(&bad, kErrKvRange);
     else
-      need += held_pages(kv, (int32_t)(len + c)) - held_pages(kv, (int32_t)len);
+      need = min(need + held_pages(kv, (int32_t)(len + c)) - held_pages(kv, (int32_t)len), over);
   }
-  int all;
-  scan_excl(need, &all);        // synchronises: bad is whole
-  if (!bad && all > 0 && find_free(kv, all, list, refs) < all) {
+  const int all = (int)sum_up_to(need, over);     // synchronises: bad is whole
+  if (!bad && all > kv.pages) {
+    if (threadIdx.x == 0) bad = kErrKvFull;
+  } else if (!bad && all > 0 && find_free(kv, all, list, refs) < all) {
     if (threadIdx.x == 0) bad = kErrKvFull;
   }
   __syncthreads();

@@ -239,6 +239,20 @@ def test_append_strided_and_int16(engine, dtype):
         assert torch.equal(at[1], (i16[i, 2:, :128].double() / 512).to(dtype))
 
 
+def test_a_list_that_asks_for_more_pages_than_an_integer_holds(engine):
+    S, most = 1100, 1 << 21                        # 1100 times 2^21 pages: over 2^31
+    zeros = lambda n: torch.zeros(n, dtype=torch.int32, device=DEV)
+    kv = PagedKV(engine, torch.zeros(3, 1, 2, 1, 16, 64, device=DEV), zeros(3),
+                 torch.empty(S, most, dtype=torch.int32, device=DEV), zeros(S))
+    seqs, counts = ints(list(range(S))), ints([16 * most] * S)
+    for n in (S, 1):
+        torch.cuda.synchronize()
+        kv.extend_async(seqs[:n], counts[:n])
+        with pytest.raises(AssertionError, match="too few free pages"):
+            engine.sync()
+        assert not kv.refs.any() and not kv.lens.any()
+
+
 def test_compact_reports_tables_that_disagree_with_the_counts(engine):
     b = Both(engine, 9, 5, 6)
     assert b.both("extend", [0, 1, 2], [40, 40, 20])
