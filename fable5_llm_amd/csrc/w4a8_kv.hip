@@ -4,6 +4,8 @@
 // device's own counts and tables, so that a step with them can be captured
 // and replayed, and is the same from run to run: free pages are handed out
 // lowest first, in the order of the list.
+#include <algorithm>
+
 #include "w4a8_mixers.h"
 
 namespace w4a8 {
@@ -524,8 +526,10 @@ hipError_t launch_kv_extend(const KvCache &kv, const int32_t *seqs, const int32_
 hipError_t launch_kv_fork(const KvCache &kv, const int32_t *parents, const int32_t *children,
                           int32_t n, hipStream_t s) {
   kv_fork_kernel<<<1, kOne, 0, s>>>(kv, parents, children, n);
-  const int runs = kv.layers * 2 * kv.heads;
-  kv_fork_rows_kernel<<<dim3(n, runs < 64 ? runs : 64), 256, 0, s>>>(kv, parents, children);
+  // a workgroup per run of a last page, up to 64; a launch has fewer than 2^32 threads
+  const int runs = std::min(kv.layers * 2 * kv.heads, 64);
+  const int rows = std::max(std::min(runs, (1 << 23) / n), 1);
+  kv_fork_rows_kernel<<<dim3(n, rows), 256, 0, s>>>(kv, parents, children);
   return hipGetLastError();
 }
 

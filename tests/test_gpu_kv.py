@@ -239,6 +239,23 @@ def test_append_strided_and_int16(engine, dtype):
         assert torch.equal(at[1], (i16[i, 2:, :128].double() / 512).to(dtype))
 
 
+def test_lists_of_the_largest_size(engine):
+    # 2^20 entries, padding but for a few
+    b = Both(engine, 60, 8, 6)
+    n = 1 << 20
+    def full(*at):
+        x = [-1] * n
+        for i, v in at:
+            x[i] = v
+        return x
+    assert b.both("extend", full((5, 2), (n - 1, 0)), full((5, 20), (n - 1, 7)))
+    b.append([2] * 20 + [0] * 7, list(range(20)) + list(range(7)))
+    assert b.both("fork", full((0, 2), (n // 2, 0), (n - 1, 2)), full((0, 3), (n // 2, 4), (n - 1, 5)))
+    b.check()
+    assert b.both("free", full((0, 2), (n - 2, 2), (n - 1, 4)))
+    b.check()
+
+
 def test_a_list_that_asks_for_more_pages_than_an_integer_holds(engine):
     S, most = 1100, 1 << 21                        # 1100 times 2^21 pages: over 2^31
     zeros = lambda n: torch.zeros(n, dtype=torch.int32, device=DEV)
