@@ -116,6 +116,9 @@ attend_kernel(KvCache kv, Attend a) {
   constexpr int ROWS = F32 ? 4 : 8;                // value rows of a lane group
   constexpr int SPLIT = I16 && !F32 ? 2 : 1;       // operands q and P are the sum of
   constexpr int LD = D + 4;                        // floats of a head's row in LDS
+  // a float16 weight's exponent ends at 2^-24: weights there are 2^14 as large,
+  // and so are their sum and the output until it is divided by it
+  constexpr float LIFT = __is_same(T, _Float16) ? 14.f : 0.f;
   __shared__ float obuf[2][16 * LD];
   __shared__ float mbuf[kWaves][16], lbuf[kWaves][16];
 
@@ -275,7 +278,7 @@ attend_kernel(KvCache kv, Attend a) {
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        sc[j][i] = exp2_of(sc[j][i] - base);
+        sc[j][i] = exp2_of(sc[j][i] - (base - LIFT));
         sum += sc[j][i];
       }
     l = l * fall + sum;

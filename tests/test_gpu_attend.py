@@ -181,6 +181,27 @@ def test_scores_far_apart(engine):
     check(kv, 0, q, [0], run(engine, kv, 0, q, [0]))
 
 
+@pytest.mark.parametrize("int16", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_many_small_weights(engine, dtype, int16):
+    # weights of 2^-25 of the largest, which carries no value: they are not lost.
+    # out = N 2^-25 V / (1 + N 2^-25); scores of 0 and 25 log 2 are off by 2^-24
+    # of 25 at most.  int16 out: N 2^-25 V = 0.125, at a step of 2^-15
+    N, V = (4096, 1024.0) if int16 else (4096, 1.0)
+    kv = make(engine, torch.Generator().manual_seed(1), [N + 1], 1, 64, 16, dtype,
+              fill=torch.zeros_like)
+    first = int(kv.tables[0, 0])
+    for p in kv.tables[0, :-(-(N + 1) // 16)].tolist():
+        kv.pool[p, 0, 1] = V
+    kv.pool[first, 0, 0, 0, 0, 0] = 25.0
+    kv.pool[first, 0, 1, 0, 0] = 0.0
+    q = torch.zeros(1, 2, 64, dtype=torch.int16 if int16 else dtype, device=DEV)
+    q[..., 0] = 1
+    check(kv, 0, q, [0], run(engine, kv, 0, q, [0], scale=math.log(2.0),
+                             **(dict(out_frac=15) if int16 else {})),
+          scale=math.log(2.0), **(dict(out_unit=2.0 ** -15) if int16 else {}))
+
+
 def test_infinite_scores(engine):
     # a key that scores -infinity weighs nothing; a row of such keys gets zeros;
     # +infinity and NaN make the row NaN, and no other row
