@@ -6,6 +6,7 @@ Host-array methods (numpy in, numpy out) are synchronous; *_async methods
 take torch tensors already on the device and enqueue on the context stream.
 """
 import ctypes
+import weakref
 from array import array
 
 import numpy as np
@@ -118,9 +119,12 @@ class Context:
         cu, grid = ctypes.c_int32(), ctypes.c_int32()
         N.check(N.lib().w4a8_ctx_info(self.h, ctypes.byref(cu), ctypes.byref(grid)))
         self.num_cu, self.grid = int(cu.value), int(grid.value)
+        self.caches = weakref.WeakSet()      # open PagedKVs, closed with the context
 
     def close(self):
         if self.h:
+            for kv in list(self.caches):
+                kv.close()
             N.lib().w4a8_ctx_destroy(self.h)
             self.h = None
 

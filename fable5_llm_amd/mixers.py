@@ -120,6 +120,7 @@ class PagedKV:
             tables.shape[1], pool.data_ptr(), refs.data_ptr(), tables.data_ptr(),
             lens.data_ptr(), ctypes.byref(h)), "kv_create")
         self.ctx, self.h = ctx, h
+        ctx.caches.add(self)
         self.pool, self.refs, self.tables, self.lens = pool, refs, tables, lens
         self.kv_heads, self.page_tokens, self.head_dim = heads, page, dim
         self.scale = 1.0 / math.sqrt(dim)
@@ -224,9 +225,11 @@ class PagedKV:
                                            _list(dst, self.ctx, "dst", n), n), "kv_copy")
 
     def close(self):
-        if self.h and self.ctx.h:
+        """Frees the handle's scratch memory, not the caller's tensors; done
+        by the context's close() too."""
+        if self.h:
             N.lib().w4a8_kv_destroy(self.h)
-        self.h = None
+            self.h = None
 
     def __enter__(self):
         return self
@@ -236,7 +239,8 @@ class PagedKV:
 
     def __del__(self):
         try:
-            self.close()
+            if self.h and self.ctx.h:
+                self.close()
         except Exception:
             pass
 

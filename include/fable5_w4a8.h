@@ -427,10 +427,11 @@ int w4a8_plan_destroy(w4a8_plan *plan);
  *   lens    int32[seqs]: its tokens; the first ceil(len / page_tokens) entries
  *           of its table are in use
  * An empty cache is refs and lens of zeros.  page_tokens: a power of two,
- * 16..1024; head_dim: 64, 128 or 256; max_pages * page_tokens: at most 2^30.  The calls below change refs, tables
- * and lens on the context's stream, so calls on one cache from several
- * streams need ordering by the caller; one handle serves one cache (its
- * scratch memory is part of the cache's state). */
+ * 16..1024; head_dim: 64, 128 or 256; max_pages * page_tokens: at most 2^30.
+ * The calls below change refs, tables and lens on the context's stream, so
+ * calls on one cache from several streams need ordering by the caller; one
+ * handle serves one cache (its scratch memory is part of the cache's state),
+ * and is destroyed before its context. */
 typedef struct w4a8_kv w4a8_kv;
 int w4a8_kv_create(w4a8_ctx *ctx, int32_t dtype, int32_t pages, int32_t layers,
                    int32_t kv_heads, int32_t page_tokens, int32_t head_dim,
@@ -515,15 +516,15 @@ typedef struct {
   int64_t tokens, rows, hk, hv, dk, dv, nslots;
   int64_t dtype, frac, out_frac;            /* of q, k, v and of out; fracs: I16 */
   int64_t norm;
-  int64_t fresh;                            /* states start from zeros, unread */
+  int64_t fresh;         /* chunk: states start from zeros, unread.  step: ignored */
   double scale, eps;
 } w4a8_delta;
 /* one token of each row */
 int w4a8_delta_step_async(w4a8_ctx *ctx, const w4a8_delta *d);
 /* whole prompts, in chunks of 64 tokens (an infinity or a NaN among a token's
-   inputs can reach every output of its chunk).  Token strides of v and
-   out: at most 2^23.  Bounds that do not lie in
-   order within the tokens: nothing is run, and the next sync reports it. */
+   inputs can reach every output of its chunk).  Token strides of v and out: at
+   most 2^23.  Bounds that do not lie in order within the tokens: nothing is
+   run, and the next sync reports it. */
 int w4a8_delta_chunk_workspace(w4a8_ctx *ctx, int64_t tokens, int64_t rows,
                                int64_t hk, int64_t hv, int64_t dk, int32_t dtype,
                                int64_t *bytes);

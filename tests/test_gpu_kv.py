@@ -289,6 +289,18 @@ def test_compact_reports_tables_that_disagree_with_the_counts(engine):
     b.check()
 
 
+def test_a_cache_ends_with_its_context(engine):
+    from fable5_llm_amd.engine import Context
+    ctx = Context(0)
+    kv, other = (PagedKV.empty(ctx, 4, 1, 1, 16, 64, 2, 2, torch.float32) for _ in range(2))
+    other.close()
+    ctx.close()
+    with pytest.raises(ValueError, match="null cache"):
+        kv.free_async(ints([0]))
+    kv.close()
+    del kv, other
+
+
 def test_copy_pages(engine):
     kv = PagedKV.empty(engine, 300, 3, 2, 16, 64, 1, 1, torch.bfloat16)
     kv.pool.normal_()
