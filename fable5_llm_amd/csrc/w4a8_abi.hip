@@ -2092,7 +2092,7 @@ int delta_launch(w4a8_ctx *c, const w4a8_delta *d, bool chunk) {
   p.out_unit = 1.f / unit_of(p.dtype, d->out_frac);
   p.err = c->d_err;
   DeviceGuard g(c->device);
-  HIP_TRY(launch_delta(p, c->stream));
+  HIP_TRY(launch_delta(p, c->num_cu, c->stream));
   return W4A8_OK;
 }
 

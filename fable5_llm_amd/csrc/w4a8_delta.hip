@@ -5,6 +5,8 @@
 // (q and k divided by their norms first where asked).  Both dot products of a
 // token are taken of the old state in one pass over it: S^T q after the update
 // is e^g S^T q + (k . q) u.
+#include <algorithm>
+
 #include "w4a8_mixers.h"
 
 namespace w4a8 {
@@ -259,7 +261,7 @@ struct Space {
   }
 };
 
-// A workgroup per chunk and key head.  It lays K, Q and K transposed out as
+// A workgroup per chunk, key head and share of its value heads.  It lays K, Q and K transposed out as
 // the operands that delta_scan_kernel reads, in whole lines (read where they
 // lie, rows of a prompt 4 KB apart all fall to one channel of the L2: 70 us of
 // the scan's 257 at 8192 tokens, 16 key heads of 128).  Tiles of M and P are
@@ -276,7 +278,7 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(Delta p) {
   const int slot = blockIdx.x, hk = blockIdx.y;
   int row;
   if (!bounds_ok(p, slot, &row)) {
-    if (slot == 0 && hk == 0 && threadIdx.x == 0) atomicOr(p.err, kErrDelta);
+    if (slot == 0 && hk == 0 && blockIdx.z == 0 && threadIdx.x == 0) atomicOr(p.err, kErrDelta);
     return;
   }
   if (row < 0) return;
@@ -285,7 +287,9 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(Delta p) {
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Space<DK, T> space(p, slot);
-  const int per = p.hv / p.hk;
+  const int per = p.hv / p.hk, share = (per + (int)gridDim.z - 1) / (int)gridDim.z;
+  const int head0 = blockIdx.z * share, head1 = min(per, head0 + share);
+  const bool rows_too = blockIdx.z == 0;           // the first share writes K and Q
 
   // rows 16 w + r of x, elements 32 s + 8 g .., as terms (zeros past the
   // chunk's end), written as operand; the sum of their squares
@@ -309,7 +313,8 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(Delta p) {
       }
       split<NK, 8>(y, f[s]);
 #pragma unroll
-      for (int i = 0; i < NK; ++i) out[((w * NS + s) * NK + i) * 64] = f[s][i];
+      for (int i = 0; i < NK; ++i)
+        if (rows_too) out[((w * NS + s) * NK + i) * 64] = f[s][i];
     }
     sum += __shfl_xor(sum, 16);
     return sum + __shfl_xor(sum, 32);
@@ -341,7 +346,7 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(Delta p) {
         kq[c] = mfma_terms<NK, NK, 2>(kc, qw[s], kq[c]);
       }
   }
-  if (w < NS) {   // rows d = 32 w + 2 r + e of K transposed: pairs of its columns
+  if (rows_too && w < NS) {   // rows d = 32 w + 2 r + e of K transposed: pairs of its columns
     bf16x8 *out = space.rows(hk, 2) + lane;
 #pragma unroll
     for (int s = 0; s < 2; ++s)
@@ -380,8 +385,8 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(Delta p) {
       }
   };
 
-  for (int first = 0; first < per; first += HEADS) {
-    const int count = min(HEADS, per - first);
+  for (int first = head0; first < head1; first += HEADS) {
+    const int count = min(HEADS, head1 - first);
     if (w < count) {   // a wavefront per head: its tokens' factors
       const int h = hk * per + first + w;
       const bool on = lane < len;
@@ -793,22 +798,30 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
 }
 
 template <int DK, typename T>
-void launch_typed(const Delta &d, hipStream_t s) {
+void launch_typed(const Delta &d, int num_cu, hipStream_t s) {
   if (!d.cu) {
     delta_step_kernel<DK, T><<<dim3(d.rows, d.hv, (d.dv + 63) / 64), 256, 0, s>>>(d);
     return;
   }
-  delta_prep_kernel<DK, T><<<dim3(d.tokens / C + d.rows, d.hk), 256, 0, s>>>(d);
+  // A key head's value heads one after another where the chunks fill the chip
+  // twice, otherwise each in a workgroup of its own (which lays out K and Q
+  // again, but for the writing), up to that: 9 chunks of 16 key and 32 value
+  // heads 30.9 -> 27.9 us with the scan, 48 of 1 and 8 97.5 -> 72.5; beyond it,
+  // 31 chunks of 16 and 32, 70 -> 75.
+  const int64_t units = (d.tokens / C + (int64_t)d.rows) * d.hk;
+  const int shares =
+      (int)std::max<int64_t>(std::min<int64_t>(d.hv / d.hk, 2 * num_cu / units), 1);
+  delta_prep_kernel<DK, T><<<dim3(d.tokens / C + d.rows, d.hk, shares), 256, 0, s>>>(d);
   const int64_t each = ((int64_t)d.rows * d.hv + 7) / 8;
   delta_scan_kernel<DK, T><<<(uint32_t)(8 * each * (d.dv / 16)), 512, 0, s>>>(d);
 }
 
 template <int DK>
-void launch_dim(const Delta &d, hipStream_t s) {
-  if (d.dtype == DT_F32) launch_typed<DK, float>(d, s);
-  else if (d.dtype == DT_BF16) launch_typed<DK, __bf16>(d, s);
-  else if (d.dtype == DT_F16) launch_typed<DK, _Float16>(d, s);
-  else launch_typed<DK, int16_t>(d, s);
+void launch_dim(const Delta &d, int num_cu, hipStream_t s) {
+  if (d.dtype == DT_F32) launch_typed<DK, float>(d, num_cu, s);
+  else if (d.dtype == DT_BF16) launch_typed<DK, __bf16>(d, num_cu, s);
+  else if (d.dtype == DT_F16) launch_typed<DK, _Float16>(d, num_cu, s);
+  else launch_typed<DK, int16_t>(d, num_cu, s);
 }
 
 }  // namespace
@@ -820,9 +833,9 @@ int64_t delta_workspace(int64_t tokens, int64_t rows, int64_t hk, int64_t hv, in
   return (tokens / C + rows) * (hv * kHeadBytes + hk * rows_bytes(dk, terms));
 }
 
-hipError_t launch_delta(const Delta &d, hipStream_t s) {
-  if (d.dk == 64) launch_dim<64>(d, s);
-  else launch_dim<128>(d, s);
+hipError_t launch_delta(const Delta &d, int num_cu, hipStream_t s) {
+  if (d.dk == 64) launch_dim<64>(d, num_cu, s);
+  else launch_dim<128>(d, num_cu, s);
   return hipGetLastError();
 }
 

@@ -99,6 +99,6 @@ struct Delta {
 constexpr int64_t kDeltaStride = 1 << 23;   // of v's and out's tokens, whole prompts
 int64_t delta_workspace(int64_t tokens, int64_t rows, int64_t hk, int64_t hv, int64_t dk,
                         int dtype);
-hipError_t launch_delta(const Delta &d, hipStream_t s);
+hipError_t launch_delta(const Delta &d, int num_cu, hipStream_t s);
 
 }  // namespace w4a8
