@@ -499,6 +499,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
   __shared__ bf16x8 Sb[3][NS][64];                // the state, k-step s by wavefront s
   __shared__ __align__(16) bf16x4 Rb[3][2][64][2], Ub[OT][2][64][2], Wb[3][2][64][2];
   __shared__ __align__(16) T Ts[8][16 * 16];      // a wavefront's tokens' values or outputs
+  __shared__ __align__(16) float Fs[2][kVecFloats];   // a chunk's factors and the next one's
   const int tiles = p.dv / 16, units = p.rows * p.hv, each = (units + 7) / 8;
   // a head's columns, and heads that share keys, on one XCD (workgroups go
   // round the eight of them)
@@ -533,8 +534,8 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
     return ((const bf16x8 *)(ws + which * kTriBytes) + (tri_of(w, s) * 3 + i) * 64)[lane];
   };
   // a, b or c of tokens 16 w + 4 g ..
-  auto factor = [&](int which) {
-    return *(const f32x4 *)((const float *)(ws + 2 * kTriBytes) + 64 * which + 16 * w + 4 * g);
+  auto factor = [&](int ch, int which) {
+    return *(const f32x4 *)(Fs[ch & 1] + 64 * which + 16 * w + 4 * g);
   };
   // Values and outputs move in pieces of 16 bytes, PIECES a row of 16 columns
   // (single values would be four loads and four stores for one), and change
@@ -590,8 +591,6 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
     struct In {
       bf16x8 k[NS][NK], m[2][3], kt[2][2][NK];
       u32x4 v;
-      f32x4 a, c;
-      float fall;
     };
     const uint8_t *const kb0 = kb, *const vb0 = vb, *const ws0 = ws;
     auto next = [&](int ch) {                     // its operands are loaded from here on
@@ -608,7 +607,6 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
         for (int s = 0; s < NS; ++s)
           x.k[s][i] = ((const bf16x8 *)kb + ((w * NS + s) * NK + i) * 64)[lane];
       x.v = *(const u32x4 *)(vb + v_at);
-      x.a = factor(0);
     };
     auto load_solve = [&](In &x) {
 #pragma unroll
@@ -616,7 +614,6 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
         x.m[0][i] = tri(0, 0, i);
         if constexpr (HI) x.m[1][i] = tri(0, 1, i);
       }
-      x.c = factor(2);
     };
     auto load_update = [&](In &x) {
       if constexpr (STATE) {
@@ -628,7 +625,6 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
             for (int i = 0; i < NK; ++i)
               x.kt[s][e][i] =
                   ((const bf16x8 *)(kb + kt_off) + (((w * 2 + s) * 2 + e) * NK + i) * 64)[lane];
-        x.fall = ((const float *)(ws + 2 * kTriBytes) + 192)[lane];
       }
     };
     // Loads go out behind a segment's reads of LDS, in the time those take.
@@ -645,6 +641,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
         exchange();
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = tile[(4 * g + i) * 16 + r];
+        const f32x4 a = factor(ch, 0);
         __builtin_amdgcn_sched_barrier(0);
         load_update(x);
         __builtin_amdgcn_sched_barrier(0);
@@ -653,7 +650,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
         for (int s = 0; s < NS; ++s) ks = mfma_terms<NK, 3, 2>(x.k[s], sb[s], ks);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          z[i] = (16 * w + 4 * g + i < len ? to_float(v[i], p.unit) : 0.f) - x.a[i] * ks[i];
+          z[i] = (16 * w + 4 * g + i < len ? to_float(v[i], p.unit) : 0.f) - a[i] * ks[i];
         put_rows(Rb, z, Int<3>());
       }
       lds_barrier();
@@ -665,12 +662,13 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
           b[0][i] = *(const bf16x8 *)Rb[i][0][lane];
           if constexpr (HI) b[1][i] = *(const bf16x8 *)Rb[i][1][lane];
         }
+        const f32x4 c = factor(ch, 2);
         __builtin_amdgcn_sched_barrier(0);
         load_rows(x);
         __builtin_amdgcn_sched_barrier(0);
         f32x4 u = mfma_terms<3, 3, 2>(x.m[0], b[0], f32x4{0, 0, 0, 0});
         if constexpr (HI) u = mfma_terms<3, 3, 2>(x.m[1], b[1], u);
-        put_rows(Wb, u * x.c, Int<3>());
+        put_rows(Wb, u * c, Int<3>());
         put_rows(Ub, u, Int<OT>());
       }
       lds_barrier();
@@ -681,11 +679,12 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
           b[0][i] = *(const bf16x8 *)Wb[i][0][lane];
           b[1][i] = *(const bf16x8 *)Wb[i][1][lane];
         }
+        const float fall = Fs[ch & 1][192];
         __builtin_amdgcn_sched_barrier(0);
         load_solve(x);
         __builtin_amdgcn_sched_barrier(0);
-        S[0] *= x.fall;
-        S[1] *= x.fall;
+        S[0] *= fall;
+        S[1] *= fall;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           S[0] = mfma_terms<NK, 3, 2>(x.kt[s][0], b[s], S[0]);
@@ -722,7 +721,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
     const int64_t o_step = p.out_token * C * (int)sizeof(T);
     const uint32_t o_at = piece_at(C, p.out_token);
     bf16x8 q[NS][NK], m[2][OT];
-    f32x4 b, o{0, 0, 0, 0};
+    f32x4 o{0, 0, 0, 0}, factors;
     const uint8_t *const qb0 = qb, *const ws0 = ws;
     // a chunk's rows of Q and their factors; its rows of P
     auto load_rows = [&](int ch) {
@@ -733,7 +732,13 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
 #pragma unroll
         for (int s = 0; s < NS; ++s)
           q[s][i] = ((const bf16x8 *)qb + ((w * NS + s) * NK + i) * 64)[lane];
-      b = factor(1);
+    };
+    // a chunk's factors go to LDS for every wavefront, by the first of these
+    auto load_factors = [&](int ch) {
+      if (w == 0) factors = ((const f32x4 *)(ws0 + (int64_t)ch * kHeadBytes + 2 * kTriBytes))[lane];
+    };
+    auto put_factors = [&](int ch) {
+      if (w == 0) *(f32x4 *)(Fs[ch & 1] + 4 * lane) = factors;
     };
     auto load_weights = [&](int ch) {
       ws = ws0 + (int64_t)ch * kHeadBytes;
@@ -752,14 +757,17 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
       if (lane < 16 * PIECES && 16 * w + prow < len) *(u32x4 *)(ob + o_at) = x;
       ob += o_step;
     };
+    load_factors(0);
     load_rows(0);
     load_weights(0);
+    put_factors(0);
     lds_barrier();
     for (int ch = 0; ch < n; ++ch) {
       // beside the chain's first segment the last chunk's outputs are written,
       // beside its second Q S0 is made, beside its third P U: no segment has
       // more than its share of the loads and stores
       if (ch) write(ch - 1);
+      load_factors(min(ch + 1, n - 1));
       lds_barrier();
       {
         bf16x8 sb[NS][OT];
@@ -770,7 +778,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
         o = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < NS; ++s) o = mfma_terms<NK, OT, OT - 1>(q[s], sb[s], o);
-        o *= b;
+        o *= factor(ch, 1);
       }
       load_rows(min(ch + 1, n - 1));
       lds_barrier();
@@ -783,6 +791,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
       o = mfma_terms<OT, OT, OT - 1>(m[0], ub[0], o);
       if constexpr (HI) o = mfma_terms<OT, OT, OT - 1>(m[1], ub[1], o);
       load_weights(min(ch + 1, n - 1));
+      put_factors(ch + 1);
       lds_barrier();
     }
     write(n - 1);
