@@ -43,7 +43,9 @@ __device__ __forceinline__ int slot_of(const Delta &p, int row, bool tell) {
 
 // One token of each row: a wavefront holds 16 columns of a head's state in
 // registers, lane (rg, cq) = (lane >> 2, lane & 3) its rows NR rg .. and
-// columns 4 cq ...
+// columns 4 cq .., so that a state is read and written once, in 64-byte runs.
+// Bound by that: 125 rows of 32 heads of 128 x 128, 527 MB in 106 us, 4.97 TB/s,
+// what a large copy reaches; one row, 4.2 MB, 5.4 us of which 2 are a launch's.
 template <int DK, typename T>
 __global__ __launch_bounds__(256) void delta_step_kernel(Delta p) {
   constexpr int NR = DK / 16;
@@ -131,8 +133,8 @@ constexpr int C = 64;
 constexpr int kTriBytes = 6 * 3 * 64 * 16;       // M or P: operands of tri_of, three terms
 constexpr int kVecFloats = 256;                  // a, b, c of 64 tokens, e^(G_C) 64 times
 constexpr int kHeadBytes = 2 * kTriBytes + kVecFloats * 4;   // of a chunk and value head
-// K, Q and K transposed of a chunk and key head, as operands
-constexpr int64_t rows_bytes(int64_t dk, int terms) { return 3 * C * dk * 2 * terms; }
+// K and Q of a chunk and key head, as operands
+constexpr int64_t rows_bytes(int64_t dk, int terms) { return 2 * C * dk * 2 * terms; }
 constexpr float kNoDecay = -200.f;               // e^g is 0 in float32 from here on down
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -211,10 +213,8 @@ __device__ __forceinline__ void lds_barrier() {
 
 // The order of a chunk's tokens in an operand of k-steps s = 0, 1: slot j of
 // lane group g is token 32 s + 16 (j >> 2) + 4 g + (j & 3), so that a lane's
-// four results of row tiles 2 s and 2 s + 1 are its own eight slots.
-__device__ __forceinline__ int token_of(int s, int g, int j) {
-  return 32 * s + 16 * (j >> 2) + 4 * g + (j & 3);
-}
+// four results of row tiles 2 s and 2 s + 1 are its own eight slots.  The state's
+// rows d are in the same order.
 // M and P as operands: row tile w (of 16 tokens) and k-step s <= w / 2
 __device__ __forceinline__ constexpr int tri_of(int w, int s) {
   return w < 2 ? w : w == 2 ? 2 + s : 4 + s;
@@ -254,21 +254,25 @@ struct Space {
   __device__ Space(const Delta &p, int64_t c)
       : ws((uint8_t *)p.ws), chunks(p.tokens / C + p.rows), chunk(c), heads(p.hv) {}
   __device__ uint8_t *head(int h) const { return ws + (h * chunks + chunk) * kHeadBytes; }
-  // 0: K, 1: Q, 2: K transposed
+  // 0: K, 1: Q
   __device__ bf16x8 *rows(int hk, int which) const {
     return (bf16x8 *)(ws + heads * chunks * kHeadBytes + (hk * chunks + chunk) * kRows +
-                      which * (kRows / 3));
+                      which * (kRows / 2));
   }
 };
 
-// A workgroup per chunk, key head and share of its value heads.  It lays K, Q and K transposed out as
-// the operands that delta_scan_kernel reads, in whole lines (read where they
-// lie, rows of a prompt 4 KB apart all fall to one channel of the L2: 70 us of
-// the scan's 257 at 8192 tokens, 16 key heads of 128).  Tiles of M and P are
-// made transposed (rows j, columns t), which leaves a lane with four
+// A workgroup per chunk, key head and share of its value heads.  It lays K and
+// Q out as the operands that delta_scan_kernel reads, in whole lines (read where
+// they lie, rows of a prompt 4 KB apart all fall to one channel of the L2: the
+// scan of 8192 tokens, 16 key heads of 128, took 34 us more).  Tiles of M and P
+// are made transposed (rows j, columns t), which leaves a lane with four
 // neighbouring slots of their operand: nothing is rearranged.
+//
+// Bound by memory: 8192 bfloat16 tokens, 16 key and 32 value heads of 128, 67 MB
+// read and 195 MB written in 69 us (3.8 TB/s).
 template <int DK, typename T>
-__global__ __launch_bounds__(256, 3) void delta_prep_kernel(Delta p) {
+__global__ __launch_bounds__(256, DK == 64 || Terms<T>::n == 1 ? 3 : 2) void
+delta_prep_kernel(Delta p) {
   constexpr int NK = Terms<T>::n, NS = DK / 32, LD = 68, HEADS = 4;
   __shared__ bf16x8 Ks[4][NS][NK][64];             // K by row tiles, as operand
   __shared__ double Gs[HEADS][C];                  // log2(e) times the running sum of g
@@ -344,28 +348,6 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(Delta p) {
         for (int i = 0; i < NK; ++i) kc[i] = Ks[c][s][i][lane];
         kk[c] = mfma_terms<NK, NK, 2>(kc, kw[s], kk[c]);
         kq[c] = mfma_terms<NK, NK, 2>(kc, qw[s], kq[c]);
-      }
-  }
-  if (rows_too && w < NS) {   // rows d = 32 w + 2 r + e of K transposed: pairs of its columns
-    bf16x8 *out = space.rows(hk, 2) + lane;
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int i = 0; i < NK; ++i) {
-        uint32_t x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int t = token_of(s, g, j);
-          x[j] = ((const uint32_t *)&Ks[t >> 4][w][i][(t & 15) + 16 * (r >> 2)])[r & 3];
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          u32x4 y;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            y[j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], e ? 0x07060302u : 0x05040100u);
-          out[(((w * 2 + s) * 2 + e) * NK + i) * 64] = __builtin_bit_cast(bf16x8, y);
-        }
       }
   }
   // row tile w of M (which 0) or P out of its transposed tiles X[c], c <= w
@@ -481,14 +463,17 @@ __global__ __launch_bounds__(256, 3) void delta_prep_kernel(Delta p) {
 // wavefronts on 16 tokens each: the chain of a chunk, S0 -> V - a K S0 -> U ->
 // S, on four of them and the outputs, b Q S0 + P U, on the other four, so that
 // the chain's trips through LDS are filled with the outputs' products.  Where
-// there is one row, a chunk's chain and the instructions issued along it are
-// what bounds the kernel.  So every operand is loaded right after an earlier
-// chunk's use of its registers, spread over the step.
+// there is one row, a chunk's chain is what bounds the kernel, and beside it the
+// bytes that a CU's vector cache passes on (each column tile reads K, Q, M and P
+// for itself).  So operands are loaded as soon as an earlier chunk has used
+// their registers, the factors once per workgroup, and K transposed for the
+// update comes out of LDS by transposed reads instead of from memory again.
+// 8192 bfloat16 tokens of 32 heads of 128 x 128: 208 us, 1.6 us a chunk; of 8
+// heads, a quarter of the chip, 1.1 us a chunk.
 //
 // Wavefront w of the chain has rows 32 w .. of the state too: lane (r, g) rows
-// 32 w + 8 g + e of column r, in register [e & 1][e >> 1], which is its slots
-// of the state as an operand; its results of U are slots of that operand
-// likewise (token_of).
+// 32 w + 8 g + 4 e + i of column r, in register S[e][i], which is its slots of
+// the state as an operand; its results of U are slots of that operand likewise.
 //
 // Outputs are rounded to 16 bits (bfloat16, float16): two terms of their
 // operands, an error of 2^-17, are enough for them.
@@ -499,6 +484,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
   __shared__ bf16x8 Sb[3][NS][64];                // the state, k-step s by wavefront s
   __shared__ __align__(16) bf16x4 Rb[3][2][64][2], Ub[OT][2][64][2], Wb[3][2][64][2];
   __shared__ __align__(16) T Ts[8][16 * 16];      // a wavefront's tokens' values or outputs
+  __shared__ __align__(16) uint8_t Kl[NK][C * DK * 2];   // K by rows, see k_at
   __shared__ __align__(16) float Fs[2][kVecFloats];   // a chunk's factors and the next one's
   const int tiles = p.dv / 16, units = p.rows * p.hv, each = (units + 7) / 8;
   // a head's columns, and heads that share keys, on one XCD (workgroups go
@@ -565,13 +551,13 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) S[e][i] = state[(int64_t)(2 * i + e) * p.dv];
+        for (int i = 0; i < 4; ++i) S[e][i] = state[(int64_t)(4 * e + i) * p.dv];
     }
     auto put_state = [&]() {
       bf16x8 t[3];
       float x[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = S[j & 1][j >> 1];
+      for (int j = 0; j < 8; ++j) x[j] = S[j >> 2][j & 3];
       split<3, 8>(x, t);
 #pragma unroll
       for (int i = 0; i < 3; ++i) Sb[i][w][lane] = t[i];
@@ -584,12 +570,18 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
       for (int i = 0; i < terms.value; ++i) b[i][w >> 1][lane][w & 1] = t[i];
     };
     const uint8_t *kb = (const uint8_t *)space.rows(hk, 0);
-    const int64_t kt_off = Space<DK, T>::kRows / 3 * 2;
+    // K goes to LDS by rows, in the order of the pieces of 16 bytes changed so
+    // that neither these writes (a lane's token is 16 w + r) nor the transposed
+    // reads (16 lanes: 4 tokens of a group, 4 pieces each) meet in a bank
+    constexpr int TURN = DK == 128 ? 0 : 1;
+    auto turn_of = [&](int t) { return ((t >> TURN) & (DK == 128 ? 3 : 1)) << 2 | ((t >> 2) & 3); };
+    auto k_at = [&](int t, int at) { return t * DK * 2 + ((at ^ turn_of(t)) * 16); };
+    const int kt_at = k_at(4 * g + (r >> 2), 4 * w + (r & 3));
     const uint8_t *vb = (const uint8_t *)((const T *)p.v + begin * p.v_token + h * p.v_head);
     const int64_t v_step = p.v_token * C * (int)sizeof(T);
     uint32_t v_at = piece_at(C, p.v_token);
     struct In {
-      bf16x8 k[NS][NK], m[2][3], kt[2][2][NK];
+      bf16x8 k[NS][NK], m[2][3];
       u32x4 v;
     };
     const uint8_t *const kb0 = kb, *const vb0 = vb, *const ws0 = ws;
@@ -615,17 +607,19 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
         if constexpr (HI) x.m[1][i] = tri(0, 1, i);
       }
     };
-    auto load_update = [&](In &x) {
-      if constexpr (STATE) {
+    // K transposed as operand: rows d = 32 w + 8 (m >> 2) + 4 e + (m & 3) of
+    // tile e, four tokens of a lane's slots at a time
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4 lds_x4;
+    auto transposed = [&](int s, int e, int i) {
+      s16x4 t[2];
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int i = 0; i < NK; ++i)
-              x.kt[s][e][i] =
-                  ((const bf16x8 *)(kb + kt_off) + (((w * 2 + s) * 2 + e) * NK + i) * 64)[lane];
-      }
+      for (int j = 0; j < 2; ++j)
+        t[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_x4 *)(Kl[i] + kt_at + (32 * s + 16 * j) * DK * 2 + 8 * e));
+      bf16x8 x;
+      __builtin_memcpy(&x, t, sizeof(x));
+      return x;
     };
     // Loads go out behind a segment's reads of LDS, in the time those take.
     auto step = [&](int ch, In &x) {
@@ -643,8 +637,6 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
         for (int i = 0; i < 4; ++i) v[i] = tile[(4 * g + i) * 16 + r];
         const f32x4 a = factor(ch, 0);
         __builtin_amdgcn_sched_barrier(0);
-        load_update(x);
-        __builtin_amdgcn_sched_barrier(0);
         f32x4 ks{0, 0, 0, 0}, z;
 #pragma unroll
         for (int s = 0; s < NS; ++s) ks = mfma_terms<NK, 3, 2>(x.k[s], sb[s], ks);
@@ -652,9 +644,14 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
         for (int i = 0; i < 4; ++i)
           z[i] = (16 * w + 4 * g + i < len ? to_float(v[i], p.unit) : 0.f) - a[i] * ks[i];
         put_rows(Rb, z, Int<3>());
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int i = 0; i < NK; ++i) *(bf16x8 *)(Kl[i] + k_at(16 * w + r, 4 * s + g)) = x.k[s][i];
       }
       lds_barrier();
       next(ch + 1);
+      bf16x8 kt[2][2][NK];
       {
         bf16x8 b[2][3];
 #pragma unroll
@@ -663,6 +660,13 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
           if constexpr (HI) b[1][i] = *(const bf16x8 *)Rb[i][1][lane];
         }
         const f32x4 c = factor(ch, 2);
+        if constexpr (STATE)
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+              for (int i = 0; i < NK; ++i) kt[s][e][i] = transposed(s, e, i);
         __builtin_amdgcn_sched_barrier(0);
         load_rows(x);
         __builtin_amdgcn_sched_barrier(0);
@@ -687,8 +691,8 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
         S[1] *= fall;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          S[0] = mfma_terms<NK, 3, 2>(x.kt[s][0], b[s], S[0]);
-          S[1] = mfma_terms<NK, 3, 2>(x.kt[s][1], b[s], S[1]);
+          S[0] = mfma_terms<NK, 3, 2>(kt[s][0], b[s], S[0]);
+          S[1] = mfma_terms<NK, 3, 2>(kt[s][1], b[s], S[1]);
         }
         put_state();
       } else {
@@ -711,7 +715,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) state[(int64_t)(2 * i + e) * p.dv] = S[e][i];
+        for (int i = 0; i < 4; ++i) state[(int64_t)(4 * e + i) * p.dv] = S[e][i];
   };
 
   auto output = [&](auto upper) {
