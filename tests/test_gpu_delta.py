@@ -112,7 +112,10 @@ def spans_of(lens):
 @pytest.mark.parametrize("lens,hk,hv,dk,dv", [
     ([1], 1, 1, 64, 16), ([64], 1, 2, 64, 64), ([63, 65, 0, 1, 128], 2, 2, 128, 32),
     ([0, 200], 1, 3, 128, 128), ([300], 2, 4, 128, 80), ([129, 7, 64, 2], 1, 2, 64, 256),
-    ([70, 40], 1, 6, 128, 16), ([5] * 40, 1, 1, 64, 16)])
+    ([70, 40], 1, 6, 128, 16), ([5] * 40, 1, 1, 64, 16),
+    # a key head's six value heads in one workgroup, in shares of two, and in
+    # shares of which the last ones are empty
+    ([1] * 520, 1, 6, 64, 16), ([3] * 130, 1, 6, 64, 16), ([2] * 100, 1, 6, 128, 16)])
 def test_chunk(engine, dtype, lens, hk, hv, dk, dv):
     gen = torch.Generator().manual_seed(sum(lens) + dv)
     cu = spans_of(lens)
