@@ -271,8 +271,7 @@ struct Space {
 // Bound by memory: 8192 bfloat16 tokens, 16 key and 32 value heads of 128, 67 MB
 // read and 195 MB written in 69 us (3.8 TB/s).
 template <int DK, typename T>
-__global__ __launch_bounds__(256, DK == 64 || Terms<T>::n == 1 ? 3 : 2) void
-delta_prep_kernel(Delta p) {
+__global__ __launch_bounds__(256, 2) void delta_prep_kernel(Delta p) {
   constexpr int NK = Terms<T>::n, NS = DK / 32, LD = 68, HEADS = 4;
   __shared__ bf16x8 Ks[4][NS][NK][64];             // K by row tiles, as operand
   __shared__ double Gs[HEADS][C];                  // log2(e) times the running sum of g
@@ -363,7 +362,8 @@ delta_prep_kernel(Delta p) {
         for (int j = 0; j < 8; ++j) x[j] = X[2 * s + (j >> 2)][j & 3];
         split<N, 8>(x, t);
 #pragma unroll
-        for (int i = 0; i < N; ++i) out[(tri_of(w, s) * 3 + i) * 64] = t[i];
+        for (int i = 0; i < N; ++i)
+          __builtin_nontemporal_store(t[i], &out[(tri_of(w, s) * 3 + i) * 64]);
       }
   };
 
@@ -758,7 +758,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
       for (int i = 0; i < 4; ++i) tile[(4 * g + i) * 16 + r] = from_float<T>(o[i], p.out_unit);
       exchange();
       const u32x4 x = *(const u32x4 *)(tile + prow * 16 + piece * (16 / (int)sizeof(T)));
-      if (lane < 16 * PIECES && 16 * w + prow < len) *(u32x4 *)(ob + o_at) = x;
+      if (lane < 16 * PIECES && 16 * w + prow < len) store16_nt(ob + o_at, x);
       ob += o_step;
     };
     load_factors(0);
