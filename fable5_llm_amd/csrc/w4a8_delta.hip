@@ -269,7 +269,9 @@ struct Space {
 // neighbouring slots of their operand: nothing is rearranged.
 //
 // Bound by memory: 8192 bfloat16 tokens, 16 key and 32 value heads of 128, 67 MB
-// read and 195 MB written in 69 us (3.8 TB/s).
+// read and 195 MB written in 66-69 us (3.9 TB/s).  M and P, which no cache holds
+// until they are read, are written past them: prep and scan 268 -> 244 us; K and
+// Q too, 257.
 template <int DK, typename T>
 __global__ __launch_bounds__(256, 2) void delta_prep_kernel(Delta p) {
   constexpr int NK = Terms<T>::n, NS = DK / 32, LD = 68, HEADS = 4;
@@ -468,8 +470,8 @@ __global__ __launch_bounds__(256, 2) void delta_prep_kernel(Delta p) {
 // for itself).  So operands are loaded as soon as an earlier chunk has used
 // their registers, the factors once per workgroup, and K transposed for the
 // update comes out of LDS by transposed reads instead of from memory again.
-// 8192 bfloat16 tokens of 32 heads of 128 x 128: 208 us, 1.6 us a chunk; of 8
-// heads, a quarter of the chip, 1.1 us a chunk.
+// 8192 bfloat16 tokens of 32 heads of 128 x 128: 188-200 us, 1.5 us a chunk; of
+// 8 heads, a quarter of the chip, 1.1 us a chunk.
 //
 // Wavefront w of the chain has rows 32 w .. of the state too: lane (r, g) rows
 // 32 w + 8 g + 4 e + i of column r, in register S[e][i], which is its slots of
