@@ -7,7 +7,8 @@ Everything is enqueued on the context's stream and nothing waits.  Lists
 entry is padding; what they hold is checked on the device and reported, as an
 AssertionError, by the next Context.sync().  Activations are float32,
 bfloat16, float16 or the engine's own int16 with `frac` fraction bits; they
-may be strided, with a contiguous last dimension, 16-byte aligned.
+may be strided, with a contiguous last dimension, 16-byte aligned.  No output
+or workspace overlaps an input.
 """
 import ctypes
 import math

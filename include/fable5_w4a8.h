@@ -410,9 +410,9 @@ int w4a8_plan_destroy(w4a8_plan *plan);
  * rows) and heads are arguments, in elements.  Sums, softmax statistics and
  * states are held in 32 bits.  Lists of sequences, pages and slots are int32
  * device arrays of at most 2^20 entries; a negative entry is padding and is
- * skipped.  What a list or
- * a table holds is checked on the device: an entry outside the cache is not
- * followed, and the next w4a8_ctx_sync() returns W4A8_E_RANGE. */
+ * skipped.  What a list or a table holds is checked on the device: an entry
+ * outside the cache is not followed, and the next w4a8_ctx_sync() returns
+ * W4A8_E_RANGE.  No output or workspace overlaps an input. */
 #define W4A8_DT_F32   0
 #define W4A8_DT_BF16  1
 #define W4A8_DT_F16   2

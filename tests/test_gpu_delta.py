@@ -313,6 +313,42 @@ def test_bad_bounds_are_reported(engine, cu):
     assert (out == 1).all() and torch.equal(d["state"], state)   # nothing was run
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_two_contexts_at_once(engine, dtype):
+    # prompts and single tokens on two streams, each with states and workspace
+    # of its own: what each gives alone, bit for bit
+    from fable5_llm_amd.engine import Context
+    gen = torch.Generator().manual_seed(31)
+    cu = spans_of([200, 333, 64])
+    jobs = []
+    with Context(0) as other:
+        for ctx in (engine, other):
+            d = inputs(gen, cu[-1], 2, 4, 128, 128, dtype, 3)
+            one = {n: (x if n == "state" else x[:3]) for n, x in d.items()}
+            jobs.append((ctx, d, one, torch.zeros_like(d["v"]), torch.zeros_like(one["v"]),
+                         ctx.delta_chunk_workspace(cu[-1], 3, 4), ints(cu), d["state"].clone()))
+
+        def work(ctx, d, one, out, o1, ws, c, first):
+            ctx.delta_chunk_async(**d, out=out, cu=c, ws=ws)
+            ctx.delta_step_async(**one, out=o1)
+
+        torch.cuda.synchronize()
+        want = []
+        for job in jobs:
+            for _ in range(4):
+                work(*job)
+            job[0].sync()
+            want.append([x.clone() for x in (job[3], job[4], job[1]["state"])])
+            job[1]["state"].copy_(job[-1])
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for job in jobs:
+                work(*job)
+        for job, w in zip(jobs, want):
+            job[0].sync()
+            assert all(torch.equal(a, b) for a, b in zip((job[3], job[4], job[1]["state"]), w))
+
+
 def test_captured_step_replays(engine):
     gen = torch.Generator().manual_seed(28)
     d = inputs(gen, 70, 2, 4, 128, 128, torch.bfloat16, 2)
