@@ -44,6 +44,15 @@ __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
+// Barrier of the workgroup for LDS alone: loads from memory stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // Per cache type: a lane's 16 bytes as matrix operand.
 template <typename T>
 struct Half {
@@ -97,19 +106,21 @@ __device__ __forceinline__ void store_out(const Attend &a, int cache_dtype, int6
 }
 
 // I16: q is int16 (its value of a step is part of a.scale), exact as the sum
-// of two 8-bit halves in the cache's type; P then goes as the sum of two
-// values too, so that a 16-bit result keeps its bits.  Otherwise P is rounded
-// to the cache's type for the second product, its sum is not: an error of
-// half a step of that type per token, which averages out over the tokens.
+// of two 8-bit halves in the cache's type.  Over a 16-bit cache P goes into the
+// second product as the sum of two values of that type, off by half a step
+// squared (bfloat16 2^-16, float16 2^-22) of a weight, so that the output's own
+// rounding is the only one that counts.
 // Workgroups: key-value heads fastest, then a row's splits, then rows.  Two a CU
-// at least (a head of 256 of 16-bit values would take 267 registers and leave
-// one: two rows of 131,072 tokens 183 us, held to 256 174); not where the
-// registers needed are far over it.
+// at least, but for heads of 256 of float32 (whose registers are far over that)
+// and of int16 rows, which two a CU make no faster.  A head of 256 of 16-bit
+// values is held to that by keeping q in LDS: 244 registers (with q in
+// registers, six values spilled: two rows of 131,072 tokens 177 us, so 167.5;
+// one row of 511 tokens 9.9, so 10.3).
 //
 // Bound by the reading of keys and values where the cache is long: 2 rows of
-// 131,072 tokens, 4 heads of 256, 1.07 GB in 165 us, 6.5 TB/s.  Short ones are
-// latency, four loads one after another and one turn of the tiles: 8.2 us for
-// one row of 511 tokens.
+// 131,072 tokens, 4 heads of 256, 1.07 GB in 164 us, 6.5 TB/s (int16 rows the
+// same).  Short ones are latency, four loads one after another and one turn of
+// the tiles: 8.5 us for one row of 511 tokens.
 template <int D, typename T, bool I16>
 __global__ __launch_bounds__(64 * kWaves, D == 256 && (I16 || sizeof(T) == 4) ? 1 : 2) void
 attend_kernel(KvCache kv, Attend a) {
@@ -120,13 +131,18 @@ attend_kernel(KvCache kv, Attend a) {
   constexpr int VEC = F32 ? 4 : (D == 64 ? 4 : 8); // elements of a value load
   constexpr int NC = D / (16 * VEC);               // loads of a value row
   constexpr int ROWS = F32 ? 4 : 8;                // value rows of a lane group
-  constexpr int SPLIT = I16 && !F32 ? 2 : 1;       // operands q and P are the sum of
+  constexpr int QT = I16 && !F32 ? 2 : 1;          // values that q is the sum of
+  constexpr int PT = F32 ? 1 : 2;                  // and that P is
   constexpr int LD = D + 4;                        // floats of a head's row in LDS
   // a float16 weight's exponent ends at 2^-24: weights there are 2^14 as large,
   // and so are their sum and the output until it is divided by it
   constexpr float LIFT = __is_same(T, _Float16) ? 14.f : 0.f;
   __shared__ float obuf[2][16 * LD];
   __shared__ float mbuf[kWaves][16], lbuf[kWaves][16];
+  // q in LDS where registers are short
+  constexpr bool QL = D == 256 && !F32;
+  constexpr int QS = QL ? KS / kWaves : KS;        // steps of q a wavefront holds
+  __shared__ __align__(16) T qbuf[QL ? QT * KS : 1][64][8];
 
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -147,20 +163,22 @@ attend_kernel(KvCache kv, Attend a) {
   }
   if (split >= R.used) return;
 
-  // q as B operand: head r, elements 8 g .. (4 g ..) of each step
+  // q as B operand: head r, elements 8 g .. (4 g ..) of each step; a wavefront
+  // makes every fourth step where they go to LDS
   typedef typename Half<T>::x8 x8;
-  x8 qh[SPLIT][F32 ? 1 : KS];
+  x8 qh[QT][F32 ? 1 : QS];
   f32x4 qf[F32 ? KS : 1];
   {
     const int64_t at = row * a.q_row + hq * a.q_head;
     const bool on = r < heads;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
+    for (int n = 0; n < QS; ++n) {
+      const int s = QL ? n * kWaves + wave : n;
       if constexpr (F32) {
         const int64_t e = at + s * 16 + g * 4;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          qf[s][i] = !on ? 0.f : I16 ? (float)((const int16_t *)a.q)[e + i]
+          qf[n][i] = !on ? 0.f : I16 ? (float)((const int16_t *)a.q)[e + i]
                                      : ((const float *)a.q)[e + i];
       } else {
         const int64_t e = at + s * 32 + g * 8;
@@ -170,11 +188,11 @@ attend_kernel(KvCache kv, Attend a) {
           for (int i = 0; i < 8; ++i) {
             const int x = (int16_t)(w[i >> 1] >> (16 * (i & 1)));
             const int lo = (int)(int8_t)x;
-            qh[0][s][i] = (T)(float)(x - lo);
-            qh[1][s][i] = (T)(float)lo;
+            qh[0][n][i] = (T)(float)(x - lo);
+            qh[1][n][i] = (T)(float)lo;
           }
         } else {
-          qh[0][s] = __builtin_bit_cast(x8, w);
+          qh[0][n] = __builtin_bit_cast(x8, w);
         }
       }
     }
@@ -245,6 +263,8 @@ attend_kernel(KvCache kv, Attend a) {
   f32x4 sc[NT];
   // scores of tokens t + 16 j + 4 g + i for head r
   auto scores = [&]() {
+    int at = lane;
+    if constexpr (QL) asm volatile("" : "+v"(at));  // read again every turn, not kept
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       sc[j] = f32x4{0, 0, 0, 0};
@@ -258,7 +278,10 @@ attend_kernel(KvCache kv, Attend a) {
         } else {
           const x8 k8 = __builtin_bit_cast(x8, kr[j][s]);
 #pragma unroll
-          for (int q = 0; q < SPLIT; ++q) sc[j] = mfma(k8, qh[q][s], sc[j]);
+          for (int q = 0; q < QT; ++q) {
+            if constexpr (QL) sc[j] = mfma(k8, *(const x8 *)qbuf[q * KS + s][at], sc[j]);
+            else sc[j] = mfma(k8, qh[q][s], sc[j]);
+          }
         }
       }
     }
@@ -312,12 +335,12 @@ attend_kernel(KvCache kv, Attend a) {
                 __builtin_amdgcn_mfma_f32_16x16x4f32(v4[e], sc[0][i], acc[c * VEC + e], 0, 0, 0);
         }
     } else {
-      x8 p[SPLIT];
+      x8 p[PT];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float w = sc[i >> 2][i & 3];
         p[0][i] = (T)w;
-        if constexpr (SPLIT == 2) p[1][i] = (T)(w - (float)p[0][i]);
+        p[1][i] = (T)(w - (float)p[0][i]);
       }
 #pragma unroll
       for (int c = 0; c < NC; ++c)
@@ -330,7 +353,7 @@ attend_kernel(KvCache kv, Attend a) {
                                          e & 1 ? 0x07060302u : 0x05040100u);
           const x8 v = __builtin_bit_cast(x8, w);
 #pragma unroll
-          for (int q = 0; q < SPLIT; ++q) acc[c * VEC + e] = mfma(v, p[q], acc[c * VEC + e]);
+          for (int q = 0; q < PT; ++q) acc[c * VEC + e] = mfma(v, p[q], acc[c * VEC + e]);
         }
     }
   };
@@ -344,6 +367,15 @@ attend_kernel(KvCache kv, Attend a) {
     load_keys(t);
     __builtin_amdgcn_sched_barrier(0);
     load_values();
+  }
+  if constexpr (QL) {
+#pragma unroll
+    for (int q = 0; q < QT; ++q)
+#pragma unroll
+      for (int n = 0; n < QS; ++n) *(x8 *)qbuf[q * KS + n * kWaves + wave][lane] = qh[q][n];
+    lds_barrier();
+  }
+  if (t < R.t1) {
     for (; t + kStep < R.t1; t += kStep) {
       int now[NT];
 #pragma unroll
