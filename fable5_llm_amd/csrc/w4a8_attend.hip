@@ -400,10 +400,10 @@ attend_kernel(KvCache kv, Attend a) {
     lbuf[wave][r] = l;
   }
   __syncthreads();
-  float M = mbuf[0][r], L = 0.f;
+  float top = mbuf[0][r], L = 0.f;
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) M = fmaxf(M, mbuf[w][r]);
-  M = base_of(M);
+  for (int w = 1; w < kWaves; ++w) top = fmaxf(top, mbuf[w][r]);
+  const float M = base_of(top);
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) L += lbuf[w][r] * exp2_of(mbuf[w][r] - M);
   const float mine = exp2_of(m - M);
@@ -469,7 +469,7 @@ attend_kernel(KvCache kv, Attend a) {
                   acc[c * VEC + e + 3][i]};
   if (g == 0) {
     float *ml = a.part + (int64_t)a.rows * a.hq * a.splits * D + slot * 2;
-    ml[0] = M;
+    ml[0] = top;                // -infinity where nothing weighs: no bound on the others'
     ml[1] = L;
   }
 }

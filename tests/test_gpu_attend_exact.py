@@ -2,7 +2,7 @@
 counts.  Per output, with u half a step of the cache's type, A = sum p |v| / sum
 p, X the largest sum |q k| scale of a row's scores and V the largest |v|:
 
-    u |out|          the output's rounding
+    u |out|          the output's rounding (int16: half of one step instead)
   + u^2 A            a weight as the sum of two values of the type
   + 2^-39 n V        float16: what lies below the second value's last bit,
                      2^-25 of weights held 2^14 as large
@@ -18,20 +18,21 @@ from test_gpu_attend import DEV, U, make, rows_of, run
 pytestmark = pytest.mark.gpu
 
 
-def check(kv, layer, q, seqs, got, scale=None):
+def check(kv, layer, q, seqs, got, scale=None, unit=1.0, out_unit=None):
     dim, u = kv.head_dim, U[kv.pool.dtype]
     scale = 1.0 / math.sqrt(dim) if scale is None else scale
     lens, per = kv.lens.tolist(), q.shape[1] // kv.kv_heads
-    q, got = q.double().cpu(), got.double().cpu()
+    q, got = q.double().cpu() * unit, got.double().cpu() * (out_unit or 1.0)
     low = 2.0 ** -39 if kv.pool.dtype == torch.float16 else 0.0
     for i, s in enumerate(seqs):
         n = lens[s]
         k, v = (x.repeat_interleave(per, 0) for x in rows_of(kv, layer, s, n))
         sc = (k @ q[i][:, :, None])[:, :, 0] * scale
-        X = (k.abs() @ q[i].abs()[:, :, None]).amax().item() * scale
+        dots = (k.abs() @ q[i].abs()[:, :, None]) * scale
+        X = dots[torch.isfinite(dots)].max().item()
         p = torch.softmax(sc, -1)[:, None]
         want, A = (p @ v)[:, 0], (p @ v.abs())[:, 0]
-        tol = u * want.abs() + u * u * A + low * n * v.abs().max() + \
+        tol = (0.5 * out_unit if out_unit else u * want.abs()) + u * u * A + low * n * v.abs().max() + \
             2.0 ** -24 * A * (X * (dim + 4) + n + 16)
         off = (got[i] - want).abs() / tol
         assert not torch.isnan(got[i]).any() and off.max() <= 1, (i, s, n, float(off.max()))
@@ -47,3 +48,20 @@ def test_weights_keep_more_bits_than_the_output(engine, dtype, dim, heads, group
     q = torch.randn(len(lens), heads * group, dim, generator=gen).to(DEV).to(dtype)
     seqs = [3, 1, 0, 5, 4, 2]
     check(kv, 0, q, seqs, run(engine, kv, 0, q, seqs))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("empty", [(0,), (1,), (3,), (0, 1), (2, 3), (0, 2)])
+def test_a_split_without_a_finite_score_weighs_nothing(engine, dtype, dim, empty):
+    # four workgroups of 128 tokens a row: some with scores of -infinity alone,
+    # the others' so far below zero that 2^score is 0
+    gen = torch.Generator().manual_seed(dim)
+    kv = make(engine, gen, [500, 400], 2, dim, 16, dtype)
+    for s in (0, 1):
+        for j, page in enumerate(kv.tables[s, :-(-[500, 400][s] // 16)].tolist()):
+            kv.pool[page, 0, 0, :, :, 0] = -float("inf") if j // 8 in empty else -480.0
+    q = torch.randn(2, 6, dim, generator=gen).to(DEV).to(dtype)
+    q[:, :, 0] = 1.0
+    out = run(engine, kv, 0, q, [0, 1], scale=1.0)
+    check(kv, 0, q, [0, 1], out, scale=1.0)
