@@ -106,7 +106,8 @@ __device__ __forceinline__ void store_out(const Attend &a, int cache_dtype, int6
 }
 
 // I16: q is int16 (its value of a step is part of a.scale), exact as the sum
-// of two 8-bit halves in the cache's type.  Over a 16-bit cache P goes into the
+// of two 8-bit values of the cache's type, both of q's sign and neither zero
+// unless q is: times an infinite key they are that infinity, not a NaN.  Over a 16-bit cache P goes into the
 // second product as the sum of two values of that type, off by half a step
 // squared (bfloat16 2^-16, float16 2^-22) of a weight, so that the output's own
 // rounding is the only one that counts.
@@ -187,9 +188,10 @@ attend_kernel(KvCache kv, Attend a) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int x = (int16_t)(w[i >> 1] >> (16 * (i & 1)));
-            const int lo = (int)(int8_t)x;
-            qh[0][n][i] = (T)(float)(x - lo);
-            qh[1][n][i] = (T)(float)lo;
+            const int lo = x < 0 ? -(-x & 255) : x & 255, hi = x - lo;
+            const bool both = hi != 0 && lo != 0;
+            qh[0][n][i] = (T)(both ? (float)hi : 0.5f * (float)x);
+            qh[1][n][i] = (T)(both ? (float)lo : 0.5f * (float)x);
           }
         } else {
           qh[0][n] = __builtin_bit_cast(x8, w);

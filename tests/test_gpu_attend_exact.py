@@ -65,3 +65,28 @@ def test_a_split_without_a_finite_score_weighs_nothing(engine, dtype, dim, empty
     q[:, :, 0] = 1.0
     out = run(engine, kv, 0, q, [0, 1], scale=1.0)
     check(kv, 0, q, [0, 1], out, scale=1.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_int16_rows_over_keys_of_infinity(engine, dtype, dim):
+    # q of every kind of bits (a byte of zeros above or below, either sign) against
+    # keys that are infinite in one place: -infinity weighs nothing, and the rest
+    # of the row is what it is without them; +infinity makes the row NaN
+    steps = [256, 1, -1, 255, -255, -256, 127, 128, 129, -128, -32768, 32767, 32512, 3, 511, -512]
+    gen = torch.Generator().manual_seed(dim)
+    lens = [300] * len(steps)
+    kv = make(engine, gen, lens, 1, dim, 16, dtype)
+    q = torch.randint(-40, 41, (len(steps), 4, dim), generator=gen, dtype=torch.int16).to(DEV)
+    for i, x in enumerate(steps):
+        q[i, :, 5] = x
+        for j in (0, 3, 18):
+            kv.pool[kv.tables[i, j], 0, 0, :, 7, 5] = -float("inf") if x > 0 else float("inf")
+    # 13 fraction bits: the largest q is 4, scores stay within a few
+    out = run(engine, kv, 0, q, list(range(len(steps))), frac=13, out_frac=12)
+    check(kv, 0, q, list(range(len(steps))), out, unit=2.0 ** -13, out_unit=2.0 ** -12)
+    for i, x in enumerate(steps):
+        kv.pool[kv.tables[i, 0], 0, 0, :, 7, 5] *= -1
+    torch.cuda.synchronize()
+    out = run(engine, kv, 0, q, list(range(len(steps))), frac=13, out_frac=12)
+    assert (out == -32768).all()                   # NaN as int16
