@@ -309,7 +309,7 @@ attend_kernel(KvCache kv, Attend a) {
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        sc[j][i] = exp2_of(sc[j][i] - (base - LIFT));
+        sc[j][i] = exp2_of(sc[j][i] - base + LIFT);   // a base of millions has no bits for LIFT
         sum += sc[j][i];
       }
     l = l * fall + sum;

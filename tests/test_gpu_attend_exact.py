@@ -90,3 +90,22 @@ def test_int16_rows_over_keys_of_infinity(engine, dtype, dim):
     torch.cuda.synchronize()
     out = run(engine, kv, 0, q, list(range(len(steps))), frac=13, out_frac=12)
     assert (out == -32768).all()                   # NaN as int16
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("size", [600.0, 1100.0, 1.2e4, 6e4])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_of_millions(engine, dtype, size, sign):
+    # scores of 2^k for whole k, exact in float32 as 64 equal products; the
+    # largest weighs 1, those 64 and more below it nothing, whatever their size
+    kv = make(engine, torch.Generator().manual_seed(3), [300, 200], 1, 64, 16, dtype)
+    near = 2.0 ** math.floor(math.log2(size))
+    for s in (0, 1):
+        for j, page in enumerate(kv.tables[s, :-(-[300, 200][s] // 16)].tolist()):
+            kv.pool[page, 0, 0] = sign * near * (1.0 if sign < 0 else 0.5)
+            if j == 5:
+                kv.pool[page, 0, 0, :, 3] = sign * near * (0.5 if sign < 0 else 1.0)
+    q = torch.full((2, 2, 64), near, device=DEV).to(dtype)
+    out = run(engine, kv, 0, q, [0, 1], scale=1.0)
+    for s in (0, 1):
+        assert torch.equal(out[s], kv.pool[kv.tables[s, 5], 0, 1, :, 3].expand(2, -1))
