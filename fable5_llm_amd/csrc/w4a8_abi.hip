@@ -29,7 +29,8 @@ struct w4a8_ctx {
   int grid = 0;            // persistent GEMV grid
   int grid_override = 0;
   int32_t *d_tables = nullptr;
-  int32_t *d_err = nullptr;
+  int32_t *d_err = nullptr;      // error word, and how often it was taken
+  int32_t err_taken = 0;
   uint64_t *d_partials = nullptr;
   int partials_cap = 0;
   int32_t *d_result = nullptr;   // head argmax {idx, val}
@@ -191,7 +192,8 @@ int take_err(w4a8_ctx *c) {
   int32_t h = 0;
   HIP_TRY(hipMemcpy(&h, c->d_err, sizeof(h), hipMemcpyDeviceToHost));
   if (h) {
-    HIP_TRY(hipMemset(c->d_err, 0, sizeof(int32_t)));
+    const int32_t next[2] = {0, c->err_taken = (c->err_taken + 1) & 0x3FFFFFFF};
+    HIP_TRY(hipMemcpy(c->d_err, next, sizeof(next), hipMemcpyHostToDevice));
     // a wait that gave up leaves the launch's results undefined (an
     // overflow found after it is one of them), so it is reported first
     if (h & 2)
@@ -206,13 +208,16 @@ int take_err(w4a8_ctx *c) {
     if (h & 1) return fail(W4A8_E_Y32_OVF, "y32 overflow — sh miscomputed");
     if (h & 16) return fail(W4A8_E_RANGE, "MOVX source is not int8-packed");
     if (h & kErrKvFull)
-      return fail(W4A8_E_RANGE, "KV cache: too few free pages; the call changed nothing");
+      return fail(W4A8_E_RANGE, "KV cache: too few free pages; neither the call nor those on the cache "
+                                "behind it changed anything");
     if (h & kErrKvList)
       return fail(W4A8_E_RANGE, "KV cache: a sequence listed twice, or a fork's child that is "
-                                "not empty or a parent too; the call changed nothing");
+                                "not empty or a parent too; neither the call nor those on the "
+                                "cache behind it changed anything");
     if (h & kErrKvRange)
       return fail(W4A8_E_RANGE, "KV cache: a sequence, position, length or page outside the "
-                                "cache; it was not followed");
+                                "cache; it was not followed (an extend or fork that names it, "
+                                "and the calls on the cache behind that, changed nothing)");
     if (h & kErrDelta)
       return fail(W4A8_E_RANGE, "delta rule: a state slot named twice or outside the states "
                                 "(that row was not run), or bounds that do not lie in order "

@@ -25,6 +25,14 @@ __device__ __forceinline__ int32_t held_pages(const KvCache &kv, int32_t len) {
   return (int32_t)(((int64_t)len + kv.page() - 1) >> kv.lg_page);
 }
 
+// what a reserve or a fork found wrong, by its first thread: reported, and the
+// cache stopped; nothing more where the cache was stopped already
+__device__ __forceinline__ void refuse(const KvCache &kv, int bad) {
+  if (bad & kKvSkip) return;
+  atomicOr(kv.err, bad);
+  kv.scratch[kKvStop] = kv.err[1] + 1;
+}
+
 // exclusive scan of one value per thread of a kOne-thread workgroup, and the
 // total; every thread of it calls
 __device__ int scan_excl(int v, int *total) {
@@ -126,6 +134,7 @@ __global__ __launch_bounds__(kOne) void kv_extend_kernel(KvCache kv, const int32
                                                          const int32_t *counts, int n) {
   __shared__ int bad;
   const FirstRefs refs = first_refs(kv, 1);
+  const bool stopped = kv_stopped(kv);
   int32_t *mark = marks(kv), *list = list_a(kv);
   if (threadIdx.x == 0) bad = 0;
   __syncthreads();
@@ -146,10 +155,11 @@ __global__ __launch_bounds__(kOne) void kv_extend_kernel(KvCache kv, const int32
     else
       need = min(need + held_pages(kv, (int32_t)(len + c)) - held_pages(kv, (int32_t)len), over);
   }
+  if (stopped && threadIdx.x == 0) atomicOr(&bad, kKvSkip);
   const int all = (int)sum_up_to(need, over);     // synchronises: bad is whole
-  if (!bad && all > kv.pages) {
-    if (threadIdx.x == 0) bad = kErrKvFull;
-  } else if (!bad && all > 0 && find_free(kv, all, list, refs) < all) {
+  const bool fine = bad == 0;
+  __syncthreads();                                // and read by all
+  if (fine && (all > kv.pages || (all > 0 && find_free(kv, all, list, refs) < all))) {
     if (threadIdx.x == 0) bad = kErrKvFull;
   }
   __syncthreads();
@@ -192,7 +202,7 @@ __global__ __launch_bounds__(kOne) void kv_extend_kernel(KvCache kv, const int32
       }
     }
   } else if (threadIdx.x == 0) {
-    atomicOr(kv.err, bad);
+    refuse(kv, bad);
   }
   for (int i = threadIdx.x; i < n; i += kOne) {
     const int s = seqs[i];
@@ -209,6 +219,7 @@ __global__ __launch_bounds__(kOne) void kv_fork_kernel(KvCache kv, const int32_t
                                                        const int32_t *children, int n) {
   __shared__ int bad;
   const FirstRefs refs = first_refs(kv, 1);
+  const bool stopped = kv_stopped(kv);
   int32_t *mark = marks(kv), *job = jobs(kv), *list = list_a(kv);
   if (threadIdx.x == 0) bad = 0;
   __syncthreads();
@@ -235,6 +246,7 @@ __global__ __launch_bounds__(kOne) void kv_fork_kernel(KvCache kv, const int32_t
     if (p >= 0 && c >= 0 && p < kv.seqs && atomicAdd(mark + p, 0) != 0)
       atomicOr(&bad, kErrKvList);
   }
+  if (stopped && threadIdx.x == 0) atomicOr(&bad, kKvSkip);
   __syncthreads();
   const bool fine = bad == 0;
   if (fine && all > 0 && find_free(kv, all, list, refs) < all) {
@@ -263,7 +275,7 @@ __global__ __launch_bounds__(kOne) void kv_fork_kernel(KvCache kv, const int32_t
       }
     }
   } else if (threadIdx.x == 0) {
-    atomicOr(kv.err, bad);
+    refuse(kv, bad);
   }
   if (threadIdx.x == 0) kv.scratch[0] = bad == 0;
   for (int i = threadIdx.x; i < n; i += kOne) {
@@ -312,8 +324,9 @@ __global__ __launch_bounds__(256) void kv_fork_rows_kernel(KvCache kv, const int
 // A workgroup per listed sequence; a sequence listed again, or already empty,
 // is left alone.  3.1 us for 32 sequences of up to 1,500 tokens.
 __global__ __launch_bounds__(256) void kv_free_kernel(KvCache kv, const int32_t *seqs) {
+  const bool stopped = kv_stopped(kv);
   const int i = blockIdx.x, s = seqs[i];
-  if (s < 0) return;
+  if (s < 0 || stopped) return;
   if (s >= kv.seqs) {
     if (threadIdx.x == 0) atomicOr(kv.err, kErrKvRange);
     return;
@@ -345,6 +358,7 @@ __global__ __launch_bounds__(256) void kv_free_kernel(KvCache kv, const int32_t 
 __global__ __launch_bounds__(kOne) void kv_compact_kernel(KvCache kv) {
   int32_t *holes = list_a(kv), *to = list_b(kv);
   FirstRefs refs = first_refs(kv, 0);
+  if (kv_stopped(kv)) return;
   int used = 0, U;
 #pragma unroll
   for (int i = 0; i < kRefsPerThread; ++i) used += refs.r[i] != 0;
@@ -417,6 +431,7 @@ __device__ __forceinline__ void copy_piece(uint8_t *b, const uint8_t *a, int64_t
 // no copy reads what another writes.  Bound by HBM: 238 MB read and written in
 // 44 us, 5.4 TB/s.
 __global__ __launch_bounds__(256) void kv_move_kernel(KvCache kv) {
+  if (kv_stopped(kv)) return;
   const int moves = kv.scratch[0], U = kv.scratch[1];
   const int32_t *holes = list_a(kv), *to = list_b(kv);
   for (int s = blockIdx.x; s < kv.seqs; s += gridDim.x) {
@@ -443,6 +458,7 @@ __global__ __launch_bounds__(256) void kv_move_kernel(KvCache kv) {
 
 __global__ __launch_bounds__(256) void kv_copy_kernel(KvCache kv, const int32_t *src,
                                                       const int32_t *dst, int n) {
+  if (kv_stopped(kv)) return;
   const int64_t pieces = (kv.page_bytes + kPiece - 1) / kPiece;
   for (int64_t w = blockIdx.x; w < n * pieces; w += gridDim.x) {
     const int m = (int)(w / pieces);
@@ -489,8 +505,9 @@ __global__ __launch_bounds__(64 * kAppendWaves) void kv_append_kernel(KvCache kv
 #pragma unroll
   for (int u = 0; u < U; ++u)
     if (lane + 64 * u < all) load(lane + 64 * u, v[u]);
+  const bool stopped = kv_stopped(kv);
   const int s = a.seqs[i];
-  if (s < 0) return;
+  if (s < 0 || stopped) return;
   bool ok = s < kv.seqs;
   int page = -1, pos = 0;
   if (ok) {

@@ -16,6 +16,7 @@ constexpr int kErrKvRange = 32;    // a sequence, position or page outside the c
 constexpr int kErrKvFull = 64;     // too few free pages
 constexpr int kErrKvList = 128;    // a sequence listed twice, or a child not empty
 constexpr int kErrDelta = 256;     // a state slot or a prompt's bounds
+constexpr int kKvSkip = 1 << 30;   // never in the word: the call comes behind a refused one
 
 // 16-byte loads and stores that pass the caches by: data read or written once
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -35,7 +36,7 @@ struct KvCache {
   uint8_t *pool;
   int32_t *refs, *tables, *lens;
   int32_t *scratch;           // kv_scratch_words(seqs, pages) words, marks zero
-  int32_t *err;
+  int32_t *err;               // the context's error word, and how often it was taken
   int32_t pages, seqs, max_pages, lg_page;
   int32_t layers, heads, dim, esize, dtype;
   int64_t page_bytes;
@@ -46,6 +47,14 @@ struct KvCache {
 constexpr int kKvHead = 64;
 inline size_t kv_scratch_words(int64_t seqs, int64_t pages) {
   return kKvHead + 2 * (size_t)seqs + 2 * (size_t)pages;
+}
+// word of scratch that a refused reserve or fork leaves: 1 + how often the
+// error word had been taken.  Until the next time, calls that change the cache
+// do nothing: those behind the refused one count on it (an append without
+// positions would overwrite the token before).
+constexpr int kKvStop = 2;
+__device__ __forceinline__ bool kv_stopped(const KvCache &kv) {
+  return kv.scratch[kKvStop] == kv.err[1] + 1;
 }
 hipError_t launch_kv_extend(const KvCache &kv, const int32_t *seqs, const int32_t *counts,
                             int32_t n, hipStream_t s);

@@ -150,7 +150,9 @@ class PagedKV:
 
     def extend_async(self, seqs, counts):
         """Sequence seqs[i] grows by counts[i] tokens, pages added as needed:
-        lowest free page first, in the order of the list, all or nothing."""
+        lowest free page first, in the order of the list, all or nothing.  A
+        refused call (the next sync reports it) stops the cache until that
+        sync: calls behind it change nothing."""
         p = _list(seqs, self.ctx, "seqs")
         N.check(N.lib().w4a8_kv_extend_async(
             self.h, p, _list(counts, self.ctx, "counts", seqs.shape[0]), seqs.shape[0]),
@@ -204,7 +206,8 @@ class PagedKV:
 
     def fork_async(self, parents, children):
         """Sequence children[i], empty, becomes a copy of parents[i]: full
-        pages shared, the used tokens of the last page copied."""
+        pages shared, the used tokens of the last page copied; all or nothing,
+        and what it stops, as extend_async."""
         p = _list(parents, self.ctx, "parents")
         n = parents.shape[0]
         N.check(N.lib().w4a8_kv_fork_async(

@@ -442,7 +442,11 @@ int w4a8_kv_destroy(w4a8_kv *kv);
 /* sequence d_seqs[i] grows by d_counts[i] tokens: pages are added as needed,
    the lowest free ones first, in the order of the list.  All or nothing: with
    too few free pages, a sequence listed twice or outside the cache, or one
-   that would pass max_pages, nothing changes and the next sync reports it. */
+   that would pass max_pages, nothing changes and the next sync reports it.
+   Until then the calls on the cache behind it (extend, append, fork, free,
+   compact, copy) change nothing either, replays of captured ones included: an
+   append at the last token would otherwise overwrite the token before.  The
+   cache is as it was before the refused call, which may be made again. */
 int w4a8_kv_extend_async(w4a8_kv *kv, const int32_t *d_seqs,
                          const int32_t *d_counts, int32_t n);
 /* token i's keys and values of one layer, k and v [n][kv_heads][head_dim] of
@@ -456,7 +460,7 @@ int w4a8_kv_append_async(w4a8_kv *kv, int32_t layer, int32_t dtype, int32_t frac
 /* sequence d_children[i], empty, becomes a copy of d_parents[i]: full pages
    are shared, the used tokens of a last page that is not full are copied to a
    free page (lowest first, in the order of the list).  A parent may be listed
-   many times.  All or nothing as above; a child listed twice, not empty, or a
+   many times.  All or nothing, and what it stops, as above; a child listed twice, not empty, or a
    parent too, is refused. */
 int w4a8_kv_fork_async(w4a8_kv *kv, const int32_t *d_parents,
                        const int32_t *d_children, int32_t n);
