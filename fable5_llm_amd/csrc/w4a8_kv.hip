@@ -353,12 +353,14 @@ __global__ __launch_bounds__(256) void kv_free_kernel(KvCache kv, const int32_t 
 // ------------------------------------------------------------------ compact
 // First kernel, one workgroup: U pages are in use; the k-th page in use at U
 // or above moves to the k-th free page below U (there are as many of either).
-// list_a: where it is, list_b[page]: where it goes; the counts move with it.
-// scratch[0] = moves, scratch[1] = U.  8.7 us for 2,048 pages.
+// list_a: the free pages that are filled.  list_b[page]: where a page at U or
+// above goes; which page comes to a filled one; -1 for the others.  The counts
+// move too.  scratch[0] = moves, scratch[1] = U.  8.7 us for 2,048 pages.
 __global__ __launch_bounds__(kOne) void kv_compact_kernel(KvCache kv) {
   int32_t *holes = list_a(kv), *to = list_b(kv);
   FirstRefs refs = first_refs(kv, 0);
   if (kv_stopped(kv)) return;
+  for (int p = threadIdx.x; p < kv.pages; p += kOne) to[p] = -1;
   int used = 0, U;
 #pragma unroll
   for (int i = 0; i < kRefsPerThread; ++i) used += refs.r[i] != 0;
@@ -392,14 +394,11 @@ __global__ __launch_bounds__(kOne) void kv_compact_kernel(KvCache kv) {
     from += all;
 #pragma unroll
     for (int i = 0; i < kRefsPerThread; ++i)
-      if (r[i] == 0 && p0 + i >= U && p0 + i < kv.pages) to[p0 + i] = -1;
-#pragma unroll
-    for (int i = 0; i < kRefsPerThread; ++i)
       if (r[i] != 0 && p0 + i >= U) {
         const int hole = at < min(moves, U) ? holes[at] : -1;
         if (hole >= 0) {
           to[p0 + i] = hole;
-          to[hole] = p0 + i;      // below U: the page that comes here
+          to[hole] = p0 + i;
           kv.refs[hole] = r[i];
           kv.refs[p0 + i] = 0;
         }
@@ -439,12 +438,12 @@ __global__ __launch_bounds__(256) void kv_move_kernel(KvCache kv) {
     int32_t *row = kv.tables + (int64_t)s * kv.max_pages;
     for (int j = threadIdx.x; j < held; j += 256) {
       const int p = row[j];
-      if (p >= 0 && p < U) continue;
-      const int q = (uint32_t)p < (uint32_t)kv.pages ? to[p] : -1;
-      if (q < 0)              // no page, or one that no sequence holds
-        atomicOr(kv.err, kErrKvRange);
-      else
-        row[j] = q;
+      const bool page = (uint32_t)p < (uint32_t)kv.pages;
+      const int q = page ? to[p] : -1;
+      // no page, or one that no sequence held: at U or above it goes nowhere,
+      // below U another one comes there
+      if (!page || (p < U) != (q < 0)) atomicOr(kv.err, kErrKvRange);
+      else if (q >= 0) row[j] = q;
     }
   }
   const int64_t pieces = (kv.page_bytes + kPiece - 1) / kPiece;
