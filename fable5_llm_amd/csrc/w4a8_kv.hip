@@ -321,21 +321,22 @@ __global__ __launch_bounds__(256) void kv_fork_rows_kernel(KvCache kv, const int
 }
 
 // --------------------------------------------------------------------- free
-// A workgroup per listed sequence; a sequence listed again, or already empty,
-// is left alone.  3.1 us for 32 sequences of up to 1,500 tokens.
+// A workgroup per listed sequence, which takes its length: of the workgroups of
+// one listed again, and of an empty one, there is nothing left to free.  3.1 us
+// for 32 sequences of up to 1,500 tokens; 2^20 entries take 2^20 workgroups'
+// time (each looking through those before it would be 2^39 comparisons).
 __global__ __launch_bounds__(256) void kv_free_kernel(KvCache kv, const int32_t *seqs) {
+  __shared__ int taken;
   const bool stopped = kv_stopped(kv);
-  const int i = blockIdx.x, s = seqs[i];
+  const int s = seqs[blockIdx.x];
   if (s < 0 || stopped) return;
   if (s >= kv.seqs) {
     if (threadIdx.x == 0) atomicOr(kv.err, kErrKvRange);
     return;
   }
-  int again = 0;
-  for (int j = threadIdx.x; j < i; j += 256) again |= seqs[j] == s;
-  if (__syncthreads_or(again)) return;
-  const int len = kv.lens[s];
-  const int held = min(held_pages(kv, max(len, 0)), kv.max_pages);
+  if (threadIdx.x == 0) taken = atomicExch(kv.lens + s, 0);
+  __syncthreads();
+  const int held = min(held_pages(kv, max(taken, 0)), kv.max_pages);
   const int32_t *row = kv.tables + (int64_t)s * kv.max_pages;
   for (int j = threadIdx.x; j < held; j += 256) {
     const int page = row[j];
@@ -346,8 +347,6 @@ __global__ __launch_bounds__(256) void kv_free_kernel(KvCache kv, const int32_t 
       atomicOr(kv.err, kErrKvRange);
     }
   }
-  __syncthreads();
-  if (threadIdx.x == 0) kv.lens[s] = 0;
 }
 
 // ------------------------------------------------------------------ compact
