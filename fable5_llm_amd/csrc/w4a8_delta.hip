@@ -30,7 +30,7 @@ __device__ __forceinline__ T from_float(float x, float out_unit) {
 
 // The slot of a row's state, -1 for none: a padded row, or a slot that an
 // earlier row names too or that lies outside the states, which is reported.
-// The whole workgroup asks.
+// The whole workgroup asks, of a call with one token a row.
 __device__ __forceinline__ int slot_of(const Delta &p, int row, bool tell) {
   const int slot = p.slots ? p.slots[row] : row;
   int taken = 0;
@@ -225,23 +225,62 @@ __device__ __forceinline__ int first_chunk(const Delta &p, int row) {
   return p.cu[row] / C + row;
 }
 
-// Whether every row's bounds lie in order within the tokens (the whole
-// workgroup asks), and which row chunk `slot` belongs to (-1: none).
-__device__ __forceinline__ bool bounds_ok(const Delta &p, int slot, int *row) {
-  __shared__ int found;
-  if (threadIdx.x == 0) found = -1;
-  __syncthreads();
-  int bad = 0;
-  for (int j = threadIdx.x; j < p.rows; j += blockDim.x) {
-    const int t0 = p.cu[j], t1 = p.cu[j + 1];
-    const bool off = t0 < 0 || t1 < t0 || t1 > p.tokens;
-    bad |= off;
-    const int at = slot - (t0 / C + j);
-    if (!off && at >= 0 && at < (t1 - t0 + C - 1) / C) found = j;
+// Chunks that the workspace has room for, and where behind them the rows'
+// verdicts lie: each row's slot (-1: none), then for every kCheck rows whether
+// the bounds of one of them are out of order.
+constexpr int kCheck = 256;
+__device__ __forceinline__ int64_t chunks_of(const Delta &p) { return p.tokens / C + p.rows; }
+__device__ __forceinline__ int32_t *row_slots(const Delta &p, int64_t chunk_bytes) {
+  return (int32_t *)((uint8_t *)p.ws + chunks_of(p) * chunk_bytes);
+}
+__device__ __forceinline__ int32_t *row_faults(const Delta &p, int64_t chunk_bytes) {
+  return row_slots(p, chunk_bytes) + p.rows;
+}
+
+// The verdicts on rows kCheck part .., by a workgroup of kCheck threads: what it
+// finds wrong is reported here.  A row's slot is looked for among the earlier
+// rows' a tile of them at a time.
+__device__ void check_rows(const Delta &p, int part, int32_t *slots, int32_t *faults) {
+  __shared__ __align__(16) int32_t tile[kCheck];
+  const int j = part * kCheck + threadIdx.x;
+  const bool on = j < p.rows;
+  const int t0 = on ? p.cu[j] : 0, t1 = on ? p.cu[j + 1] : 0;
+  int slot = !on ? -1 : p.slots ? p.slots[j] : j;
+  bool taken = slot >= p.nslots;
+  const int last = min(part * kCheck + kCheck, p.rows);
+  for (int base = 0; p.slots && base < last; base += kCheck) {
+    const int i = base + threadIdx.x;
+    __syncthreads();
+    tile[threadIdx.x] = i < last ? p.slots[i] : -1;
+    __syncthreads();
+    const int n = min(kCheck, last - base);
+    for (int k = 0; k < n; ++k) taken |= tile[k] == slot && base + k < j && slot >= 0;
   }
-  bad = __syncthreads_or(bad);
-  *row = found;
-  return !bad;
+  const int bad = __syncthreads_or(t0 < 0 || t1 < t0 || t1 > p.tokens);
+  const int wrong = __syncthreads_or(taken);
+  if (on) slots[j] = taken ? -1 : slot;
+  if (threadIdx.x == 0) {
+    faults[part] = bad;
+    if (bad || wrong) atomicOr(p.err, kErrDelta);
+  }
+}
+
+// Which row chunk `slot` of the workspace belongs to, -1: none (a row's chunks
+// are fewer than its room, or its bounds are out of order).  The last row whose
+// first chunk is not behind it, looked for among blockDim.x rows at a time; the
+// whole workgroup asks.
+__device__ __forceinline__ int row_of(const Delta &p, int slot) {
+  int lo = 0, n = p.rows;
+  while (n > 1) {
+    const int step = (n + (int)blockDim.x - 1) / (int)blockDim.x, at = (int)threadIdx.x * step;
+    const int before = __syncthreads_count(at < n && first_chunk(p, lo + at) <= slot);
+    if (before == 0) return -1;
+    lo = __builtin_amdgcn_readfirstlane(lo + (before - 1) * step);
+    n = __builtin_amdgcn_readfirstlane(min(step, n - (before - 1) * step));
+  }
+  const int t0 = p.cu[lo], t1 = p.cu[lo + 1], at = slot - (t0 / C + lo);
+  if (t0 < 0 || t1 < t0 || t1 > p.tokens || at < 0 || at >= (t1 - t0 + C - 1) / C) return -1;
+  return lo;
 }
 
 // A chunk in the workspace: M, P and factors per value head, rows per key head;
@@ -252,7 +291,9 @@ struct Space {
   uint8_t *ws;
   int64_t chunks, chunk, heads;
   __device__ Space(const Delta &p, int64_t c)
-      : ws((uint8_t *)p.ws), chunks(p.tokens / C + p.rows), chunk(c), heads(p.hv) {}
+      : ws((uint8_t *)p.ws), chunks(chunks_of(p)), chunk(c), heads(p.hv) {}
+  // of a chunk, all heads
+  static __device__ int64_t bytes(const Delta &p) { return (int64_t)p.hv * kHeadBytes + p.hk * kRows; }
   __device__ uint8_t *head(int h) const { return ws + (h * chunks + chunk) * kHeadBytes; }
   // 0: K, 1: Q
   __device__ bf16x8 *rows(int hk, int which) const {
@@ -261,7 +302,8 @@ struct Space {
   }
 };
 
-// A workgroup per chunk, key head and share of its value heads.  It lays K and
+// A workgroup per chunk, key head and share of its value heads, and behind the
+// chunks' one per kCheck rows for the verdicts on them.  It lays K and
 // Q out as the operands that delta_scan_kernel reads, in whole lines (read where
 // they lie, rows of a prompt 4 KB apart all fall to one channel of the L2: the
 // scan of 8192 tokens, 16 key heads of 128, took 34 us more).  Tiles of M and P
@@ -281,11 +323,13 @@ __global__ __launch_bounds__(256, 2) void delta_prep_kernel(Delta p) {
   __shared__ __align__(16) float At[C * LD];       // A transposed
   __shared__ __align__(16) float Tt[4][16 * 20];   // its diagonal blocks' inverses, transposed
   const int slot = blockIdx.x, hk = blockIdx.y;
-  int row;
-  if (!bounds_ok(p, slot, &row)) {
-    if (slot == 0 && hk == 0 && blockIdx.z == 0 && threadIdx.x == 0) atomicOr(p.err, kErrDelta);
+  if (slot >= chunks_of(p)) {
+    const int64_t bytes = Space<DK, T>::bytes(p);
+    if (hk == 0 && blockIdx.z == 0)
+      check_rows(p, slot - (int)chunks_of(p), row_slots(p, bytes), row_faults(p, bytes));
     return;
   }
+  const int row = row_of(p, slot);
   if (row < 0) return;
   const int chunk = slot - first_chunk(p, row);
   const int t0 = p.cu[row] + chunk * C, len = min(C, p.cu[row + 1] - t0);
@@ -495,9 +539,11 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
   const int unit = xcd * each + at / tiles;
   if (at / tiles >= each || unit >= units) return;
   const int row = unit / p.hv, h = unit - row * p.hv, hk = h / (p.hv / p.hk);
-  int dummy;
-  if (!bounds_ok(p, -1, &dummy)) return;          // reported by delta_prep_kernel
-  const int slot = slot_of(p, row, h == 0 && at % tiles == 0);
+  const int32_t *faults = row_faults(p, Space<DK, T>::bytes(p));
+  const int slot = row_slots(p, Space<DK, T>::bytes(p))[row];
+  int bad = 0;
+  for (int i = threadIdx.x; i < (p.rows + kCheck - 1) / kCheck; i += 512) bad |= faults[i];
+  if (__syncthreads_or(bad)) return;              // reported by delta_prep_kernel
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
   const int col = (at % tiles) * 16 + r;
@@ -826,7 +872,8 @@ void launch_typed(const Delta &d, int num_cu, hipStream_t s) {
   const int64_t units = (d.tokens / C + (int64_t)d.rows) * d.hk;
   const int shares =
       (int)std::max<int64_t>(std::min<int64_t>(d.hv / d.hk, 2 * num_cu / units), 1);
-  delta_prep_kernel<DK, T><<<dim3(d.tokens / C + d.rows, d.hk, shares), 256, 0, s>>>(d);
+  const int parts = (d.rows + kCheck - 1) / kCheck;
+  delta_prep_kernel<DK, T><<<dim3(d.tokens / C + d.rows + parts, d.hk, shares), 256, 0, s>>>(d);
   const int64_t each = ((int64_t)d.rows * d.hv + 7) / 8;
   delta_scan_kernel<DK, T><<<(uint32_t)(8 * each * (d.dv / 16)), 512, 0, s>>>(d);
 }
@@ -845,7 +892,9 @@ int64_t delta_workspace(int64_t tokens, int64_t rows, int64_t hk, int64_t hv, in
                         int dtype) {
   const int terms = dtype == DT_F32 ? Terms<float>::n
                     : dtype == DT_BF16 ? Terms<__bf16>::n : Terms<_Float16>::n;
-  return (tokens / C + rows) * (hv * kHeadBytes + hk * rows_bytes(dk, terms));
+  const int64_t verdicts = 4 * (rows + (rows + kCheck - 1) / kCheck);
+  return (tokens / C + rows) * (hv * kHeadBytes + hk * rows_bytes(dk, terms)) +
+         (verdicts + 15) / 16 * 16;
 }
 
 hipError_t launch_delta(const Delta &d, int num_cu, hipStream_t s) {
