@@ -41,6 +41,63 @@ __device__ __forceinline__ int slot_of(const Delta &p, int row, bool tell) {
   return taken ? -1 : slot;
 }
 
+// The same for the rows kCheck part .., one a thread of a workgroup of kCheck,
+// which compares them with all earlier ones, a tile of them at a time.
+constexpr int kCheck = 256;
+__device__ __forceinline__ int claim_slot(const Delta &p, int part) {
+  constexpr int TILE = 8 * kCheck;
+  __shared__ __align__(16) int32_t tile[TILE];
+  const int first = part * kCheck, j = first + (int)threadIdx.x;
+  const int slot = j >= p.rows ? -1 : p.slots ? p.slots[j] : j;
+  bool taken = slot >= p.nslots;
+  for (int base = 0; p.slots && base < first + kCheck; base += TILE) {
+    int32_t x[TILE / kCheck];
+#pragma unroll
+    for (int i = 0; i < TILE / kCheck; ++i) {
+      const int at = base + i * kCheck + (int)threadIdx.x;
+      x[i] = at < p.rows ? p.slots[at] : -1;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TILE / kCheck; ++i) tile[i * kCheck + threadIdx.x] = x[i];
+    __syncthreads();
+    const int whole = min(first - base, TILE);      // of them, all earlier than this part's
+#pragma unroll 16
+    for (int k = 0; k < whole; k += 4) {
+      const int4 t = *(const int4 *)(tile + k);
+      taken |= (t.x == slot) | (t.y == slot) | (t.z == slot) | (t.w == slot);
+    }
+    if (whole < TILE)
+#pragma unroll 16
+      for (int k = 0; k < kCheck; k += 4) {
+        const int4 t = *(const int4 *)(tile + whole + k);
+        const int mine = (int)threadIdx.x - k;      // rows of it before this thread's
+        taken |= ((t.x == slot) & (mine > 0)) | ((t.y == slot) & (mine > 1)) |
+                 ((t.z == slot) & (mine > 2)) | ((t.w == slot) & (mine > 3));
+      }
+  }
+  taken = taken && slot >= 0;
+  if (__syncthreads_or(taken) && threadIdx.x == 0) atomicOr(p.err, kErrDelta);
+  return taken ? -1 : slot;
+}
+
+// Of many rows, each workgroup of delta_step_kernel looking through the earlier
+// ones costs more than a kernel that does it once, and leaves a row's slot where
+// the row's workgroups will write their outputs, in the first 4 bytes of each
+// one's columns: 2^20 rows of 4 heads 567 -> 33 ms (8.5 of them the states'),
+// 65,536 of 1 head 0.76 -> 0.61, 16,384 of 4 0.31 -> 0.25; but 16,384 of 1 0.08
+// -> 0.16, so it is done where rows have workgroups enough.
+constexpr int kManyRows = 16384, kManyUnits = 65536;
+template <typename T>
+__global__ __launch_bounds__(kCheck) void delta_claim_kernel(Delta p) {
+  const int slot = claim_slot(p, blockIdx.x);
+  const int64_t row = (int64_t)blockIdx.x * kCheck + threadIdx.x;
+  if (row >= p.rows) return;
+  for (int h = 0; h < p.hv; ++h)
+    for (int col = 0; col < p.dv; col += 64)
+      *(int32_t *)((T *)p.out + row * p.out_token + h * p.out_head + col) = slot;
+}
+
 // One token of each row: a wavefront holds 16 columns of a head's state in
 // registers, lane (rg, cq) = (lane >> 2, lane & 3) its rows NR rg .. and
 // columns 4 cq .., so that a state is read and written once, in 64-byte runs.
@@ -50,7 +107,14 @@ template <int DK, typename T>
 __global__ __launch_bounds__(256) void delta_step_kernel(Delta p) {
   constexpr int NR = DK / 16;
   const int row = blockIdx.x, h = blockIdx.y;
-  const int slot = slot_of(p, row, h == 0 && blockIdx.z == 0);
+  int slot;
+  if (p.claimed) {
+    slot = *(const int32_t *)((const T *)p.out + row * p.out_token + h * p.out_head +
+                              blockIdx.z * 64);
+    __syncthreads();             // read by all before it is written over
+  } else {
+    slot = slot_of(p, row, h == 0 && blockIdx.z == 0);
+  }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int rg = lane >> 2, col = (blockIdx.z * 4 + wave) * 16 + (lane & 3) * 4;
   if (col >= p.dv) return;
@@ -228,7 +292,6 @@ __device__ __forceinline__ int first_chunk(const Delta &p, int row) {
 // Chunks that the workspace has room for, and where behind them the rows'
 // verdicts lie: each row's slot (-1: none), then for every kCheck rows whether
 // the bounds of one of them are out of order.
-constexpr int kCheck = 256;
 __device__ __forceinline__ int64_t chunks_of(const Delta &p) { return p.tokens / C + p.rows; }
 __device__ __forceinline__ int32_t *row_slots(const Delta &p, int64_t chunk_bytes) {
   return (int32_t *)((uint8_t *)p.ws + chunks_of(p) * chunk_bytes);
@@ -238,30 +301,17 @@ __device__ __forceinline__ int32_t *row_faults(const Delta &p, int64_t chunk_byt
 }
 
 // The verdicts on rows kCheck part .., by a workgroup of kCheck threads: what it
-// finds wrong is reported here.  A row's slot is looked for among the earlier
-// rows' a tile of them at a time.
+// finds wrong is reported here.
 __device__ void check_rows(const Delta &p, int part, int32_t *slots, int32_t *faults) {
-  __shared__ __align__(16) int32_t tile[kCheck];
-  const int j = part * kCheck + threadIdx.x;
+  const int j = part * kCheck + (int)threadIdx.x;
   const bool on = j < p.rows;
   const int t0 = on ? p.cu[j] : 0, t1 = on ? p.cu[j + 1] : 0;
-  int slot = !on ? -1 : p.slots ? p.slots[j] : j;
-  bool taken = slot >= p.nslots;
-  const int last = min(part * kCheck + kCheck, p.rows);
-  for (int base = 0; p.slots && base < last; base += kCheck) {
-    const int i = base + threadIdx.x;
-    __syncthreads();
-    tile[threadIdx.x] = i < last ? p.slots[i] : -1;
-    __syncthreads();
-    const int n = min(kCheck, last - base);
-    for (int k = 0; k < n; ++k) taken |= tile[k] == slot && base + k < j && slot >= 0;
-  }
+  const int slot = claim_slot(p, part);
+  if (on) slots[j] = slot;
   const int bad = __syncthreads_or(t0 < 0 || t1 < t0 || t1 > p.tokens);
-  const int wrong = __syncthreads_or(taken);
-  if (on) slots[j] = taken ? -1 : slot;
   if (threadIdx.x == 0) {
     faults[part] = bad;
-    if (bad || wrong) atomicOr(p.err, kErrDelta);
+    if (bad) atomicOr(p.err, kErrDelta);
   }
 }
 
@@ -861,6 +911,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
 template <int DK, typename T>
 void launch_typed(const Delta &d, int num_cu, hipStream_t s) {
   if (!d.cu) {
+    if (d.claimed) delta_claim_kernel<T><<<(d.rows + kCheck - 1) / kCheck, kCheck, 0, s>>>(d);
     delta_step_kernel<DK, T><<<dim3(d.rows, d.hv, (d.dv + 63) / 64), 256, 0, s>>>(d);
     return;
   }
@@ -897,7 +948,9 @@ int64_t delta_workspace(int64_t tokens, int64_t rows, int64_t hk, int64_t hv, in
          (verdicts + 15) / 16 * 16;
 }
 
-hipError_t launch_delta(const Delta &d, int num_cu, hipStream_t s) {
+hipError_t launch_delta(Delta d, int num_cu, hipStream_t s) {
+  d.claimed = !d.cu && d.slots && d.rows >= kManyRows &&
+              (int64_t)d.rows * d.hv * ((d.dv + 63) / 64) >= kManyUnits;
   if (d.dk == 64) launch_dim<64>(d, num_cu, s);
   else launch_dim<128>(d, num_cu, s);
   return hipGetLastError();

@@ -104,10 +104,11 @@ struct Delta {
   float scale, eps;
   float unit, out_unit;         // DT_I16: the value of a step of q, k, v; 1 / that of out
   int32_t *err;
+  int32_t claimed;              // one token per row: the rows' slots lie in out (launch_delta)
 };
 constexpr int64_t kDeltaStride = 1 << 23;   // of v's and out's tokens, whole prompts
 int64_t delta_workspace(int64_t tokens, int64_t rows, int64_t hk, int64_t hv, int64_t dk,
                         int dtype);
-hipError_t launch_delta(const Delta &d, int num_cu, hipStream_t s);
+hipError_t launch_delta(Delta d, int num_cu, hipStream_t s);
 
 }  // namespace w4a8

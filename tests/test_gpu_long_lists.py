@@ -159,3 +159,50 @@ def test_prompts_in_proportion(engine):
         torch.cuda.empty_cache()
     print(times)
     assert times[1 << 18] < 4 * 32 * times[1 << 13], times
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,dv", [(16383, 256), (16400, 256), (33000, 80), (70001, 16)])
+def test_a_token_of_many_rows(engine, dtype, rows, dv):
+    # slots in any order, padded rows, rows that name an earlier one's slot or none
+    # of the states, near and far; out in every other head of a wider row.  One
+    # token of 64 terms: 8 sqrt(65) 2^-24 of the largest state, 8, and half a step
+    gen = torch.Generator().manual_seed(rows)
+    d, _ = prompts(gen, torch.ones(rows, dtype=torch.int64), dtype, dv=dv)
+    slots = torch.randperm(rows, generator=gen)
+    slots[[5, 300, rows - 2]] = -1
+    slots[rows - 1] = slots[3]
+    slots[256], slots[513], slots[1] = slots[255], slots[2], slots[0]
+    slots[700] = rows
+    good = slots.clone()
+    good[[rows - 1, 256, 513, 1, 700]] = -1
+    first = d["state"].clone()
+    wide = torch.full((rows, 2, dv), 3.0, device=DEV).to(dtype)
+    sl = slots.to(torch.int32).to(DEV)
+    torch.cuda.synchronize()
+    engine.delta_step_async(**d, out=wide[:, 1:], slots=sl)
+    with pytest.raises(AssertionError, match="state slot"):
+        engine.sync()
+    at = torch.nonzero(good >= 0)[:, 0].to(DEV)
+    s = good[good >= 0].to(DEV)
+    want, w_out = first[:, 0].double(), torch.zeros(rows, dv, device=DEV, dtype=torch.float64)
+    want[s], w_out[at] = token(d, want[s], at)
+    assert want.abs().max() < 8
+    tol = 8 * 65 ** 0.5 * 2.0 ** -24 * 8
+    assert (d["state"][:, 0].double() - want).abs().max() <= tol
+    half = torch.finfo(dtype).eps / 2
+    assert ((wide[:, 1].double() - w_out).abs() <= tol + half * w_out.abs()).all()
+    assert (wide[:, 0] == 3).all()
+
+
+def test_tokens_in_proportion(engine):
+    times = {}
+    for rows in (1 << 15, 1 << 20):
+        gen = torch.Generator().manual_seed(3)
+        d, _ = prompts(gen, torch.ones(rows, dtype=torch.int64), torch.bfloat16)
+        out, sl = torch.ones_like(d["v"]), torch.randperm(rows, generator=gen)
+        sl = sl.to(torch.int32).to(DEV)
+        times[rows] = seconds(engine, lambda: engine.delta_step_async(**d, out=out, slots=sl),
+                              lambda: None)
+    print(times)
+    assert times[1 << 20] < 4 * 32 * times[1 << 15], times
