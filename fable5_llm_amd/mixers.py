@@ -8,7 +8,13 @@ entry is padding; what they hold is checked on the device and reported, as an
 AssertionError, by the next Context.sync().  Activations are float32,
 bfloat16, float16 or the engine's own int16 with `frac` fraction bits; they
 may be strided, with a contiguous last dimension, 16-byte aligned.  No output
-or workspace overlaps an input.
+or workspace overlaps an input or another output.
+
+A call's tensors, lists and workspaces too, are used after it has returned:
+they are made before the context's stream gets to the call, and kept, unwritten,
+until the work is done (a tensor made in the call's own brackets is torch's
+again at once).  A captured graph needs its PagedKVs open as long as it is
+replayed.
 """
 import ctypes
 import math

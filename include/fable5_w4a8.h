@@ -412,7 +412,11 @@ int w4a8_plan_destroy(w4a8_plan *plan);
  * device arrays of at most 2^20 entries; a negative entry is padding and is
  * skipped.  What a list or a table holds is checked on the device: an entry
  * outside the cache is not followed, and the next w4a8_ctx_sync() returns
- * W4A8_E_RANGE.  No output or workspace overlaps an input. */
+ * W4A8_E_RANGE.  No output or workspace overlaps an input or another output.
+ * Buffers, lists and workspaces among them, are used on the context's stream
+ * after the call has returned and stay until the work is done; a cache is not
+ * destroyed while a captured graph with calls on it may be replayed.  An int16
+ * output saturates (a NaN: at the lowest value). */
 #define W4A8_DT_F32   0
 #define W4A8_DT_BF16  1
 #define W4A8_DT_F16   2
@@ -452,7 +456,8 @@ int w4a8_kv_extend_async(w4a8_kv *kv, const int32_t *d_seqs,
 /* token i's keys and values of one layer, k and v [n][kv_heads][head_dim] of
    the cache's dtype or int16, to sequence d_seqs[i] at position d_pos[i] <
    its length (null: its last token).  Two tokens for the same place leave
-   either one's values there. */
+   either one's values there; a place in a page that other sequences hold too
+   is theirs as well. */
 int w4a8_kv_append_async(w4a8_kv *kv, int32_t layer, int32_t dtype, int32_t frac,
                          const void *d_k, int64_t k_token, int64_t k_head,
                          const void *d_v, int64_t v_token, int64_t v_head,
