@@ -42,32 +42,31 @@ __device__ __forceinline__ int slot_of(const Delta &p, int row, bool tell) {
 }
 
 // The same for the rows kCheck part .., one a thread of a workgroup of kCheck,
-// which compares them with all earlier ones, a tile of them at a time.
-constexpr int kCheck = 256;
-__device__ __forceinline__ int claim_slot(const Delta &p, int part) {
-  constexpr int TILE = 8 * kCheck;
-  __shared__ __align__(16) int32_t tile[TILE];
+// which compares them with all earlier ones, a tile (of kTile, in LDS) of them at
+// a time.
+constexpr int kCheck = 256, kTile = 8 * kCheck;
+__device__ __forceinline__ int claim_slot(const Delta &p, int part, int32_t *tile) {
   const int first = part * kCheck, j = first + (int)threadIdx.x;
   const int slot = j >= p.rows ? -1 : p.slots ? p.slots[j] : j;
   bool taken = slot >= p.nslots;
-  for (int base = 0; p.slots && base < first + kCheck; base += TILE) {
-    int32_t x[TILE / kCheck];
+  for (int base = 0; p.slots && base < first + kCheck; base += kTile) {
+    int32_t x[kTile / kCheck];
 #pragma unroll
-    for (int i = 0; i < TILE / kCheck; ++i) {
+    for (int i = 0; i < kTile / kCheck; ++i) {
       const int at = base + i * kCheck + (int)threadIdx.x;
       x[i] = at < p.rows ? p.slots[at] : -1;
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < TILE / kCheck; ++i) tile[i * kCheck + threadIdx.x] = x[i];
+    for (int i = 0; i < kTile / kCheck; ++i) tile[i * kCheck + threadIdx.x] = x[i];
     __syncthreads();
-    const int whole = min(first - base, TILE);      // of them, all earlier than this part's
+    const int whole = min(first - base, kTile);      // of them, all earlier than this part's
 #pragma unroll 16
     for (int k = 0; k < whole; k += 4) {
       const int4 t = *(const int4 *)(tile + k);
       taken |= (t.x == slot) | (t.y == slot) | (t.z == slot) | (t.w == slot);
     }
-    if (whole < TILE)
+    if (whole < kTile)
 #pragma unroll 16
       for (int k = 0; k < kCheck; k += 4) {
         const int4 t = *(const int4 *)(tile + whole + k);
@@ -90,7 +89,8 @@ __device__ __forceinline__ int claim_slot(const Delta &p, int part) {
 constexpr int kManyRows = 16384, kManyUnits = 65536;
 template <typename T>
 __global__ __launch_bounds__(kCheck) void delta_claim_kernel(Delta p) {
-  const int slot = claim_slot(p, blockIdx.x);
+  __shared__ __align__(16) int32_t tile[kTile];
+  const int slot = claim_slot(p, blockIdx.x, tile);
   const int64_t row = (int64_t)blockIdx.x * kCheck + threadIdx.x;
   if (row >= p.rows) return;
   for (int h = 0; h < p.hv; ++h)
@@ -302,11 +302,12 @@ __device__ __forceinline__ int32_t *row_faults(const Delta &p, int64_t chunk_byt
 
 // The verdicts on rows kCheck part .., by a workgroup of kCheck threads: what it
 // finds wrong is reported here.
-__device__ void check_rows(const Delta &p, int part, int32_t *slots, int32_t *faults) {
+__device__ void check_rows(const Delta &p, int part, int32_t *slots, int32_t *faults,
+                           int32_t *tile) {
   const int j = part * kCheck + (int)threadIdx.x;
   const bool on = j < p.rows;
   const int t0 = on ? p.cu[j] : 0, t1 = on ? p.cu[j + 1] : 0;
-  const int slot = claim_slot(p, part);
+  const int slot = claim_slot(p, part, tile);
   if (on) slots[j] = slot;
   const int bad = __syncthreads_or(t0 < 0 || t1 < t0 || t1 > p.tokens);
   if (threadIdx.x == 0) {
@@ -375,8 +376,10 @@ __global__ __launch_bounds__(256, 2) void delta_prep_kernel(Delta p) {
   const int slot = blockIdx.x, hk = blockIdx.y;
   if (slot >= chunks_of(p)) {
     const int64_t bytes = Space<DK, T>::bytes(p);
+    static_assert(sizeof(At) >= kTile * sizeof(int32_t), "no tile of slots");
     if (hk == 0 && blockIdx.z == 0)
-      check_rows(p, slot - (int)chunks_of(p), row_slots(p, bytes), row_faults(p, bytes));
+      check_rows(p, slot - (int)chunks_of(p), row_slots(p, bytes), row_faults(p, bytes),
+                 (int32_t *)At);
     return;
   }
   const int row = row_of(p, slot);
