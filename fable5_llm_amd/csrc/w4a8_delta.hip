@@ -192,7 +192,10 @@ __global__ __launch_bounds__(256) void delta_step_kernel(Delta p) {
 // int16 of two, bfloat16 of one), and of the products of two operands' terms
 // those below 2^-24 are left out.  So a state keeps its 24 bits through a
 // prompt; a norm of q or k is a factor of its row, applied to the sums.
-// A token that holds an infinity or a NaN spoils its whole chunk.
+// (Exactly: from 2^-103 up to where bfloat16 ends, 2^128 - 2^119.)  From a token
+// with an infinity or a NaN in k, v, g or beta on, its head's outputs, for v its
+// column's alone, and the state are NaN; the tokens before it are what they are
+// without it.
 constexpr int C = 64;
 constexpr int kTriBytes = 6 * 3 * 64 * 16;       // M or P: operands of tri_of, three terms
 constexpr int kVecFloats = 256;                  // a, b, c of 64 tokens, e^(G_C) 64 times
@@ -238,6 +241,7 @@ __device__ __forceinline__ f32x4 mfma_terms(const bf16x8 *a, const bf16x8 *b, f3
 }
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
 // x[0 .. M) as a sum of N vectors of bfloat16, a pair of values per conversion
 // (whose result is kept as one word: taken apart, the compiler converts each
@@ -371,6 +375,7 @@ __global__ __launch_bounds__(256, 2) void delta_prep_kernel(Delta p) {
   __shared__ bf16x8 Ks[4][NS][NK][64];             // K by row tiles, as operand
   __shared__ double Gs[HEADS][C];                  // log2(e) times the running sum of g
   __shared__ __align__(16) float betas[HEADS][C], rks[C], rqs[C];
+  __shared__ int firsts[HEADS];
   __shared__ __align__(16) float At[C * LD];       // A transposed
   __shared__ __align__(16) float Tt[4][16 * 20];   // its diagonal blocks' inverses, transposed
   const int slot = blockIdx.x, hk = blockIdx.y;
@@ -429,7 +434,7 @@ __global__ __launch_bounds__(256, 2) void delta_prep_kernel(Delta p) {
     for (int i = 0; i < NK; ++i) Ks[w][s][i][lane] = kw[s][i];
   if (g == 0) {
     const bool on = 16 * w + r < len;
-    rks[16 * w + r] = !on ? 0.f : p.norm ? 1.f / sqrtf(kk2 + p.eps) : 1.f;
+    rks[16 * w + r] = !on ? 0.f : !finite(kk2) ? NAN : p.norm ? 1.f / sqrtf(kk2 + p.eps) : 1.f;
     rqs[16 * w + r] = !on ? 0.f : (p.norm ? 1.f / sqrtf(qq2 + p.eps) : 1.f) * p.scale;
   }
   __syncthreads();
@@ -481,11 +486,15 @@ __global__ __launch_bounds__(256, 2) void delta_prep_kernel(Delta p) {
         const double y = __shfl_up(G, d);
         if (lane >= d) G += y;
       }
+      // from the first token on whose k, g or beta is no number, M is 0 and a NaN
+      const uint64_t odd = __ballot(!finite((float)G) || !finite(bt) || !finite(rks[lane]));
+      const int first = odd ? __builtin_ctzll(odd) : C;
+      if (lane == 0) firsts[w] = first;
       Gs[w][lane] = G;
-      betas[w][lane] = bt;
+      betas[w][lane] = lane < first ? bt : 0.f;
       const double GC = __shfl(G, 63);
       float *vec = (float *)(space.head(h) + 2 * kTriBytes);
-      vec[lane] = on ? exp2_of((float)G) * rks[lane] : 0.f;
+      vec[lane] = !on ? 0.f : lane < first ? exp2_of((float)G) * rks[lane] : NAN;
       vec[64 + lane] = on ? exp2_of((float)G) * rqs[lane] : 0.f;
       vec[128 + lane] = on ? exp2_of((float)(GC - G)) * rks[lane] : 0.f;
       vec[192 + lane] = exp2_of((float)GC);
@@ -497,6 +506,7 @@ __global__ __launch_bounds__(256, 2) void delta_prep_kernel(Delta p) {
         const int t = 16 * w + r;
         const double Gt = Gs[b][t];
         const float rqt = rqs[t], bt = betas[b][t] * rks[t];
+        const int before = min(t, t < firsts[b] ? C : 0);   // of the tokens that A_t has
         f32x4 P[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -507,7 +517,7 @@ __global__ __launch_bounds__(256, 2) void delta_prep_kernel(Delta p) {
             for (int i = 0; i < 4; ++i) {
               const int j = 16 * c + 4 * g + i;
               const float dec = exp2_of((float)(Gt - Gs[b][j])) * rkj[i];
-              At[j * LD + t] = j < t ? bt * dec * kk[c][i] : 0.f;
+              At[j * LD + t] = j < before ? bt * dec * kk[c][i] : 0.f;
               P[c][i] = j <= t ? rqt * dec * kq[c][i] : 0.f;
             }
           }
@@ -577,7 +587,7 @@ __global__ __launch_bounds__(256, 2) void delta_prep_kernel(Delta p) {
 // Outputs are rounded to 16 bits (bfloat16, float16): two terms of their
 // operands, an error of 2^-17, are enough for them.
 template <int DK, typename T>
-__global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
+__global__ __launch_bounds__(512, DK == 64 && sizeof(T) == 2 ? 4 : 1) void delta_scan_kernel(Delta p) {
   constexpr int NK = Terms<T>::n, NS = DK / 32;
   constexpr int OT = out_terms<T>();
   __shared__ bf16x8 Sb[3][NS][64];                // the state, k-step s by wavefront s
@@ -585,6 +595,9 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
   __shared__ __align__(16) T Ts[8][16 * 16];      // a wavefront's tokens' values or outputs
   __shared__ __align__(16) uint8_t Kl[NK][C * DK * 2];   // K by rows, see k_at
   __shared__ __align__(16) float Fs[2][kVecFloats];   // a chunk's factors and the next one's
+  __shared__ int seen;                            // whether a chunk of the row was odd
+  __shared__ __align__(16) int odds[4];           // this one's tokens, by wavefront,
+  __shared__ int firsts[4][16];                   // and each column's first odd one
   const int tiles = p.dv / 16, units = p.rows * p.hv, each = (units + 7) / 8;
   // a head's columns, and heads that share keys, on one XCD (workgroups go
   // round the eight of them)
@@ -637,13 +650,31 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
     return (uint32_t)(min(16 * w + prow, len - 1) * (int)token + col - r) * (uint32_t)sizeof(T) +
            (uint32_t)piece * 16;
   };
+  // A token is odd in a column whose V - a K S0 is no finite number (k, v, g, beta
+  // or the state were not).  0 times it would spoil the tokens before it in the
+  // chunk's products.  So a row in which one was seen is walked again, from its
+  // state, which is written last, and then the column's tokens from the first odd
+  // one on are taken out of the products, and made NaN through Q S0 and the state's
+  // factor.  (Deciding it chunk by chunk took 8192 tokens 258 us, not 244.  And no
+  // branch stands between a product and the first use of its result: the compiler
+  // does not wait for it across one.)
+  auto any_odd = [&](int4 o) {
+    return __builtin_amdgcn_readfirstlane(o.x | o.y | o.z | o.w) != 0;
+  };
+  auto first_odd = [&]() {
+    int first = C;
+    for (int i = 0; i < 4; ++i)
+      if (odds[i]) first = min(first, firsts[i][r]);
+    return first;
+  };
   auto exchange = [&]() {                         // a wavefront's writes before its reads
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
   };
 
-  auto chain = [&](auto upper) {
+  auto chain = [&](auto upper, auto again) {
+    constexpr bool AGAIN = again.value;
     constexpr bool HI = upper.value;              // w >= 2: two k-steps of M
     constexpr bool STATE = NS == 4 || !HI;        // rows of the state
     float *state = p.state + (((int64_t)slot * p.hv + h) * DK + 32 * w + 8 * g) * p.dv + col;
@@ -722,6 +753,36 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
       __builtin_memcpy(&x, t, sizeof(x));
       return x;
     };
+    // U and W once more without the odd tokens; the first one of the column
+    auto without_odd = [&](int ch, In &x) {
+      auto take_out = [&](bf16x4 (*b)[2][64][2], auto terms, int first) {
+        for (int i = 0; i < terms.value; ++i)
+          for (int e = 0; e < 4; ++e)
+            if (16 * w + 4 * g + e >= first) b[i][w >> 1][lane][w & 1][e] = (__bf16)0.f;
+      };
+      const int first = first_odd();
+      take_out(Rb, Int<3>(), first);
+      lds_barrier();
+      const uint8_t *const after = ws;
+      ws = ws0 + (int64_t)ch * kHeadBytes;
+      load_solve(x);
+      bf16x8 b[2][3];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        b[0][i] = *(const bf16x8 *)Rb[i][0][lane];
+        if constexpr (HI) b[1][i] = *(const bf16x8 *)Rb[i][1][lane];
+      }
+      f32x4 u = mfma_terms<3, 3, 2>(x.m[0], b[0], f32x4{0, 0, 0, 0});
+      if constexpr (HI) u = mfma_terms<3, 3, 2>(x.m[1], b[1], u);
+      put_rows(Wb, u * factor(ch, 2), Int<3>());
+      put_rows(Ub, u, Int<OT>());
+      take_out(Wb, Int<3>(), first);
+      take_out(Ub, Int<OT>(), first);
+      lds_barrier();
+      ws = after;
+      load_solve(x);
+      return first;
+    };
     // Loads go out behind a segment's reads of LDS, in the time those take.
     auto step = [&](int ch, In &x) {
       const int len = min(C, end - begin - ch * C);
@@ -777,6 +838,8 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
         put_rows(Ub, u, Int<OT>());
       }
       lds_barrier();
+      int4 o4{0, 0, 0, 0};
+      if constexpr (AGAIN) o4 = *(const int4 *)odds;
       if constexpr (STATE) {
         bf16x8 b[2][3];
 #pragma unroll
@@ -784,10 +847,19 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
           b[0][i] = *(const bf16x8 *)Wb[i][0][lane];
           b[1][i] = *(const bf16x8 *)Wb[i][1][lane];
         }
-        const float fall = Fs[ch & 1][192];
+        float fall = Fs[ch & 1][192];
         __builtin_amdgcn_sched_barrier(0);
         load_solve(x);
         __builtin_amdgcn_sched_barrier(0);
+        if constexpr (AGAIN)
+          if (any_odd(o4)) {
+            if (without_odd(ch, x) < C) fall = NAN;
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+              b[0][i] = *(const bf16x8 *)Wb[i][0][lane];
+              b[1][i] = *(const bf16x8 *)Wb[i][1][lane];
+            }
+          }
         S[0] *= fall;
         S[1] *= fall;
 #pragma unroll
@@ -798,6 +870,8 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
         put_state();
       } else {
         load_solve(x);
+        if constexpr (AGAIN)
+          if (any_odd(o4)) without_odd(ch, x);
       }
       lds_barrier();
     };
@@ -812,14 +886,17 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
     load_solve(in);
     lds_barrier();
     for (int ch = 0; ch < n; ++ch) step(ch, in);
+    if constexpr (!AGAIN) lds_barrier();            // the last outputs were looked at
     if constexpr (STATE)
+      if (AGAIN || !seen)
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) state[(int64_t)(4 * e + i) * p.dv] = S[e][i];
+          for (int i = 0; i < 4; ++i) state[(int64_t)(4 * e + i) * p.dv] = S[e][i];
   };
 
-  auto output = [&](auto upper) {
+  auto output = [&](auto upper, auto again) {
+    constexpr bool AGAIN = again.value, LATE = NS * NK <= 4;
     constexpr bool HI = upper.value;
     const uint8_t *qb = (const uint8_t *)space.rows(hk, 1);
     uint8_t *ob = (uint8_t *)((T *)p.out + begin * p.out_token + h * p.out_head);
@@ -829,7 +906,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
     f32x4 o{0, 0, 0, 0}, factors;
     const uint8_t *const qb0 = qb, *const ws0 = ws;
     // a chunk's rows of Q and their factors; its rows of P
-    auto load_rows = [&](int ch) {
+    auto load_rows = [&](int ch, bf16x8 (*q)[NK]) {
       qb = qb0 + ch * space.kRows;
       ws = ws0 + (int64_t)ch * kHeadBytes;
 #pragma unroll
@@ -861,38 +938,88 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
       const u32x4 x = *(const u32x4 *)(tile + prow * 16 + piece * (16 / (int)sizeof(T)));
       if (lane < 16 * PIECES && 16 * w + prow < len) store16_nt(ob + o_at, x);
       ob += o_step;
+      if constexpr (!AGAIN)                         // an odd token's outputs are
+        if (__any(!finite(o[0]) || !finite(o[1]) || !finite(o[2]) || !finite(o[3])) && lane == 0)
+          seen = 1;
+    };
+    // whether V - a K S0 of this wavefront's tokens, by its first terms, is odd
+    auto look_for_odd = [&]() {
+      bool odd[4], any = false;
+      uint32_t z[2];
+      __builtin_memcpy(z, &Rb[0][w >> 1][lane][w & 1], sizeof(z));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        odd[e] = (z[e >> 1] >> (16 * (e & 1)) & 0x7F80) == 0x7F80;
+        any |= odd[e];
+      }
+      any = __any(any);
+      if (any) {
+        int first = C;
+#pragma unroll
+        for (int e = 3; e >= 0; --e) first = odd[e] ? 16 * w + 4 * g + e : first;
+        first = min(first, __shfl_xor(first, 16));
+        first = min(first, __shfl_xor(first, 32));
+        if (g == 0) firsts[w][r] = first;
+      }
+      if (lane == 0) odds[w] = any;
     };
     load_factors(0);
-    load_rows(0);
+    load_rows(0, q);
     load_weights(0);
     put_factors(0);
     lds_barrier();
     for (int ch = 0; ch < n; ++ch) {
       // beside the chain's first segment the last chunk's outputs are written,
       // beside its second Q S0 is made, beside its third P U: no segment has
-      // more than its share of the loads and stores
+      // more than its share of the loads and stores.  Q of one term leaves the
+      // registers for the next chunk's beside it: Q S0 is read beside the second
+      // segment and made beside the third (8192 bfloat16 tokens 258 -> 244 us).
       if (ch) write(ch - 1);
       load_factors(min(ch + 1, n - 1));
       lds_barrier();
-      {
-        bf16x8 sb[NS][OT];
+      bf16x8 sb[NS][OT], qn[NS][NK];
 #pragma unroll
-        for (int s = 0; s < NS; ++s)
+      for (int s = 0; s < NS; ++s)
 #pragma unroll
-          for (int i = 0; i < OT; ++i) sb[s][i] = Sb[i][s][lane];
+        for (int i = 0; i < OT; ++i) sb[s][i] = Sb[i][s][lane];
+      const f32x4 b = factor(ch, 1);
+      if constexpr (AGAIN) look_for_odd();
+      auto q_state = [&]() {
         o = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < NS; ++s) o = mfma_terms<NK, OT, OT - 1>(q[s], sb[s], o);
-        o *= factor(ch, 1);
+        o *= b;
+      };
+      if constexpr (LATE) {
+        load_rows(min(ch + 1, n - 1), qn);
+        lds_barrier();
+        q_state();
+        __builtin_memcpy(q, qn, sizeof(q));
+      } else {
+        q_state();
+        load_rows(min(ch + 1, n - 1), q);
+        lds_barrier();
       }
-      load_rows(min(ch + 1, n - 1));
-      lds_barrier();
       bf16x8 ub[2][OT];
+      auto get_u = [&]() {
 #pragma unroll
-      for (int i = 0; i < OT; ++i) {
-        ub[0][i] = *(const bf16x8 *)Ub[i][0][lane];
-        if constexpr (HI) ub[1][i] = *(const bf16x8 *)Ub[i][1][lane];
-      }
+        for (int i = 0; i < OT; ++i) {
+          ub[0][i] = *(const bf16x8 *)Ub[i][0][lane];
+          if constexpr (HI) ub[1][i] = *(const bf16x8 *)Ub[i][1][lane];
+        }
+      };
+      int4 o4{0, 0, 0, 0};
+      if constexpr (AGAIN) o4 = *(const int4 *)odds;
+      get_u();
+      if constexpr (AGAIN)
+        if (any_odd(o4)) {
+          const int first = first_odd();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = 16 * w + 4 * g + i < first ? o[i] : NAN;
+          lds_barrier();                            // the chain's, in without_odd
+          lds_barrier();
+          get_u();
+        }
       o = mfma_terms<OT, OT, OT - 1>(m[0], ub[0], o);
       if constexpr (HI) o = mfma_terms<OT, OT, OT - 1>(m[1], ub[1], o);
       load_weights(min(ch + 1, n - 1));
@@ -900,15 +1027,22 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(Delta p) {
       lds_barrier();
     }
     write(n - 1);
+    if constexpr (!AGAIN) lds_barrier();
   };
   // the same number of barriers on every way
-  if (wave < 4) {
-    if (w < 2) chain(Int<0>());
-    else chain(Int<1>());
-  } else {
-    if (w < 2) output(Int<0>());
-    else output(Int<1>());
-  }
+  auto walk = [&](auto again) {
+    ws = space.head(h);
+    if (wave < 4) {
+      if (w < 2) chain(Int<0>(), again);
+      else chain(Int<1>(), again);
+    } else {
+      if (w < 2) output(Int<0>(), again);
+      else output(Int<1>(), again);
+    }
+  };
+  if (threadIdx.x == 0) seen = 0;                 // chain and outputs meet before it is used
+  walk(Int<0>());
+  if (seen) walk(Int<1>());
 }
 
 template <int DK, typename T>

@@ -530,9 +530,11 @@ typedef struct {
 } w4a8_delta;
 /* one token of each row */
 int w4a8_delta_step_async(w4a8_ctx *ctx, const w4a8_delta *d);
-/* whole prompts, in chunks of 64 tokens (an infinity or a NaN among a token's
-   inputs can reach every output of its chunk).  Token strides of v and out: at
-   most 2^23.  Bounds that do not lie in order within the tokens: nothing is
+/* whole prompts, in chunks of 64 tokens.  From a token on whose k, v, beta or g
+   (-infinity but: a decay to 0) holds an infinity or a NaN, its heads' outputs
+   and states are NaN (from v: that column's; from q: that token's outputs are no
+   numbers); all others are what they are without it.  Token strides of v and
+   out: at most 2^23.  Bounds that do not lie in order within the tokens: nothing is
    run, and the next sync reports it. */
 int w4a8_delta_chunk_workspace(w4a8_ctx *ctx, int64_t tokens, int64_t rows,
                                int64_t hk, int64_t hv, int64_t dk, int32_t dtype,
