@@ -262,6 +262,9 @@ _DELTA = struct.Struct("=10Q23q2d")
 
 def _delta_fault(ctx, q, k, v, g, beta, state, out):
     """What is wrong with the tensors of a delta-rule call, as a ValueError."""
+    for t, name in ((q, "q"), (k, "k"), (v, "v"), (g, "g"), (beta, "beta"), (state, "state"),
+                    (out, "out")):
+        _on(t, ctx, name)
     if q.dim() != 3 or v.dim() != 3 or state.dim() != 4:
         raise ValueError("q, k [tokens, hk, dk], v, out [tokens, hv, dv] and "
                          "state [slots, hv, dk, dv] are required")
@@ -275,7 +278,6 @@ def _delta_fault(ctx, q, k, v, g, beta, state, out):
     _act(out, ctx, "out", (tokens, hv, dv), q.dtype)
     _gate(g, ctx, "g", (tokens, hv))
     _gate(beta, ctx, "beta", (tokens, hv))
-    _on(state, ctx, "state")
     raise ValueError(f"state: must be contiguous float32 [slots, {hv}, {dk}, {dv}]")
 
 
@@ -284,9 +286,10 @@ def delta_args(ctx, q, k, v, g, beta, state, out, cu, ws, slots, scale, norm, ep
     """The checked arguments of one delta-rule call, packed as w4a8_delta.
     The checks of the tensors are one condition (a step is a few microseconds
     on the device); what does not hold is told by _delta_fault."""
-    dts, dev, qt = _dtypes(), ctx.device, q.dtype
-    dt = dts.get(qt)
+    dts, dev = _dtypes(), ctx.device
     try:
+        qt = q.dtype
+        dt = dts.get(qt)
         tokens, hk, dk = qs = q.shape
         _, hv, dv = vs = v.shape
         q0, q1, q2 = q.stride()
