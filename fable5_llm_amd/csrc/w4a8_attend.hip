@@ -480,7 +480,7 @@ attend_kernel(KvCache kv, Attend a) {
 // 2^(m_s - M) l_s.  A workgroup per row and head, D / 4 threads per split; what
 // it waits for is a chain of small loads, so the first two splits of a thread
 // are on their way before it knows how many there are.  One row of 16 heads of
-// 256 and 4 splits 1.7-2.9 us, two rows of 128 splits 5.5.
+// 256 and 4 splits 1.9-2.7 us, two rows of 64 splits 5.5.
 constexpr int kJoin = 256;
 template <int D>
 __global__ __launch_bounds__(kJoin) void attend_join_kernel(KvCache kv, Attend a) {
@@ -550,7 +550,7 @@ void launch_dim(const KvCache &kv, const Attend &a, uint32_t grid, hipStream_t s
 }  // namespace
 
 // Splits of a row: workgroups for the chip twice over at least, and no more than
-// 512 tokens of the cache's longest sequence in one (a longer one is what a
+// 512 tokens of the most that a table holds (the host knows no row's length) in one (a longer one is what a
 // ragged batch waits for), but no more than 16 for that (each is a part to
 // join), and none of less than a chunk.  Measured: 48 ragged rows to 4099, 8
 // key-value heads of 128, in 9 splits 37.5 us, in 3 51; 8 rows of 3450 in 8

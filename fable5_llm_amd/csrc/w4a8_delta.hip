@@ -102,7 +102,7 @@ __global__ __launch_bounds__(kCheck) void delta_claim_kernel(Delta p) {
 // registers, lane (rg, cq) = (lane >> 2, lane & 3) its rows NR rg .. and
 // columns 4 cq .., so that a state is read and written once, in 64-byte runs.
 // Bound by that: 125 rows of 32 heads of 128 x 128, 527 MB in 106 us, 4.97 TB/s,
-// what a large copy reaches; one row, 4.2 MB, 5.4 us of which 2 are a launch's.
+// what a large copy reaches; one row, 4.2 MB, 4.9 us of which 2 are a launch's.
 template <int DK, typename T>
 __global__ __launch_bounds__(256) void delta_step_kernel(Delta p) {
   constexpr int NR = DK / 16;
@@ -366,7 +366,7 @@ struct Space {
 // neighbouring slots of their operand: nothing is rearranged.
 //
 // Bound by memory: 8192 bfloat16 tokens, 16 key and 32 value heads of 128, 67 MB
-// read and 195 MB written in 66-69 us (3.9 TB/s).  M and P, which no cache holds
+// read and 195 MB written in 64-69 us (3.9 TB/s).  M and P, which no cache holds
 // until they are read, are written past them: prep and scan 268 -> 244 us; K and
 // Q too, 257.
 template <int DK, typename T>
@@ -577,7 +577,7 @@ __global__ __launch_bounds__(256, 2) void delta_prep_kernel(Delta p) {
 // for itself).  So operands are loaded as soon as an earlier chunk has used
 // their registers, the factors once per workgroup, and K transposed for the
 // update comes out of LDS by transposed reads instead of from memory again.
-// 8192 bfloat16 tokens of 32 heads of 128 x 128: 188-200 us, 1.5 us a chunk; of
+// 8192 bfloat16 tokens of 32 heads of 128 x 128: 192-203 us, 1.5 us a chunk; of
 // 8 heads, a quarter of the chip, 1.1 us a chunk.
 //
 // Wavefront w of the chain has rows 32 w .. of the state too: lane (r, g) rows
@@ -655,9 +655,9 @@ __global__ __launch_bounds__(512, DK == 64 && sizeof(T) == 2 ? 4 : 1) void delta
   // chunk's products.  So a row in which one was seen is walked again, from its
   // state, which is written last, and then the column's tokens from the first odd
   // one on are taken out of the products, and made NaN through Q S0 and the state's
-  // factor.  (Deciding it chunk by chunk took 8192 tokens 258 us, not 244.  And no
-  // branch stands between a product and the first use of its result: the compiler
-  // does not wait for it across one.)
+  // factor.  (Decided in the chain of every chunk, six ragged prompts took 38.4 us,
+  // not 37.3.  And no branch stands between a product and the first use of its
+  // result: the compiler does not always wait for it across one.)
   auto any_odd = [&](int4 o) {
     return __builtin_amdgcn_readfirstlane(o.x | o.y | o.z | o.w) != 0;
   };
@@ -973,7 +973,7 @@ __global__ __launch_bounds__(512, DK == 64 && sizeof(T) == 2 ? 4 : 1) void delta
       // beside its second Q S0 is made, beside its third P U: no segment has
       // more than its share of the loads and stores.  Q of one term leaves the
       // registers for the next chunk's beside it: Q S0 is read beside the second
-      // segment and made beside the third (8192 bfloat16 tokens 258 -> 244 us).
+      // segment and made beside the third (8192 bfloat16 tokens 258 -> 245 us).
       if (ch) write(ch - 1);
       load_factors(min(ch + 1, n - 1));
       lds_barrier();

@@ -211,7 +211,7 @@ __global__ __launch_bounds__(kOne) void kv_extend_kernel(KvCache kv, const int32
 }
 
 // --------------------------------------------------------------------- fork
-// First kernel, one workgroup (32 children and under 1,000 pages: 7.1 us, a chain
+// First kernel, one workgroup (32 children and under 1,000 pages: 6.8 us, a chain
 // of loads, marks and scans): the list's faults, a free page for each child
 // of a parent whose last page is not full (jobs[child], -1 where none), the
 // children's lengths.  scratch[0]: whether the second kernel runs.
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(kOne) void kv_fork_kernel(KvCache kv, const int32_t
 
 // Second kernel, a row of workgroups per pair: the shared pages' entries and
 // counts, and the used tokens of the last page, one run of memory per layer,
-// keys or values, and head (32 children, 8 layers of 4 heads of 256: 4.7 us).
+// keys or values, and head (32 children, 8 layers of 4 heads of 256: 4.6 us).
 __global__ __launch_bounds__(256) void kv_fork_rows_kernel(KvCache kv, const int32_t *parents,
                                                            const int32_t *children) {
   if (kv.scratch[0] == 0) return;
@@ -322,7 +322,7 @@ __global__ __launch_bounds__(256) void kv_fork_rows_kernel(KvCache kv, const int
 
 // --------------------------------------------------------------------- free
 // A workgroup per listed sequence, which takes its length: of the workgroups of
-// one listed again, and of an empty one, there is nothing left to free.  3.1 us
+// one listed again, and of an empty one, there is nothing left to free.  2.8 us
 // for 32 sequences of up to 1,500 tokens; 2^20 entries take 2^20 workgroups'
 // time (each looking through those before it would be 2^39 comparisons).
 __global__ __launch_bounds__(256) void kv_free_kernel(KvCache kv, const int32_t *seqs) {
@@ -354,7 +354,7 @@ __global__ __launch_bounds__(256) void kv_free_kernel(KvCache kv, const int32_t 
 // or above moves to the k-th free page below U (there are as many of either).
 // list_a: the free pages that are filled.  list_b[page]: where a page at U or
 // above goes; which page comes to a filled one; -1 for the others.  The counts
-// move too.  scratch[0] = moves, scratch[1] = U.  8.7 us for 2,048 pages.
+// move too.  scratch[0] = moves, scratch[1] = U.  8.3 us for 2,048 pages.
 __global__ __launch_bounds__(kOne) void kv_compact_kernel(KvCache kv) {
   int32_t *holes = list_a(kv), *to = list_b(kv);
   FirstRefs refs = first_refs(kv, 0);

@@ -489,7 +489,9 @@ int w4a8_kv_attend_workspace(const w4a8_kv *kv, int32_t rows, int32_t q_heads,
    of a key-value head side by side (q_heads a multiple of kv_heads).
      out = softmax(scale q K^T) V; a row without tokens gets zeros
    dtype: the cache's, or I16 (q with frac, out with out_frac fraction bits);
-   q and out share it.  d_ws: 16-byte aligned. */
+   q and out share it.  d_ws: 16-byte aligned.  rows * q_heads * a row's parts
+   (16 where rows are many and tables long, fewer for tables of under 8,192
+   tokens) are at most 2^23 in one call. */
 int w4a8_kv_attend_async(w4a8_kv *kv, int32_t layer, int32_t dtype, int32_t frac,
                          int32_t out_frac, const void *d_q, int64_t q_row,
                          int64_t q_head, void *d_out, int64_t out_row,
