@@ -107,10 +107,10 @@ __device__ __forceinline__ void store_out(const Attend &a, int cache_dtype, int6
 
 // I16: q is int16 (its value of a step is part of a.scale), exact as the sum
 // of two 8-bit values of the cache's type, both of q's sign and neither zero
-// unless q is: times an infinite key they are that infinity, not a NaN.  Over a 16-bit cache P goes into the
-// second product as the sum of two values of that type, off by half a step
-// squared (bfloat16 2^-16, float16 2^-22) of a weight, so that the output's own
-// rounding is the only one that counts.
+// unless q is: times an infinite key they are that infinity, not a NaN.  Over a
+// 16-bit cache P goes into the second product as the sum of two values of that
+// type, off by half a step squared (bfloat16 2^-16, float16 2^-22) of a weight,
+// so that the output's own rounding is the only one that counts.
 // Workgroups: key-value heads fastest, then a row's splits, then rows.  Two a CU
 // at least, but for heads of 256 of float32 (whose registers are far over that)
 // and of int16 rows, which two a CU make no faster.  A head of 256 of 16-bit
@@ -550,11 +550,11 @@ void launch_dim(const KvCache &kv, const Attend &a, uint32_t grid, hipStream_t s
 }  // namespace
 
 // Splits of a row: workgroups for the chip twice over at least, and no more than
-// 512 tokens of the most that a table holds (the host knows no row's length) in one (a longer one is what a
-// ragged batch waits for), but no more than 16 for that (each is a part to
-// join), and none of less than a chunk.  Measured: 48 ragged rows to 4099, 8
-// key-value heads of 128, in 9 splits 37.5 us, in 3 51; 8 rows of 3450 in 8
-// 25.8, in 16 29.5; 24 rows of 9216 in 16 151, in 3 168.
+// 512 tokens of the most that a table holds in one (the host knows no row's
+// length; a longer split is what a ragged batch waits for), but no more than 16
+// for that (each is a part to join), and none of less than a chunk.  Measured: 48
+// ragged rows to 4099, 8 key-value heads of 128, in 9 splits 37.5 us, in 3 51; 8
+// rows of 3450 in 8 25.8, in 16 29.5; 24 rows of 9216 in 16 151, in 3 168.
 int attend_splits(const KvCache &kv, int64_t rows, int64_t hq, int num_cu) {
   const int64_t group = hq / kv.heads, base = rows * kv.heads * ((group + 15) / 16);
   const int64_t most = (((int64_t)kv.max_pages << kv.lg_page) + kAttendChunk - 1) / kAttendChunk;
