@@ -443,7 +443,9 @@ class Context:
         """Whole prompts through the gated delta rule: the arguments of
         delta_step_async with tokens of several rows side by side, row i's
         from cu[i] to cu[i + 1] (int32 [rows + 1], on the device).  fresh: the
-        states start from zeros and are not read."""
+        states start from zeros and are not read.  From a token with an infinity
+        or a NaN in k, v, beta or g (but -infinity) on, its heads' outputs and
+        states are NaN; no earlier token's are touched."""
         N.check(N.lib().w4a8_delta_chunk_async(self.h, mixers.delta_args(
             self, q, k, v, g, beta, state, out, cu, ws, slots, scale, norm, eps, fresh, frac,
             out_frac)), "delta_chunk")
