@@ -293,8 +293,8 @@ __device__ __forceinline__ int first_chunk(const Delta &p, int row) {
   return p.cu[row] / C + row;
 }
 
-// Chunks that the workspace has room for, and where behind them the rows'
-// verdicts lie: each row's slot (-1: none), then for every kCheck rows whether
+// Chunks that the workspace has room for, and where behind them the
+// findings on the rows lie: each row's slot (-1: none), then for every kCheck rows whether
 // the bounds of one of them are out of order.
 __device__ __forceinline__ int64_t chunks_of(const Delta &p) { return p.tokens / C + p.rows; }
 __device__ __forceinline__ int32_t *row_slots(const Delta &p, int64_t chunk_bytes) {
@@ -304,7 +304,7 @@ __device__ __forceinline__ int32_t *row_faults(const Delta &p, int64_t chunk_byt
   return row_slots(p, chunk_bytes) + p.rows;
 }
 
-// The verdicts on rows kCheck part .., by a workgroup of kCheck threads: what it
+// The findings on rows kCheck part .., by a workgroup of kCheck threads: what it
 // finds wrong is reported here.
 __device__ void check_rows(const Delta &p, int part, int32_t *slots, int32_t *faults,
                            int32_t *tile) {
@@ -360,7 +360,7 @@ struct Space {
 };
 
 // A workgroup per chunk, key head and share of its value heads, and behind the
-// chunks' one per kCheck rows for the verdicts on them.  It lays K and
+// chunks' one per kCheck rows for the findings on them.  It lays K and
 // Q out as the operands that delta_scan_kernel reads, in whole lines (read where
 // they lie, rows of a prompt 4 KB apart all fall to one channel of the L2: the
 // scan of 8192 tokens, 16 key heads of 128, took 34 us more).  Tiles of M and P
@@ -1087,9 +1087,9 @@ int64_t delta_workspace(int64_t tokens, int64_t rows, int64_t hk, int64_t hv, in
                         int dtype) {
   const int terms = dtype == DT_F32 ? Terms<float>::n
                     : dtype == DT_BF16 ? Terms<__bf16>::n : Terms<_Float16>::n;
-  const int64_t verdicts = 4 * (rows + (rows + kCheck - 1) / kCheck);
+  const int64_t findings = 4 * (rows + (rows + kCheck - 1) / kCheck);
   return (tokens / C + rows) * (hv * kHeadBytes + hk * rows_bytes(dk, terms)) +
-         (verdicts + 15) / 16 * 16;
+         (findings + 15) / 16 * 16;
 }
 
 hipError_t launch_delta(Delta d, int num_cu, hipStream_t s) {
