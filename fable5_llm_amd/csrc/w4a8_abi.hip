@@ -2271,6 +2271,98 @@ int w4a8_kv_attend_async(w4a8_kv *kv, int32_t layer, int32_t dtype, int32_t frac
   return W4A8_OK;
 }
 
+namespace {
+// What a step's plan is made for; *shape is set where it can be made.
+int check_step(const w4a8_kv *kv, int32_t rows, int32_t tokens, int32_t q_heads,
+               ChunkShape *shape) {
+  if (!kv) return fail(W4A8_E_ARG, "null cache");
+  if (rows < 0 || rows > kMostRows || tokens < 0 || tokens > kMostRows)
+    return fail(W4A8_E_ARG, "a step has at most 2^20 rows and 2^20 tokens");
+  if (q_heads < 1 || q_heads > 65535 || q_heads % kv->c.heads)
+    return fail(W4A8_E_ARG, "q_heads must be a multiple of the cache's kv_heads");
+  *shape = chunk_shape(kv->c, rows, tokens, q_heads, kv->ctx->num_cu);
+  // a launch has fewer than 2^32 threads
+  if (shape->units * kv->c.heads * shape->tiles > (1 << 22))
+    return fail(W4A8_E_ARG, "a step of too many rows, tokens and heads for one call");
+  return W4A8_OK;
+}
+
+int check_plan(const ChunkShape &shape, int32_t rows, const void *d_plan, int64_t plan_bytes) {
+  const int64_t need = 4 * plan_words(shape, rows);
+  if (!d_plan || !aligned16(d_plan) || plan_bytes < need)
+    return fail(W4A8_E_ARG, "a step's plan: " + std::to_string(plan_bytes) +
+                                " bytes, the call needs " + std::to_string(need) +
+                                ", 16-byte aligned");
+  return W4A8_OK;
+}
+}  // namespace
+
+int w4a8_kv_plan_bytes(const w4a8_kv *kv, int32_t rows, int32_t tokens, int32_t q_heads,
+                       int64_t *bytes) {
+  if (!bytes) return fail(W4A8_E_ARG, "null argument");
+  ChunkShape shape;
+  if (int rc = check_step(kv, rows, tokens, q_heads, &shape)) return rc;
+  *bytes = 4 * plan_words(shape, rows);
+  return W4A8_OK;
+}
+
+int w4a8_kv_map_async(w4a8_kv *kv, const int32_t *d_seqs, const int32_t *d_counts, int32_t rows,
+                      int32_t tokens, int32_t q_heads, int32_t *d_cu, int32_t *d_token_seqs,
+                      int32_t *d_pos, int64_t *d_slots, void *d_plan, int64_t plan_bytes) {
+  KvMap m{};
+  if (int rc = check_step(kv, rows, tokens, q_heads, &m.shape)) return rc;
+  if (!d_cu || (rows > 0 && (!d_seqs || !d_counts)) ||
+      (tokens > 0 && (!d_token_seqs || !d_pos || !d_slots)))
+    return fail(W4A8_E_ARG, "null argument");
+  if ((((uintptr_t)d_seqs | (uintptr_t)d_counts | (uintptr_t)d_cu | (uintptr_t)d_token_seqs |
+        (uintptr_t)d_pos) & 3) || ((uintptr_t)d_slots & 7))
+    return fail(W4A8_E_ARG, "lists must be 4-byte, slots 8-byte aligned");
+  if (int rc = check_plan(m.shape, rows, d_plan, plan_bytes)) return rc;
+  m.seqs = d_seqs, m.counts = d_counts, m.cu = d_cu, m.token_seqs = d_token_seqs;
+  m.pos = d_pos, m.slots = d_slots, m.plan = (int32_t *)d_plan;
+  m.rows = rows, m.tokens = tokens;
+  DeviceGuard g(kv->ctx->device);
+  HIP_TRY(launch_kv_map(kv->c, m, kv->ctx->stream));
+  return W4A8_OK;
+}
+
+int w4a8_kv_attend_chunk_workspace(const w4a8_kv *kv, int32_t rows, int32_t tokens,
+                                   int32_t q_heads, int64_t *bytes) {
+  if (!bytes) return fail(W4A8_E_ARG, "null argument");
+  ChunkShape shape;
+  if (int rc = check_step(kv, rows, tokens, q_heads, &shape)) return rc;
+  *bytes = chunk_workspace(kv->c, shape);
+  return W4A8_OK;
+}
+
+int w4a8_kv_attend_chunk_async(w4a8_kv *kv, int32_t layer, const void *d_q, int64_t q_token,
+                               int64_t q_head, int32_t out_dtype, int32_t out_frac, void *d_out,
+                               int64_t out_token, int64_t out_head, const void *d_plan,
+                               int64_t plan_bytes, int32_t rows, int32_t tokens, int32_t q_heads,
+                               double scale, void *d_ws, int64_t ws_bytes) {
+  Chunk a{};
+  if (int rc = check_step(kv, rows, tokens, q_heads, &a.shape)) return rc;
+  if (layer < 0 || layer >= kv->c.layers) return fail(W4A8_E_ARG, "no such layer");
+  if (int rc = check_act(kv->c.dtype, out_dtype, out_frac)) return rc;
+  if (int rc = check_plan(a.shape, rows, d_plan, plan_bytes)) return rc;
+  if (tokens == 0 || rows == 0) return W4A8_OK;
+  if (!rows_ok(d_q, kv->c.dtype, q_token, q_head) || !rows_ok(d_out, out_dtype, out_token, out_head))
+    return fail(W4A8_E_ARG, "q and out must be 16-byte aligned, their strides whole 16 bytes");
+  const int64_t need = chunk_workspace(kv->c, a.shape);
+  if (need > 0 && (!d_ws || !aligned16(d_ws) || ws_bytes < need))
+    return fail(W4A8_E_ARG, "attention: the workspace holds " + std::to_string(ws_bytes) +
+                                " bytes, the call needs " + std::to_string(need));
+  a.q = d_q, a.out = d_out;
+  a.q_token = q_token, a.q_head = q_head, a.out_token = out_token, a.out_head = out_head;
+  a.plan = (const int32_t *)d_plan, a.part = (float *)d_ws;
+  a.tokens = tokens, a.hq = q_heads, a.layer = layer, a.dtype = out_dtype;
+  a.scale = (float)(scale * 1.4426950408889634);
+  a.out_unit = 1.f / unit_of(out_dtype, out_frac);
+  DeviceGuard g(kv->ctx->device);
+  HIP_TRY(launch_chunk(kv->c, a, kv->ctx->stream));
+  return W4A8_OK;
+}
+
 int w4a8_delta_step_async(w4a8_ctx *c, const w4a8_delta *d) { return delta_launch(c, d, false); }
 
 int w4a8_delta_chunk_workspace(w4a8_ctx *c, int64_t tokens, int64_t rows, int64_t hk, int64_t hv,

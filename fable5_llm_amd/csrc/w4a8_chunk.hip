@@ -1,0 +1,931 @@
+// Attention of several new tokens of each sequence over a paged key-value
+// cache, and where a step's tokens lie.
+//
+//   o_h = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale q_h . k_t - m),
+//
+// over the tokens t up to the query's own, in one pass with a running maximum
+// m and sum.
+#include "w4a8_mfma_ops.h"
+
+namespace w4a8 {
+
+namespace {
+
+// ---------------------------------------------------------------------- maps
+constexpr int kOne = 1024;        // threads of the single-workgroup kernel
+
+// exclusive scan of one value per thread of a kOne-thread workgroup, and the
+// total; every thread of it calls
+__device__ int scan_excl(int v, int *total) {
+  __shared__ int sums[kOne / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int x = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  __syncthreads();              // the last call's sums are read
+  if (lane == 63) sums[wave] = x;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kOne / 64; ++w) {
+    const int s = sums[w];
+    before += w < wave ? s : 0;
+    all += s;
+  }
+  *total = all;
+  return before + x - v;
+}
+
+// the sum of one value per thread, at most `most` (a bound under 2^31 / kOne
+// of each value and of the sum)
+__device__ int64_t sum_all(int64_t v) {
+  __shared__ int64_t sums[kOne / 64];
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = v;
+  __syncthreads();
+  int64_t all = 0;
+#pragma unroll
+  for (int w = 0; w < kOne / 64; ++w) all += sums[w];
+  return all;
+}
+
+struct MapRow {
+  int seq, count, len;   // seq -1: padding
+  int bad;
+};
+__device__ __forceinline__ MapRow map_row(const KvCache &kv, const KvMap &m, int row) {
+  MapRow r{m.seqs[row], m.counts[row], 0, 0};
+  if (r.count < 0) r.count = 0, r.bad = 1;
+  if (r.seq >= kv.seqs) r.seq = -1, r.bad = 1;
+  if (r.seq < 0) r.seq = -1;
+  if (r.seq >= 0) {
+    r.len = kv.lens[r.seq];
+    if (r.len < r.count || r.len > ((int64_t)kv.max_pages << kv.lg_page)) {
+      r.bad = 1;
+      r.seq = -1;
+      r.len = 0;
+    }
+  }
+  return r;
+}
+
+// Keys of a part: L = the work (tiles of a row times its tokens, all rows) over
+// the units that fill the chip, but no fewer than kLeast.
+constexpr int kLeast = 512;
+__device__ __forceinline__ int parts_of(int len, int64_t most) {
+  return len > most ? (int)((len + most - 1) / most) : 1;
+}
+
+// First kernel, one workgroup: where rows begin, how many parts theirs keys are
+// taken in, and where their units, joins and parts lie.
+__global__ __launch_bounds__(kOne) void kv_map_kernel(KvCache kv, KvMap m) {
+  const int tokens = m.shape.tokens;
+  int32_t *rows = m.plan + kPlanHead + kUnitWords * m.shape.units + kJoinWords * m.shape.joins;
+  const bool stopped = kv_stopped(kv);
+  int64_t sum = 0, work = 0;
+  int bad = 0;
+  for (int i = threadIdx.x; i < m.rows; i += kOne) {
+    const MapRow r = map_row(kv, m, i);
+    sum += r.count;
+    bad |= r.bad;
+    work += (int64_t)((r.count + tokens - 1) / tokens) * r.len;
+  }
+  sum = sum_all(sum);
+  work = sum_all(work);
+  if (bad) atomicOr(kv.err, kErrKvRange);
+  const bool fits = sum <= m.tokens && !stopped;
+  if (threadIdx.x == 0 && sum > m.tokens) atomicOr(kv.err, kErrKvRange);
+  int64_t most = (work + m.shape.split - 1) / m.shape.split;
+  if (most < kLeast) most = kLeast;
+  int cu = 0, units = 0, joins = 0, parts = 0;
+  for (int base = 0; base < m.rows; base += kOne) {
+    const int i = base + threadIdx.x;
+    MapRow r{-1, 0, 0, 0};
+    if (i < m.rows && fits) r = map_row(kv, m, i);
+    const int tiles = (r.count + tokens - 1) / tokens, n = parts_of(r.len, most);
+    const int mine = tiles * n, joined = n > 1 ? tiles : 0, split = n > 1 ? mine : 0;
+    int all[4];
+    const int at_cu = cu + scan_excl(r.count, &all[0]), at_unit = units + scan_excl(mine, &all[1]),
+              at_join = joins + scan_excl(joined, &all[2]),
+              at_part = parts + scan_excl(split, &all[3]);
+    cu += all[0], units += all[1], joins += all[2], parts += all[3];
+    if (i < m.rows) {
+      m.cu[i] = at_cu;
+      int32_t *to = rows + kRowWords * i;
+      to[0] = at_unit, to[1] = at_join, to[2] = at_part, to[3] = n;
+    }
+  }
+  if (threadIdx.x == 0) {
+    m.cu[m.rows] = cu;
+    rows[kRowWords * m.rows] = units;
+    m.plan[0] = units;
+    m.plan[1] = joins;
+    m.plan[2] = fits;
+  }
+}
+
+// the last of rows whose word (at stride) is at most v; word 0 is
+template <int STRIDE>
+__device__ __forceinline__ int row_of(const int32_t *words, int rows, int v) {
+  int lo = 0, hi = rows;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (words[STRIDE * mid] <= v) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// Second kernel, a thread per token and per unit.
+__global__ __launch_bounds__(256) void kv_map_rows_kernel(KvCache kv, KvMap m) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  const int32_t *rows =
+      m.plan + kPlanHead + kUnitWords * m.shape.units + kJoinWords * m.shape.joins;
+  const bool some = m.rows > 0 && m.plan[2] != 0;
+  if (i < m.tokens) {
+    int seq = -1, pos = -1;
+    int64_t slot = -1;
+    if (some && i < m.cu[m.rows]) {
+      const int row = row_of<1>(m.cu, m.rows, i);
+      const MapRow r = map_row(kv, m, row);
+      if (r.seq >= 0) {
+        seq = r.seq;
+        pos = r.len - r.count + (i - m.cu[row]);
+        const int page = kv.tables[(int64_t)seq * kv.max_pages + (pos >> kv.lg_page)];
+        if ((uint32_t)page < (uint32_t)kv.pages)
+          slot = ((int64_t)page << kv.lg_page) + (pos & (kv.page() - 1));
+        else
+          atomicOr(kv.err, kErrKvRange);
+      }
+    }
+    m.token_seqs[i] = seq;
+    m.pos[i] = pos;
+    m.slots[i] = slot;
+  }
+  if (!some || i >= m.plan[0]) return;
+  // a row's tiles from its last tokens, which see the most keys, to its first
+  const int row = row_of<kRowWords>(rows, m.rows, i);
+  const MapRow r = map_row(kv, m, row);
+  const int32_t *at = rows + kRowWords * row;
+  const int n = at[3], j = (i - at[0]) / n, part = i - at[0] - j * n;
+  const int tokens = m.shape.tokens, tile = (r.count + tokens - 1) / tokens - 1 - j;
+  const int tok = tile * tokens, ntok = min(tokens, r.count - tok);
+  int32_t *u = m.plan + kPlanHead + (int64_t)kUnitWords * i;
+  int pos0 = 0, k0 = 0, k1 = 0, slot = -1;
+  if (r.seq >= 0) {
+    pos0 = r.len - r.count + tok;
+    const int end = pos0 + ntok, per = ((end + n - 1) / n + 63) / 64 * 64;
+    const int used = (int)(((int64_t)end + per - 1) / per);
+    const int64_t from = (int64_t)part * per;
+    k0 = (int)(from < end ? from : end);
+    k1 = (int)(from + per < end ? from + per : end);
+    if (used > 1) slot = at[2] + j * n + part;
+    if (n > 1 && part == 0) {
+      int32_t *join = m.plan + kPlanHead + kUnitWords * m.shape.units +
+                      (int64_t)kJoinWords * (at[1] + j);
+      join[0] = m.cu[row] + tok, join[1] = ntok, join[2] = at[2] + j * n, join[3] = used;
+    }
+  }
+  u[0] = r.seq, u[1] = m.cu[row] + tok, u[2] = ntok, u[3] = pos0;
+  u[4] = k0, u[5] = k1, u[6] = slot, u[7] = 0;
+}
+
+// ----------------------------------------------------------------- attention
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
+
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+// what exponents are taken against: the maximum, or 0 where no score is above
+// -infinity, so that every weight there is 0 and not a NaN
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
+
+// Where a maximum (times scale) is this far from 0, its last bit (a sixteenth) is
+// no longer nothing to an exponent: 2^(s scale - m scale) with m scale rounded
+// would be that bit off 1 for the largest score, up to infinity.
+constexpr float kFar = 1048576.f;
+
+struct Unit {
+  int seq, tok, ntok, pos0, k0, k1, slot;
+};
+// A unit of the plan as it stands there, or one without tokens where it is not
+// what a plan of this call can hold.
+__device__ __forceinline__ Unit unit_of(const KvCache &kv, const Chunk &a, int64_t i) {
+  const int4 *p = (const int4 *)(a.plan + kPlanHead + kUnitWords * i);
+  const int4 x = p[0], y = p[1];
+  Unit u{__builtin_amdgcn_readfirstlane(x.x), __builtin_amdgcn_readfirstlane(x.y),
+         __builtin_amdgcn_readfirstlane(x.z), __builtin_amdgcn_readfirstlane(x.w),
+         __builtin_amdgcn_readfirstlane(y.x), __builtin_amdgcn_readfirstlane(y.y),
+         __builtin_amdgcn_readfirstlane(y.z)};
+  const int64_t most = (int64_t)kv.max_pages << kv.lg_page;
+  if (u.seq >= kv.seqs || u.tok < 0 || u.ntok < 0 || u.ntok > a.shape.tokens ||
+      (int64_t)u.tok + u.ntok > a.tokens || u.pos0 < 0 || u.k0 < 0 || u.k1 < u.k0 ||
+      u.k1 > most || (int64_t)u.pos0 + u.ntok > most || (u.seq < 0 && u.k1 > 0) ||
+      (u.k0 & 63) || u.slot >= a.shape.parts) {
+    if (threadIdx.x == 0) atomicOr(kv.err, kErrKvRange);
+    u.ntok = 0;
+  }
+  return u;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_four(T *p, const float *x) {
+  typedef T x4 __attribute__((ext_vector_type(4)));
+  *(x4 *)p = x4{(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
+}
+// four values of a head: rounded once
+__device__ __forceinline__ void store_out(const Chunk &a, int cache_dtype, int64_t at,
+                                          const float *x) {
+  if (a.dtype == DT_I16) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    s16x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = (int16_t)fminf(fmaxf(rintf(x[i] * a.out_unit), -32768.f), 32767.f);
+    *(s16x4 *)((int16_t *)a.out + at) = v;
+  } else if (cache_dtype == DT_F32) {
+    store_four((float *)a.out + at, x);
+  } else if (cache_dtype == DT_BF16) {
+    store_four((__bf16 *)a.out + at, x);
+  } else {
+    store_four((_Float16 *)a.out + at, x);
+  }
+}
+
+template <typename T>
+struct Of {
+  typedef T x8 __attribute__((ext_vector_type(8)));
+};
+
+// Keys of a turn: 64, or 32 where a row of them is 512 bytes or more
+template <int D, typename T>
+constexpr int kTurn = D * sizeof(T) >= 512 ? 32 : 64;
+// A turn's keys or values lie in LDS by rows, the order of a row's pieces of 16
+// bytes changed by the row so that neither 16 rows' same piece (keys) nor four
+// rows' runs of 64 bytes (values by columns) meet in a bank.
+template <int ROW>
+__device__ __forceinline__ constexpr int turn_of(int t) {
+  return ROW == 128 ? ((t >> 1) & 1) << 2 | ((t >> 2) & 3) : (t & 3) << 2 | ((t >> 2) & 3);
+}
+template <int ROW>
+__device__ __forceinline__ constexpr int lds_at(int t, int piece) {
+  return t * ROW + ((piece ^ turn_of<ROW>(t)) << 4);
+}
+
+// A value that the compiler takes as new each time, so that what is made of it
+// by an addition or two is made again and not kept in a register.
+__device__ __forceinline__ int afresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// What the kernels of either width share: a unit's place, and a turn's keys and
+// values on their way to LDS, by NW wavefronts.
+template <int D, typename T, int NW>
+struct Turns {
+  static constexpr int KT = kTurn<D, T>, ROW = D * sizeof(T), BYTES = KT * ROW;
+  static constexpr int BLOCKS = KT / 16;            // of 16 tokens, each in one page
+  // A block's keys, or its values, are a job of 16 ROW bytes: a wavefront has
+  // one or two (a block's keys and values), or shares one with another.
+  static constexpr int JOBS = 2 * BLOCKS, SHARE = NW > JOBS ? NW / JOBS : 1;
+  static constexpr int MINE = JOBS > NW ? JOBS / NW : 1;
+  static constexpr int COPIES = 16 * ROW / 1024 / SHARE;
+  static_assert(MINE <= 2 && (MINE == 1 || BLOCKS == NW) && COPIES >= 1, "copies");
+  const KvCache &kv;
+  const int32_t *table;
+  int64_t plane, kbase;
+  int k1, wave, page, lane_at;
+  int next[BLOCKS];
+  uint32_t good;                                    // blocks whose pages are the pool's
+  int bad;
+  __device__ __forceinline__ Turns(const KvCache &kv, const Unit &u, int layer, int kvh, int wave)
+      : kv(kv), table(kv.tables + (int64_t)u.seq * kv.max_pages),
+        plane((int64_t)kv.page() * D), kbase(((int64_t)layer * 2 * kv.heads + kvh) * plane),
+        k1(u.k1), wave(wave), page(kv.page()), bad(0) {
+    const int at = (threadIdx.x & 63) * 16, row = at / ROW, piece = (at % ROW) >> 4;
+    lane_at = row * ROW + ((piece ^ turn_of<ROW>(row)) << 4);
+  }
+  __device__ __forceinline__ void look_up(int t) {
+#pragma unroll
+    for (int j = 0; j < BLOCKS; ++j) {
+      const int tt = t + 16 * j;
+      next[j] = table[(tt < k1 ? tt : k1 - 1) >> kv.lg_page];
+    }
+  }
+  // the turn from t on, whose pages were looked up, to lds (keys, then values)
+  __device__ __forceinline__ void load(int t, uint32_t lds) {
+    good = 0;
+    int p[BLOCKS];
+#pragma unroll
+    for (int j = 0; j < BLOCKS; ++j) {
+      p[j] = __builtin_amdgcn_readfirstlane(next[j]);
+      const bool ok = (uint32_t)p[j] < (uint32_t)kv.pages;
+      good |= (ok ? 1u : 0u) << j;
+      bad |= !ok;
+      if (!ok) p[j] = 0;
+    }
+    const int job = MINE == 2 ? wave : wave / SHARE, j = job % BLOCKS, part = wave % SHARE;
+    int mine = p[0];
+#pragma unroll
+    for (int x = 1; x < BLOCKS; ++x) mine = j == x ? p[x] : mine;
+    const uint8_t *from = kv.pool + mine * kv.page_bytes +
+                          (kbase + (int64_t)((t + 16 * j) & (page - 1)) * D) * (int)sizeof(T);
+    const int at = afresh(lane_at);
+#pragma unroll
+    for (int x = 0; x < MINE; ++x) {
+      const int which = MINE == 2 ? x : job / BLOCKS;
+      const uint8_t *src = which ? from + kv.heads * plane * (int)sizeof(T) : from;
+      const uint32_t to = lds + which * BYTES + j * 16 * ROW + part * COPIES * 1024;
+      if constexpr (SHARE == 1) {
+#pragma unroll
+        for (int n = 0; n < COPIES; ++n)            // turn_of is a sum without carries
+          copy16(src, (at ^ (turn_of<ROW>(n * 1024 / ROW) << 4)) + n * 1024, to + n * 1024);
+      } else {
+#pragma unroll
+        for (int n = 0; n < COPIES; ++n) {
+          const int i = part * COPIES + n;
+          copy16(src, (at ^ (turn_of<ROW>(i * 1024 / ROW) << 4)) + i * 1024, to + n * 1024);
+        }
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ void turn_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// Infinities and NaNs among a masked turn's values: 0 times one would reach the
+// queries that do not see it, and what lies behind a sequence's end may be
+// anything.  give(key): adds such values of a key that a query sees to its
+// output; then they are taken out.  Every wavefront calls.
+template <typename T, typename Tn, int NW, typename Give>
+__device__ __forceinline__ void take_out_odd(uint8_t *values, int *flag, Give give) {
+  constexpr uint32_t E = sizeof(T) == 4 ? 0x7F800000u : __is_same(T, _Float16) ? 0x7C00u : 0x7F80u;
+  auto odd_bits = [](uint32_t w) {
+    if constexpr (sizeof(T) == 4) return (w & E) == E ? 0xFFFFFFFFu : 0u;
+    return ((w & E) == E ? 0xFFFFu : 0u) | ((w >> 16 & E) == E ? 0xFFFF0000u : 0u);
+  };
+  bool odd = false;
+  for (int at = threadIdx.x * 16; at < Tn::BYTES; at += NW * 1024) {
+    const u32x4 w = *(const u32x4 *)(values + at);
+    odd |= (odd_bits(w[0]) | odd_bits(w[1]) | odd_bits(w[2]) | odd_bits(w[3])) != 0;
+  }
+  if (odd) *flag = 1;
+  __syncthreads();
+  if (*flag == 0) return;
+  for (int key = 0; key < Tn::KT; ++key) give(key);
+  __syncthreads();
+  for (int at = threadIdx.x * 16; at < Tn::BYTES; at += NW * 1024) {
+    u32x4 w = *(const u32x4 *)(values + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] &= ~odd_bits(w[i]);
+    *(u32x4 *)(values + at) = w;
+  }
+  if (threadIdx.x == 0) *flag = 0;
+  __syncthreads();
+}
+
+struct Place {
+  int kvh, h0, heads;        // key-value head, first query head, query heads
+  int64_t unit;
+  int part;                  // of a unit's parts: which tile of heads
+};
+__device__ __forceinline__ Place place_of(const KvCache &kv, const Chunk &a) {
+  const int per = kv.heads * a.shape.tiles, group = a.hq / kv.heads;
+  Place p;
+  p.unit = blockIdx.x / per;
+  p.part = (int)(blockIdx.x - p.unit * per);
+  p.kvh = p.part / a.shape.tiles;
+  const int first = (p.part - p.kvh * a.shape.tiles) * a.shape.heads;
+  p.heads = min(a.shape.heads, group - first);
+  p.h0 = p.kvh * group + first;
+  return p;
+}
+
+__device__ __forceinline__ void zeros(const KvCache &kv, const Chunk &a, const Unit &u,
+                                      const Place &p) {
+  const float zero[4] = {0, 0, 0, 0};
+  const int each = p.heads * kv.dim;
+  for (int e = threadIdx.x * 4; e < u.ntok * each; e += blockDim.x * 4) {
+    const int t = e / each, x = e - t * each;
+    store_out(a, kv.dtype, (int64_t)(u.tok + t) * a.out_token + (p.h0 + x / kv.dim) * a.out_head +
+                               x % kv.dim, zero);
+  }
+}
+
+// Where a row of a unit's parts lies: its values, then (all rows') maximum and sum
+__device__ __forceinline__ float *part_row(const KvCache &kv, const Chunk &a, int slot,
+                                           const Place &p, int row) {
+  const int per = kv.heads * a.shape.tiles;
+  return a.part + (((int64_t)slot * per + p.part) * kChunkRows + row) * kv.dim;
+}
+__device__ __forceinline__ float *part_sums(const KvCache &kv, const Chunk &a, int slot,
+                                            const Place &p, int row) {
+  const int64_t per = kv.heads * a.shape.tiles;
+  return a.part + a.shape.parts * per * kChunkRows * kv.dim +
+         ((slot * per + p.part) * kChunkRows + row) * 2;
+}
+
+// Keys and values of 16 bits.
+template <int D, typename T>
+__global__ __launch_bounds__(kThreads, 2) void chunk_kernel(KvCache kv, Chunk a) {
+  typedef Turns<D, T, kWaves> Tn;
+  typedef typename Of<T>::x8 x8;
+  constexpr int KT = Tn::KT, ROW = Tn::ROW, BYTES = Tn::BYTES;
+  constexpr int KS = D / 16, NT = KT / 32, ND = D / 32;
+  constexpr bool HALF = __is_same(T, _Float16);
+  // weights are taken against a maximum that follows the largest score only when
+  // that is SLACK above it, so that sums are rarely rescaled; a float16 weight's
+  // exponent ends at 2^-24: weights there are 2^LIFT as large
+  constexpr float LIFT = HALF ? 14.f : 0.f, SLACK = HALF ? 1.f : 8.f;
+  __shared__ __align__(1024) uint8_t buf[2][2 * BYTES];
+  __shared__ int odd;
+
+  const Place P = place_of(kv, a);
+  if (P.unit >= min((int64_t)a.plan[0], a.shape.units)) return;
+  const Unit u = unit_of(kv, a, P.unit);
+  if (u.ntok == 0) return;
+  if (u.k1 == 0) return zeros(kv, a, u, P);
+  if (u.k0 >= u.k1) return;
+  const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Tn turns(kv, u, a.layer, P.kvh, wave);
+  turns.look_up(u.k0);
+  turns.load(u.k0, (uint32_t)(uintptr_t)buf[0]);
+  turns.look_up(u.k0 + KT);
+
+  // this lane's query: row of the unit, its token and head
+  const int row = wave * 32 + r, tok = row / P.heads, head = P.h0 + row - tok * P.heads;
+  const bool on = tok < u.ntok;
+  const bool work = wave * 32 < u.ntok * P.heads;
+  const int last = u.pos0 + (on ? tok : 0);         // the last key it sees
+  const int wave_last =                             // and any of this wavefront
+      u.pos0 + min(u.ntok - 1, __builtin_amdgcn_readfirstlane((wave * 32 + 31) / P.heads));
+  // a scale below 0 turns q, and 0 makes it 0 (a masked score is -infinity)
+  const float sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f;
+  const float scale = a.scale == 0.f ? 1.f : fabsf(a.scale);
+  if (threadIdx.x == 0) odd = 0;
+  x8 q[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int64_t e = (int64_t)(u.tok + tok) * a.q_token + head * a.q_head + 16 * s + 8 * g;
+    const u32x4 w = on ? *(const u32x4 *)((const uint16_t *)a.q + e) : u32x4{0, 0, 0, 0};
+    const uint32_t flip = sign < 0.f ? 0x80008000u : 0u, keep = sign == 0.f ? 0u : ~0u;
+    q[s] = __builtin_bit_cast(x8, (w ^ flip) & keep);
+  }
+
+  f32x16 o[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+  float m = -INFINITY, l = 0.f;                     // m: of scores before the scale
+  // where this lane's keys (row r, piece g of each step) and the columns of
+  // values that it reads for its group of 16 lie in LDS; a step, an element tile
+  // and a second four keys turn bits of the place
+  const int k_at = lds_at<ROW>(r, g);
+  const int v_row = 4 * g + ((lane & 15) >> 2), v_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  const int v_at = lds_at<ROW>(v_row, v_col >> 3) + (v_col & 4) * 2;
+
+  auto body = [&](int t, const uint8_t *lds, uint32_t good, bool masked) {
+    f32x16 sc[NT];
+    const int kat = afresh(k_at);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[j][i] = 0.f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const x8 k = *(const x8 *)(lds + (kat ^ (s << 5)) + 32 * j * ROW);
+        sc[j] = mfma32(k, q[s], sc[j]);
+        if (D == 256 && s % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    // result i of tile j is key t + 32 j + 8 (i >> 2) + 4 g + (i & 3)
+    if (masked) {
+      const int end = min(last, u.k1 - 1) - t - 4 * g;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const bool off = (32 * j + 8 * (i >> 2) + (i & 3) > end) | !(good >> (2 * j + (i >> 3)) & 1);
+          sc[j][i] = off ? -INFINITY : sc[j][i];
+        }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[j][i]);
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const bool rise = (top - m) * scale > SLACK;    // from -infinity too
+    if (__any(rise)) {
+      const float up = rise ? top : m;
+      const float fall = exp2_of((m - base_of(up)) * scale);
+      m = up;
+      l *= fall;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[d] *= fall;
+    }
+    const float base = base_of(m);
+    float sum = 0.f;
+    if constexpr (D == 256) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float x = (sc[j][i] - base) * scale;
+          sc[j][i] = exp2_of(LIFT > 0.f ? x + LIFT : x);
+          sum += sc[j][i];
+        }
+    } else {
+      float off = base * scale;
+      const bool far = fabsf(off) >= kFar;
+      if (__any(far)) {                             // of other queries, not a bit changes
+#pragma unroll
+        for (int j = 0; j < NT; ++j) sc[j] -= far ? base : 0.f;
+        off = far ? 0.f : off;
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float x = __builtin_fmaf(sc[j][i], scale, -off);
+          sc[j][i] = exp2_of(LIFT > 0.f ? x + LIFT : x);
+          sum += sc[j][i];
+        }
+    }
+    l += sum;
+    const int vat = afresh(v_at);
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        x8 p;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = (T)sc[j][8 * s + i];
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          // row d of V transposed: eight keys of this lane's, four at a time
+          u32x2 w[2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            w[x] = lds_columns(lds + BYTES + (vat ^ (d << 6) ^ (x << 5)) +
+                               (32 * j + 16 * s + 8 * x) * ROW);
+          o[d] = mfma32(__builtin_bit_cast(x8, w), p, o[d]);
+          if (D == 256 && d % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+  };
+  // the infinities and NaNs among a key's values, to the queries that see it
+  auto give = [&](int t, const uint8_t *values, uint32_t good, int key) {
+    const bool sees = t + key <= last && t + key < u.k1 && (good >> (key >> 4) & 1);
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int col = 32 * d + 8 * b + 4 * g;
+        typedef T x4 __attribute__((ext_vector_type(4)));
+        const x4 v = *(const x4 *)(values + lds_at<ROW>(key, col >> 3) + (col & 4) * 2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float y = (float)v[i];
+          o[d][4 * b + i] += sees && !(fabsf(y) < INFINITY) ? y : 0.f;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  };
+
+  turn_barrier();
+  const int full = min(u.pos0 + 1, u.k1);           // keys that every query sees
+  for (int t = u.k0, b = 0; t < u.k1; t += KT, b ^= 1) {
+    const uint32_t good = turns.good;
+    if (t + KT < u.k1) {
+      turns.load(t + KT, (uint32_t)(uintptr_t)buf[b ^ 1]);
+      turns.look_up(t + 2 * KT);
+    }
+    const bool masked = t + KT > full || good != (1u << Tn::BLOCKS) - 1;
+    if (masked)
+      take_out_odd<T, Tn, kWaves>(buf[b] + BYTES, &odd,
+                                  [&](int key) { give(t, buf[b] + BYTES, good, key); });
+    if (work && t <= wave_last) body(t, buf[b], good, masked);
+    turn_barrier();
+  }
+  if (turns.bad && threadIdx.x == 0) atomicOr(kv.err, kErrKvRange);
+  if (!on) return;
+  l += __shfl_xor(l, 32);
+  // result i of tile d is element 32 d + 8 (i >> 2) + 4 g + (i & 3)
+  if (u.slot < 0) {
+    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+    const int64_t at = (int64_t)(u.tok + tok) * a.out_token + head * a.out_head + 4 * g;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const float x[4] = {o[d][4 * b] * inv, o[d][4 * b + 1] * inv, o[d][4 * b + 2] * inv,
+                            o[d][4 * b + 3] * inv};
+        store_out(a, kv.dtype, at + 32 * d + 8 * b, x);
+      }
+    return;
+  }
+  float *part = part_row(kv, a, u.slot, P, row) + 4 * g;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+      *(f32x4 *)(part + 32 * d + 8 * b) =
+          f32x4{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]};
+  if (g == 0) {
+    float *ml = part_sums(kv, a, u.slot, P, row);
+    ml[0] = m * scale;
+    ml[1] = l;
+  }
+}
+
+// Keys and values of 32 bits, on the float32 matrix instructions: 16 keys by 16
+// queries, a wavefront's queries as C columns of tiles, so that q and out stay
+// in 128 registers.
+template <int D, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void chunk_f32_kernel(KvCache kv, Chunk a) {
+  typedef Turns<D, float, NW> Tn;
+  constexpr int C = kChunkRows / (16 * NW);
+  constexpr int KT = Tn::KT, ROW = Tn::ROW, BYTES = Tn::BYTES;
+  constexpr int KS = D / 16, NT = KT / 16, NC = D / 64;
+  constexpr float SLACK = 8.f;
+  __shared__ __align__(1024) uint8_t buf[2][2 * BYTES];
+  __shared__ int odd;
+
+  const Place P = place_of(kv, a);
+  if (P.unit >= min((int64_t)a.plan[0], a.shape.units)) return;
+  const Unit u = unit_of(kv, a, P.unit);
+  if (u.ntok == 0) return;
+  if (u.k1 == 0) return zeros(kv, a, u, P);
+  if (u.k0 >= u.k1) return;
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Tn turns(kv, u, a.layer, P.kvh, wave);
+  turns.look_up(u.k0);
+  turns.load(u.k0, (uint32_t)(uintptr_t)buf[0]);
+  turns.look_up(u.k0 + KT);
+
+  int row[C], tok[C], head[C], last[C];
+  bool on[C];
+  const bool work = wave * 16 * C < u.ntok * P.heads;
+  const int wave_last =
+      u.pos0 + min(u.ntok - 1, __builtin_amdgcn_readfirstlane((wave * 16 * C + 16 * C - 1) / P.heads));
+  f32x4 q[C][KS];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    row[c] = wave * 16 * C + 16 * c + r;
+    tok[c] = row[c] / P.heads;
+    head[c] = P.h0 + row[c] - tok[c] * P.heads;
+    on[c] = tok[c] < u.ntok;
+    last[c] = u.pos0 + (on[c] ? tok[c] : 0);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int64_t e = (int64_t)(u.tok + tok[c]) * a.q_token + head[c] * a.q_head + 16 * s + 4 * g;
+      q[c][s] = f32x4{0, 0, 0, 0};
+      if (on[c]) {
+        q[c][s] = *(const f32x4 *)((const float *)a.q + e);
+        if (a.scale < 0.f) q[c][s] = -q[c][s];
+        if (a.scale == 0.f) q[c][s] = f32x4{0, 0, 0, 0};
+      }
+    }
+  }
+  const float scale = a.scale == 0.f ? 1.f : fabsf(a.scale);
+  if (threadIdx.x == 0) odd = 0;
+  f32x4 o[C][NC * 4];
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int d = 0; d < NC * 4; ++d) o[c][d] = f32x4{0, 0, 0, 0};
+  float m[C], l[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) m[c] = -INFINITY, l[c] = 0.f;
+
+  // a step of 16 elements and a key of the lane's four turn bits of the place
+  const int k_at = lds_at<ROW>(r, g), v_at = lds_at<ROW>(4 * g, r);
+  auto body = [&](int t, const uint8_t *lds, uint32_t good, bool masked) {
+    f32x4 sc[C][NT];
+    const int kat = afresh(k_at);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) sc[c][j] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const f32x4 k = *(const f32x4 *)(lds + (kat ^ (s << 6)) + 16 * j * ROW);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int c = 0; c < C; ++c) sc[c][j] = mfma16(k[i], q[c][s][i], sc[c][j]);
+        if (s & 1) __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    // result i of tile j is key t + 16 j + 4 g + i
+    if (masked) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int end = min(last[c], u.k1 - 1) - t - 4 * g;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            sc[c][j][i] = ((16 * j + i > end) | !(good >> j & 1)) ? -INFINITY : sc[c][j][i];
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[c][j][i]);
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const bool rise = (top - m[c]) * scale > SLACK;
+      if (__any(rise)) {
+        const float up = rise ? top : m[c];
+        const float fall = exp2_of((m[c] - base_of(up)) * scale);
+        m[c] = up;
+        l[c] *= fall;
+#pragma unroll
+        for (int d = 0; d < NC * 4; ++d) o[c][d] *= fall;
+      }
+      const float base = base_of(m[c]);
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sc[c][j][i] = exp2_of((sc[c][j][i] - base) * scale);
+          l[c] += sc[c][j][i];
+        }
+    }
+    const int vat = afresh(v_at);
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int d = 0; d < NC; ++d) {
+          const f32x4 v = *(const f32x4 *)(lds + BYTES + (vat ^ (i << 6)) + 256 * d +
+                                           (16 * j + i) * ROW);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+              o[c][4 * d + e] = mfma16(v[e], sc[c][j][i], o[c][4 * d + e]);
+          if (d & 1) __builtin_amdgcn_sched_barrier(0);
+        }
+  };
+  auto give = [&](int t, const uint8_t *values, uint32_t good, int key) {
+#pragma unroll
+    for (int d = 0; d < NC; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4 v = *(const f32x4 *)(values + lds_at<ROW>(key, 16 * d + 4 * g + i));
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const bool sees = t + key <= last[c] && t + key < u.k1 && (good >> (key >> 4) & 1);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            o[c][4 * d + e][i] += sees && !(fabsf(v[e]) < INFINITY) ? v[e] : 0.f;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  };
+
+  turn_barrier();
+  const int full = min(u.pos0 + 1, u.k1);
+  for (int t = u.k0, b = 0; t < u.k1; t += KT, b ^= 1) {
+    const uint32_t good = turns.good;
+    if (t + KT < u.k1) {
+      turns.load(t + KT, (uint32_t)(uintptr_t)buf[b ^ 1]);
+      turns.look_up(t + 2 * KT);
+    }
+    const bool masked = t + KT > full || good != (1u << Tn::BLOCKS) - 1;
+    if (masked)
+      take_out_odd<float, Tn, NW>(buf[b] + BYTES, &odd,
+                                  [&](int key) { give(t, buf[b] + BYTES, good, key); });
+    if (work && t <= wave_last) body(t, buf[b], good, masked);
+    turn_barrier();
+  }
+  if (turns.bad && threadIdx.x == 0) atomicOr(kv.err, kErrKvRange);
+  // result i of o[4 d + e] is element (16 d + 4 g + i) * 4 + e
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    float sum = l[c] + __shfl_xor(l[c], 16);
+    sum += __shfl_xor(sum, 32);
+    if (!on[c]) continue;
+    const float inv = u.slot >= 0 ? 1.f : sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+    const int64_t at = (int64_t)(u.tok + tok[c]) * a.out_token + head[c] * a.out_head;
+    float *part = u.slot >= 0 ? part_row(kv, a, u.slot, P, row[c]) : nullptr;
+#pragma unroll
+    for (int d = 0; d < NC; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = (16 * d + 4 * g + i) * 4;
+        const float x[4] = {o[c][4 * d][i] * inv, o[c][4 * d + 1][i] * inv,
+                            o[c][4 * d + 2][i] * inv, o[c][4 * d + 3][i] * inv};
+        if (part) *(f32x4 *)(part + e) = f32x4{x[0], x[1], x[2], x[3]};
+        else store_out(a, kv.dtype, at + e, x);
+      }
+    if (part && g == 0) {
+      float *ml = part_sums(kv, a, u.slot, P, row[c]);
+      ml[0] = m[c] * scale;
+      ml[1] = sum;
+    }
+  }
+}
+
+// The parts of a tile joined: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
+// D / 4 threads per row, a workgroup per tile of tokens and heads.
+template <int D>
+__global__ __launch_bounds__(kThreads) void chunk_join_kernel(KvCache kv, Chunk a) {
+  constexpr int LANES = D / 4, ROWS = kThreads / LANES;
+  const Place P = place_of(kv, a);
+  if (P.unit >= min((int64_t)a.plan[1], a.shape.joins)) return;
+  const int4 j = *(const int4 *)(a.plan + kPlanHead + kUnitWords * a.shape.units +
+                                 kJoinWords * P.unit);
+  if (j.w <= 1 || j.x < 0 || j.y < 0 || j.y > a.shape.tokens || (int64_t)j.x + j.y > a.tokens ||
+      j.z < 0 || (int64_t)j.z + j.w > a.shape.parts)
+    return;
+  const int lane = threadIdx.x % LANES, rows = j.y * P.heads;
+  for (int row = threadIdx.x / LANES; row < rows; row += ROWS) {
+    float m = -INFINITY, l = 0.f;
+    f32x4 o{0, 0, 0, 0};
+    for (int s = 0; s < j.w; ++s) {
+      const float *ml = part_sums(kv, a, j.z + s, P, row);
+      const f32x4 so = *(const f32x4 *)(part_row(kv, a, j.z + s, P, row) + lane * 4);
+      const float top = fmaxf(m, ml[0]), base = base_of(top);
+      const float x = exp2_of(m - base), y = exp2_of(ml[0] - base);
+      m = top;
+      l = l * x + ml[1] * y;
+      o = o * x + so * y;
+    }
+    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+    const float x[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+    const int tok = row / P.heads;
+    store_out(a, kv.dtype, (int64_t)(j.x + tok) * a.out_token + (P.h0 + row - tok * P.heads) * a.out_head +
+                               lane * 4, x);
+  }
+}
+
+template <int D>
+void launch_dim(const KvCache &kv, const Chunk &a, uint32_t grid, hipStream_t s) {
+  constexpr int F32 = D == 256 ? 8 : 4;
+  if (kv.dtype == DT_F32) chunk_f32_kernel<D, F32><<<grid, 64 * F32, 0, s>>>(kv, a);
+  else if (kv.dtype == DT_BF16) chunk_kernel<D, __bf16><<<grid, kThreads, 0, s>>>(kv, a);
+  else chunk_kernel<D, _Float16><<<grid, kThreads, 0, s>>>(kv, a);
+  const uint32_t joins = (uint32_t)(kv.heads * a.shape.tiles * a.shape.joins);
+  if (joins) chunk_join_kernel<D><<<joins, kThreads, 0, s>>>(kv, a);
+}
+
+}  // namespace
+
+// A unit has up to kChunkRows rows: every query head of a key-value head that
+// fits, and as many tokens.  A row's keys are split (kv_map_kernel) so that the
+// units of `split` tiles' work fill the chip; with W = the sum over rows of
+// tiles times tokens and L = W / split or more keys a part, parts beyond the
+// first and tiles that are split are at most W / L each.
+ChunkShape chunk_shape(const KvCache &kv, int64_t rows, int64_t tokens, int64_t hq, int num_cu) {
+  ChunkShape c{};
+  const int64_t group = hq / kv.heads;
+  c.heads = (int32_t)(group < kChunkRows ? group : kChunkRows);
+  c.tiles = (int32_t)((group + c.heads - 1) / c.heads);
+  c.tokens = kChunkRows / c.heads;
+  const int64_t per = (int64_t)kv.heads * c.tiles, most = rows < tokens ? rows : tokens;
+  const int64_t tiles = tokens / c.tokens + most;
+  c.split = (4ll * num_cu + per - 1) / per;
+  const bool can = (((int64_t)kv.max_pages << kv.lg_page) > kLeast) && tiles > 0;
+  c.joins = can ? (tiles < c.split ? tiles : c.split) : 0;
+  c.units = tiles + (can ? c.split : 0);
+  c.parts = can ? c.joins + c.split : 0;
+  return c;
+}
+
+int64_t chunk_workspace(const KvCache &kv, const ChunkShape &c) {
+  return c.parts * kv.heads * c.tiles * kChunkRows * (kv.dim + 2) * 4;
+}
+
+hipError_t launch_kv_map(const KvCache &kv, const KvMap &m, hipStream_t s) {
+  kv_map_kernel<<<1, kOne, 0, s>>>(kv, m);
+  const int64_t n = m.tokens > m.shape.units ? m.tokens : m.shape.units;
+  if (n > 0) kv_map_rows_kernel<<<(uint32_t)((n + 255) / 256), 256, 0, s>>>(kv, m);
+  return hipGetLastError();
+}
+
+hipError_t launch_chunk(const KvCache &kv, const Chunk &a, hipStream_t s) {
+  const uint32_t grid = (uint32_t)(kv.heads * a.shape.tiles * a.shape.units);
+  if (grid == 0) return hipSuccess;
+  if (kv.dim == 64) launch_dim<64>(kv, a, grid, s);
+  else if (kv.dim == 128) launch_dim<128>(kv, a, grid, s);
+  else launch_dim<256>(kv, a, grid, s);
+  return hipGetLastError();
+}
+
+}  // namespace w4a8

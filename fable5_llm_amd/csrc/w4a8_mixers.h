@@ -88,6 +88,50 @@ int attend_splits(const KvCache &kv, int64_t rows, int64_t hq, int num_cu);
 int64_t attend_workspace(const KvCache &kv, int64_t rows, int64_t hq, int num_cu);
 hipError_t launch_attend(const KvCache &kv, const Attend &a, hipStream_t s);
 
+// A step's new tokens, several of each sequence, and their attention
+// (w4a8_chunk.hip).  The plan of a step, int32 words on the device: a head of
+// kPlanHead, then units and joins; a row's place in them behind those.
+//   unit   a run of a row's tokens and of the keys before them, a workgroup's
+//          work for each of the key-value heads' tiles of query heads
+//   join   a run of tokens whose keys several units took
+constexpr int kPlanHead = 16, kUnitWords = 8, kJoinWords = 4, kRowWords = 4;
+constexpr int kChunkRows = 128;     // query rows (tokens x heads) of a unit
+struct ChunkShape {
+  int32_t heads;                    // query heads of a unit, of one key-value head
+  int32_t tiles;                    // head tiles of a key-value head
+  int32_t tokens;                   // tokens of a unit
+  int64_t split;                    // units of a full chip, see chunk_shape
+  int64_t units, joins, parts;      // at most
+};
+ChunkShape chunk_shape(const KvCache &kv, int64_t rows, int64_t tokens, int64_t hq, int num_cu);
+inline int64_t plan_words(const ChunkShape &c, int64_t rows) {
+  return kPlanHead + kUnitWords * c.units + kJoinWords * c.joins + kRowWords * (rows + 1);
+}
+struct KvMap {
+  const int32_t *seqs, *counts;     // of rows
+  int32_t *cu, *token_seqs, *pos;   // outputs
+  int64_t *slots;
+  int32_t *plan;
+  int32_t rows, tokens;
+  ChunkShape shape;
+};
+hipError_t launch_kv_map(const KvCache &kv, const KvMap &m, hipStream_t s);
+
+struct Chunk {
+  const void *q;                    // [tokens][hq][dim], strides in elements
+  void *out;
+  int64_t q_token, q_head, out_token, out_head;
+  const int32_t *plan;
+  float *part;                      // [parts][kv heads][head tiles][rows of a unit][dim], then
+                                    // {max, sum} of each row
+  int32_t tokens, hq, layer, dtype;
+  ChunkShape shape;
+  float scale;                      // of the scores, log2(e) included
+  float out_unit;                   // DT_I16: 1 / the value of one step of out
+};
+int64_t chunk_workspace(const KvCache &kv, const ChunkShape &c);
+hipError_t launch_chunk(const KvCache &kv, const Chunk &a, hipStream_t s);
+
 // The gated delta rule: q, k [tokens][hk][dk], v, out [tokens][hv][dv], g and
 // beta [tokens][hv], state [slots][hv][dk][dv].
 struct Delta {

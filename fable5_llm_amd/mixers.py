@@ -92,6 +92,31 @@ def _workspace(ctx, nbytes):
     return torch.empty(int(nbytes), dtype=torch.uint8, device=torch.device("cuda", ctx.device))
 
 
+class ChunkMaps:
+    """Where the tokens of a step lie (PagedKV.chunk_maps makes it, PagedKV.map_async
+    fills it, for all layers of the step):
+
+      cu      int32 [rows + 1]: row i's tokens are cu[i] .. cu[i + 1] - 1
+      seqs    int32 [tokens]: each token's sequence
+      pos     int32 [tokens]: its position in the sequence
+      slots   int64 [tokens]: its place in the pool, page * page_tokens + place
+              in the page; -1 in all three for padding and behind the last row
+      plan    uint8: the attention's pieces of work"""
+
+    def __init__(self, kv, rows, tokens, q_heads):
+        import torch
+        b = ctypes.c_int64()
+        N.check(N.lib().w4a8_kv_plan_bytes(kv.h, rows, tokens, q_heads, ctypes.byref(b)),
+                "kv_plan_bytes")
+        ints = dict(dtype=torch.int32, device=torch.device("cuda", kv.ctx.device))
+        self.cu, self.seqs, self.pos = (torch.empty(n, **ints)
+                                        for n in (rows + 1, tokens, tokens))
+        self.slots = torch.empty(tokens, dtype=torch.int64, device=ints["device"])
+        self.plan = _workspace(kv.ctx, b.value)
+        self.rows, self.tokens, self.q_heads = rows, tokens, q_heads
+        self.cache = kv
+
+
 class PagedKV:
     """A key-value cache in pages, over the caller's device tensors:
 
@@ -209,6 +234,55 @@ class PagedKV:
             _list(seqs, self.ctx, "seqs", n),
             None if upto is None else _list(upto, self.ctx, "upto", n), n, hq,
             self.scale if scale is None else scale, ws.data_ptr(), ws.nbytes), "kv_attend")
+
+    def chunk_maps(self, rows, tokens, q_heads):
+        """Device memory for the maps of steps with this many rows, tokens and
+        query heads, until map_async fills it of no meaning."""
+        return ChunkMaps(self, rows, tokens, q_heads)
+
+    def _maps(self, maps):
+        if not isinstance(maps, ChunkMaps):
+            raise ValueError("maps: must be made by chunk_maps")
+        if maps.cache is not self:
+            raise ValueError("maps: are another cache's")
+        return maps
+
+    def map_async(self, seqs, counts, maps):
+        """Where a step's tokens lie: the last counts[i] tokens of sequence
+        seqs[i] for each row i, side by side in the order of the list."""
+        m = self._maps(maps)
+        N.check(N.lib().w4a8_kv_map_async(
+            self.h, _list(seqs, self.ctx, "seqs", m.rows),
+            _list(counts, self.ctx, "counts", m.rows), m.rows, m.tokens, m.q_heads,
+            m.cu.data_ptr(), m.seqs.data_ptr(), m.pos.data_ptr(), m.slots.data_ptr(),
+            m.plan.data_ptr(), m.plan.nbytes), "kv_map")
+
+    def attend_chunk_workspace(self, maps):
+        """Device memory for attend_chunk_async with these maps; calls that can
+        overlap, graphs' replays among them, need one each."""
+        m, b = self._maps(maps), ctypes.c_int64()
+        N.check(N.lib().w4a8_kv_attend_chunk_workspace(self.h, m.rows, m.tokens, m.q_heads,
+                                                       ctypes.byref(b)),
+                "kv_attend_chunk_workspace")
+        return _workspace(self.ctx, b.value)
+
+    def attend_chunk_async(self, layer, q, out, maps, ws, scale=None, out_frac=0):
+        """out [tokens, q_heads, head_dim] = attention of a step's tokens, each
+        over the tokens of its sequence up to itself.  q: of the cache's type;
+        out: that too, or int16.  scale: 1 / sqrt(head_dim) unless given.  Tokens
+        of a padded row get zeros, those behind the last row's are left alone."""
+        m = self._maps(maps)
+        shape = (m.tokens, m.q_heads, self.head_dim)
+        qp, q0, q1 = _act(q, self.ctx, "q", shape, self.dtype)
+        op, o0, o1 = _act(out, self.ctx, "out", shape)
+        _on(ws, self.ctx, "ws")
+        if not ws.is_contiguous():
+            raise ValueError("ws: must be contiguous")
+        N.check(N.lib().w4a8_kv_attend_chunk_async(
+            self.h, layer, qp, q0, q1, self._act_type(out, "out"), out_frac, op, o0, o1,
+            m.plan.data_ptr(), m.plan.nbytes, m.rows, m.tokens, m.q_heads,
+            self.scale if scale is None else scale, ws.data_ptr(), ws.nbytes),
+            "kv_attend_chunk")
 
     def fork_async(self, parents, children):
         """Sequence children[i], empty, becomes a copy of parents[i]: full

@@ -499,6 +499,49 @@ int w4a8_kv_attend_async(w4a8_kv *kv, int32_t layer, int32_t dtype, int32_t frac
                          const int32_t *d_upto, int32_t rows, int32_t q_heads,
                          double scale, void *d_ws, int64_t ws_bytes);
 
+/* ---- a step of several new tokens of each sequence ----
+ * A step: rows i (a sequence d_seqs[i], negative: a padded row) with
+ * d_counts[i] new tokens each, side by side in the order of the list, in
+ * activations of `tokens` tokens; those behind the last row's are no row's.
+ * The new tokens of a row are the last d_counts[i] that its sequence holds
+ * (w4a8_kv_extend_async came before); a sequence may be listed more than once.
+ *
+ * Where they lie: d_cu int32[rows + 1], row i's tokens are d_cu[i] ..
+ * d_cu[i + 1] - 1; for each of `tokens` tokens its sequence, its position in it
+ * (int32) and its slot of the cache (int64: page * page_tokens + place in the
+ * page), -1 for one of a padded row, of no row or of none of the pool's pages.
+ * d_plan: what w4a8_kv_attend_chunk_async goes by, w4a8_kv_plan_bytes bytes,
+ * 16-byte aligned; both hold until the cache changes, for all layers.
+ * A row whose sequence is outside the cache or holds fewer tokens than its
+ * count is treated as padding, and a step of more tokens than `tokens` (or on a
+ * cache that a refused call has stopped) as one without rows; the next sync
+ * reports it. */
+int w4a8_kv_plan_bytes(const w4a8_kv *kv, int32_t rows, int32_t tokens,
+                       int32_t q_heads, int64_t *bytes);
+int w4a8_kv_map_async(w4a8_kv *kv, const int32_t *d_seqs, const int32_t *d_counts,
+                      int32_t rows, int32_t tokens, int32_t q_heads, int32_t *d_cu,
+                      int32_t *d_token_seqs, int32_t *d_pos, int64_t *d_slots,
+                      void *d_plan, int64_t plan_bytes);
+/* bytes of workspace w4a8_kv_attend_chunk_async needs for such a step (may be
+   0).  Calls that can overlap need one each. */
+int w4a8_kv_attend_chunk_workspace(const w4a8_kv *kv, int32_t rows, int32_t tokens,
+                                   int32_t q_heads, int64_t *bytes);
+/* Attention of a step's new tokens, each over its sequence's tokens up to
+   itself: q [tokens][q_heads][head_dim] of the cache's dtype, query heads of a
+   key-value head side by side.
+     out = softmax(scale q K^T) V
+   out_dtype: the cache's, or I16 (with out_frac fraction bits).  Tokens of a
+   padded row get zeros; those of no row are left alone.  Weights go into the
+   second product rounded to the cache's dtype.  An infinity or a NaN in a key
+   or value reaches no token before its own.  rows, tokens and q_heads: the
+   plan's. */
+int w4a8_kv_attend_chunk_async(w4a8_kv *kv, int32_t layer, const void *d_q,
+                               int64_t q_token, int64_t q_head, int32_t out_dtype,
+                               int32_t out_frac, void *d_out, int64_t out_token,
+                               int64_t out_head, const void *d_plan, int64_t plan_bytes,
+                               int32_t rows, int32_t tokens, int32_t q_heads,
+                               double scale, void *d_ws, int64_t ws_bytes);
+
 /* The gated delta rule.  Per token t and value head h (key head h / (hv /
  * hk)), with the head's state S float32 [dk][dv]:
  *   S <- exp(g) S;  u = beta (v - S^T k);  S <- S + k u^T;  out = scale S^T q
