@@ -19,7 +19,7 @@ ALU_SHIFT32, ALU_SILU32, ALU_EMUL32, ALU_SHIFT32W = 1, 6, 8, 9
 MOVY_PAIRS32, MOVY_INT16 = 0, 1
 PLAN_GRAPH, PLAN_PERSISTENT, PLAN_PERSISTENT_COOP = 0, 1, 2
 FENCE_ALL, FENCE_AUTO = 0, 1
-DT_F32, DT_BF16, DT_F16, DT_I16 = 0, 1, 2, 3
+DT_F32, DT_BF16, DT_F16, DT_I16, DT_I32 = 0, 1, 2, 3, 4
 WAIT_NONE, WAIT_GRID, WAIT_INPUT = 0, 1, 2   # w4a8_plan_fences
 
 _P = ctypes.c_void_p
@@ -88,6 +88,10 @@ SIGNATURES = {
     "w4a8_kv_attend_chunk_workspace": [_P, _I32, _I32, _I32, _P],
     "w4a8_kv_attend_chunk_async": [_P, _I32, _P, _I64, _I64, _I32, _I32, _P, _I64, _I64, _P,
                                    _I64, _I32, _I32, _I32, ctypes.c_double, _P, _I64],
+    "w4a8_rotary_async": [_P, _P],
+    "w4a8_kv_append_rotary_async": [_P, _I32, _P],
+    "w4a8_logprobs_workspace": [_P, _I64, _I64, _P],
+    "w4a8_logprobs_async": [_P, _P],
     "w4a8_delta_step_async": [_P, _P],
     "w4a8_delta_chunk_workspace": [_P, _I64, _I64, _I64, _I64, _I64, _I32, _P],
     "w4a8_delta_chunk_async": [_P, _P],

@@ -218,6 +218,9 @@ int take_err(w4a8_ctx *c) {
       return fail(W4A8_E_RANGE, "KV cache: a sequence, position, length or page outside the "
                                 "cache; it was not followed (an extend or fork that names it, "
                                 "and the calls on the cache behind that, changed nothing)");
+    if (h & kErrToken)
+      return fail(W4A8_E_RANGE, "log probabilities: a token outside the vocabulary (its log "
+                                "probability was left 0)");
     if (h & kErrDelta)
       return fail(W4A8_E_RANGE, "delta rule: a state slot named twice or outside the states "
                                 "(that row was not run), or bounds that do not lie in order "
@@ -2360,6 +2363,138 @@ int w4a8_kv_attend_chunk_async(w4a8_kv *kv, int32_t layer, const void *d_q, int6
   a.out_unit = 1.f / unit_of(out_dtype, out_frac);
   DeviceGuard g(kv->ctx->device);
   HIP_TRY(launch_chunk(kv->c, a, kv->ctx->stream));
+  return W4A8_OK;
+}
+
+namespace {
+const char *rotary_fault(const w4a8_rotary *d, bool append) {
+  if (d->dtype < DT_F32 || d->dtype > DT_I16 || d->out_dtype < DT_F32 || d->out_dtype > DT_I16)
+    return "unknown dtype";
+  if (d->out_dtype != d->dtype && d->dtype != DT_I16)
+    return "out must have the dtype of q and k, which may be int16";
+  if (d->frac < 0 || d->frac > 31 || d->out_frac < 0 || d->out_frac > 31)
+    return "fraction bits must be 0..31";
+  if (d->dim < 16 || d->dim > 256 || d->dim % 16) return "dim must be a multiple of 16, 16..256";
+  if (d->rot < 0 || d->rot > d->dim || d->rot % 16)
+    return "rot must be a multiple of 16, at most dim";
+  if (d->rot > 0 && (!d->freq || ((uintptr_t)d->freq & 7))) return "freq must be 8-byte aligned";
+  if (d->tokens < 0 || d->tokens > kMostRows) return "at most 2^20 tokens";
+  if (d->q_heads < 0 || d->k_heads < 0 || d->q_heads > 65535 || d->k_heads > 65535 ||
+      d->q_heads + d->k_heads < 1)
+    return "heads out of range";
+  if (((uintptr_t)d->q_norm | (uintptr_t)d->k_norm) & 3) return "norms must be 4-byte aligned";
+  if (!(d->amplitude == d->amplitude) || !(d->eps >= 0.0)) return "amplitude or eps is no number";
+  // a launch has fewer than 2^32 threads
+  if (d->tokens * (d->q_heads + 2 * d->k_heads) > (1 << 27))
+    return "too many tokens and heads for one call";
+  if (d->tokens == 0) return nullptr;
+  const int t = (int)d->dtype, o = (int)d->out_dtype;
+  if (!d->pos || ((uintptr_t)d->pos & 3)) return "pos must be 4-byte aligned";
+  if (d->q_heads > 0 && (!rows_ok(d->q, t, d->q_token, d->q_head) ||
+                         !rows_ok(d->q_out, o, d->q_out_token, d->q_out_head)))
+    return "q and its out must be 16-byte aligned, their strides whole 16 bytes";
+  if (d->k_heads > 0 && !rows_ok(d->k, t, d->k_token, d->k_head))
+    return "k must be 16-byte aligned, its strides whole 16 bytes";
+  if (d->k_heads > 0 && !append && !rows_ok(d->k_out, o, d->k_out_token, d->k_out_head))
+    return "k's out must be 16-byte aligned, its strides whole 16 bytes";
+  if (append && (!rows_ok(d->v, t, d->v_token, d->v_head) || !d->slots ||
+                 ((uintptr_t)d->slots & 7)))
+    return "v must be 16-byte, slots 8-byte aligned, v's strides whole 16 bytes";
+  return nullptr;
+}
+
+int rotary_launch(w4a8_ctx *c, const KvCache &kv, const w4a8_rotary *d, int32_t layer,
+                  bool append) {
+  if (const char *why = rotary_fault(d, append)) return fail(W4A8_E_ARG, std::string("rotary: ") + why);
+  if (d->tokens == 0) return W4A8_OK;
+  Rotary a{};
+  a.q = d->q, a.k = d->k, a.v = d->v, a.q_out = d->q_out, a.k_out = d->k_out;
+  a.pos = d->pos, a.slots = append ? d->slots : nullptr, a.freq = d->freq;
+  a.q_norm = d->q_norm, a.k_norm = d->k_norm;
+  a.q_token = d->q_token, a.q_head = d->q_head, a.k_token = d->k_token, a.k_head = d->k_head;
+  a.v_token = d->v_token, a.v_head = d->v_head;
+  a.q_out_token = d->q_out_token, a.q_out_head = d->q_out_head;
+  a.k_out_token = d->k_out_token, a.k_out_head = d->k_out_head;
+  a.tokens = (int32_t)d->tokens, a.hq = (int32_t)d->q_heads, a.hk = (int32_t)d->k_heads;
+  a.dim = (int32_t)d->dim, a.rot = (int32_t)d->rot, a.pairs = d->pairs != 0;
+  a.in_dtype = (int32_t)d->dtype, a.out_dtype = (int32_t)d->out_dtype, a.layer = layer;
+  for (a.lanes = 1; a.lanes * 16 < a.dim;) a.lanes *= 2;
+  a.unit = unit_of(a.in_dtype, d->frac), a.out_per = 1.f / unit_of(a.out_dtype, d->out_frac);
+  a.amplitude = (float)d->amplitude, a.eps = (float)d->eps, a.per_dim = 1.f / (float)d->dim;
+  DeviceGuard g(c->device);
+  HIP_TRY(launch_rotary(kv, a, c->num_cu, c->stream));
+  return W4A8_OK;
+}
+}  // namespace
+
+int w4a8_rotary_async(w4a8_ctx *c, const w4a8_rotary *d) {
+  if (!c || !d) return fail(W4A8_E_ARG, "null argument");
+  return rotary_launch(c, KvCache{}, d, 0, false);
+}
+
+int w4a8_kv_append_rotary_async(w4a8_kv *kv, int32_t layer, const w4a8_rotary *d) {
+  if (!kv || !d) return fail(W4A8_E_ARG, "null argument");
+  if (layer < 0 || layer >= kv->c.layers) return fail(W4A8_E_ARG, "no such layer");
+  if (d->dim != kv->c.dim || d->k_heads != kv->c.heads || d->out_dtype != kv->c.dtype)
+    return fail(W4A8_E_ARG, "rotary: dim, k_heads and out_dtype are the cache's");
+  return rotary_launch(kv->ctx, kv->c, d, layer, true);
+}
+
+namespace {
+int check_logits(const w4a8_ctx *c, int64_t rows, int64_t vocab) {
+  if (!c) return fail(W4A8_E_ARG, "null argument");
+  if (rows < 0 || rows > kMostRows || vocab < 1 || vocab > (1 << 24))
+    return fail(W4A8_E_ARG, "log probabilities: at most 2^20 rows, of 1 to 2^24 logits");
+  if (rows * logprobs_splits(rows ? rows : 1, vocab, c->num_cu) > (1 << 23))
+    return fail(W4A8_E_ARG, "log probabilities: too many rows and logits for one call");
+  return W4A8_OK;
+}
+}  // namespace
+
+int w4a8_logprobs_workspace(const w4a8_ctx *c, int64_t rows, int64_t vocab, int64_t *bytes) {
+  if (!bytes) return fail(W4A8_E_ARG, "null argument");
+  if (int rc = check_logits(c, rows, vocab)) return rc;
+  *bytes = rows ? logprobs_workspace(rows, vocab, c->num_cu) : 0;
+  return W4A8_OK;
+}
+
+int w4a8_logprobs_async(w4a8_ctx *c, const w4a8_logprobs *d) {
+  if (!c || !d) return fail(W4A8_E_ARG, "null argument");
+  if (int rc = check_logits(c, d->rows, d->vocab)) return rc;
+  if (d->dtype < DT_F32 || d->dtype > DT_I32 || d->dtype == DT_I16)
+    return fail(W4A8_E_ARG, "logits are float32, bfloat16, float16 or int32");
+  if (d->k < 0 || d->k > 32 || d->k > d->vocab)
+    return fail(W4A8_E_ARG, "log probabilities: 0 to 32 alternatives, of as many logits");
+  const float scale = (float)(d->scale * 1.4426950408889634);
+  if (!(scale > 0.f) || !(scale < INFINITY))
+    return fail(W4A8_E_ARG, "log probabilities: scale must be above 0 and finite");
+  if (d->rows == 0) return W4A8_OK;
+  const int size = d->dtype == DT_I32 ? 4 : dtype_size((int)d->dtype);
+  if (!d->logits || ((uintptr_t)d->logits & (size - 1)) || d->row < 0)
+    return fail(W4A8_E_ARG, "logits must be aligned to their size");
+  if ((!d->logp != !d->ids) || (d->k > 0 && (!d->top_logp || !d->top_ids)) ||
+      (((uintptr_t)d->ids | (uintptr_t)d->logp | (uintptr_t)d->entropy | (uintptr_t)d->top_logp |
+        (uintptr_t)d->top_ids) & 3))
+    return fail(W4A8_E_ARG, "log probabilities: ids and logp, top_logp and top_ids come together, "
+                            "4-byte aligned");
+  const int64_t need = logprobs_workspace(d->rows, d->vocab, c->num_cu);
+  if (!d->ws || !aligned16(d->ws) || d->ws_bytes < need)
+    return fail(W4A8_E_ARG, "log probabilities: the workspace holds " +
+                                std::to_string(d->ws_bytes) + " bytes, the call needs " +
+                                std::to_string(need));
+  Logprobs a{};
+  a.logits = d->logits, a.ids = d->ids;
+  a.logp = d->logp, a.entropy = d->entropy, a.top_logp = d->top_logp, a.top_ids = d->top_ids;
+  a.row = d->row, a.rows = d->rows, a.vocab = d->vocab;
+  a.k = (int32_t)d->k, a.dtype = (int32_t)d->dtype;
+  a.blocks = logprobs_blocks(d->vocab);
+  a.splits = logprobs_splits(d->rows, d->vocab, c->num_cu);
+  a.parts = (float *)d->ws;
+  a.keys = a.k > 0 ? (uint32_t *)(a.parts + a.rows * a.splits * 4) : nullptr;
+  a.scale = scale;
+  a.err = c->d_err;
+  DeviceGuard g(c->device);
+  HIP_TRY(launch_logprobs(a, c->stream));
   return W4A8_OK;
 }
 

@@ -8,7 +8,7 @@
 namespace w4a8 {
 
 // element types of activations and caches (W4A8_DT_*)
-enum Dtype { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2, DT_I16 = 3 };
+enum Dtype { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2, DT_I16 = 3, DT_I32 = 4 };
 inline int dtype_size(int d) { return d == DT_F32 ? 4 : 2; }
 
 // bits of the context's error word
@@ -16,6 +16,7 @@ constexpr int kErrKvRange = 32;    // a sequence, position or page outside the c
 constexpr int kErrKvFull = 64;     // too few free pages
 constexpr int kErrKvList = 128;    // a sequence listed twice, or a child not empty
 constexpr int kErrDelta = 256;     // a state slot or a prompt's bounds
+constexpr int kErrToken = 512;     // a token outside the vocabulary
 constexpr int kKvSkip = 1 << 30;   // never in the word: the call comes behind a refused one
 
 // 16-byte loads and stores that pass the caches by: data read or written once
@@ -131,6 +132,42 @@ struct Chunk {
 };
 int64_t chunk_workspace(const KvCache &kv, const ChunkShape &c);
 hipError_t launch_chunk(const KvCache &kv, const Chunk &a, hipStream_t s);
+
+// Heads rotated to their tokens' positions (w4a8_rotary.hip); with slots, k and v
+// go into the cache's layer.
+struct Rotary {
+  const void *q, *k, *v;            // [tokens][heads][dim], strides in elements
+  void *q_out, *k_out;              // q_out may be q, k_out k
+  const int32_t *pos;
+  const int64_t *slots;
+  const double *freq;               // [rot / 2]: radians a position
+  const float *q_norm, *k_norm;     // [dim] or null
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, q_out_token, q_out_head, k_out_token,
+      k_out_head;
+  int32_t tokens, hq, hk, dim, rot, pairs, in_dtype, out_dtype, layer;
+  int32_t lanes;                    // of a head: a power of two
+  float unit, out_per;              // DT_I16: the value of a step, 1 / that of out
+  float amplitude, eps, per_dim;    // per_dim: 1 / dim
+};
+hipError_t launch_rotary(const KvCache &kv, const Rotary &a, int num_cu, hipStream_t s);
+
+// What rows of logits say (w4a8_logprobs.hip)
+struct Logprobs {
+  const void *logits;               // [rows][vocab], rows `row` elements apart
+  const int32_t *ids;
+  float *logp, *entropy, *top_logp; // [rows], [rows], [rows][k]; the first two may be null
+  int32_t *top_ids;                 // [rows][k]
+  float *parts;                     // [rows][splits][4]
+  uint32_t *keys;                   // [rows][blocks], null without alternatives
+  int64_t row, rows, vocab;
+  int32_t k, dtype, blocks, splits;
+  float scale;                      // log2(e) included
+  int32_t *err;
+};
+int logprobs_blocks(int64_t vocab);
+int logprobs_splits(int64_t rows, int64_t vocab, int num_cu);
+int64_t logprobs_workspace(int64_t rows, int64_t vocab, int num_cu);
+hipError_t launch_logprobs(const Logprobs &a, hipStream_t s);
 
 // The gated delta rule: q, k [tokens][hk][dk], v, out [tokens][hv][dv], g and
 // beta [tokens][hv], state [slots][hv][dk][dv].

@@ -417,6 +417,40 @@ class Context:
             self.h, gate.h, up.h, down.h, pg, pu, pd, _dptr(x16), _dptr(norm_w),
             int(in_f), 1 if one_plus else 0, _dptr(mlp_out), _dptr(res_out)), "mlp")
 
+    # ------------------------------------------------ positions (async)
+    def rotary_async(self, q, k, pos, freq, q_out, k_out, layout="halves", amplitude=1.0,
+                     q_norm=None, k_norm=None, eps=1e-6, frac=0, out_frac=0):
+        """Heads of q [tokens, q_heads, dim] and k [tokens, k_heads, dim] (one of
+        them may be None, with its out) rotated to the tokens' positions pos
+        (int32, negative: nothing of that token is written), into q_out and
+        k_out, which may be q and k.  freq: float64 [rot / 2] on the device,
+        radians a position (mixers.rotary_frequencies); the first rot elements
+        of a head are rotated, as pairs (i, i + rot / 2) ("halves") or (2 i, 2 i
+        + 1) ("pairs"), and multiplied by amplitude.  q_norm, k_norm: float32
+        [dim], the weights of a root-mean-square norm of each head before that.
+        q and k of one type, q_out and k_out too: the same, or any if int16
+        (frac, out_frac: fraction bits)."""
+        N.check(N.lib().w4a8_rotary_async(self.h, mixers.rotary_args(
+            self, q, k, None, pos, None, freq, q_out, k_out, layout, amplitude, q_norm, k_norm,
+            eps, frac, out_frac)), "rotary")
+
+    # ------------------------------------------------- log probabilities (async)
+    def logprobs_workspace(self, rows, vocab):
+        """Device memory for logprobs_async with this many rows and logits;
+        calls that can overlap need one each."""
+        return mixers.logprobs_workspace(self, rows, vocab)
+
+    def logprobs_async(self, logits, ids, logp, ws, entropy=None, top_logp=None, top_ids=None,
+                       scale=1.0):
+        """What rows of logits [rows, vocab] (float32, bfloat16, float16, or int32
+        as a head's y32) say, with y = scale * logits: the log probability logp
+        [rows] of token ids[row] (negative: none, 0; both may be None), the
+        entropy [rows] in nats, and the best alternatives top_ids [rows, k], k up
+        to 32, with their log probabilities top_logp: largest logit first, of
+        equal ones the lowest index.  Outputs float32, ids int32."""
+        N.check(N.lib().w4a8_logprobs_async(self.h, mixers.logprobs_args(
+            self, logits, ids, logp, ws, entropy, top_logp, top_ids, scale)), "logprobs")
+
     # ------------------------------------------- gated delta rule (async)
     def delta_step_async(self, q, k, v, g, beta, state, out, slots=None, scale=None, norm=True,
                          eps=1e-6, frac=0, out_frac=0):

@@ -257,6 +257,18 @@ class PagedKV:
             m.cu.data_ptr(), m.seqs.data_ptr(), m.pos.data_ptr(), m.slots.data_ptr(),
             m.plan.data_ptr(), m.plan.nbytes), "kv_map")
 
+    def append_rotary_async(self, layer, q, k, v, pos, slots, freq, q_out, layout="halves",
+                            amplitude=1.0, q_norm=None, k_norm=None, eps=1e-6, frac=0):
+        """A layer's q [n, heads, head_dim], normalised and rotated to the tokens'
+        positions, into q_out, and k, v [n, kv_heads, head_dim], k likewise, into
+        the tokens' slots of the cache (map_async's pos and slots; negative: a
+        padded token, nothing of it is written).  q, k and v: of the cache's
+        type, or int16 with frac; q_out: the cache's type.  The other arguments:
+        Context.rotary_async's."""
+        N.check(N.lib().w4a8_kv_append_rotary_async(self.h, layer, rotary_args(
+            self.ctx, q, k, v, pos, slots, freq, q_out, None, layout, amplitude, q_norm, k_norm,
+            eps, frac, 0, (self.kv_heads, self.head_dim, self.dtype))), "kv_append_rotary")
+
     def attend_chunk_workspace(self, maps):
         """Device memory for attend_chunk_async with these maps; calls that can
         overlap, graphs' replays among them, need one each."""
@@ -327,6 +339,150 @@ class PagedKV:
                 self.close()
         except Exception:
             pass
+
+
+# w4a8_rotary: ten pointers, ten strides, tokens, q_heads, k_heads, dim, rot, pairs,
+# dtype, frac, out_dtype, out_frac, amplitude, eps
+_ROTARY = struct.Struct("=10Q20q2d")
+
+
+def _vector(t, ctx, name, dtype, n):
+    _on(t, ctx, name)
+    if t.dim() != 1 or t.dtype != dtype or not t.is_contiguous() or \
+            (n is not None and t.shape[0] != n):
+        raise ValueError(f"{name}: must be a contiguous {dtype} vector"
+                         + ("" if n is None else f" of {n} entries"))
+    return t.data_ptr()
+
+
+def rotary_args(ctx, q, k, v, pos, slots, freq, q_out, k_out, layout, amplitude, q_norm, k_norm,
+                eps, frac, out_frac, cache=None):
+    """The checked arguments of one rotary call, packed as w4a8_rotary.  cache:
+    (heads, dim, type) of the cache that k and v go into."""
+    import torch
+    if layout not in ("halves", "pairs"):
+        raise ValueError(f"layout: 'halves' or 'pairs', not {layout!r}")
+    dts = _dtypes()
+    if q is None and (k is None or cache):
+        raise ValueError("q: is needed" if cache else "q, k: one of them is needed")
+    x = k if q is None else q
+    _on(x, ctx, "k" if q is None else "q")
+    if x.dim() != 3:
+        raise ValueError("q and k: [tokens, heads, dim] is required")
+    tokens, dim, dtype = x.shape[0], x.shape[2], x.dtype
+    dt = dts.get(dtype)
+    if dt is None:
+        raise ValueError(f"q and k: float32, bfloat16, float16 or int16, not {dtype}")
+    if cache:
+        heads, cdim, ctype = cache
+        if dt != N.DT_I16 and dtype != ctype:
+            raise ValueError(f"q: must be {ctype}, as the cache, or int16")
+        if dim != cdim:
+            raise ValueError(f"q: has heads of {dim}, the cache of {cdim}")
+    out_type = cache[2] if cache else (q_out if q is not None else k_out).dtype
+    if dts.get(out_type) is None or (out_type != dtype and dt != N.DT_I16):
+        raise ValueError(f"out: must be {dtype}, as q and k")
+    qh, qp, q0, q1, qo, qo0, qo1 = (0,) * 7
+    kh, kp, k0, k1, ko, ko0, ko1, vp, v0, v1 = (0,) * 10
+    if q is not None:
+        qh = q.shape[1]
+        qp, q0, q1 = _act(q, ctx, "q", (tokens, qh, dim), dtype)
+        qo, qo0, qo1 = _act(q_out, ctx, "q_out", (tokens, qh, dim), out_type)
+    if k is not None or cache:
+        _on(k, ctx, "k")
+        kh = cache[0] if cache else k.shape[1] if k.dim() == 3 else 0
+        kp, k0, k1 = _act(k, ctx, "k", (tokens, kh, dim), dtype)
+        if cache:
+            vp, v0, v1 = _act(v, ctx, "v", (tokens, kh, dim), dtype)
+        else:
+            ko, ko0, ko1 = _act(k_out, ctx, "k_out", (tokens, kh, dim), out_type)
+    return _ROTARY.pack(
+        qp, kp, vp, qo, ko, _list(pos, ctx, "pos", tokens),
+        _vector(slots, ctx, "slots", torch.int64, tokens) if cache else 0,
+        _vector(freq, ctx, "freq", torch.float64, None),
+        *(0 if w is None else _vector(w, ctx, n, torch.float32, dim)
+          for w, n in ((q_norm, "q_norm"), (k_norm, "k_norm"))),
+        q0, q1, k0, k1, v0, v1, qo0, qo1, ko0, ko1, tokens, qh, kh, dim, 2 * freq.shape[0],
+        layout == "pairs", dt, frac, dts[out_type], out_frac, amplitude, eps)
+
+
+def rotary_frequencies(rot, base=10000.0, stretch=None, factor=1.0, trained=None, fast=32.0,
+                       slow=1.0):
+    """(freq, amplitude) for the rotary calls: radians a position of rot / 2
+    pairs, float64 on the host, f_i = base^(-2 i / rot).  For contexts `factor`
+    times as long as the `trained` tokens:
+
+      stretch="positions"  f / factor: all positions drawn together
+      stretch="base"       base factor^(rot / (rot - 2)) in place of base: the
+                           fastest pair as it was, the slowest f / factor
+      stretch="parts"      pairs that turn `fast` times or more within `trained`
+                           as they were, those of `slow` or fewer f / factor, in
+                           between a ramp over the turns; amplitude 0.1 log
+                           factor + 1"""
+    import torch
+    if rot < 2 or rot % 2:
+        raise ValueError("rot: must be even, 2 or more")
+    if not base > 0 or not factor >= 1:
+        raise ValueError("base must be above 0, factor 1 or more")
+    if stretch == "base":
+        if rot < 4:
+            raise ValueError("rot: 4 or more with stretch='base'")
+        base = base * factor ** (rot / (rot - 2))
+    f = float(base) ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)
+    if stretch == "positions":
+        return f / factor, 1.0
+    if stretch == "parts":
+        if not trained or not trained > 0 or not fast > slow:
+            raise ValueError("trained tokens, and fast above slow, are needed")
+        keep = ((trained * f / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
+        return f * keep + f / factor * (1 - keep), 0.1 * math.log(factor) + 1.0
+    if stretch not in (None, "base"):
+        raise ValueError(f"stretch: None, 'positions', 'base' or 'parts', not {stretch!r}")
+    return f, 1.0
+
+
+# w4a8_logprobs: seven pointers, ws_bytes, row, rows, vocab, k, dtype, scale
+_LOGPROBS = struct.Struct("=7Q6qd")
+
+
+def logprobs_args(ctx, logits, ids, logp, ws, entropy, top_logp, top_ids, scale):
+    """The checked arguments of one logprobs call, packed as w4a8_logprobs."""
+    import torch
+    _on(logits, ctx, "logits")
+    types = {torch.float32: N.DT_F32, torch.bfloat16: N.DT_BF16, torch.float16: N.DT_F16,
+             torch.int32: N.DT_I32}
+    if logits.dim() != 2 or logits.dtype not in types:
+        raise ValueError("logits: [rows, vocab] of float32, bfloat16, float16 or int32 is required")
+    rows, vocab = logits.shape
+    if logits.stride(1) != 1 and vocab > 1:
+        raise ValueError("logits: the last dimension must be contiguous")
+    if (ids is None) != (logp is None) or (top_ids is None) != (top_logp is None):
+        raise ValueError("ids and logp, top_ids and top_logp come together")
+    k = 0
+    if top_ids is not None:
+        for t, name, dtype in ((top_ids, "top_ids", torch.int32),
+                               (top_logp, "top_logp", torch.float32)):
+            _on(t, ctx, name)
+            if t.dim() != 2 or t.shape[0] != rows or t.shape != top_ids.shape or \
+                    t.dtype != dtype or not t.is_contiguous():
+                raise ValueError(f"{name}: must be contiguous {dtype} [rows, k]")
+        k = top_ids.shape[1]
+    _on(ws, ctx, "ws")
+    if not ws.is_contiguous():
+        raise ValueError("ws: must be contiguous")
+    return _LOGPROBS.pack(
+        logits.data_ptr(), 0 if ids is None else _list(ids, ctx, "ids", rows),
+        *(0 if t is None else _vector(t, ctx, n, torch.float32, rows)
+          for t, n in ((logp, "logp"), (entropy, "entropy"))),
+        *((top_logp.data_ptr(), top_ids.data_ptr()) if k else (0, 0)), ws.data_ptr(), ws.nbytes,
+        logits.stride(0) if rows > 1 else 0, rows, vocab, k, types[logits.dtype], scale)
+
+
+def logprobs_workspace(ctx, rows, vocab):
+    b = ctypes.c_int64()
+    N.check(N.lib().w4a8_logprobs_workspace(ctx.h, rows, vocab, ctypes.byref(b)),
+            "logprobs_workspace")
+    return _workspace(ctx, b.value)
 
 
 # w4a8_delta: ten pointers, ws_bytes, ten strides, tokens, rows, hk, hv, dk, dv,

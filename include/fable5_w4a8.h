@@ -421,6 +421,7 @@ int w4a8_plan_destroy(w4a8_plan *plan);
 #define W4A8_DT_BF16  1
 #define W4A8_DT_F16   2
 #define W4A8_DT_I16   3   /* activations only */
+#define W4A8_DT_I32   4   /* logits only */
 
 /* A paged cache over device memory of the caller:
  *   pool    [pages][layers][keys, values][kv_heads][page_tokens][head_dim] of
@@ -541,6 +542,66 @@ int w4a8_kv_attend_chunk_async(w4a8_kv *kv, int32_t layer, const void *d_q,
                                int64_t out_head, const void *d_plan, int64_t plan_bytes,
                                int32_t rows, int32_t tokens, int32_t q_heads,
                                double scale, void *d_ws, int64_t ws_bytes);
+
+/* Heads rotated to their tokens' positions, and normalised first where a norm's
+ * weights are given: for a head x of q or k at position p, y = x / sqrt(mean x^2
+ * + eps) * norm, and for the pairs (a, b) = (y[i], y[i + rot / 2]), or (y[2 i],
+ * y[2 i + 1]) with `pairs`, i < rot / 2, t = p * freq[i]:
+ *   (a, b) -> amplitude * (a cos t - b sin t, b cos t + a sin t)
+ * Elements from rot on pass through.  The angle is taken in 64 bits.  freq:
+ * radians a position, what a stretched context's rule makes of them included.
+ * q [tokens][q_heads][dim], k, v [tokens][k_heads][dim]; either of q_heads and
+ * k_heads may be 0.  A token with a negative position is padding: nothing of
+ * it is written.  q_out may be q, and k_out k, with the same strides.  dim: a
+ * multiple of 16, 16..256; rot: one too, 0..dim.  At most 2^20 tokens.  All
+ * members are 8 bytes wide. */
+typedef struct {
+  const void *q, *k, *v; /* v: append only */
+  void *q_out, *k_out;   /* k_out: not of append */
+  const int32_t *pos;    /* [tokens] */
+  const int64_t *slots;  /* [tokens], append only: w4a8_kv_map_async's */
+  const double *freq;    /* [rot / 2], device */
+  const float *q_norm, *k_norm;   /* [dim], or null: not normalised */
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head; /* strides, in elements */
+  int64_t q_out_token, q_out_head, k_out_token, k_out_head;
+  int64_t tokens, q_heads, k_heads, dim, rot, pairs;
+  int64_t dtype, frac;            /* of q, k and v; frac: I16 */
+  int64_t out_dtype, out_frac;    /* dtype again, or any where that is I16 */
+  double amplitude, eps;
+} w4a8_rotary;
+int w4a8_rotary_async(w4a8_ctx *ctx, const w4a8_rotary *r);
+/* The same for a layer's q into q_out, and k and v into their slots of the
+   cache, whose dtype is out_dtype.  A token without a slot is padding too; one
+   outside the pool is reported by the next sync.  Two tokens with the same slot
+   leave either one's values there. */
+int w4a8_kv_append_rotary_async(w4a8_kv *kv, int32_t layer, const w4a8_rotary *r);
+
+/* What rows of logits say.  With y = scale * logits, per row: the log
+ * probability y[id] - log sum e^y of token ids[row] (negative: none, 0), the
+ * entropy in nats, and the k best alternatives, largest logit first, of equal
+ * ones the lowest index first, with their log probabilities.  Logits of
+ * -infinity (tokens ruled out) weigh nothing; a row of nothing else has log
+ * probabilities of -infinity and an entropy of 0; one with a NaN or +infinity
+ * has no numbers (and some alternatives' indices).  I32: a head's y32, or any
+ * whole numbers.  An id outside the vocabulary is reported by the next sync. */
+typedef struct {
+  const void *logits;    /* [rows][vocab], aligned to an element */
+  const int32_t *ids;    /* [rows], or null */
+  float *logp;           /* [rows], with ids */
+  float *entropy;        /* [rows], or null */
+  float *top_logp;       /* [rows][k] */
+  int32_t *top_ids;      /* [rows][k] */
+  void *ws;              /* w4a8_logprobs_workspace bytes, 16-byte aligned */
+  int64_t ws_bytes;
+  int64_t row;           /* stride of rows, in elements */
+  int64_t rows, vocab;   /* at most 2^20, and 2^24 */
+  int64_t k;             /* 0..32, at most vocab */
+  int64_t dtype;         /* F32, BF16, F16 or I32 */
+  double scale;          /* above 0: 1 / temperature, times the value of a step of I32 */
+} w4a8_logprobs;
+int w4a8_logprobs_workspace(const w4a8_ctx *ctx, int64_t rows, int64_t vocab,
+                            int64_t *bytes);
+int w4a8_logprobs_async(w4a8_ctx *ctx, const w4a8_logprobs *l);
 
 /* The gated delta rule.  Per token t and value head h (key head h / (hv /
  * hk)), with the head's state S float32 [dk][dv]:
