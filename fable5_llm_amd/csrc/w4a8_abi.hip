@@ -2359,6 +2359,7 @@ int w4a8_kv_attend_chunk_async(w4a8_kv *kv, int32_t layer, const void *d_q, int6
   a.q_token = q_token, a.q_head = q_head, a.out_token = out_token, a.out_head = out_head;
   a.plan = (const int32_t *)d_plan, a.part = (float *)d_ws;
   a.tokens = tokens, a.hq = q_heads, a.layer = layer, a.dtype = out_dtype;
+  a.most_joins = 8 * kv->ctx->num_cu;
   a.scale = (float)(scale * 1.4426950408889634);
   a.out_unit = 1.f / unit_of(out_dtype, out_frac);
   DeviceGuard g(kv->ctx->device);

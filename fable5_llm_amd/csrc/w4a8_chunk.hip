@@ -76,7 +76,7 @@ __device__ __forceinline__ MapRow map_row(const KvCache &kv, const KvMap &m, int
 
 // Keys of a part: L = the work (tiles of a row times its tokens, all rows) over
 // the units that fill the chip, but no fewer than kLeast.
-constexpr int kLeast = 512;
+constexpr int kLeast = 128;
 __device__ __forceinline__ int parts_of(int len, int64_t most) {
   return len > most ? (int)((len + most - 1) / most) : 1;
 }
@@ -168,12 +168,14 @@ __global__ __launch_bounds__(256) void kv_map_rows_kernel(KvCache kv, KvMap m) {
     m.slots[i] = slot;
   }
   if (!some || i >= m.plan[0]) return;
-  // a row's tiles from its last tokens, which see the most keys, to its first
+  // a row's tiles from its last tokens, which see the most keys, to its first,
+  // those of the same part of the keys side by side
   const int row = row_of<kRowWords>(rows, m.rows, i);
   const MapRow r = map_row(kv, m, row);
   const int32_t *at = rows + kRowWords * row;
-  const int n = at[3], j = (i - at[0]) / n, part = i - at[0] - j * n;
-  const int tokens = m.shape.tokens, tile = (r.count + tokens - 1) / tokens - 1 - j;
+  const int tokens = m.shape.tokens, tiles = (r.count + tokens - 1) / tokens;
+  const int n = at[3], part = (i - at[0]) / tiles, j = i - at[0] - part * tiles;
+  const int tile = tiles - 1 - j;
   const int tok = tile * tokens, ntok = min(tokens, r.count - tok);
   int32_t *u = m.plan + kPlanHead + (int64_t)kUnitWords * i;
   int pos0 = 0, k0 = 0, k1 = 0, slot = -1;
@@ -394,11 +396,11 @@ struct Place {
   int64_t unit;
   int part;                  // of a unit's parts: which tile of heads
 };
-__device__ __forceinline__ Place place_of(const KvCache &kv, const Chunk &a) {
+__device__ __forceinline__ Place place_of(const KvCache &kv, const Chunk &a, int64_t i) {
   const int per = kv.heads * a.shape.tiles, group = a.hq / kv.heads;
   Place p;
-  p.unit = blockIdx.x / per;
-  p.part = (int)(blockIdx.x - p.unit * per);
+  p.unit = i / per;
+  p.part = (int)(i - p.unit * per);
   p.kvh = p.part / a.shape.tiles;
   const int first = (p.part - p.kvh * a.shape.tiles) * a.shape.heads;
   p.heads = min(a.shape.heads, group - first);
@@ -445,7 +447,7 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(KvCache kv, Chunk a)
   __shared__ __align__(1024) uint8_t buf[2][2 * BYTES];
   __shared__ int odd;
 
-  const Place P = place_of(kv, a);
+  const Place P = place_of(kv, a, blockIdx.x);
   if (P.unit >= min((int64_t)a.plan[0], a.shape.units)) return;
   const Unit u = unit_of(kv, a, P.unit);
   if (u.ntok == 0) return;
@@ -521,10 +523,9 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(KvCache kv, Chunk a)
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[j][i]);
-    top = fmaxf(top, __shfl_xor(top, 32));
-    const bool rise = (top - m) * scale > SLACK;    // from -infinity too
-    if (__any(rise)) {
-      const float up = rise ? top : m;
+    if (__any((top - m) * scale > SLACK)) {         // from -infinity too
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float up = (top - m) * scale > SLACK ? top : m;
       const float fall = exp2_of((m - base_of(up)) * scale);
       m = up;
       l *= fall;
@@ -550,12 +551,12 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(KvCache kv, Chunk a)
         for (int j = 0; j < NT; ++j) sc[j] -= far ? base : 0.f;
         off = far ? 0.f : off;
       }
+      off -= LIFT;
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float x = __builtin_fmaf(sc[j][i], scale, -off);
-          sc[j][i] = exp2_of(LIFT > 0.f ? x + LIFT : x);
+          sc[j][i] = exp2_of(__builtin_fmaf(sc[j][i], scale, -off));
           sum += sc[j][i];
         }
     }
@@ -659,7 +660,7 @@ __global__ __launch_bounds__(64 * NW, 2) void chunk_f32_kernel(KvCache kv, Chunk
   __shared__ __align__(1024) uint8_t buf[2][2 * BYTES];
   __shared__ int odd;
 
-  const Place P = place_of(kv, a);
+  const Place P = place_of(kv, a, blockIdx.x);
   if (P.unit >= min((int64_t)a.plan[0], a.shape.units)) return;
   const Unit u = unit_of(kv, a, P.unit);
   if (u.ntok == 0) return;
@@ -745,11 +746,10 @@ __global__ __launch_bounds__(64 * NW, 2) void chunk_f32_kernel(KvCache kv, Chunk
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[c][j][i]);
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      const bool rise = (top - m[c]) * scale > SLACK;
-      if (__any(rise)) {
-        const float up = rise ? top : m[c];
+      if (__any((top - m[c]) * scale > SLACK)) {
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float up = (top - m[c]) * scale > SLACK ? top : m[c];
         const float fall = exp2_of((m[c] - base_of(up)) * scale);
         m[c] = up;
         l[c] *= fall;
@@ -843,35 +843,51 @@ __global__ __launch_bounds__(64 * NW, 2) void chunk_f32_kernel(KvCache kv, Chunk
 }
 
 // The parts of a tile joined: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
-// D / 4 threads per row, a workgroup per tile of tokens and heads.
+// D / 4 threads per row; a workgroup takes the rows that its threads make of one
+// tile after another, so that few are launched where nothing was split.
 template <int D>
 __global__ __launch_bounds__(kThreads) void chunk_join_kernel(KvCache kv, Chunk a) {
-  constexpr int LANES = D / 4, ROWS = kThreads / LANES;
-  const Place P = place_of(kv, a);
-  if (P.unit >= min((int64_t)a.plan[1], a.shape.joins)) return;
-  const int4 j = *(const int4 *)(a.plan + kPlanHead + kUnitWords * a.shape.units +
-                                 kJoinWords * P.unit);
-  if (j.w <= 1 || j.x < 0 || j.y < 0 || j.y > a.shape.tokens || (int64_t)j.x + j.y > a.tokens ||
-      j.z < 0 || (int64_t)j.z + j.w > a.shape.parts)
-    return;
-  const int lane = threadIdx.x % LANES, rows = j.y * P.heads;
-  for (int row = threadIdx.x / LANES; row < rows; row += ROWS) {
+  constexpr int LANES = D / 4, ROWS = kThreads / LANES, GROUPS = kChunkRows / ROWS, AT_ONCE = 4;
+  const int per = kv.heads * a.shape.tiles, lane = threadIdx.x % LANES;
+  const int64_t all = min((int64_t)a.plan[1], a.shape.joins) * per * GROUPS;
+  for (int64_t w = blockIdx.x; w < all; w += gridDim.x) {
+    const int64_t unit = w / GROUPS;
+    const int row = (int)(w - unit * GROUPS) * ROWS + threadIdx.x / LANES;
+    const Place P = place_of(kv, a, unit);
+    const int4 j = *(const int4 *)(a.plan + kPlanHead + kUnitWords * a.shape.units +
+                                   kJoinWords * P.unit);
+    if (j.w <= 1 || j.x < 0 || j.y < 0 || j.y > a.shape.tokens ||
+        (int64_t)j.x + j.y > a.tokens || j.z < 0 || (int64_t)j.z + j.w > a.shape.parts ||
+        row >= j.y * P.heads)
+      continue;
     float m = -INFINITY, l = 0.f;
     f32x4 o{0, 0, 0, 0};
-    for (int s = 0; s < j.w; ++s) {
-      const float *ml = part_sums(kv, a, j.z + s, P, row);
-      const f32x4 so = *(const f32x4 *)(part_row(kv, a, j.z + s, P, row) + lane * 4);
-      const float top = fmaxf(m, ml[0]), base = base_of(top);
-      const float x = exp2_of(m - base), y = exp2_of(ml[0] - base);
-      m = top;
-      l = l * x + ml[1] * y;
-      o = o * x + so * y;
+    for (int s0 = 0; s0 < j.w; s0 += AT_ONCE) {
+      f32x4 so[AT_ONCE];
+      float sm[AT_ONCE], sl[AT_ONCE];
+#pragma unroll
+      for (int x = 0; x < AT_ONCE; ++x) {
+        const int s = j.z + min(s0 + x, j.w - 1);
+        const float *ml = part_sums(kv, a, s, P, row);
+        so[x] = *(const f32x4 *)(part_row(kv, a, s, P, row) + lane * 4);
+        sm[x] = ml[0];
+        sl[x] = ml[1];
+      }
+#pragma unroll
+      for (int x = 0; x < AT_ONCE; ++x) {
+        if (s0 + x >= j.w) break;
+        const float top = fmaxf(m, sm[x]), base = base_of(top);
+        const float f = exp2_of(m - base), y = exp2_of(sm[x] - base);
+        m = top;
+        l = l * f + sl[x] * y;
+        o = o * f + so[x] * y;
+      }
     }
     const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
     const float x[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
     const int tok = row / P.heads;
-    store_out(a, kv.dtype, (int64_t)(j.x + tok) * a.out_token + (P.h0 + row - tok * P.heads) * a.out_head +
-                               lane * 4, x);
+    store_out(a, kv.dtype, (int64_t)(j.x + tok) * a.out_token +
+                               (P.h0 + row - tok * P.heads) * a.out_head + lane * 4, x);
   }
 }
 
@@ -881,8 +897,11 @@ void launch_dim(const KvCache &kv, const Chunk &a, uint32_t grid, hipStream_t s)
   if (kv.dtype == DT_F32) chunk_f32_kernel<D, F32><<<grid, 64 * F32, 0, s>>>(kv, a);
   else if (kv.dtype == DT_BF16) chunk_kernel<D, __bf16><<<grid, kThreads, 0, s>>>(kv, a);
   else chunk_kernel<D, _Float16><<<grid, kThreads, 0, s>>>(kv, a);
-  const uint32_t joins = (uint32_t)(kv.heads * a.shape.tiles * a.shape.joins);
-  if (joins) chunk_join_kernel<D><<<joins, kThreads, 0, s>>>(kv, a);
+  constexpr int GROUPS = kChunkRows / (kThreads / (D / 4));
+  const int64_t joins = kv.heads * a.shape.tiles * a.shape.joins * GROUPS;
+  if (joins)
+    chunk_join_kernel<D><<<(uint32_t)(joins < a.most_joins ? joins : a.most_joins), kThreads, 0,
+                           s>>>(kv, a);
 }
 
 }  // namespace

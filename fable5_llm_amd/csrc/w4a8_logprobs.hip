@@ -29,6 +29,12 @@ struct Logit {
   static constexpr Max none() { return -INFINITY; }
   static __device__ __forceinline__ Max of(T x) { return (float)x; }
   static __device__ __forceinline__ Max larger(Max a, Max b) { return fmaxf(a, b); }
+  // of three, a NaN none: without the steps that fmaxf takes for signalling ones
+  static __device__ __forceinline__ Max larger(Max a, Max b, Max c) {
+    float m;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(a), "v"(b), "v"(c));
+    return m;
+  }
   // x - m; 0 below nothing at all
   static __device__ __forceinline__ float less(Max x, Max m) {
     return x - (m == -INFINITY ? 0.f : m);
@@ -37,6 +43,9 @@ struct Logit {
     const uint32_t b = __float_as_uint(x + 0.f);
     return x != x ? 0u : b ^ ((int32_t)b < 0 ? 0xFFFFFFFFu : 0x80000000u);
   }
+  static __device__ __forceinline__ Max from_key(uint32_t k) {
+    return k == 0 ? NAN : __uint_as_float(k ^ ((int32_t)k < 0 ? 0x80000000u : 0xFFFFFFFFu));
+  }
 };
 template <>
 struct Logit<int32_t> {
@@ -44,11 +53,28 @@ struct Logit<int32_t> {
   static constexpr Max none() { return INT32_MIN; }
   static __device__ __forceinline__ Max of(int32_t x) { return x; }
   static __device__ __forceinline__ Max larger(Max a, Max b) { return max(a, b); }
+  static __device__ __forceinline__ Max larger(Max a, Max b, Max c) { return max(max(a, b), c); }
   static __device__ __forceinline__ float less(Max x, Max m) {
     return -(float)((uint32_t)m - (uint32_t)x);
   }
   static __device__ __forceinline__ uint32_t key(Max x) { return (uint32_t)x ^ 0x80000000u; }
+  static __device__ __forceinline__ Max from_key(uint32_t k) { return (Max)(k ^ 0x80000000u); }
 };
+
+// the largest of 64 lanes' values, in lane 63: neighbours, fours, rows' halves and
+// rows of 16, then rows one after another
+__device__ __forceinline__ uint32_t largest_of_lanes(uint32_t x) {
+#define W4A8_STEP(ctrl, rows) \
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xF, false))
+  W4A8_STEP(0xB1, 0xF);    // quad_perm [1,0,3,2]
+  W4A8_STEP(0x4E, 0xF);    // quad_perm [2,3,0,1]
+  W4A8_STEP(0x141, 0xF);   // row_half_mirror
+  W4A8_STEP(0x140, 0xF);   // row_mirror
+  W4A8_STEP(0x142, 0xA);   // row_bcast15 -> rows 1, 3
+  W4A8_STEP(0x143, 0xC);   // row_bcast31 -> rows 2, 3
+#undef W4A8_STEP
+  return x;
+}
 
 // A running maximum m with Z = sum 2^d and T = sum d 2^d, d = (x - m) scale (in
 // powers of two)
@@ -156,20 +182,44 @@ __global__ __launch_bounds__(kThreads) void logprobs_sums_kernel(Logprobs a) {
     };
     auto top = L::none();
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (in(i)) top = L::larger(top, L::of(p.x[i]));
+    for (int i = 0; i < kPer; i += 2)
+      top = L::larger(in(i) ? L::of(p.x[i]) : L::none(), in(i + 1) ? L::of(p.x[i + 1]) : L::none(),
+                      top);
     sums.raise(L::larger(sums.m, top), a.scale);
+    float Z = 0.f, S = 0.f;
+    bool done = false;
+    if constexpr (ALL && !__is_same(T, int32_t)) {
+      // one multiply-add a difference, against the scaled maximum as it is rounded;
+      // what that is off by is taken out of the sums
+      const float ref = sums.m * a.scale;
+      if (!__any(!(fabsf(ref) < 1e38f))) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const float d = in(i) ? L::less(L::of(p.x[i]), sums.m) * a.scale : -INFINITY;
-      const float e = exp2_of(d);
-      sums.Z += e;
-      sums.S += e * fmaxf(d, -3e38f);   // a logit of -infinity: 0, not 0 times that
+        for (int i = 0; i < kPer; ++i) {
+          const float d = __builtin_fmaf(L::of(p.x[i]), a.scale, -ref), e = exp2_of(d);
+          Z += e;
+          S += e * d;
+        }
+        done = !__any(S != S);              // a logit of -infinity: 0 times that
+        const float off = __builtin_fmaf(sums.m, a.scale, -ref), f = exp2_of(-off);
+        S = (S - off * Z) * f;
+        Z *= f;
+      }
     }
-    if (a.keys) {
+    if (!done) {
+      Z = S = 0.f;
 #pragma unroll
-      for (int d = 1; d < 64; d <<= 1) top = L::larger(top, __shfl_xor(top, d));
-      if (lane == 0) a.keys[r * a.blocks + b] = L::key(top);
+      for (int i = 0; i < kPer; ++i) {
+        const float d = in(i) ? L::less(L::of(p.x[i]), sums.m) * a.scale : -INFINITY;
+        const float e = exp2_of(d);
+        Z += e;
+        S += e * fmaxf(d, -3e38f);
+      }
+    }
+    sums.Z += Z;
+    sums.S += S;
+    if (a.keys) {
+      const uint32_t key = largest_of_lanes(L::key(top));
+      if (lane == 63) a.keys[r * a.blocks + b] = key;
     }
   };
   Piece<T> p{}, next{};
@@ -208,6 +258,7 @@ __device__ __forceinline__ int count(int mine) {
 template <typename F>
 __device__ __forceinline__ uint32_t reached_by(int want, F how_many) {
   uint32_t v = 0;
+#pragma unroll 1
   for (int bit = 31; bit >= 0; --bit) {
     const uint32_t to = v | 1u << bit;
     if (how_many(to) >= want) v = to;
@@ -217,18 +268,31 @@ __device__ __forceinline__ uint32_t reached_by(int want, F how_many) {
 
 // Second kernel, a workgroup per row: the splits' sums joined, the given token,
 // and the best: the k blocks, what in them is at least the last of their maxima
-// (k logits or more, mostly few more), and of those each one's rank.
+// (k logits or more, mostly few more), and of those each one's rank.  What it
+// waits for is two rounds of loads: sums, maxima and the token; the blocks.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(Logprobs a) {
   typedef Logit<T> L;
+  constexpr int kLocal = 4096, kRanked = 1024;
+  // a thread reads 16 bytes of a block, AT_ONCE of them before it looks at any
+  constexpr int V = 16 / sizeof(T), SIDE = kThreads / (kBlock / V), AT_ONCE = 4;
   __shared__ float whole[3];
-  __shared__ uint32_t keys[4096];
+  __shared__ __align__(16) uint32_t keys[kLocal];
   __shared__ uint64_t list[kList];
   __shared__ int32_t blocks[32];
+  __shared__ uint32_t smallest;
   __shared__ int listed;
   const int64_t r = blockIdx.x;
   const T *row = (const T *)a.logits + r * a.row;
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, k = a.k, nb = min(k, a.blocks);
+  const uint32_t *from = a.keys + r * a.blocks;
+  const bool local = a.blocks <= kLocal;
+  const int id = a.logp ? a.ids[r] : -1;
+  if (k > 0 && local)
+    for (int i = threadIdx.x; i < (a.blocks + 3) / 4 * 4; i += kThreads)
+      keys[i] = i < a.blocks ? from[i] : 0u;
+  T given{};
+  if (threadIdx.x == 0 && id >= 0 && id < a.vocab) given = row[id];
   if (threadIdx.x < 64) {
     Sums<T> sums;
     for (int i = lane; i < a.splits; i += 64)
@@ -242,115 +306,169 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Logprobs a) {
   __syncthreads();
   const Sums<T> sums = Sums<T>::from(whole);
   const float logZ = log2f(sums.Z);
-  auto logp = [&](T x) {
-    const float d = L::less(L::of(x), sums.m) * a.scale;
+  auto logp = [&](typename L::Max x) {
+    const float d = L::less(x, sums.m) * a.scale;
     // a row of -infinity alone: Z = 0
     return sums.Z == 0.f ? -INFINITY : (d - logZ) * 0.6931471805599453f;
   };
   if (threadIdx.x == 0) {
-    const int id = a.ids ? a.ids[r] : -1;
-    if (a.logp) {
-      if (id >= a.vocab) atomicOr(a.err, kErrToken);
-      a.logp[r] = id >= 0 && id < a.vocab ? logp(row[id]) : 0.f;
-    }
+    if (id >= a.vocab) atomicOr(a.err, kErrToken);
+    if (a.logp) a.logp[r] = id >= 0 && id < a.vocab ? logp(L::of(given)) : 0.f;
     if (a.entropy)
       a.entropy[r] = sums.Z == 0.f ? 0.f : (logZ - sums.S / sums.Z) * 0.6931471805599453f;
   }
-  if (a.k == 0) return;
+  if (k == 0) return;
 
-  // the k blocks, in the order of the row
-  const uint32_t *from = a.keys + r * a.blocks;
-  const bool local = a.blocks <= 4096;
-  if (local)
-    for (int i = threadIdx.x; i < a.blocks; i += kThreads) keys[i] = from[i];
-  __syncthreads();
-  auto key_of = [&](int i) { return local ? keys[i] : from[i]; };
-  const int k = a.k, nb = min(k, a.blocks);
+  // f(place, key, rank) of the first n of LDS's keys, in order of size and place;
+  // `padded`, a multiple of 4, of them are there
+  auto rank_keys = [&](int padded, int n, auto f) {
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const uint32_t mine = keys[i];
+      int rank = 0;
+#pragma unroll 2
+      for (int j = 0; j < padded; j += 4) {
+        const u32x4 x = *(const u32x4 *)(keys + j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) rank += (x[e] > mine) | ((x[e] == mine) & (j + e < i));
+      }
+      f(i, mine, rank);
+    }
+    __syncthreads();
+  };
+  // the k blocks, and the last one's maximum
   uint32_t least = 0;
-  if (a.blocks > k)
+  if (a.blocks <= k) {
+    if ((int)threadIdx.x < a.blocks) blocks[threadIdx.x] = threadIdx.x;
+    __syncthreads();
+  } else if (a.blocks <= kRanked) {
+    rank_keys((a.blocks + 3) / 4 * 4, a.blocks, [&](int i, uint32_t key, int rank) {
+      if (rank < k) blocks[rank] = i;
+      if (rank == k - 1) smallest = key;
+    });
+    least = smallest;
+  } else {
+    auto key_of = [&](int i) { return local ? keys[i] : from[i]; };
     least = reached_by(k, [&](uint32_t v) {
       int mine = 0;
       for (int i = threadIdx.x; i < a.blocks; i += kThreads) mine += key_of(i) >= v;
       return count(mine);
     });
-  int above = 0;
-  for (int i = threadIdx.x; i < a.blocks; i += kThreads) above += key_of(i) > least;
-  int equals = nb - count(above);          // so many of the first that equal it
-  if (a.blocks <= k) {
-    if ((int)threadIdx.x < a.blocks) blocks[threadIdx.x] = threadIdx.x;
-    __syncthreads();
-  } else if (threadIdx.x < 64) {
-    for (int base = 0, n = 0; base < a.blocks; base += 64) {
-      const int i = base + lane;
-      const uint32_t key = i < a.blocks ? key_of(i) : 0;
-      const uint64_t same = __ballot(i < a.blocks && key == least);
-      const int before = __popcll(same & ((1ull << lane) - 1));
-      const bool take = i < a.blocks && (key > least || (key == least && before < equals));
-      const uint64_t taken = __ballot(take);
-      if (take) blocks[n + __popcll(taken & ((1ull << lane) - 1))] = i;
-      n += __popcll(taken);
-      equals -= min(equals, (int)__popcll(same));
+    int above = 0;
+    for (int i = threadIdx.x; i < a.blocks; i += kThreads) above += key_of(i) > least;
+    int equals = k - count(above);         // so many of the first that equal it
+    if (threadIdx.x < 64) {
+      for (int base = 0, n = 0; base < a.blocks; base += 64) {
+        const int i = base + lane;
+        const uint32_t key = i < a.blocks ? key_of(i) : 0;
+        const uint64_t same = __ballot(i < a.blocks && key == least);
+        const int before = __popcll(same & ((1ull << lane) - 1));
+        const bool take = i < a.blocks && (key > least || (key == least && before < equals));
+        const uint64_t taken = __ballot(take);
+        if (take) blocks[n + __popcll(taken & ((1ull << lane) - 1))] = i;
+        n += __popcll(taken);
+        equals -= min(equals, (int)__popcll(same));
+      }
     }
+    __syncthreads();
   }
-  __syncthreads();
 
-  // what in them is at least v, by its key and place: every thread its own
+  // The blocks' logits as 16 bytes a thread, of SIDE blocks at once, AT_ONCE times
+  // before any is looked at: f(keys, first place).  Those of no row have key 0.
   const int shift = shift_of(row);
+  const int side = SIDE == 1 ? 0 : (int)threadIdx.x / (kBlock / V);
+  const int mine_at = ((int)threadIdx.x - side * (kBlock / V)) * V;
   auto each = [&](auto f) {
-    for (int j = 0; j < nb; ++j) {
-      const int64_t first = (int64_t)blocks[j] * kBlock - shift;
+#pragma unroll 1
+    for (int j0 = 0; j0 < nb; j0 += AT_ONCE * SIDE) {
+      u32x4 x[AT_ONCE];
+      int64_t at[AT_ONCE];
 #pragma unroll
-      for (int i = 0; i < kBlock / kThreads; ++i) {
-        const int64_t at = first + i * kThreads + threadIdx.x;
-        if (at >= 0 && at < a.vocab) f(L::key(L::of(row[at])), (uint32_t)at);
+      for (int j = 0; j < AT_ONCE; ++j) {
+        const int b = j0 + j * SIDE + side;
+        at[j] = b < nb ? (int64_t)blocks[b] * kBlock - shift + mine_at : a.vocab;
+        // what lies beside a row's ends in its 16 bytes is read one by one below
+        const bool whole = at[j] >= 0 && at[j] + V <= a.vocab;
+        x[j] = whole ? *(const u32x4 *)(row + at[j]) : u32x4{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) {
+        struct Vec { T e[V]; };
+        Vec v = __builtin_bit_cast(Vec, x[j]);
+        const bool whole = at[j] >= 0 && at[j] + V <= a.vocab;
+        uint32_t key[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) key[e] = whole ? L::key(L::of(v.e[e])) : 0u;
+        if (!whole && at[j] < a.vocab) {
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (at[j] + e >= 0 && at[j] + e < a.vocab) key[e] = L::key(L::of(row[at[j] + e]));
+        }
+        f(key, at[j]);
       }
     }
-  };
-  auto list_up = [&](uint32_t v, uint32_t last) {     // those of v itself up to place last
-    each([&](uint32_t key, uint32_t at) {
-      if (key > v || (key == v && at <= last)) {
-        const int n = atomicAdd(&listed, 1);
-        if (n < kList) list[n] = (uint64_t)key << 32 | (uint32_t)~at;
-      }
-    });
-    __syncthreads();
   };
   if (a.blocks <= k && a.vocab > kList) {
     // no block was left out: the k-th of the threads' maxima
     uint32_t top = 0;
-    each([&](uint32_t key, uint32_t) { top = max(top, key); });
-    least = reached_by(k, [&](uint32_t v) { return count(top >= v); });
-  }
-  list_up(least, 0xFFFFFFFFu);
-  if (listed > kList) {
-    // many at least as large: the k-th largest, and which of its equals count
-    const uint32_t kth = reached_by(k, [&](uint32_t v) {
-      int mine = 0;
-      each([&](uint32_t key, uint32_t) { mine += key >= v; });
-      return count(mine);
+#pragma unroll 1
+    for (int64_t i = threadIdx.x; i < a.vocab; i += kThreads) top = max(top, L::key(L::of(row[i])));
+    keys[threadIdx.x] = top;
+    __syncthreads();
+    rank_keys(kThreads, kThreads, [&](int, uint32_t key, int rank) {
+      if (rank == k - 1) smallest = key;
     });
-    int more = 0;
-    each([&](uint32_t key, uint32_t) { more += key > kth; });
-    const int rest = k - count(more);
+    least = smallest;
+  }
+  auto put = [&](uint32_t key, int64_t at) {
+    const int n = atomicAdd(&listed, 1);
+    if (n < kList) list[n] = (uint64_t)key << 32 | (uint32_t)~(uint32_t)at;
+  };
+  each([&](const uint32_t *key, int64_t at) {
+    uint32_t top = key[0];
+#pragma unroll
+    for (int e = 1; e < V; ++e) top = max(top, key[e]);
+    if (top < least) return;
+    for (int e = 0; e < V; ++e)
+      if (at + e >= 0 && at + e < a.vocab && key[e] >= least) put(key[e], at + e);
+  });
+  __syncthreads();
+  if (listed > kList) {
+    // many at least as large: the k-th largest, and which of its equals count;
+    // rarely needed, and kept short
+    auto all = [&](auto f) {
+      int mine = 0;
+#pragma unroll 1
+      for (int j = 0; j < nb * (kBlock / kThreads); ++j) {
+        const int64_t at = (int64_t)blocks[j / (kBlock / kThreads)] * kBlock - shift +
+                           j % (kBlock / kThreads) * kThreads + threadIdx.x;
+        if (at >= 0 && at < a.vocab) mine += f(L::key(L::of(row[at])), at);
+      }
+      return count(mine);
+    };
+    const uint32_t kth = reached_by(k, [&](uint32_t v) {
+      return all([&](uint32_t key, int64_t) { return key >= v; });
+    });
+    const int rest = k - all([&](uint32_t key, int64_t) { return key > kth; });
     // the place of the rest-th of them: not below the last whose earlier are fewer
     const uint32_t first = ~reached_by(rest, [&](uint32_t v) {
-      int mine = 0;
-      each([&](uint32_t key, uint32_t at) { mine += key == kth && ~at >= v; });
-      return count(mine);
+      return all([&](uint32_t key, int64_t at) { return key == kth && ~(uint32_t)at >= v; });
     });
     if (threadIdx.x == 0) listed = 0;
     __syncthreads();
-    list_up(kth, first);
+    all([&](uint32_t key, int64_t at) {
+      if (key > kth || (key == kth && (uint32_t)at <= first)) put(key, at);
+      return 0;
+    });
   }
   const int n = min(listed, kList);
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const uint64_t mine = list[i];
     int rank = 0;
+#pragma unroll 4
     for (int j = 0; j < n; ++j) rank += list[j] > mine;
     if (rank < k) {
-      const uint32_t at = ~(uint32_t)mine;
-      a.top_ids[r * k + rank] = (int32_t)at;
-      a.top_logp[r * k + rank] = logp(row[at]);
+      a.top_ids[r * k + rank] = (int32_t)~(uint32_t)mine;
+      a.top_logp[r * k + rank] = logp(L::from_key((uint32_t)(mine >> 32)));
     }
   }
 }
@@ -368,7 +486,7 @@ void launch_typed(const Logprobs &a, hipStream_t s) {
 int logprobs_blocks(int64_t vocab) { return (int)((vocab + 7 + kBlock - 1) / kBlock); }
 int logprobs_splits(int64_t rows, int64_t vocab, int num_cu) {
   const int64_t blocks = logprobs_blocks(vocab), most = (blocks + kWaves - 1) / kWaves;
-  const int64_t want = (8ll * num_cu + rows - 1) / rows;
+  const int64_t want = (16ll * num_cu + rows - 1) / rows;
   return (int)(want < most ? want : most);
 }
 int64_t logprobs_workspace(int64_t rows, int64_t vocab, int num_cu) {

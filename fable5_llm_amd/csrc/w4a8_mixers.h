@@ -126,6 +126,7 @@ struct Chunk {
   float *part;                      // [parts][kv heads][head tiles][rows of a unit][dim], then
                                     // {max, sum} of each row
   int32_t tokens, hq, layer, dtype;
+  int32_t most_joins;               // workgroups of the second kernel, at most
   ChunkShape shape;
   float scale;                      // of the scores, log2(e) included
   float out_unit;                   // DT_I16: 1 / the value of one step of out
