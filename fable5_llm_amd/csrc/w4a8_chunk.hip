@@ -179,13 +179,15 @@ __global__ __launch_bounds__(256) void kv_map_rows_kernel(KvCache kv, KvMap m) {
   const int tok = tile * tokens, ntok = min(tokens, r.count - tok);
   int32_t *u = m.plan + kPlanHead + (int64_t)kUnitWords * i;
   int pos0 = 0, k0 = 0, k1 = 0, slot = -1;
+  bool none = false;                        // a part behind the tile's last key
   if (r.seq >= 0) {
     pos0 = r.len - r.count + tok;
     const int end = pos0 + ntok, per = ((end + n - 1) / n + 63) / 64 * 64;
     const int used = (int)(((int64_t)end + per - 1) / per);
     const int64_t from = (int64_t)part * per;
-    k0 = (int)(from < end ? from : end);
-    k1 = (int)(from + per < end ? from + per : end);
+    none = from >= end;
+    k0 = none ? 0 : (int)from;
+    k1 = none ? 0 : (int)(from + per < end ? from + per : end);
     if (used > 1) slot = at[2] + j * n + part;
     if (n > 1 && part == 0) {
       int32_t *join = m.plan + kPlanHead + kUnitWords * m.shape.units +
@@ -193,7 +195,7 @@ __global__ __launch_bounds__(256) void kv_map_rows_kernel(KvCache kv, KvMap m) {
       join[0] = m.cu[row] + tok, join[1] = ntok, join[2] = at[2] + j * n, join[3] = used;
     }
   }
-  u[0] = r.seq, u[1] = m.cu[row] + tok, u[2] = ntok, u[3] = pos0;
+  u[0] = r.seq, u[1] = m.cu[row] + tok, u[2] = none ? 0 : ntok, u[3] = pos0;
   u[4] = k0, u[5] = k1, u[6] = slot, u[7] = 0;
 }
 
@@ -224,7 +226,7 @@ __device__ __forceinline__ Unit unit_of(const KvCache &kv, const Chunk &a, int64
          __builtin_amdgcn_readfirstlane(y.z)};
   const int64_t most = (int64_t)kv.max_pages << kv.lg_page;
   if (u.seq >= kv.seqs || u.tok < 0 || u.ntok < 0 || u.ntok > a.shape.tokens ||
-      (int64_t)u.tok + u.ntok > a.tokens || u.pos0 < 0 || u.k0 < 0 || u.k1 < u.k0 ||
+      (int64_t)u.tok + u.ntok > a.tokens || u.pos0 < 0 || u.k0 < 0 || (u.k1 > 0 && u.k1 <= u.k0) ||
       u.k1 > most || (int64_t)u.pos0 + u.ntok > most || (u.seq < 0 && u.k1 > 0) ||
       (u.k0 & 63) || u.slot >= a.shape.parts) {
     if (threadIdx.x == 0) atomicOr(kv.err, kErrKvRange);
@@ -452,7 +454,6 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(KvCache kv, Chunk a)
   const Unit u = unit_of(kv, a, P.unit);
   if (u.ntok == 0) return;
   if (u.k1 == 0) return zeros(kv, a, u, P);
-  if (u.k0 >= u.k1) return;
   const int lane = threadIdx.x & 63, r = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Tn turns(kv, u, a.layer, P.kvh, wave);
@@ -665,7 +666,6 @@ __global__ __launch_bounds__(64 * NW, 2) void chunk_f32_kernel(KvCache kv, Chunk
   const Unit u = unit_of(kv, a, P.unit);
   if (u.ntok == 0) return;
   if (u.k1 == 0) return zeros(kv, a, u, P);
-  if (u.k0 >= u.k1) return;
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Tn turns(kv, u, a.layer, P.kvh, wave);
