@@ -101,6 +101,7 @@ struct ChunkShape {
   int32_t heads;                    // query heads of a unit, of one key-value head
   int32_t tiles;                    // head tiles of a key-value head
   int32_t tokens;                   // tokens of a unit
+  int32_t least;                    // keys of a part, at least
   int64_t split;                    // units of a full chip, see chunk_shape
   int64_t units, joins, parts;      // at most
 };
