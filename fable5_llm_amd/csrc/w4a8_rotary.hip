@@ -26,14 +26,25 @@ struct Unit<int16_t> {
   }
 };
 
+// eight elements as they lie in memory, and as numbers
 template <typename T>
-__device__ __forceinline__ void load8(float *x, const void *p, int64_t at, float unit) {
-  alignas(16) T v[8];
+struct Raw {
+  u32x4 w[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ Raw<T> load8(const void *p, int64_t at) {
+  Raw<T> r;
 #pragma unroll
-  for (int i = 0; i < (int)sizeof(v) / 16; ++i)
-    ((u32x4 *)v)[i] = ((const u32x4 *)((const T *)p + at))[i];
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+    r.w[i] = load16_nt((const u32x4 *)((const T *)p + at) + i);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void numbers(float *x, const Raw<T> &r, float unit) {
+  struct Eight { T v[8]; };
+  const Eight e = __builtin_bit_cast(Eight, r);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = Unit<T>::in(v[i], unit);
+  for (int i = 0; i < 8; ++i) x[i] = Unit<T>::in(e.v[i], unit);
 }
 template <typename T>
 __device__ __forceinline__ void store8(void *p, int64_t at, const float *x, float per) {
@@ -78,7 +89,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(KvCache kv, Rotary a) 
   const bool here = lane * 16 < a.dim, rotated = lane * 16 < a.rot;
   const bool split = rotated && !a.pairs;
   const int at0 = split ? 8 * lane : 16 * lane, at1 = split ? a.rot / 2 + 8 * lane : at0 + 8;
-  float x[U][16];
+  Raw<IN> raw[U][2];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int h = h0 + u;
@@ -89,11 +100,10 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(KvCache kv, Rotary a) 
           q ? token * a.q_token + h * a.q_head
             : k ? token * a.k_token + (h - a.hq) * a.k_head
                 : token * a.v_token + (h - a.hq - a.hk) * a.v_head;
-      load8<IN>(x[u], src, at + at0, a.unit);
-      load8<IN>(x[u] + 8, src, at + at1, a.unit);
+      raw[u][0] = load8<IN>(src, at + at0);
+      raw[u][1] = load8<IN>(src, at + at1);
     } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[u][i] = 0.f;
+      raw[u][0] = raw[u][1] = Raw<IN>{};
     }
   }
   const int pos = a.pos[token];
@@ -122,27 +132,30 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(KvCache kv, Rotary a) 
     const int h = h0 + u;
     if (u >= heads) break;
     const bool q = h < a.hq, k = h < a.hq + a.hk;
+    float x[16];
+    numbers(x, raw[u][0], a.unit);
+    numbers(x + 8, raw[u][1], a.unit);
     const float *w = q ? a.q_norm : k ? a.k_norm : nullptr;
     if (w) {
       float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sum += x[u][i] * x[u][i];
+      for (int i = 0; i < 16; ++i) sum += x[i] * x[i];
       for (int d = 1; d < lanes; d <<= 1) sum += __shfl_xor(sum, d);
       const float inv = 1.f / sqrtf(sum * a.per_dim + a.eps);
       if (here) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          x[u][i] *= inv * w[at0 + i];
-          x[u][8 + i] *= inv * w[at1 + i];
+          x[i] *= inv * w[at0 + i];
+          x[8 + i] *= inv * w[at1 + i];
         }
       }
     }
     if (!here) continue;
     if (k && rotated) {
       auto turn = [&](int i, int ia, int ib) {
-        const float p = x[u][ia], r = x[u][ib];
-        x[u][ia] = p * c[i] - r * s[i];
-        x[u][ib] = r * c[i] + p * s[i];
+        const float p = x[ia], r = x[ib];
+        x[ia] = p * c[i] - r * s[i];
+        x[ib] = r * c[i] + p * s[i];
       };
       if (a.pairs) {
 #pragma unroll
@@ -156,16 +169,16 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(KvCache kv, Rotary a) 
       void *dst = q ? a.q_out : a.k_out;
       const int64_t at = q ? token * a.q_out_token + h * a.q_out_head
                            : token * a.k_out_token + (h - a.hq) * a.k_out_head;
-      store8<OUT>(dst, at + at0, x[u], a.out_per);
-      store8<OUT>(dst, at + at1, x[u] + 8, a.out_per);
+      store8<OUT>(dst, at + at0, x, a.out_per);
+      store8<OUT>(dst, at + at1, x + 8, a.out_per);
     } else {
       const int which = k ? 0 : 1, kh = h - a.hq - (k ? 0 : a.hk);
       uint8_t *base = kv.pool + (slot >> kv.lg_page) * kv.page_bytes;
       const int64_t at =
           ((((int64_t)a.layer * 2 + which) * kv.heads + kh) * kv.page() + (slot & (kv.page() - 1))) *
           kv.dim;
-      store8<OUT>(base, at + at0, x[u], 1.f);
-      store8<OUT>(base, at + at1, x[u] + 8, 1.f);
+      store8<OUT>(base, at + at0, x, 1.f);
+      store8<OUT>(base, at + at1, x + 8, 1.f);
     }
   }
 }
@@ -177,7 +190,7 @@ void launch_typed(const KvCache &kv, const Rotary &a, int num_cu, hipStream_t s)
   auto blocks = [&](int u) {
     return (uint32_t)(((int64_t)a.tokens * ((all + u - 1) / u) + each - 1) / each);
   };
-  if (items > few) rotary_kernel<IN, OUT, 4><<<blocks(4), kThreads, 0, s>>>(kv, a);
+  if (items > few) rotary_kernel<IN, OUT, 6><<<blocks(6), kThreads, 0, s>>>(kv, a);
   else rotary_kernel<IN, OUT, 1><<<blocks(1), kThreads, 0, s>>>(kv, a);
 }
 
