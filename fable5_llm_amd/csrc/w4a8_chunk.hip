@@ -183,7 +183,7 @@ __global__ __launch_bounds__(kOne) void kv_map_kernel(KvCache kv, KvMap m) {
   if (row < m.rows) r = map_row(kv, m, row);
   if (r.bad && blockIdx.x == 0) atomicOr(kv.err, kErrKvRange);
   int64_t sum = r.count;
-  int64_t work = (int64_t)((r.count + m.shape.tokens - 1) / m.shape.tokens) * r.len;
+  int64_t work = ((int64_t)r.count + m.shape.tokens - 1) / m.shape.tokens * r.len;
   sum_all(sum, work);
   const bool fits = sum <= m.tokens && !stopped;
   if (row == 0 && blockIdx.x == 0 && sum > m.tokens) atomicOr(kv.err, kErrKvRange);
@@ -225,7 +225,7 @@ __global__ __launch_bounds__(kOne) void kv_map_rows_kernel(KvCache kv, KvMap m) 
     const MapRow r = map_row(kv, m, i);
     sum += r.count;
     bad |= r.bad;
-    work += (int64_t)((r.count + m.shape.tokens - 1) / m.shape.tokens) * r.len;
+    work += ((int64_t)r.count + m.shape.tokens - 1) / m.shape.tokens * r.len;
   }
   sum_all(sum, work);
   if (bad) atomicOr(kv.err, kErrKvRange);

@@ -461,6 +461,11 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Logprobs a) {
     });
   }
   const int n = min(listed, kList);
+  // only a row of NaNs has fewer: any indices
+  for (int i = n + threadIdx.x; i < k; i += kThreads) {
+    a.top_ids[r * k + i] = i;
+    a.top_logp[r * k + i] = NAN;
+  }
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const uint64_t mine = list[i];
     int rank = 0;

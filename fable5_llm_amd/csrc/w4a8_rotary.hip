@@ -111,7 +111,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(KvCache kv, Rotary a) 
   if (a.slots) {
     const bool stopped = kv_stopped(kv);
     slot = a.slots[token];
-    if (slot >= (int64_t)kv.pages << kv.lg_page) {
+    if (pos >= 0 && slot >= (int64_t)kv.pages << kv.lg_page) {
       if (lane == 0) atomicOr(kv.err, kErrKvRange);
       slot = -1;
     }

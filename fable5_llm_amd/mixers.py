@@ -379,7 +379,10 @@ def rotary_args(ctx, q, k, v, pos, slots, freq, q_out, k_out, layout, amplitude,
             raise ValueError(f"q: must be {ctype}, as the cache, or int16")
         if dim != cdim:
             raise ValueError(f"q: has heads of {dim}, the cache of {cdim}")
-    out_type = cache[2] if cache else (q_out if q is not None else k_out).dtype
+    if not cache:
+        y, name = (q_out, "q_out") if q is not None else (k_out, "k_out")
+        _on(y, ctx, name)
+    out_type = cache[2] if cache else y.dtype
     if dts.get(out_type) is None or (out_type != dtype and dt != N.DT_I16):
         raise ValueError(f"out: must be {dtype}, as q and k")
     qh, qp, q0, q1, qo, qo0, qo1 = (0,) * 7

@@ -98,6 +98,18 @@ def test_sizes(engine, dtype, rows, vocab, k):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [1024 * 1024 - 3, 1100003, 4200001])
+def test_more_blocks_than_are_ranked_at_once(engine, dtype, vocab):
+    # over 1,024 blocks of 1,024 logits, and over 4,096; among 7 values in a
+    # second row, so that blocks' maxima are equal everywhere
+    gen = torch.Generator().manual_seed(vocab)
+    x = logits(gen, 2, vocab, dtype)
+    x[1] = torch.randint(0, 7, (vocab,), generator=gen).to(DEV).to(dtype)
+    for k in (1, 32):
+        check(engine, x, ints([vocab - 1, 5]), k, 1e-6 if dtype == torch.int32 else 1.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_rows_at_any_place(engine, dtype):
     # rows that begin at every element of 16 bytes, apart by odd strides
     gen = torch.Generator().manual_seed(4)
@@ -169,6 +181,15 @@ def test_a_row_without_numbers_spoils_no_other(engine, dtype, bad):
         assert torch.equal(g[::2], w[::2])
     assert torch.isnan(got[1][1]) and not torch.isfinite(got[2][1]).any()
     assert ((got[3][1] >= 0) & (got[3][1] < 9000)).all() and not torch.isfinite(got[0][1])
+
+
+@pytest.mark.parametrize("vocab", [40, 5000, 70000])
+def test_a_row_of_nans_has_indices(engine, vocab):
+    x = torch.full((2, vocab), math.nan, device=DEV)
+    x[1, 3] = 1.0
+    logp, ent, tl, ti = run(engine, x, ints([0, 3]), 32)
+    assert torch.isnan(logp).all() and torch.isnan(ent).all() and torch.isnan(tl).all()
+    assert ((ti >= 0) & (ti < vocab)).all()
 
 
 def test_extremes(engine):

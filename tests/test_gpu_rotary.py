@@ -242,7 +242,8 @@ def test_wrong_tensors(engine):
     norm = torch.ones(64, device=DEV)
     f(q[:0], None, pos[:0], freq, q[:0], None)
     for call in (lambda: f(q.cpu(), k, pos, freq, q, k), lambda: f(None, None, pos, freq, None, None),
-                 lambda: f(q, k, pos[:2], freq, q, k), lambda: f(q, k, pos.long(), freq, q, k),
+                 lambda: f(q, k, pos, freq, None, k), lambda: f(None, k, pos, freq, None, None),
+                 lambda: f(q, k, pos, freq, q, None), lambda: f(q, k, pos[:2], freq, q, k), lambda: f(q, k, pos.long(), freq, q, k),
                  lambda: f(q, k, pos, freq.float(), q, k), lambda: f(q, k, pos, freq[:7], q, k),
                  lambda: f(q, k, pos, frequencies(80)[0], q, k),
                  lambda: f(q, k.half(), pos, freq, q, k.half()),
