@@ -6,8 +6,10 @@ hand-written HIP kernels for gfx950 behind the C ABI of
 include/fable5_w4a8.h.
 
   engine        Context / Weights handle API (host and device buffers)
-  mixers        PagedKV: attention over a paged key-value cache and the cache's
-                pages; the gated delta rule's arguments (Context.delta_*)
+  mixers        PagedKV: attention over a paged key-value cache, of single
+                tokens and of prompts' chunks, and the cache's pages; rotary
+                positions, log probabilities and the gated delta rule's arguments
+                (Context.rotary_async, logprobs_async, delta_*)
   w4a8_ref      matvec_y32, rshift_round, row image packing (reference names)
   fixedpoint    dyn_quant_i8
   layer_fixed   matvec_fx, matvec_to, rmsnorm_fx, mlp_fx, MOVY/ALU ops, head

@@ -12,7 +12,9 @@ namespace w4a8 {
 namespace {
 
 // ---------------------------------------------------------------------- maps
-constexpr int kOne = 1024;        // threads of the single-workgroup kernel
+// What a map writes is a word or two a token; it costs its launch and a chain of
+// dependent loads: a row's words, its length, and its tokens' table entries.
+constexpr int kOne = 1024;        // threads of a workgroup that takes in all rows
 
 // exclusive scans of N values per thread of a kOne-thread workgroup, and their
 // totals; every thread of it calls
@@ -175,8 +177,12 @@ __device__ __forceinline__ void put_head(const KvMap &m, int units, int joins, b
 // Rows of a step whose units are put in order: 3,001 tokens of 13 rows 149 -> 131
 // us, 2,000 of 20 rows 103 -> 83.  Many rows' lie mixed as they come.
 constexpr int kSorted = 128;
+
 // Steps of up to kOne rows in one launch: every workgroup takes in all rows, a
-// thread each, and then writes kOne tokens and units of its own.
+// thread each, and then writes kOne tokens and units of its own.  61 rows of a token
+// 8.7 us (7.5 under the profiler, of which an empty kernel is 4.4), 300 rows of up
+// to 40 9.7; one workgroup for the rows and a second launch for the tokens took
+// 11.6 and 14.6.
 __global__ __launch_bounds__(kOne) void kv_map_kernel(KvCache kv, KvMap m) {
   __shared__ int32_t at[6][kOne + 1];       // where a row's tokens, units, joins, parts begin,
                                             // its parts, its units' place in the plan
@@ -326,9 +332,9 @@ __device__ __forceinline__ Unit unit_of(const KvCache &kv, const Chunk &a, int64
   }
   const int64_t most = (int64_t)kv.max_pages << kv.lg_page;
   if (u.seq >= kv.seqs || u.tok < 0 || u.ntok < 0 || u.ntok > a.shape.tokens ||
-      (int64_t)u.tok + u.ntok > a.tokens || u.pos0 < 0 || u.k0 < 0 || (u.k1 > 0 && u.k1 <= u.k0) ||
-      u.k1 > most || (int64_t)u.pos0 + u.ntok > most || (u.seq < 0 && u.k1 > 0) ||
-      (u.k0 & 63) || u.slot >= a.shape.parts) {
+      (int64_t)u.tok + u.ntok > a.tokens || u.pos0 < 0 || u.k0 < 0 || u.k1 < 0 ||
+      (u.k1 > 0 && u.k1 <= u.k0) || u.k1 > most || (int64_t)u.pos0 + u.ntok > most ||
+      (u.seq < 0 && u.k1 > 0) || (u.k0 & 63) || u.slot >= a.shape.parts) {
     if (threadIdx.x == 0) atomicOr(kv.err, kErrKvRange);
     u.ntok = 0;
   }
@@ -542,7 +548,23 @@ __device__ __forceinline__ float *part_sums(const KvCache &kv, const Chunk &a, i
          ((slot * per + p.part) * kChunkRows + row) * 2;
 }
 
-// Keys and values of 16 bits.
+// Keys and values of 16 bits, on 32 x 32 x 16 matrix instructions: a wavefront has
+// 32 of the unit's rows.  S^T = K q^T leaves 16 keys of one query in a lane, which
+// are, rounded once to the cache's type, the B operand of o^T = V^T p^T as they
+// are: no weight passes through LDS, and a query's maximum and sum are a lane's own
+// and its partner's.  V is read by columns from where it lies by rows.  Keys and
+// values of the next turn are copied to LDS while this one is worked on; a turn's 32
+// or 64 keys serve 128 rows, so that LDS is read once for 128 operations a byte.
+//
+// Bound by the matrix units and the clock that their power leaves them: 8,192
+// tokens of a prompt, 16 query heads of 256, 549 us, 1.0 PFLOP/s (a large product
+// reaches 1.17); without conflicts in LDS, at 2.1 of 2.4 GHz.  Turns whose products
+// begin before the last turn's weights are done gain nothing there.  Short calls
+// wait: 17 tokens over 511 keys, 12.5 us, of which 2 before the first turn, 1.1 a
+// turn and 2.6 for the parts' stores.
+//
+// At D = 256 (s - m) scale takes two operations, elsewhere one multiply-add and the
+// branch for far maxima: that branch's registers do not fit beside 128 of out.
 template <int D, typename T>
 __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(KvCache kv, Chunk a) {
   typedef Turns<D, T, kWaves> Tn;
@@ -762,7 +784,10 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(KvCache kv, Chunk a)
 
 // Keys and values of 32 bits, on the float32 matrix instructions: 16 keys by 16
 // queries, a wavefront's queries as C columns of tiles, so that q and out stay
-// in 128 registers.
+// in 128 registers.  Weights stay in 32 bits.  At the float32 matrix rate, an eighth
+// of the 16-bit one, this is bound by the matrix units once the chip is full: 1,000
+// tokens of five rows over up to 2,000 keys, 8 heads of 64, 27 us of 6 at that rate
+// (few units of uneven length), and 8.5 for the join.
 template <int D, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void chunk_f32_kernel(KvCache kv, Chunk a) {
   typedef Turns<D, float, NW> Tn;
@@ -960,7 +985,8 @@ __global__ __launch_bounds__(64 * NW, 2) void chunk_f32_kernel(KvCache kv, Chunk
 // The parts of a tile joined: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
 // A thread takes four elements of a row; a workgroup ROWS rows and FOURS such fours
 // of them (128 bytes of a part, 64 of out side by side), one tile's after another,
-// so that few are launched where nothing was split.
+// so that few are launched where nothing was split.  Bound by its reads: 21 us behind
+// 100 tokens over 131,072 keys, 4 where there is little (2.6 where nothing is).
 template <int D>
 struct JoinShape {
   static constexpr int FOURS = D / 4 < 32 ? D / 4 : 32, ROWS = kThreads / FOURS;
@@ -1042,6 +1068,10 @@ ChunkShape chunk_shape(const KvCache &kv, int64_t rows, int64_t tokens, int64_t 
   c.tokens = kChunkRows / c.heads;
   const int64_t per = (int64_t)kv.heads * c.tiles, most = rows < tokens ? rows : tokens;
   const int64_t tiles = tokens / c.tokens + most;
+  // Two units a compute unit, as its LDS holds: 100 tokens over 131,072 keys 292 us
+  // (one 360), 1,000 float32 tokens of five rows 35 (one 42), 700 of three over up
+  // to 9,000 keys 55 (four 65, one 49), 64 of two over up to 60,000 of 64 elements
+  // 56 (four 81, one 50)
   c.split = (2ll * num_cu + per - 1) / per;
   // two turns of the kernels: 17 tokens over 511 keys of 256 bfloat16 16.1 us in
   // parts of 128 keys, 15.2 in parts of 64; five rows of float32 keys of 64 35, 43

@@ -1,6 +1,8 @@
 // Declarations of the mixers between a step's sites: attention over a paged
-// key-value cache (w4a8_attend.hip), the cache's pages (w4a8_kv.hip) and the
-// gated delta rule (w4a8_delta.hip), shared with the C ABI (w4a8_abi.hip).
+// key-value cache (w4a8_attend.hip; of several new tokens a sequence, w4a8_chunk.hip),
+// the cache's pages (w4a8_kv.hip), rotary positions (w4a8_rotary.hip), what logits say
+// (w4a8_logprobs.hip) and the gated delta rule (w4a8_delta.hip), shared with the C ABI
+// (w4a8_abi.hip).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>

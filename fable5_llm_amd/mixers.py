@@ -1,6 +1,8 @@
 """The mixers between a step's sites, on device tensors: attention over a
-paged key-value cache with the cache's pages (PagedKV), and the gated delta
-rule (the delta_* methods of engine.Context).
+paged key-value cache with the cache's pages, for single tokens and for several
+of each sequence (PagedKV); rotary positions, log probabilities and the gated
+delta rule (rotary_async, logprobs_async and the delta_* methods of
+engine.Context).
 
 Everything is enqueued on the context's stream and nothing waits.  Lists
 (sequences, positions, pages, slots) are int32 device tensors, a negative
