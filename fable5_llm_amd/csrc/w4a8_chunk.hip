@@ -175,7 +175,8 @@ __device__ __forceinline__ void put_head(const KvMap &m, int units, int joins, b
 }
 
 // Rows of a step whose units are put in order: 3,001 tokens of 13 rows 149 -> 131
-// us, 2,000 of 20 rows 103 -> 83.  Many rows' lie mixed as they come.
+// us, 2,000 of 20 rows 103 -> 83, a layer, for 1.5 us of the map (eight rows' sizes at a
+// time; one after another 10).  Many rows' lie mixed as they come.
 constexpr int kSorted = 128;
 
 // Steps of up to kOne rows in one launch: every workgroup takes in all rows, a
@@ -206,7 +207,7 @@ __global__ __launch_bounds__(kOne) void kv_map_kernel(KvCache kv, KvMap m) {
   for (int i = 0; i < 4; ++i) at[i][row] = p.add[i];
   at[4][row] = p.parts;
   at[5][row] = p.add[1];
-  if (m.rows <= kSorted && all[1] > m.shape.split) {
+  if (m.rows > 1 && m.rows <= kSorted && all[1] > m.shape.split) {
     // more units than the chip takes at once: the rows with the longest ones first,
     // in every workgroup the same way
     __shared__ int2 size[kSorted];          // keys of a unit, at most; units
@@ -215,10 +216,13 @@ __global__ __launch_bounds__(kOne) void kv_map_kernel(KvCache kv, KvMap m) {
     __syncthreads();
     if (row < m.rows) {
       int before = 0;
-#pragma unroll 8
-      for (int i = 0; i < kSorted; ++i) {
-        const int2 x = size[i];
-        before += x.x > keys || (x.x == keys && i < row) ? x.y : 0;
+      for (int at8 = 0; at8 < m.rows; at8 += 8) {       // zeros behind the last
+        int2 x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = size[at8 + i];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          before += ((x[i].x > keys) | ((x[i].x == keys) & (at8 + i < row))) ? x[i].y : 0;
       }
       at[5][row] = before;
     }
@@ -560,8 +564,8 @@ __device__ __forceinline__ float *part_sums(const KvCache &kv, const Chunk &a, i
 // tokens of a prompt, 16 query heads of 256, 549 us, 1.0 PFLOP/s (a large product
 // reaches 1.17); without conflicts in LDS, at 2.1 of 2.4 GHz.  Turns whose products
 // begin before the last turn's weights are done gain nothing there.  Short calls
-// wait: 17 tokens over 511 keys, 12.5 us, of which 2 before the first turn, 1.1 a
-// turn and 2.6 for the parts' stores.
+// wait: 17 tokens over 511 keys, 9.8 us, of which 2 before the first turn, 1.1 a turn
+// and 2.6 for the parts' stores.
 //
 // At D = 256 (s - m) scale takes two operations, elsewhere one multiply-add and the
 // branch for far maxima: that branch's registers do not fit beside 128 of out.
@@ -985,8 +989,8 @@ __global__ __launch_bounds__(64 * NW, 2) void chunk_f32_kernel(KvCache kv, Chunk
 // The parts of a tile joined: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
 // A thread takes four elements of a row; a workgroup ROWS rows and FOURS such fours
 // of them (128 bytes of a part, 64 of out side by side), one tile's after another,
-// so that few are launched where nothing was split.  Bound by its reads: 21 us behind
-// 100 tokens over 131,072 keys, 4 where there is little (2.6 where nothing is).
+// so that few are launched where nothing was split.  Bound by its reads: 10 us behind
+// 100 tokens over 131,072 keys, 5 where there is little (2.6 where nothing is).
 template <int D>
 struct JoinShape {
   static constexpr int FOURS = D / 4 < 32 ? D / 4 : 32, ROWS = kThreads / FOURS;
