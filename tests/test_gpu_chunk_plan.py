@@ -71,3 +71,20 @@ def test_units_in_order(engine, rows):
     if rows >= 65:
         q = random_q(gen, total, 16, 64, torch.bfloat16)
         check(kv, 0, q, seqs, count, run(engine, kv, 0, q, m))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=str)
+@pytest.mark.parametrize("counts,lens", [((5, 1, 3, 2), (200, 3000, 1500, 31)),
+                                         ((1, 200, 0, 3), (129, 333, 50, 4000))], ids=str)
+def test_rows_in_parts_and_in_order(engine, counts, lens, dtype):
+    # 32 units fill the chip; the long rows' parts come to more with the short rows
+    gen = torch.Generator().manual_seed(len(lens))
+    kv = make(engine, gen, list(lens), 16, 64, 16, dtype)
+    m = mapped(engine, kv, [0, 1, 2, 3], list(counts), 16)
+    plan = m.plan.view(torch.int32)
+    assert plan[0] > -(-2 * torch.cuda.get_device_properties(0).multi_processor_count // 16)
+    assert plan[1] >= 2                  # rows whose parts are joined
+    q = random_q(gen, sum(counts), 16, 64, dtype)
+    out = run(engine, kv, 0, q, m)
+    check(kv, 0, q, [0, 1, 2, 3], counts, out)
+    assert torch.equal(out, run(engine, kv, 0, q, m))
