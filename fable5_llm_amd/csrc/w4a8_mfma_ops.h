@@ -36,12 +36,12 @@ __device__ __forceinline__ u32x2 lds_columns(const void *p) {
 }
 
 // 16 bytes a lane from memory (a uniform address and a lane's offset) into LDS
-// at a uniform address and 16 bytes a lane from there (M0, which no other
-// instruction of these kernels uses).  The compiler does not
+// at a uniform address and 16 bytes a lane from there (M0: one wait state between its
+// write and the copy, which nothing else puts there).  The compiler does not
 // count them: a wait for them comes before the barrier that their readers wait at.
 __device__ __forceinline__ void copy16(const void *base, uint32_t offset, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1"
-               :: "v"(offset), "s"(base), "s"(lds) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :: "v"(offset), "s"(base), "s"(lds) : "memory", "m0");
 }
 
 }  // namespace w4a8

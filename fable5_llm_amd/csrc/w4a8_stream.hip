@@ -139,9 +139,10 @@ __device__ __forceinline__ int lane_now() {
 __device__ __forceinline__ void wait_vm_all() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // lane l copies 16 bytes from src (its own address, agent-coherent) to LDS
-// lds_base + 16 * l; lds_base must be uniform
+// lds_base + 16 * l; lds_base must be uniform.  One wait state between the write of
+// M0 and the copy, which the compiler does not put into an asm string.
 __device__ __forceinline__ void copy16_sc1(const void *src, uint32_t lds_base) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off sc1"
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off sc1"
                :: "v"(src), "s"(lds_base) : "memory", "m0");
 }
 
