@@ -481,7 +481,9 @@ __device__ __forceinline__ void turn_barrier() {
 // Infinities and NaNs among a masked turn's values: 0 times one would reach the
 // queries that do not see it, and what lies behind a sequence's end may be
 // anything.  give(key): adds such values of a key that a query sees to its
-// output; then they are taken out.  Every wavefront calls.
+// output; then they are taken out.  Every wavefront calls.  That comes before the
+// turn's maximum, so an infinity may be all that a query's output holds while its
+// maximum is -infinity, and its factor there is 1 and not 0.
 template <typename T, typename Tn, int NW, typename Give>
 __device__ __forceinline__ void take_out_odd(uint8_t *values, int *flag, Give give) {
   constexpr uint32_t E = sizeof(T) == 4 ? 0x7F800000u : __is_same(T, _Float16) ? 0x7C00u : 0x7F80u;
@@ -507,6 +509,24 @@ __device__ __forceinline__ void take_out_odd(uint8_t *values, int *flag, Give gi
   }
   if (threadIdx.x == 0) *flag = 0;
   __syncthreads();
+}
+
+// Outputs times a factor f >= 0, a power of two; where 32 bits hold none so small and
+// f is 0, an infinity stays one and all else becomes 0: three factors of 2^-126 bring
+// any number below the least.
+template <int N, typename V>
+__device__ __forceinline__ void fall_by(V (&o)[N], float f) {
+  constexpr float LEAST = 1.17549435e-38f;          // 2^-126
+  const bool none = f == 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) o[i] *= none ? LEAST : f;
+  if (__any(none)) {
+    const float again = none ? LEAST : 1.f;
+#pragma unroll 1
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] *= again;
+  }
 }
 
 struct Place {
@@ -570,7 +590,7 @@ __device__ __forceinline__ float *part_sums(const KvCache &kv, const Chunk &a, i
 // At D = 256 (s - m) scale takes two operations, elsewhere one multiply-add and the
 // branch for far maxima: that branch's registers do not fit beside 128 of out.
 template <int D, typename T>
-__global__ __launch_bounds__(kThreads, 2) void chunk_kernel(KvCache kv, Chunk a) {
+__global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void chunk_kernel(KvCache kv, Chunk a) {
   typedef Turns<D, T, kWaves> Tn;
   typedef typename Of<T>::x8 x8;
   constexpr int KT = Tn::KT, ROW = Tn::ROW, BYTES = Tn::BYTES;
@@ -663,11 +683,10 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(KvCache kv, Chunk a)
     if (__any((top - m) * scale > SLACK)) {         // from -infinity too
       top = fmaxf(top, __shfl_xor(top, 32));
       const float up = (top - m) * scale > SLACK ? top : m;
-      const float fall = exp2_of((m - base_of(up)) * scale);
+      const float fall = m == -INFINITY ? 1.f : exp2_of((m - up) * scale);
       m = up;
       l *= fall;
-#pragma unroll
-      for (int d = 0; d < ND; ++d) o[d] *= fall;
+      fall_by(o, fall);
     }
     const float base = base_of(m);
     float sum = 0.f;
@@ -892,11 +911,10 @@ __global__ __launch_bounds__(64 * NW, 2) void chunk_f32_kernel(KvCache kv, Chunk
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
         const float up = (top - m[c]) * scale > SLACK ? top : m[c];
-        const float fall = exp2_of((m[c] - base_of(up)) * scale);
+        const float fall = m[c] == -INFINITY ? 1.f : exp2_of((m[c] - up) * scale);
         m[c] = up;
         l[c] *= fall;
-#pragma unroll
-        for (int d = 0; d < NC * 4; ++d) o[c][d] *= fall;
+        fall_by(o[c], fall);
       }
       const float base = base_of(m[c]);
 #pragma unroll
@@ -1031,10 +1049,13 @@ __global__ __launch_bounds__(kThreads) void chunk_join_kernel(KvCache kv, Chunk 
       for (int x = 0; x < AT_ONCE; ++x) {
         if (s0 + x >= j.w) break;
         const float top = fmaxf(m, sm[x]), base = base_of(top);
-        const float f = exp2_of(m - base), y = exp2_of(sm[x] - base);
+        const float f = m == -INFINITY ? 1.f : exp2_of(m - base), y = exp2_of(sm[x] - base);
         m = top;
         l = l * f + sl[x] * y;
-        o = o * f + so[x] * y;
+        f32x4 was[1] = {o}, part[1] = {so[x]};
+        fall_by(was, f);
+        fall_by(part, y);
+        o = was[0] + part[0];
       }
     }
     const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;

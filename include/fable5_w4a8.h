@@ -534,8 +534,9 @@ int w4a8_kv_attend_chunk_workspace(const w4a8_kv *kv, int32_t rows, int32_t toke
    out_dtype: the cache's, or I16 (with out_frac fraction bits).  Tokens of a
    padded row get zeros; those of no row are left alone.  Weights go into the
    second product rounded to the cache's dtype.  An infinity or a NaN in a key
-   or value reaches no token before its own.  rows, tokens and q_heads: the
-   plan's. */
+   or value reaches no token before its own; an infinite value makes that element
+   of the tokens that see it that infinity (where both are seen, or it weighs 0,
+   some number that is not finite).  rows, tokens and q_heads: the plan's. */
 int w4a8_kv_attend_chunk_async(w4a8_kv *kv, int32_t layer, const void *d_q,
                                int64_t q_token, int64_t q_head, int32_t out_dtype,
                                int32_t out_frac, void *d_out, int64_t out_token,
