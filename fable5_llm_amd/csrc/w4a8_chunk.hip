@@ -312,10 +312,16 @@ __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2
 // -infinity, so that every weight there is 0 and not a NaN
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
 
-// Where a maximum (times scale) is this far from 0, its last bit (a sixteenth) is
-// no longer nothing to an exponent: 2^(s scale - m scale) with m scale rounded
-// would be that bit off 1 for the largest score, up to infinity.
-constexpr float kFar = 1048576.f;
+// Where a maximum (times scale) is this far from 0, its rounding (below that half of
+// 2^-13) is no longer nothing to an exponent: in 2^(s scale - m scale) with m scale rounded
+// it is a factor that all weights against m have, and those against the next maximum
+// have another.  Two of them are 2^-13.5 of a weight at most, a sixth of what its own
+// rounding to float16 may be.
+constexpr float kFar = 2048.f;
+// of scores, in powers of two; what is below 0 or 0 is part of q
+__device__ __forceinline__ float scale_of(const Chunk &a) {
+  return a.scale == 0.f ? 1.f : fabsf(a.scale);
+}
 
 struct Unit {
   int seq, tok, ntok, pos0, k0, k1, slot;
@@ -558,7 +564,8 @@ __device__ __forceinline__ void zeros(const KvCache &kv, const Chunk &a, const U
 }
 
 // Where four elements, 4 e .., of a row of a unit's part lie: 32 rows' side by
-// side, as the lanes of a wavefront hold them; then (all rows') maximum and sum.
+// side, as the lanes of a wavefront hold them; then (all rows') maximum, of scores
+// before the scale so that large ones' differences are exact, and sum.
 __device__ __forceinline__ float *part_at(const KvCache &kv, const Chunk &a, int slot,
                                           const Place &p, int row, int e) {
   const int per = kv.heads * a.shape.tiles;
@@ -621,7 +628,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void chunk_kernel(KvCach
       u.pos0 + min(u.ntok - 1, __builtin_amdgcn_readfirstlane((wave * 32 + 31) / P.heads));
   // a scale below 0 turns q, and 0 makes it 0 (a masked score is -infinity)
   const float sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f;
-  const float scale = a.scale == 0.f ? 1.f : fabsf(a.scale);
+  const float scale = scale_of(a);
   if (threadIdx.x == 0) odd = 0;
   x8 q[KS];
 #pragma unroll
@@ -800,7 +807,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void chunk_kernel(KvCach
           f32x4{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]};
   if (g == 0) {
     float *ml = part_sums(kv, a, u.slot, P, row);
-    ml[0] = m * scale;
+    ml[0] = m;
     ml[1] = l;
   }
 }
@@ -854,7 +861,7 @@ __global__ __launch_bounds__(64 * NW, 2) void chunk_f32_kernel(KvCache kv, Chunk
       }
     }
   }
-  const float scale = a.scale == 0.f ? 1.f : fabsf(a.scale);
+  const float scale = scale_of(a);
   if (threadIdx.x == 0) odd = 0;
   const uint32_t lds = (uint32_t)(uintptr_t)buf;
   __builtin_amdgcn_sched_barrier(0);
@@ -998,13 +1005,14 @@ __global__ __launch_bounds__(64 * NW, 2) void chunk_f32_kernel(KvCache kv, Chunk
       }
     if (part && g == 0) {
       float *ml = part_sums(kv, a, u.slot, P, row[c]);
-      ml[0] = m[c] * scale;
+      ml[0] = m[c];
       ml[1] = sum;
     }
   }
 }
 
-// The parts of a tile joined: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
+// The parts of a tile joined, with c = the scale in powers of two:
+//   out = sum_s 2^(c (m_s - M)) o_s / sum_s 2^(c (m_s - M)) l_s.
 // A thread takes four elements of a row; a workgroup ROWS rows and FOURS such fours
 // of them (128 bytes of a part, 64 of out side by side), one tile's after another,
 // so that few are launched where nothing was split.  Bound by its reads: 10 us behind
@@ -1019,6 +1027,7 @@ __global__ __launch_bounds__(kThreads) void chunk_join_kernel(KvCache kv, Chunk 
   typedef JoinShape<D> J;
   constexpr int AT_ONCE = 4;
   const int per = kv.heads * a.shape.tiles;
+  const float scale = scale_of(a);
   const int64_t all = min((int64_t)a.plan[1], a.shape.joins) * per * J::GROUPS;
   for (int64_t w = blockIdx.x; w < all; w += gridDim.x) {
     const int64_t unit = w / J::GROUPS;
@@ -1049,7 +1058,8 @@ __global__ __launch_bounds__(kThreads) void chunk_join_kernel(KvCache kv, Chunk 
       for (int x = 0; x < AT_ONCE; ++x) {
         if (s0 + x >= j.w) break;
         const float top = fmaxf(m, sm[x]), base = base_of(top);
-        const float f = m == -INFINITY ? 1.f : exp2_of(m - base), y = exp2_of(sm[x] - base);
+        const float f = m == -INFINITY ? 1.f : exp2_of((m - base) * scale);
+        const float y = exp2_of((sm[x] - base) * scale);
         m = top;
         l = l * f + sl[x] * y;
         f32x4 was[1] = {o}, part[1] = {so[x]};
