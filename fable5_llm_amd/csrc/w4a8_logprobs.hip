@@ -18,6 +18,7 @@ constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kBlock = 1024;      // logits of a block
 constexpr int kPer = kBlock / 64; // of a lane
 constexpr int kList = 1024;       // candidates that are ranked in LDS
+constexpr float kFar = 16777216.f; // 2^24: scaled logits of a last bit above 1 lie beyond
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -192,9 +193,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_sums_kernel(Logprobs a) {
     bool done = false;
     if constexpr (ALL && !__is_same(T, int32_t)) {
       // one multiply-add a difference, against the scaled maximum as it is rounded;
-      // what that is off by is taken out of the sums
+      // what that is off by, half a power of two at most, is taken out of the sums
       const float ref = sums.m * a.scale;
-      if (!__any(!(fabsf(ref) < 1e38f))) {
+      if (!__any(!(fabsf(ref) < kFar))) {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
           const float d = __builtin_fmaf(L::of(p.x[i]), a.scale, -ref), e = exp2_of(d);
