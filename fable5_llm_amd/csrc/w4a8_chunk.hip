@@ -181,9 +181,9 @@ constexpr int kSorted = 128;
 
 // Steps of up to kOne rows in one launch: every workgroup takes in all rows, a
 // thread each, and then writes kOne tokens and units of its own.  61 rows of a token
-// 8.7 us (7.5 under the profiler, of which an empty kernel is 4.4), 300 rows of up
-// to 40 9.7; one workgroup for the rows and a second launch for the tokens took
-// 11.6 and 14.6.
+// 8 us (7.9 under the profiler, of which an empty kernel is 4.4), 300 rows of 16,381
+// tokens 9, 1,024 rows of a token 10.5; one workgroup for the rows and a second launch
+// for the tokens took 11.6 and 14.6 for the first two.
 __global__ __launch_bounds__(kOne) void kv_map_kernel(KvCache kv, KvMap m) {
   __shared__ int32_t at[6][kOne + 1];       // where a row's tokens, units, joins, parts begin,
                                             // its parts, its units' place in the plan
@@ -248,7 +248,9 @@ __global__ __launch_bounds__(kOne) void kv_map_kernel(KvCache kv, KvMap m) {
 }
 
 // More rows: first one workgroup, which leaves where rows' tokens, units, joins and
-// parts begin behind the plan's joins;
+// parts begin behind the plan's joins, a round of loads for each kOne rows and another
+// for their scans (2,000 rows of 16,000 tokens 19.6 us in all, 10.7 of them here; 1,025
+// rows of a token 17.5);
 __global__ __launch_bounds__(kOne) void kv_map_rows_kernel(KvCache kv, KvMap m) {
   int32_t *rows = m.plan + kPlanHead + kUnitWords * m.shape.units + kJoinWords * m.shape.joins;
   const bool stopped = kv_stopped(kv);
@@ -587,15 +589,28 @@ __device__ __forceinline__ float *part_sums(const KvCache &kv, const Chunk &a, i
 // values of the next turn are copied to LDS while this one is worked on; a turn's 32
 // or 64 keys serve 128 rows, so that LDS is read once for 128 operations a byte.
 //
-// Bound by the matrix units and the clock that their power leaves them: 8,192
-// tokens of a prompt, 16 query heads of 256, 549 us, 1.0 PFLOP/s (a large product
-// reaches 1.17); without conflicts in LDS, at 2.1 of 2.4 GHz.  Turns whose products
-// begin before the last turn's weights are done gain nothing there.  Short calls
-// wait: 17 tokens over 511 keys, 9.8 us, of which 2 before the first turn, 1.1 a turn
-// and 2.6 for the parts' stores.
+// No one unit is the bound: a wavefront's products, exponents and reads of LDS follow
+// one another, and the two wavefronts of a SIMD cover each other in part.  8,192
+// tokens of a prompt, 16 query heads of 256, take 533-571 us on several cards,
+// 0.96-1.03 PFLOP/s, with the matrix units busy 45 % of the cycles at 1.9 of 2.4 GHz (a
+// product of 8,192 x 8,192 x 8,192: 1.35-1.39 PFLOP/s, 70 % at 1.8), and no conflicts
+// in LDS; 100 tokens over 131,072 keys, heads of 128, 291-300 us, 36 %.  At heads of
+// 256 turns whose products begin before the last turn's weights are done gained
+// nothing; at fewer that was not tried.  Short calls wait: 17 tokens over 511 keys,
+// 10-11 us, of which 2 before the first turn, 1.1 a turn and 2.6 for the parts' stores.
+//
+// Weights are rounded once to the cache's type for the second product, beside the
+// rounding of the output: errors against 64 bits of 1.25 to 1.42 times what the latter
+// alone leaves (bfloat16 0.0022 for 0.0016, float16 0.00025 for 0.0002; two roundings
+// of one size and no relation, so the square root of 2 at most).  As sums of two
+// values, as for a single token, they leave none of it, for half as many products
+// again: the prompt took 775 us where it takes 569, 100 tokens over 131,072 391 for 299,
+// 17 over 511 15.1 for 14.6; and an infinite value would meet a second part of 0.
 //
 // At D = 256 (s - m) scale takes two operations, elsewhere one multiply-add and the
 // branch for far maxima: that branch's registers do not fit beside 128 of out.
+// At D = 64 registers are held to 128, four wavefronts a SIMD (8,192 tokens of a prompt,
+// 64 heads of 64, 629 us; with the 140 that it takes otherwise 640).
 template <int D, typename T>
 __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void chunk_kernel(KvCache kv, Chunk a) {
   typedef Turns<D, T, kWaves> Tn;
@@ -815,9 +830,11 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 4 : 2) void chunk_kernel(KvCach
 // Keys and values of 32 bits, on the float32 matrix instructions: 16 keys by 16
 // queries, a wavefront's queries as C columns of tiles, so that q and out stay
 // in 128 registers.  Weights stay in 32 bits.  At the float32 matrix rate, an eighth
-// of the 16-bit one, this is bound by the matrix units once the chip is full: 1,000
-// tokens of five rows over up to 2,000 keys, 8 heads of 64, 27 us of 6 at that rate
-// (few units of uneven length), and 8.5 for the join.
+// of the 16-bit one, this is bound by the matrix units once the chip is full: 4,096
+// tokens of a prompt, 32 heads of 128, 1.17 ms, 117 of 153 TFLOP/s.  1,000 tokens of
+// five rows over up to 2,000 keys, 8 heads of 64, take 27 us of 6 at that rate (few units
+// of uneven length: the matrix units are busy 22 % of the cycles), and 6.5 for the
+// join.
 template <int D, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void chunk_f32_kernel(KvCache kv, Chunk a) {
   typedef Turns<D, float, NW> Tn;
@@ -1015,8 +1032,8 @@ __global__ __launch_bounds__(64 * NW, 2) void chunk_f32_kernel(KvCache kv, Chunk
 //   out = sum_s 2^(c (m_s - M)) o_s / sum_s 2^(c (m_s - M)) l_s.
 // A thread takes four elements of a row; a workgroup ROWS rows and FOURS such fours
 // of them (128 bytes of a part, 64 of out side by side), one tile's after another,
-// so that few are launched where nothing was split.  Bound by its reads: 10 us behind
-// 100 tokens over 131,072 keys, 5 where there is little (2.6 where nothing is).
+// so that few are launched where nothing was split.  Bound by its reads: 8.4 us behind
+// 100 tokens over 131,072 keys; 4.4 where there is little, and as much where nothing is.
 template <int D>
 struct JoinShape {
   static constexpr int FOURS = D / 4 < 32 ? D / 4 : 32, ROWS = kThreads / FOURS;
@@ -1103,13 +1120,16 @@ ChunkShape chunk_shape(const KvCache &kv, int64_t rows, int64_t tokens, int64_t 
   c.tokens = kChunkRows / c.heads;
   const int64_t per = (int64_t)kv.heads * c.tiles, most = rows < tokens ? rows : tokens;
   const int64_t tiles = tokens / c.tokens + most;
-  // Two units a compute unit, as its LDS holds: 100 tokens over 131,072 keys 292 us
-  // (one 360), 1,000 float32 tokens of five rows 35 (one 42), 700 of three over up
-  // to 9,000 keys 55 (four 65, one 49), 64 of two over up to 60,000 of 64 elements
-  // 56 (four 81, one 50)
+  // Two units a compute unit, as its LDS holds: 100 tokens over 131,072 keys 296 us
+  // (one 362, four 303), 1,000 float32 tokens of five rows 33 (48, 33), 2,000 of twenty 83
+  // (92, 106), 64 of two over up to 60,000 of 64 elements 44 (43, 58); the other way
+  // 700 of three over up to 9,000 keys 54 (47, 62), 3,001 of thirteen 132 (127, 135)
   c.split = (2ll * num_cu + per - 1) / per;
-  // two turns of the kernels: 17 tokens over 511 keys of 256 bfloat16 16.1 us in
-  // parts of 128 keys, 15.2 in parts of 64; five rows of float32 keys of 64 35, 43
+  // two turns of the kernels.  17 tokens over 511 keys in parts of 64 keys and of 128:
+  // 256 bfloat16 elements a key 14.3 and 15.8 us, float32 128 19.5 and 27.4, 256 28.3 and
+  // 43.5; bfloat16 64 and 128 11 and 12 either way, float32 64 15.2 and 18.4.  1,000 tokens
+  // of five rows over up to 2,000: float32 256 100 and 92, 128 53 and 53, 64 34 and
+  // 34; bfloat16 256 36 and 34, 128 23 and 23, 64 18.9 and 17.7
   c.least = kv.dim * kv.esize >= 512 ? 64 : 128;
   const bool can = (((int64_t)kv.max_pages << kv.lg_page) > c.least) && tiles > 0;
   c.joins = can ? (tiles < c.split ? tiles : c.split) : 0;

@@ -162,7 +162,7 @@ __device__ __forceinline__ void load_block(Piece<T> &p, const T *row, int64_t vo
 }
 
 // First kernel: `splits` workgroups a row, a wavefront a block at a time.  Bound by
-// HBM and the exponents beside it: 509 rows of 248,320 bfloat16 logits 48 us, 5.3 TB/s
+// HBM and the exponents beside it: 509 rows of 248,320 bfloat16 logits 48-49 us, 5.2 TB/s
 // (reads alone reach 7.35).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void logprobs_sums_kernel(Logprobs a) {

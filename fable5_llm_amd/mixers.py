@@ -423,7 +423,11 @@ def rotary_frequencies(rot, base=10000.0, stretch=None, factor=1.0, trained=None
       stretch="parts"      pairs that turn `fast` times or more within `trained`
                            as they were, those of `slow` or fewer f / factor, in
                            between a ramp over the turns; amplitude 0.1 log
-                           factor + 1"""
+                           factor + 1
+
+    A checkpoint trained with another rule (a ramp over the pairs' index between
+    those of `fast` and `slow` turns is common, and gives the pairs between other
+    frequencies) needs its own: the calls take any."""
     import torch
     if rot < 2 or rot % 2:
         raise ValueError("rot: must be even, 2 or more")

@@ -574,7 +574,7 @@ int w4a8_rotary_async(w4a8_ctx *ctx, const w4a8_rotary *r);
 /* The same for a layer's q into q_out, and k and v into their slots of the
    cache, whose dtype is out_dtype.  A token without a slot is padding too; one
    outside the pool is reported by the next sync.  Two tokens with the same slot
-   leave either one's values there. */
+   leave either one's values there, piece by piece. */
 int w4a8_kv_append_rotary_async(w4a8_kv *kv, int32_t layer, const w4a8_rotary *r);
 
 /* What rows of logits say.  With y = scale * logits, per row: the log
